@@ -74,6 +74,16 @@ _PROTOTYPES: dict[str, tuple[object, list[object]]] = {
     "aa_context_lengths": (
         c_int, [c_void_p] + [_I64] * 5 + [c_int] + [c_void_p] * 3 + [c_size_t, c_void_p]
     ),
+    "aa_adaln_fwd": (c_int, [c_void_p, c_void_p]),
+    "aa_adaln_bwd_workspace": (c_size_t, [_I64] * 3 + [c_int]),
+    "aa_adaln_bwd": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
+    "aa_rowquant_int8": (c_int, [c_void_p, _I64, _I64, c_int, c_void_p, c_void_p, c_int, c_void_p]),
+    "aa_int8_linear": (c_int, [c_void_p] * 5 + [_I64] * 3 + [c_int, c_void_p]),
+    "aa_gelu8_fwd": (c_int, [c_void_p] * 4 + [_I64] * 2 + [c_int, c_void_p]),
+    "aa_gelu8_bwd": (c_int, [c_void_p] * 4 + [_I64] * 2 + [c_int, c_void_p]),
+    "aa_lora8_fwd": (c_int, [c_void_p] * 5 + [_I64] * 3 + [c_int, c_void_p]),
+    "aa_lora8_bwd_workspace": (c_size_t, [_I64] * 3),
+    "aa_lora8_bwd": (c_int, [c_void_p] * 6 + [c_void_p, c_size_t] + [_I64] * 3 + [c_int, c_void_p]),
 }
 
 EXPORTED = tuple(_PROTOTYPES)
@@ -134,6 +144,66 @@ class AttnBwdArgs(Structure):
         ("hd", c_int64),
         ("softmax_scale", c_float),
         ("dtype", c_int),
+    ]
+
+
+class AdalnArgs(Structure):
+    """Mirror of aa_adaln_args."""
+
+    _fields_ = [
+        ("x", c_void_p),
+        ("y", c_void_p),
+        ("gate", c_void_p),
+        ("scale", c_void_p),
+        ("shift", c_void_p),
+        ("gate_stride", c_int64),
+        ("scale_stride", c_int64),
+        ("shift_stride", c_int64),
+        ("weight", c_void_p),
+        ("r", c_void_p),
+        ("h", c_void_p),
+        ("q", c_void_p),
+        ("q_scale", c_void_p),
+        ("stats", c_void_p),
+        ("B", c_int64),
+        ("S", c_int64),
+        ("D", c_int64),
+        ("eps", c_float),
+        ("branch_scale", c_float),
+        ("dtype", c_int),
+        ("mod_dtype", c_int),
+    ]
+
+
+class AdalnBwdArgs(Structure):
+    """Mirror of aa_adaln_bwd_args."""
+
+    _fields_ = [
+        ("dr", c_void_p),
+        ("dh", c_void_p),
+        ("x", c_void_p),
+        ("y", c_void_p),
+        ("gate", c_void_p),
+        ("scale", c_void_p),
+        ("gate_stride", c_int64),
+        ("scale_stride", c_int64),
+        ("weight", c_void_p),
+        ("stats", c_void_p),
+        ("dx", c_void_p),
+        ("dy", c_void_p),
+        ("dgate", c_void_p),
+        ("dscale", c_void_p),
+        ("dshift", c_void_p),
+        ("dweight", c_void_p),
+        ("gate_rows", c_int64),
+        ("scale_rows", c_int64),
+        ("shift_rows", c_int64),
+        ("B", c_int64),
+        ("S", c_int64),
+        ("D", c_int64),
+        ("branch_scale", c_float),
+        ("dtype", c_int),
+        ("mod_dtype", c_int),
     ]
 
 
@@ -247,6 +317,8 @@ __all__ = [
     "AA_EINVAL",
     "AA_EUNSUPPORTED",
     "AA_OK",
+    "AdalnArgs",
+    "AdalnBwdArgs",
     "AttnBwdArgs",
     "AttnFwdArgs",
     "EXPORTED",

@@ -29,7 +29,7 @@ LIB_PATH = HERE / LIB_NAME
 SOURCES = (
     "abi.hip", "prologue.hip", "ctx_scale.hip", "context.hip", "rowquant.hip", "attn_fwd.hip",
     "attn_fwd_pp.hip", "attn_fwd_ks.hip", "attn_fwd_d384.hip", "attn_bwd.hip", "attn_bwd_dq_ks.hip",
-    "attn_bwd_dkdv.hip", "qkv_proj.hip",
+    "attn_bwd_dkdv.hip", "qkv_proj.hip", "adaln.hip", "int8_linear.hip", "ckpt8.hip",
 )
 ARCH = "gfx950"
 # The measurement's MFMA-rate calibration (bench.py), a library of its own so

@@ -1,0 +1,320 @@
+"""Norms, gate, residual and modulation around a block's sublayers on MI355X, opt-in.
+
+What stands between two sublayers of the block (src/kernels/adaln.py:298-314 in the
+reference, whose ops this module does not register: import `anima_flat_amd.kernels.adaln`
+to use it; its ops live in the `anima_flat_amd::` namespace):
+
+  residual_adaln       r = x + branch_scale * gate * norm(y); h = LayerNorm(r) * (1 + scale) + shift
+  adaln                h = LayerNorm(x) * (1 + scale) + shift (in front of the first sublayer)
+  residual_adaln_int8  residual_adaln with h as int8 codes and a scale per token, for
+                       kernels.int8.int8_linear (inference; src/kernels/fp8.py:56-97 in int8)
+
+One kernel forward (aa_adaln_fwd), one backward and, where the modulation or the norm's
+weight is trained, a second that adds up its partial sums (aa_adaln_bwd). All arithmetic is
+fp32; r and h are rounded to bf16 once each, and the norm is taken of the unrounded r.
+Gradients are deterministic.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+
+from .. import _lib
+from .common import _check, aligned, custom_op
+from .rope import _f32
+
+MAX_D = 8192
+
+
+def _mod_code(t: torch.Tensor) -> int:
+    return 2 if t.dtype == torch.float32 else 0
+
+
+def _mod_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else 0
+
+
+def _forward(x, y, gate, scale, shift, weight, eps, branch_scale, want_stats, int8):
+    B, S, D = x.shape
+    x, y, gate, scale, shift = (None if t is None else aligned(t) for t in (x, y, gate, scale, shift))
+    r = torch.empty_like(x) if y is not None else None
+    h = q = qs = None
+    if int8:
+        q = torch.empty(B, S, D, dtype=torch.int8, device=x.device)
+        qs = torch.empty(B * S, 1, dtype=torch.float32, device=x.device)
+    else:
+        h = torch.empty_like(x)
+    stats = torch.empty(B * S if want_stats else 0, 4, dtype=torch.float32, device=x.device)
+    w = None if weight is None else aligned(_f32(weight))
+    a = _lib.AdalnArgs(
+        x=x.data_ptr(), y=_lib.ptr(y), gate=_lib.ptr(gate), scale=scale.data_ptr(), shift=shift.data_ptr(),
+        gate_stride=0 if gate is None else _mod_stride(gate), scale_stride=_mod_stride(scale),
+        shift_stride=_mod_stride(shift), weight=_lib.ptr(w), r=_lib.ptr(r), h=_lib.ptr(h), q=_lib.ptr(q),
+        q_scale=_lib.ptr(qs), stats=stats.data_ptr() if want_stats else None, B=B, S=S, D=D, eps=eps,
+        branch_scale=branch_scale, dtype=_lib.dtype_code(x), mod_dtype=_mod_code(scale),
+    )
+    with torch.cuda.device(x.device):
+        _lib.check(_lib.lib().aa_adaln_fwd(ctypes.byref(a), _lib.stream(x)), "adaln")
+    return r, h, q, qs, stats
+
+
+def _backward(dr, dh, x, y, gate, scale, weight, stats, shift_rows, branch_scale, mods):
+    """(dx, dy, dgate, dscale, dshift, dweight); what is not computed has no elements."""
+    B, S, D = x.shape
+    dr, dh = (None if t is None else aligned(t.contiguous()) for t in (dr, dh))
+    x, y, gate, scale = (None if t is None else aligned(t) for t in (x, y, gate, scale))
+    dx = torch.empty_like(x)
+    dy = torch.empty_like(x) if y is not None else x.new_empty(0)
+    dgate, dscale, dshift, dweight = (x.new_empty(0) for _ in range(4))
+    if mods:
+        dscale, dshift = torch.empty_like(scale, memory_format=torch.contiguous_format), scale.new_empty(shift_rows, D)
+        if y is not None:
+            dgate = torch.empty_like(gate, memory_format=torch.contiguous_format)
+        if weight is not None:
+            dweight = torch.empty(D, dtype=torch.float32, device=x.device)
+    out = dx, dy, dgate, dscale, dshift, dweight
+    if x.numel() == 0:
+        for t in out:
+            t.zero_()
+        return out
+    w = None if weight is None else aligned(_f32(weight))
+
+    def p(t):
+        return t.data_ptr() if t.numel() else None
+
+    a = _lib.AdalnBwdArgs(
+        dr=_lib.ptr(dr), dh=_lib.ptr(dh), x=x.data_ptr(), y=_lib.ptr(y), gate=_lib.ptr(gate),
+        scale=scale.data_ptr(), gate_stride=0 if gate is None else _mod_stride(gate),
+        scale_stride=_mod_stride(scale), weight=_lib.ptr(w), stats=stats.data_ptr(), dx=dx.data_ptr(),
+        dy=p(dy), dgate=p(dgate), dscale=p(dscale), dshift=p(dshift), dweight=p(dweight),
+        gate_rows=1 if gate is None else gate.shape[0], scale_rows=scale.shape[0], shift_rows=shift_rows,
+        B=B, S=S, D=D, branch_scale=branch_scale, dtype=_lib.dtype_code(x), mod_dtype=_mod_code(scale),
+    )
+    with torch.cuda.device(x.device):
+        ws_bytes = _lib.lib().aa_adaln_bwd_workspace(B, S, D, int(mods))
+        ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=x.device) if ws_bytes else None
+        _lib.check(
+            _lib.lib().aa_adaln_bwd(ctypes.byref(a), _lib.ptr(ws), ws_bytes, _lib.stream(x)), "adaln_bwd"
+        )
+    return out
+
+
+# --------------------------------------------------------------------- ops --
+
+
+@custom_op("anima_flat_amd::residual_adaln", mutates_args=())
+def _residual_adaln(
+    x: torch.Tensor, y: torch.Tensor, gate: torch.Tensor, scale: torch.Tensor, shift: torch.Tensor,
+    weight: Optional[torch.Tensor], eps: float, branch_scale: float, want_stats: bool,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    r, h, _, _, stats = _forward(x, y, gate, scale, shift, weight, eps, branch_scale, want_stats, False)
+    return r, h, stats
+
+
+@_residual_adaln.register_fake
+def _(x, y, gate, scale, shift, weight, eps, branch_scale, want_stats):
+    rows = x.shape[0] * x.shape[1] if want_stats else 0
+    return torch.empty_like(x), torch.empty_like(x), x.new_empty((rows, 4), dtype=torch.float32)
+
+
+@custom_op("anima_flat_amd::adaln", mutates_args=())
+def _adaln(
+    x: torch.Tensor, scale: torch.Tensor, shift: torch.Tensor, eps: float, want_stats: bool
+) -> tuple[torch.Tensor, torch.Tensor]:
+    _, h, _, _, stats = _forward(x, None, None, scale, shift, None, eps, 1.0, want_stats, False)
+    return h, stats
+
+
+@_adaln.register_fake
+def _(x, scale, shift, eps, want_stats):
+    rows = x.shape[0] * x.shape[1] if want_stats else 0
+    return torch.empty_like(x), x.new_empty((rows, 4), dtype=torch.float32)
+
+
+@custom_op("anima_flat_amd::residual_adaln_int8", mutates_args=())
+def _residual_adaln_int8(
+    x: torch.Tensor, y: torch.Tensor, gate: torch.Tensor, scale: torch.Tensor, shift: torch.Tensor,
+    weight: Optional[torch.Tensor], eps: float, branch_scale: float,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    r, _, q, qs, _ = _forward(x, y, gate, scale, shift, weight, eps, branch_scale, False, True)
+    return r, q, qs
+
+
+@_residual_adaln_int8.register_fake
+def _(x, y, gate, scale, shift, weight, eps, branch_scale):
+    rows = x.shape[0] * x.shape[1]
+    return torch.empty_like(x), torch.empty_like(x, dtype=torch.int8), x.new_empty((rows, 1), dtype=torch.float32)
+
+
+@custom_op("anima_flat_amd::adaln_bwd", mutates_args=())
+def _adaln_bwd(
+    dr: Optional[torch.Tensor], dh: Optional[torch.Tensor], x: torch.Tensor, y: Optional[torch.Tensor],
+    gate: Optional[torch.Tensor], scale: torch.Tensor, weight: Optional[torch.Tensor], stats: torch.Tensor,
+    shift_rows: int, branch_scale: float, mods: bool,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _backward(dr, dh, x, y, gate, scale, weight, stats, shift_rows, branch_scale, mods)
+
+
+@_adaln_bwd.register_fake
+def _(dr, dh, x, y, gate, scale, weight, stats, shift_rows, branch_scale, mods):
+    D = x.shape[2]
+    return (
+        torch.empty_like(x),
+        torch.empty_like(x) if y is not None else x.new_empty(0),
+        gate.new_empty(gate.shape) if mods and y is not None else x.new_empty(0),
+        scale.new_empty(scale.shape) if mods else x.new_empty(0),
+        scale.new_empty((shift_rows, D)) if mods else x.new_empty(0),
+        x.new_empty(D, dtype=torch.float32) if mods and weight is not None else x.new_empty(0),
+    )
+
+
+def _residual_adaln_setup(ctx, inputs, output):
+    x, y, gate, scale, shift, weight, _, ctx.branch_scale, want_stats = inputs
+    if not want_stats:
+        raise RuntimeError("residual_adaln: a call that needs gradients keeps its statistics (want_stats)")
+    ctx.set_materialize_grads(False)
+    ctx.mods = any(ctx.needs_input_grad[2:6])
+    ctx.shift_rows = shift.shape[0]
+    ctx.save_for_backward(x, y, gate, scale, weight, output[2])
+
+
+def _residual_adaln_backward(ctx, dr, dh, _):
+    x, y, gate, scale, weight, stats = ctx.saved_tensors
+    if dr is None and dh is None:
+        return (None,) * 9
+    dx, dy, dgate, dscale, dshift, dweight = _adaln_bwd(
+        dr, dh, x, y, gate, scale, weight, stats, ctx.shift_rows, ctx.branch_scale, ctx.mods
+    )
+    if not ctx.mods:
+        return (dx, dy) + (None,) * 7
+    dw = None if weight is None else dweight.to(weight.dtype)
+    return dx, dy, dgate, dscale, dshift, dw, None, None, None
+
+
+torch.library.register_autograd(
+    "anima_flat_amd::residual_adaln", _residual_adaln_backward, setup_context=_residual_adaln_setup
+)
+
+
+def _adaln_setup(ctx, inputs, output):
+    x, scale, shift, _, want_stats = inputs
+    if not want_stats:
+        raise RuntimeError("adaln: a call that needs gradients keeps its statistics (want_stats)")
+    ctx.set_materialize_grads(False)
+    ctx.mods = any(ctx.needs_input_grad[1:3])
+    ctx.shift_rows = shift.shape[0]
+    ctx.save_for_backward(x, scale, output[1])
+
+
+def _adaln_backward(ctx, dh, _):
+    x, scale, stats = ctx.saved_tensors
+    if dh is None:
+        return (None,) * 5
+    dx, _, _, dscale, dshift, _ = _adaln_bwd(
+        None, dh, x, None, None, scale, None, stats, ctx.shift_rows, 1.0, ctx.mods
+    )
+    return (dx, dscale, dshift, None, None) if ctx.mods else (dx,) + (None,) * 4
+
+
+torch.library.register_autograd("anima_flat_amd::adaln", _adaln_backward, setup_context=_adaln_setup)
+
+
+# -------------------------------------------------------------- public API --
+
+
+def _rows(t: torch.Tensor, x: torch.Tensor, name: str) -> torch.Tensor:
+    """A modulation as [1 or B, D] rows with unit stride that the kernel can read."""
+    B, _, D = x.shape
+    if t.ndim == 3 and t.shape[1] == 1:
+        t = t[:, 0]
+    if t.ndim == 1:
+        t = t[None]
+    if t.ndim != 2 or t.shape[1] != D or t.shape[0] not in (1, B):
+        raise ValueError(f"{name} must be [B, D], [B, 1, D], [1, D] or [D]")
+    if t.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"{name} must be bfloat16 or float32")
+    unit = 16 // t.element_size()
+    if t.stride(1) != 1 or (t.shape[0] > 1 and (t.stride(0) % unit or t.stride(0) < D)):
+        t = t.contiguous()
+    return t
+
+
+def _tokens(x: torch.Tensor, name: str) -> torch.Tensor:
+    if x.ndim != 3 or x.shape[2] == 0:
+        raise ValueError(f"{name} must be [B, S, D]")
+    if x.dtype != torch.bfloat16:
+        raise ValueError(f"unsupported dtype {x.dtype}: only bfloat16 is implemented")
+    if x.shape[2] % 8 or x.shape[2] > MAX_D:
+        raise ValueError(f"D must be a multiple of 8 and at most {MAX_D}")
+    return x.contiguous()
+
+
+def _arguments(x, y, gate, scale, shift, weight):
+    tensors = [t for t in (x, y, gate, scale, shift, weight) if t is not None]
+    _check(*tensors)
+    if any(t.device != x.device for t in tensors):
+        raise ValueError("all tensors must be on one device")
+    if y is not None and y.shape != x.shape:
+        raise ValueError("y must have x's shape")
+    if weight is not None and (weight.shape != x.shape[2:] or weight.dtype not in (torch.bfloat16, torch.float32)):
+        raise ValueError("weight must be [D], bfloat16 or float32")
+    x = _tokens(x, "x")
+    y = None if y is None else _tokens(y, "y")
+    mods = [None if t is None else _rows(t, x, n) for t, n in ((gate, "gate"), (scale, "scale"), (shift, "shift"))]
+    if len({t.dtype for t in mods if t is not None}) > 1:
+        mods = [None if t is None else t.float() for t in mods]
+    return x, y, *mods, None if weight is None else weight.contiguous()
+
+
+def _wants_grad(*ts) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+def residual_adaln(x, y, gate, scale, shift, weight=None, eps=1e-6, branch_scale=1.0):
+    """Add a sublayer's gated output to the residual stream and norm the sum for the next one.
+
+    Args:
+        x: Residual stream `[B, S, D]`, bfloat16 (D a multiple of 8, at most 8192).
+        y: The sublayer's output, x's shape.
+        gate, scale, shift: Modulation, one row per batch item or one for all: `[B, D]`,
+            `[B, 1, D]`, `[1, D]` or `[D]`, bfloat16 or float32 (mixed ones are widened).
+            Views such as `mod.chunk(3, -1)` are read in place.
+        weight: RMSNorm weight `[D]` of a norm on y in front of the gate, or None.
+        eps: Epsilon of both norms.
+        branch_scale: Constant factor of the gated branch.
+
+    Returns:
+        `(r, h)`: `r = x + branch_scale * gate * y` (y normed with `weight`) and
+        `h = LayerNorm(r) * (1 + scale) + shift`, both bfloat16 `[B, S, D]`. Differentiable
+        in every tensor.
+
+    Raises:
+        ValueError: If a tensor is not on CUDA, or its shape or dtype is not supported.
+    """
+    x, y, gate, scale, shift, weight = _arguments(x, y, gate, scale, shift, weight)
+    stats = _wants_grad(x, y, gate, scale, shift, weight)
+    r, h, _ = _residual_adaln(x, y, gate, scale, shift, weight, eps, branch_scale, stats)
+    return r, h
+
+
+def adaln(x, scale, shift, eps=1e-6):
+    """`LayerNorm(x) * (1 + scale) + shift`, arguments as for `residual_adaln`."""
+    x, _, _, scale, shift, _ = _arguments(x, None, None, scale, shift, None)
+    return _adaln(x, scale, shift, eps, _wants_grad(x, scale, shift))[0]
+
+
+def residual_adaln_int8(x, y, gate, scale, shift, weight=None, eps=1e-6, branch_scale=1.0):
+    """`residual_adaln` with h as int8 tokens for `int8_linear`. Inference only (no autograd).
+
+    Returns:
+        `(r, q, s)`: r bfloat16, q int8 `[B, S, D]` and float32 scales `[B * S, 1]` with
+        `h ~ q * s`, rounded from the fp32 h. A token with a value that is not finite has
+        the scale NaN.
+    """
+    x, y, gate, scale, shift, weight = _arguments(x, y, gate, scale, shift, weight)
+    if _wants_grad(x, y, gate, scale, shift, weight):
+        raise RuntimeError("residual_adaln_int8 has no backward: use residual_adaln for training")
+    return _residual_adaln_int8(x, y, gate, scale, shift, weight, eps, branch_scale)

@@ -25,6 +25,12 @@ def _check(*ts: torch.Tensor) -> None:
             raise ValueError("CUDA tensors required")
 
 
+def aligned(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy of it where its first element is not at a 16-byte boundary (for the
+    ops' own functions: tracing tensors have no address)."""
+    return t.clone() if t.data_ptr() % 16 else t
+
+
 def is_registered(qualname: str) -> bool:
     """True if the torch.library op `ns::name` exists in this process."""
     ns, name = qualname.split("::", 1)

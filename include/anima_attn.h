@@ -53,6 +53,7 @@ enum {
 enum {
   AA_DTYPE_BF16 = 0,
   AA_DTYPE_FP16 = 1, /* reserved: rejected with AA_EUNSUPPORTED */
+  AA_DTYPE_FP32 = 2, /* modulation rows of aa_adaln_fwd / _bwd only */
 };
 
 /* ABI version of the loaded library (AA_ABI_VERSION when built from this header). */
@@ -338,6 +339,149 @@ int aa_context_lengths(const void* ctx, int64_t B, int64_t S, int64_t C,
  */
 int aa_rowquant(const void* x, int64_t rows, int64_t K, int gelu,
                 void* q, float* s, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Norms, gate and residual around the sublayers                             */
+/* ------------------------------------------------------------------------ */
+
+typedef struct aa_adaln_args {
+  const void* x;        /* [B, S, D] residual stream */
+  const void* y;        /* [B, S, D] the sublayer's output, or NULL: no residual add */
+  const void* gate;     /* rows of D (mod_dtype), batch item b's at b * gate_stride; unused without y */
+  const void* scale;
+  const void* shift;
+  int64_t gate_stride;  /* elements; 0: one row for all batch items */
+  int64_t scale_stride;
+  int64_t shift_stride;
+  const float* weight;  /* [D] RMSNorm weight of a norm on y, or NULL: y as it is */
+  void* r;              /* [B, S, D] x + branch_scale * gate * norm(y); unused without y */
+  void* h;              /* [B, S, D] modulated norm of r, or NULL when q is set */
+  void* q;              /* [B, S, D] int8 codes of h in place of h, or NULL */
+  float* q_scale;       /* [B * S] scales of q */
+  float* stats;         /* [B * S, 4] for aa_adaln_bwd, or NULL */
+  int64_t B, S, D;
+  float eps;
+  float branch_scale;
+  int dtype;            /* of x, y, r, h */
+  int mod_dtype;        /* of gate, scale, shift: AA_DTYPE_BF16 or AA_DTYPE_FP32 */
+} aa_adaln_args;
+
+/*
+ * n = y, or y * rsqrt(mean(y^2) + eps) * weight; r = x + branch_scale * gate * n
+ * (r = x without y); h = (r - mean(r)) * rsqrt(var(r) + eps) * (1 + scale) + shift,
+ * per token over D channels, all in fp32; r and h are rounded to bf16 once each
+ * (h is that of the fp32 r). With q: s = max(max|h|, 1e-12) / 127 and
+ * q = round-to-nearest-even(h / s) per token; a token with a value that is not
+ * finite has the scale NaN.
+ * x, y, r, h, q contiguous; D a multiple of 8, at most 8192; 16-byte aligned
+ * pointers and modulation rows.
+ * Stands for the work of src/kernels/adaln.py:298-314 (residual_adaln, adaln;
+ * kernel adaln.py:10-46) and, with q, of src/kernels/fp8.py:56-97 in int8.
+ */
+int aa_adaln_fwd(const aa_adaln_args* args, void* stream);
+
+typedef struct aa_adaln_bwd_args {
+  const void* dr;       /* [B, S, D] gradient of r (of h's input x without y), or NULL: zero */
+  const void* dh;       /* [B, S, D] gradient of h, or NULL: zero */
+  const void* x;        /* x, y, gate, scale, weight, strides: as in the forward */
+  const void* y;
+  const void* gate;
+  const void* scale;
+  int64_t gate_stride;
+  int64_t scale_stride;
+  const float* weight;
+  const float* stats;   /* from aa_adaln_fwd */
+  void* dx;             /* [B, S, D] */
+  void* dy;             /* [B, S, D]; unused without y */
+  void* dgate;          /* [gate_rows, D] in mod_dtype, or NULL: not computed */
+  void* dscale;
+  void* dshift;
+  float* dweight;       /* [D], or NULL */
+  int64_t gate_rows;    /* B, or 1: the sum over all batch items */
+  int64_t scale_rows;
+  int64_t shift_rows;
+  int64_t B, S, D;
+  float branch_scale;
+  int dtype;
+  int mod_dtype;
+} aa_adaln_bwd_args;
+
+/* Bytes of workspace aa_adaln_bwd needs on the current device, 16-byte aligned:
+ * partial sums of the modulation's and the weight's gradients; 0 when none of
+ * them is asked for (sums == 0). */
+size_t aa_adaln_bwd_workspace(int64_t B, int64_t S, int64_t D, int sums);
+
+/*
+ * Gradients of aa_adaln_fwd (not of its int8 form), every sum in a fixed order.
+ * Stands for the work of the backward in src/kernels/adaln.py (kernel :111-172).
+ */
+int aa_adaln_bwd(const aa_adaln_bwd_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Int8 products                                                             */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * Per-row int8 quantisation of x [rows, K] bf16 (contiguous): y = x or GELU(x)
+ * (gelu != 0), s[row] = max(max|y|, 1e-12) / 127 (float), q = round-to-nearest-
+ * even(y / s) (int8 [rows, K]). A row with a value that is not finite has the
+ * scale NaN and codes 0. K a multiple of 8 and at most 8192; x 16-byte and q
+ * 8-byte aligned.
+ */
+int aa_rowquant_int8(const void* x, int64_t rows, int64_t K, int gelu,
+                     void* q, float* s, int dtype, void* stream);
+
+/*
+ * y[m, n] = s[m] * weight_scale[n] * sum_k q[m, k] weight[n, k], the sum exact
+ * in int32; q [M, K], weight [N, K] int8, y [M, N] of `dtype` (bf16), all
+ * contiguous and 16-byte aligned; s [M], weight_scale [N] float.
+ * K a multiple of 16 and at most 65536; N a multiple of 8.
+ * Stands for the work of src/kernels/fp8.py:234-257 (fp8_linear) in int8.
+ */
+int aa_int8_linear(const void* q, const float* s, const void* weight, const float* weight_scale,
+                   void* y, int64_t M, int64_t N, int64_t K, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Activations kept in 8 bits for the backward pass                          */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * The 8-bit checkpoint of rows x [rows, K] bf16: per row, groups of 32 channels
+ * (G = ceil(K / 32), the last one may be shorter) share a step, a power of two
+ * 2^(e - 127) with 2^6 <= max|x| / step < 2^7 (e >= 1): code = round-to-nearest-
+ * even(x / step) clamped to +-127. codes: int8 [rows, 32 G], zero past K;
+ * exps: uint8 biased exponents e, 255 for a group with a value that is not
+ * finite (it reads back as NaN).
+ *
+ * aa_gelu8_fwd: y = GELU(x) (erf form), and the checkpoint, exps [rows, G];
+ * codes NULL: y only. aa_gelu8_bwd: dx = dy * GELU'(code * step).
+ * x, y, dy, dx [rows, K] contiguous, codes: 16-byte aligned; K a multiple of 8,
+ * at most 65536.
+ */
+int aa_gelu8_fwd(const void* x, void* y, void* codes, void* exps, int64_t rows, int64_t K,
+                 int dtype, void* stream);
+int aa_gelu8_bwd(const void* dy, const void* codes, const void* exps, void* dx, int64_t rows,
+                 int64_t K, int dtype, void* stream);
+
+/*
+ * t = x a^T (x [M, K], a [R, K], t [M, R], bf16, contiguous), and x's checkpoint
+ * with exps [G, Mp], Mp = M rounded up to a multiple of 16; codes NULL: t only.
+ * R a multiple of 8, at most 64; K a multiple of 8, at most 65536; all pointers
+ * 16-byte aligned.
+ */
+int aa_lora8_fwd(const void* x, const void* a, void* t, void* codes, void* exps, int64_t M,
+                 int64_t K, int64_t R, int dtype, void* stream);
+
+/* Bytes of workspace aa_lora8_bwd needs on the current device for da. */
+size_t aa_lora8_bwd_workspace(int64_t M, int64_t K, int64_t R);
+
+/*
+ * dx = dt a [M, K] and da = dt^T (codes * step) [R, K] (bf16; either may be
+ * NULL: not computed), every sum in a fixed order.
+ */
+int aa_lora8_bwd(const void* dt, const void* a, const void* codes, const void* exps, void* dx,
+                 void* da, void* workspace, size_t workspace_bytes, int64_t M, int64_t K,
+                 int64_t R, int dtype, void* stream);
 
 #ifdef __cplusplus
 }
