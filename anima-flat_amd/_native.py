@@ -29,6 +29,12 @@ NATIVE_OPS = frozenset({
     "anima_flat_amd::kv_proj_norm",
 })
 
+# The block's operators around attention (kernels.adaln, kernels.int8, kernels.ckpt8).
+NATIVE_BLOCK_OPS = frozenset("anima_flat_amd::" + name for name in (
+    "residual_adaln", "adaln", "residual_adaln_int8", "adaln_bwd", "rowquant_int8", "int8_linear",
+    "gelu8", "gelu8_bwd", "lora_down8", "lora_down8_bwd",
+))
+
 _ext = None
 _missing = False
 
@@ -79,7 +85,7 @@ def _load():
 
 def attach(qualname: str, impl) -> None:
     """Give op `qualname` its native kernels, if it has any."""
-    if qualname in NATIVE_OPS:
+    if qualname in NATIVE_OPS or qualname in NATIVE_BLOCK_OPS:
         ext = _load()
         if ext is not None:
             ext.attach(qualname, impl)

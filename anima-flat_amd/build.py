@@ -144,7 +144,9 @@ def _torch_commands() -> tuple[list[str], list[str]]:
     link_cmd = [
         "g++", "-shared", "-fPIC", "-o", str(TORCH_LIB_PATH) + ".tmp", obj, f"-L{root}/lib", f"-L{HERE}",
         "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python", "-lc10", "-lc10_hip", "-lanima_attn",
-        "-Wl,-rpath,$ORIGIN",
+        # Every entry point is looked up when the extension loads: beside a library without one
+        # of them it does not load, instead of ending the process at the first call.
+        "-Wl,-rpath,$ORIGIN", "-Wl,-z,now",
     ]
     return compile_cmd, link_cmd
 

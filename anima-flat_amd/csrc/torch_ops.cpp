@@ -23,8 +23,10 @@
 #include <functional>
 #include <map>
 #include <memory>
+#include <optional>
 #include <string>
 #include <tuple>
+#include <utility>
 #include <vector>
 
 #include "../../include/anima_attn.h"
@@ -389,6 +391,287 @@ T2 kv_proj_norm(const Tensor& x, const Tensor& w, const Tensor& kw, int64_t head
   return python_impl<T2>("kv_proj_norm", x, w, kw, heads, eps);
 }
 
+// ------------------------------------------------------ norms of the block --
+
+using T6 = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;
+using OptT = std::optional<Tensor>;
+
+// Contiguous bf16 [B, S, D] at a 16-byte boundary, on the GPU of `like`.
+bool rows_ready(const Tensor& t, const Tensor& like) {
+  return t.dim() == 3 && bf16_on(t, like) && t.is_contiguous() && aligned16(t) && t.numel() > 0;
+}
+
+// Modulation rows [1 or B, D] that the kernels read in place, of mod0's dtype.
+bool mod_ready(const Tensor& t, const Tensor& x, const Tensor& mod0) {
+  const auto dtype = t.scalar_type();
+  return t.dim() == 2 && t.size(1) == x.size(2) && (t.size(0) == 1 || t.size(0) == x.size(0)) &&
+         dtype == mod0.scalar_type() && (dtype == at::kFloat || dtype == at::kBFloat16) && on_gpu(t, x) &&
+         t.stride(1) == 1 && aligned16(t) &&
+         (t.size(0) == 1 || (t.stride(0) * t.element_size() % 16 == 0 && t.stride(0) >= t.size(1)));
+}
+
+int64_t mod_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : 0; }
+
+bool adaln_ready(const Tensor& x, const Tensor* y, const Tensor* gate, const Tensor& scale, const OptT& weight) {
+  return rows_ready(x, x) && (!y || (rows_ready(*y, x) && y->sizes() == x.sizes() && gate && mod_ready(*gate, x, scale))) &&
+         mod_ready(scale, x, scale) && (!weight || (weight->numel() == x.size(2) && on_gpu(*weight, x)));
+}
+
+// fp32 weight that lives until the launch.
+Tensor f32_or_none(const OptT& weight) { return weight ? f32(*weight) : Tensor(); }
+float* float_ptr(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
+
+bool adaln_forward(const Tensor& x, const Tensor* y, const Tensor* gate, const Tensor& scale, const Tensor& shift,
+                   const OptT& weight, double eps, double branch_scale, Tensor* r, Tensor* h, Tensor* q,
+                   Tensor* qs, Tensor* stats) {
+  if (!adaln_ready(x, y, gate, scale, weight) || !mod_ready(shift, x, scale)) return false;
+  const c10::DeviceGuard guard(x.device());
+  const int64_t B = x.size(0), S = x.size(1), D = x.size(2);
+  const auto fopt = x.options().dtype(at::kFloat);
+  const Tensor w = f32_or_none(weight);
+  if (w.defined() && !aligned16(w)) return false;
+  if (r) *r = at::empty(x.sizes(), x.options());
+  if (h) *h = at::empty(x.sizes(), x.options());
+  if (q) {
+    *q = at::empty(x.sizes(), x.options().dtype(at::kChar));
+    *qs = at::empty({B * S, 1}, fopt);
+  }
+  if (stats) *stats = at::empty({B * S, 4}, fopt);
+  aa_adaln_args a = {};
+  a.x = x.data_ptr();
+  a.y = y ? y->data_ptr() : nullptr;
+  a.gate = gate ? gate->data_ptr() : nullptr;
+  a.scale = scale.data_ptr();
+  a.shift = shift.data_ptr();
+  a.gate_stride = gate ? mod_stride(*gate) : 0;
+  a.scale_stride = mod_stride(scale);
+  a.shift_stride = mod_stride(shift);
+  a.weight = float_ptr(w);
+  a.r = r ? r->data_ptr() : nullptr;
+  a.h = h ? h->data_ptr() : nullptr;
+  a.q = q ? q->data_ptr() : nullptr;
+  a.q_scale = qs ? qs->data_ptr<float>() : nullptr;
+  a.stats = stats ? stats->data_ptr<float>() : nullptr;
+  a.B = B;
+  a.S = S;
+  a.D = D;
+  a.eps = (float)eps;
+  a.branch_scale = (float)branch_scale;
+  a.dtype = AA_DTYPE_BF16;
+  a.mod_dtype = scale.scalar_type() == at::kFloat ? AA_DTYPE_FP32 : AA_DTYPE_BF16;
+  return launched(aa_adaln_fwd(&a, stream_of(x)), "adaln");
+}
+
+T3 residual_adaln(const Tensor& x, const Tensor& y, const Tensor& gate, const Tensor& scale, const Tensor& shift,
+                  const OptT& weight, double eps, double branch_scale, bool want_stats) {
+  Tensor r, h, stats;
+  if (adaln_forward(x, &y, &gate, scale, shift, weight, eps, branch_scale, &r, &h, nullptr, nullptr,
+                    want_stats ? &stats : nullptr)) {
+    if (!want_stats) stats = at::empty({0, 4}, x.options().dtype(at::kFloat));
+    return {r, h, stats};
+  }
+  return python_impl<T3>("residual_adaln", x, y, gate, scale, shift, weight, eps, branch_scale, want_stats);
+}
+
+T2 adaln(const Tensor& x, const Tensor& scale, const Tensor& shift, double eps, bool want_stats) {
+  Tensor h, stats;
+  if (adaln_forward(x, nullptr, nullptr, scale, shift, std::nullopt, eps, 1.0, nullptr, &h, nullptr, nullptr,
+                    want_stats ? &stats : nullptr)) {
+    if (!want_stats) stats = at::empty({0, 4}, x.options().dtype(at::kFloat));
+    return {h, stats};
+  }
+  return python_impl<T2>("adaln", x, scale, shift, eps, want_stats);
+}
+
+T3 residual_adaln_int8(const Tensor& x, const Tensor& y, const Tensor& gate, const Tensor& scale,
+                       const Tensor& shift, const OptT& weight, double eps, double branch_scale) {
+  Tensor r, q, qs;
+  if (adaln_forward(x, &y, &gate, scale, shift, weight, eps, branch_scale, &r, nullptr, &q, &qs, nullptr))
+    return {r, q, qs};
+  return python_impl<T3>("residual_adaln_int8", x, y, gate, scale, shift, weight, eps, branch_scale);
+}
+
+T6 adaln_bwd(const OptT& dr_, const OptT& dh_, const Tensor& x, const OptT& y, const OptT& gate, const Tensor& scale,
+             const OptT& weight, const Tensor& stats, int64_t shift_rows, double branch_scale, bool mods) {
+  const auto slow = [&] {
+    return python_impl<T6>("adaln_bwd", dr_, dh_, x, y, gate, scale, weight, stats, shift_rows, branch_scale, mods);
+  };
+  if (!adaln_ready(x, y ? &*y : nullptr, gate ? &*gate : nullptr, scale, weight)) return slow();
+  const int64_t B = x.size(0), S = x.size(1), D = x.size(2);
+  if (stats.scalar_type() != at::kFloat || stats.numel() != 4 * B * S || !stats.is_contiguous() || !on_gpu(stats, x) ||
+      (shift_rows != 1 && shift_rows != B))
+    return slow();
+  const c10::DeviceGuard guard(x.device());
+  Tensor dr, dh;
+  for (const auto& [from, to] : {std::make_pair(&dr_, &dr), std::make_pair(&dh_, &dh)}) {
+    if (!*from) continue;
+    if (!bf16_on(**from, x) || (*from)->sizes() != x.sizes()) return slow();
+    *to = (*from)->contiguous();
+    if (!aligned16(*to)) return slow();
+  }
+  const Tensor w = f32_or_none(weight);
+  if (w.defined() && !aligned16(w)) return slow();
+  const auto none = [&] { return at::empty({0}, x.options()); };
+  Tensor dx = at::empty(x.sizes(), x.options()), dy = y ? at::empty(x.sizes(), x.options()) : none();
+  Tensor dgate = none(), dscale = none(), dshift = none(), dweight = none();
+  if (mods) {
+    dscale = at::empty(scale.sizes(), scale.options());
+    dshift = at::empty({shift_rows, D}, scale.options());
+    if (y) dgate = at::empty(gate->sizes(), gate->options());
+    if (weight) dweight = at::empty({D}, x.options().dtype(at::kFloat));
+  }
+  const auto ptr = [](const Tensor& t) { return t.numel() ? t.data_ptr() : nullptr; };
+  aa_adaln_bwd_args a = {};
+  a.dr = dr.defined() ? dr.data_ptr() : nullptr;
+  a.dh = dh.defined() ? dh.data_ptr() : nullptr;
+  a.x = x.data_ptr();
+  a.y = y ? y->data_ptr() : nullptr;
+  a.gate = gate ? gate->data_ptr() : nullptr;
+  a.scale = scale.data_ptr();
+  a.gate_stride = gate ? mod_stride(*gate) : 0;
+  a.scale_stride = mod_stride(scale);
+  a.weight = float_ptr(w);
+  a.stats = stats.data_ptr<float>();
+  a.dx = dx.data_ptr();
+  a.dy = ptr(dy);
+  a.dgate = ptr(dgate);
+  a.dscale = ptr(dscale);
+  a.dshift = ptr(dshift);
+  a.dweight = (float*)ptr(dweight);
+  a.gate_rows = gate ? gate->size(0) : 1;
+  a.scale_rows = scale.size(0);
+  a.shift_rows = shift_rows;
+  a.B = B;
+  a.S = S;
+  a.D = D;
+  a.branch_scale = (float)branch_scale;
+  a.dtype = AA_DTYPE_BF16;
+  a.mod_dtype = scale.scalar_type() == at::kFloat ? AA_DTYPE_FP32 : AA_DTYPE_BF16;
+  const size_t bytes = aa_adaln_bwd_workspace(B, S, D, mods);
+  Tensor ws;
+  if (bytes) ws = at::empty({(int64_t)bytes / 4}, x.options().dtype(at::kFloat));
+  if (!launched(aa_adaln_bwd(&a, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(x)), "adaln_bwd")) return slow();
+  return {dx, dy, dgate, dscale, dshift, dweight};
+}
+
+// ----------------------------------------------------------- int8 products --
+
+T2 rowquant_int8(const Tensor& x, bool gelu) {
+  if (rows_ready(x, x)) {
+    const c10::DeviceGuard guard(x.device());
+    const int64_t rows = x.size(0) * x.size(1);
+    Tensor q = at::empty(x.sizes(), x.options().dtype(at::kChar));
+    Tensor s = at::empty({rows, 1}, x.options().dtype(at::kFloat));
+    if (launched(aa_rowquant_int8(x.data_ptr(), rows, x.size(2), gelu, q.data_ptr(), s.data_ptr<float>(),
+                                  AA_DTYPE_BF16, stream_of(x)),
+                 "rowquant_int8"))
+      return {q, s};
+  }
+  return python_impl<T2>("rowquant_int8", x, gelu);
+}
+
+Tensor int8_linear(const Tensor& q, const Tensor& s, const Tensor& w, const Tensor& ws) {
+  if (q.is_cuda() && q.dim() == 3 && w.dim() == 2 && q.scalar_type() == at::kChar && w.scalar_type() == at::kChar &&
+      q.size(2) == w.size(1) && q.numel() > 0 && q.is_contiguous() && w.is_contiguous() && aligned16(q) && aligned16(w) &&
+      on_gpu(w, q) && on_gpu(s, q) && on_gpu(ws, q) && s.scalar_type() == at::kFloat && ws.scalar_type() == at::kFloat &&
+      s.numel() == q.size(0) * q.size(1) && ws.numel() == w.size(0) && s.is_contiguous() && ws.is_contiguous()) {
+    const c10::DeviceGuard guard(q.device());
+    Tensor y = at::empty({q.size(0), q.size(1), w.size(0)}, q.options().dtype(at::kBFloat16));
+    if (launched(aa_int8_linear(q.data_ptr(), s.data_ptr<float>(), w.data_ptr(), ws.data_ptr<float>(), y.data_ptr(),
+                                s.numel(), w.size(0), w.size(1), AA_DTYPE_BF16, stream_of(q)),
+                 "int8_linear"))
+      return y;
+  }
+  return python_impl<Tensor>("int8_linear", q, s, w, ws);
+}
+
+// ------------------------------------------------------- 8-bit checkpoints --
+
+// Codes [rows, 32 G] and exponents of the given shape; empty without `keep`.
+void kept(const Tensor& x, bool keep, int64_t e0, int64_t e1, Tensor* codes, Tensor* exps) {
+  const int64_t K = x.size(2);
+  *codes = at::empty({keep ? x.size(0) * x.size(1) : 0, (K + 31) / 32 * 32}, x.options().dtype(at::kChar));
+  *exps = at::empty({keep ? e0 : 0, keep ? e1 : 0}, x.options().dtype(at::kByte));
+}
+
+T3 gelu8(const Tensor& x, bool keep) {
+  if (rows_ready(x, x)) {
+    const c10::DeviceGuard guard(x.device());
+    const int64_t rows = x.size(0) * x.size(1), K = x.size(2);
+    Tensor y = at::empty(x.sizes(), x.options()), codes, exps;
+    kept(x, keep, rows, (K + 31) / 32, &codes, &exps);
+    if (launched(aa_gelu8_fwd(x.data_ptr(), y.data_ptr(), keep ? codes.data_ptr() : nullptr,
+                              keep ? exps.data_ptr() : nullptr, rows, K, AA_DTYPE_BF16, stream_of(x)),
+                 "gelu8"))
+      return {y, codes, exps};
+  }
+  return python_impl<T3>("gelu8", x, keep);
+}
+
+// A checkpoint of `rows` rows of K channels, with exponents of n elements.
+bool kept_ready(const Tensor& codes, const Tensor& exps, const Tensor& like, int64_t rows, int64_t K, int64_t n) {
+  return codes.scalar_type() == at::kChar && exps.scalar_type() == at::kByte && on_gpu(codes, like) && on_gpu(exps, like) &&
+         codes.numel() == rows * ((K + 31) / 32 * 32) && exps.numel() == n && codes.is_contiguous() && exps.is_contiguous() &&
+         aligned16(codes) && aligned16(exps);
+}
+
+Tensor gelu8_bwd(const Tensor& dy_, const Tensor& codes, const Tensor& exps) {
+  if (dy_.dim() == 3 && bf16_on(dy_, dy_) && dy_.numel() > 0) {
+    const c10::DeviceGuard guard(dy_.device());
+    const Tensor dy = dy_.contiguous();
+    const int64_t rows = dy.size(0) * dy.size(1), K = dy.size(2);
+    if (aligned16(dy) && kept_ready(codes, exps, dy, rows, K, rows * ((K + 31) / 32))) {
+      Tensor dx = at::empty(dy.sizes(), dy.options());
+      if (launched(aa_gelu8_bwd(dy.data_ptr(), codes.data_ptr(), exps.data_ptr(), dx.data_ptr(), rows, K,
+                                AA_DTYPE_BF16, stream_of(dy)),
+                   "gelu8_bwd"))
+        return dx;
+    }
+  }
+  return python_impl<Tensor>("gelu8_bwd", dy_, codes, exps);
+}
+
+bool down_ready(const Tensor& a, const Tensor& like) {
+  return a.dim() == 2 && bf16_on(a, like) && a.is_contiguous() && aligned16(a) && a.numel() > 0;
+}
+
+T3 lora_down8(const Tensor& x, const Tensor& a, bool keep) {
+  if (rows_ready(x, x) && down_ready(a, x) && a.size(1) == x.size(2)) {
+    const c10::DeviceGuard guard(x.device());
+    const int64_t rows = x.size(0) * x.size(1), K = x.size(2), R = a.size(0);
+    Tensor t = at::empty({x.size(0), x.size(1), R}, x.options()), codes, exps;
+    kept(x, keep, (K + 31) / 32, (rows + 15) / 16 * 16, &codes, &exps);
+    if (launched(aa_lora8_fwd(x.data_ptr(), a.data_ptr(), t.data_ptr(), keep ? codes.data_ptr() : nullptr,
+                              keep ? exps.data_ptr() : nullptr, rows, K, R, AA_DTYPE_BF16, stream_of(x)),
+                 "lora_down8"))
+      return {t, codes, exps};
+  }
+  return python_impl<T3>("lora_down8", x, a, keep);
+}
+
+T2 lora_down8_bwd(const Tensor& dt_, const Tensor& a, const Tensor& codes, const Tensor& exps, bool need_x, bool need_a) {
+  if (dt_.dim() == 3 && bf16_on(dt_, dt_) && dt_.numel() > 0 && down_ready(a, dt_) && dt_.size(2) == a.size(0)) {
+    const c10::DeviceGuard guard(dt_.device());
+    const Tensor dt = dt_.contiguous();
+    const int64_t rows = dt.size(0) * dt.size(1), R = a.size(0), K = a.size(1);
+    if (aligned16(dt) &&
+        (!need_a || kept_ready(codes, exps, dt, rows, K, (K + 31) / 32 * ((rows + 15) / 16 * 16)))) {
+      Tensor dx = need_x ? at::empty({dt.size(0), dt.size(1), K}, dt.options()) : at::empty({0}, dt.options());
+      Tensor da = need_a ? at::empty({R, K}, dt.options()) : at::empty({0}, dt.options());
+      const size_t bytes = need_a ? aa_lora8_bwd_workspace(rows, K, R) : 0;
+      Tensor ws;
+      if (bytes) ws = at::empty({(int64_t)bytes / 4}, dt.options().dtype(at::kFloat));
+      if (launched(aa_lora8_bwd(dt.data_ptr(), a.data_ptr(), need_a ? codes.data_ptr() : nullptr,
+                                need_a ? exps.data_ptr() : nullptr, need_x ? dx.data_ptr() : nullptr,
+                                need_a ? da.data_ptr() : nullptr, bytes ? ws.data_ptr() : nullptr, bytes, rows, K, R,
+                                AA_DTYPE_BF16, stream_of(dt)),
+                   "lora_down8_bwd"))
+        return {dx, da};
+    }
+  }
+  return python_impl<T2>("lora_down8_bwd", dt_, a, codes, exps, need_x, need_a);
+}
+
 // ----------------------------------------------------------------- autograd --
 
 // The dispatcher's handle of one op, called below or above autograd.
@@ -426,6 +709,17 @@ ANIMA_OP(op_qkv_proj_norm_rope, "anima_flat_amd::qkv_proj_norm_rope", T3, CT, CT
          int64_t, double)
 ANIMA_OP(op_proj_head_norm, "anima_flat_amd::proj_head_norm", Tensor, CT, CT, CT, int64_t, double)
 ANIMA_OP(op_kv_proj_norm, "anima_flat_amd::kv_proj_norm", T2, CT, CT, CT, int64_t, double)
+using CO = const OptT&;
+ANIMA_OP(op_residual_adaln, "anima_flat_amd::residual_adaln", T3, CT, CT, CT, CT, CT, CO, double, double, bool)
+ANIMA_OP(op_adaln, "anima_flat_amd::adaln", T2, CT, CT, CT, double, bool)
+ANIMA_OP(op_residual_adaln_int8, "anima_flat_amd::residual_adaln_int8", T3, CT, CT, CT, CT, CT, CO, double, double)
+ANIMA_OP(op_adaln_bwd, "anima_flat_amd::adaln_bwd", T6, CO, CO, CT, CO, CO, CT, CO, CT, int64_t, double, bool)
+ANIMA_OP(op_rowquant_int8, "anima_flat_amd::rowquant_int8", T2, CT, bool)
+ANIMA_OP(op_int8_linear, "anima_flat_amd::int8_linear", Tensor, CT, CT, CT, CT)
+ANIMA_OP(op_gelu8, "anima_flat_amd::gelu8", T3, CT, bool)
+ANIMA_OP(op_gelu8_bwd, "anima_flat_amd::gelu8_bwd", Tensor, CT, CT, CT)
+ANIMA_OP(op_lora_down8, "anima_flat_amd::lora_down8", T3, CT, CT, bool)
+ANIMA_OP(op_lora_down8_bwd, "anima_flat_amd::lora_down8_bwd", T2, CT, CT, CT, CT, bool, bool)
 #undef ANIMA_OP
 
 // Whether a call is recorded for the backward; no op here has a forward-mode
@@ -434,7 +728,9 @@ template <class... A>
 bool needs_grad(const A&... args) {
   const auto any = [&](auto pred) {
     const auto one = [&](const auto& a) {
-      if constexpr (std::is_same_v<std::decay_t<decltype(a)>, Tensor>) return pred(a);
+      using A1 = std::decay_t<decltype(a)>;
+      if constexpr (std::is_same_v<A1, Tensor>) return pred(a);
+      else if constexpr (std::is_same_v<A1, OptT>) return a.has_value() && a->defined() && pred(*a);
       else return false;
     };
     return (one(args) || ...);
@@ -469,7 +765,11 @@ struct NoBackward : torch::autograd::Function<NoBackward> {
 variable_list as_list(const Tensor& t) { return {t}; }
 variable_list as_list(const T2& t) { return {std::get<0>(t), std::get<1>(t)}; }
 variable_list as_list(const T3& t) { return {std::get<0>(t), std::get<1>(t), std::get<2>(t)}; }
+variable_list as_list(const T6& t) {
+  return std::apply([](const auto&... v) { return variable_list{v...}; }, t);
+}
 void from_list(const variable_list& l, Tensor& t) { t = l[0]; }
+void from_list(const variable_list& l, T6& t) { t = {l[0], l[1], l[2], l[3], l[4], l[5]}; }
 void from_list(const variable_list& l, T2& t) { t = {l[0], l[1]}; }
 void from_list(const variable_list& l, T3& t) { t = {l[0], l[1], l[2]}; }
 
@@ -563,6 +863,142 @@ Tensor head_norm_autograd(CT x, CT w, int64_t heads, double eps) {
   return HeadNorm::apply(x, w, heads, eps);
 }
 
+// The statistics and 8-bit copies, which have no derivative, are handed past
+// the node as the LSE is.
+struct ResidualAdaln : torch::autograd::Function<ResidualAdaln> {
+  static constexpr bool is_traceable = true;
+  static variable_list forward(AutogradContext* ctx, CT x, CT y, CT gate, CT scale, CT shift, CO weight, double eps,
+                               double branch_scale, bool mods, Tensor* stats) {
+    auto [r, h, st] = op_residual_adaln().below(x, y, gate, scale, shift, weight, eps, branch_scale, true);
+    *stats = st;
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({x, y, gate, scale, weight.value_or(Tensor()), st});
+    ctx->saved_data["branch_scale"] = branch_scale;
+    ctx->saved_data["shift_rows"] = shift.size(0);
+    ctx->saved_data["mods"] = mods;
+    return {r, h};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    variable_list out(10);
+    if (!g[0].defined() && !g[1].defined()) return out;
+    const variable_list s = ctx->get_saved_variables();
+    const auto opt = [](const Tensor& t) { return t.defined() ? OptT(t) : OptT(); };
+    const bool mods = ctx->saved_data["mods"].toBool();
+    auto [dx, dy, dgate, dscale, dshift, dweight] =
+        op_adaln_bwd()(opt(g[0]), opt(g[1]), s[0], s[1], s[2], s[3], opt(s[4]), s[5],
+                       ctx->saved_data["shift_rows"].toInt(), ctx->saved_data["branch_scale"].toDouble(), mods);
+    out[0] = dx;
+    out[1] = dy;
+    if (mods) {
+      out[2] = dgate;
+      out[3] = dscale;
+      out[4] = dshift;
+      if (s[4].defined()) out[5] = dweight.to(s[4].scalar_type());
+    }
+    return out;
+  }
+};
+
+T3 residual_adaln_autograd(CT x, CT y, CT gate, CT scale, CT shift, CO weight, double eps, double branch_scale,
+                           bool want_stats) {
+  if (!needs_grad(x, y, gate, scale, shift, weight))
+    return op_residual_adaln().below(x, y, gate, scale, shift, weight, eps, branch_scale, want_stats);
+  const bool mods = gate.requires_grad() || scale.requires_grad() || shift.requires_grad() ||
+                    (weight && weight->requires_grad());
+  Tensor stats;
+  const variable_list o = ResidualAdaln::apply(x, y, gate, scale, shift, weight, eps, branch_scale, mods, &stats);
+  return {o[0], o[1], stats};
+}
+
+struct Adaln : torch::autograd::Function<Adaln> {
+  static constexpr bool is_traceable = true;
+  static Tensor forward(AutogradContext* ctx, CT x, CT scale, CT shift, double eps, bool mods, Tensor* stats) {
+    auto [h, st] = op_adaln().below(x, scale, shift, eps, true);
+    *stats = st;
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({x, scale, st});
+    ctx->saved_data["shift_rows"] = shift.size(0);
+    ctx->saved_data["mods"] = mods;
+    return h;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    variable_list out(6);
+    if (!g[0].defined()) return out;
+    const variable_list s = ctx->get_saved_variables();
+    const bool mods = ctx->saved_data["mods"].toBool();
+    const T6 r = op_adaln_bwd()(OptT(), g[0], s[0], OptT(), OptT(), s[1], OptT(), s[2],
+                                ctx->saved_data["shift_rows"].toInt(), 1.0, mods);
+    out[0] = std::get<0>(r);
+    if (mods) {
+      out[1] = std::get<3>(r);
+      out[2] = std::get<4>(r);
+    }
+    return out;
+  }
+};
+
+T2 adaln_autograd(CT x, CT scale, CT shift, double eps, bool want_stats) {
+  if (!needs_grad(x, scale, shift)) return op_adaln().below(x, scale, shift, eps, want_stats);
+  Tensor stats;
+  Tensor h = Adaln::apply(x, scale, shift, eps, scale.requires_grad() || shift.requires_grad(), &stats);
+  return {h, stats};
+}
+
+struct Gelu8 : torch::autograd::Function<Gelu8> {
+  static constexpr bool is_traceable = true;
+  static Tensor forward(AutogradContext* ctx, CT x, Tensor* codes, Tensor* exps) {
+    Tensor y;
+    std::tie(y, *codes, *exps) = op_gelu8().below(x, true);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({*codes, *exps});
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    variable_list out(3);
+    if (!g[0].defined()) return out;
+    const variable_list s = ctx->get_saved_variables();
+    out[0] = op_gelu8_bwd()(g[0], s[0], s[1]);
+    return out;
+  }
+};
+
+T3 gelu8_autograd(CT x, bool keep) {
+  if (!needs_grad(x)) return op_gelu8().below(x, keep);
+  Tensor codes, exps;
+  Tensor y = Gelu8::apply(x, &codes, &exps);
+  return {y, codes, exps};
+}
+
+struct LoraDown8 : torch::autograd::Function<LoraDown8> {
+  static constexpr bool is_traceable = true;
+  static Tensor forward(AutogradContext* ctx, CT x, CT a, bool need_x, bool need_a, Tensor* codes, Tensor* exps) {
+    Tensor t;
+    std::tie(t, *codes, *exps) = op_lora_down8().below(x, a, need_a);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({a, *codes, *exps});
+    ctx->saved_data["need_x"] = need_x;
+    ctx->saved_data["need_a"] = need_a;
+    return t;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    variable_list out(6);
+    if (!g[0].defined()) return out;
+    const variable_list s = ctx->get_saved_variables();
+    const bool need_x = ctx->saved_data["need_x"].toBool(), need_a = ctx->saved_data["need_a"].toBool();
+    auto [dx, da] = op_lora_down8_bwd()(g[0], s[0], s[1], s[2], need_x, need_a);
+    if (need_x) out[0] = dx;
+    if (need_a) out[1] = da;
+    return out;
+  }
+};
+
+T3 lora_down8_autograd(CT x, CT a, bool keep) {
+  if (!needs_grad(x, a)) return op_lora_down8().below(x, a, keep);
+  Tensor codes, exps;
+  Tensor t = LoraDown8::apply(x, a, x.requires_grad(), a.requires_grad(), &codes, &exps);
+  return {t, codes, exps};
+}
+
 // ------------------------------------------------------------- registration --
 
 // Registrations live as long as the process, as torch.library's do.
@@ -600,6 +1036,16 @@ void add_kernels(const std::string& ns, const std::string& name) {
   ANIMA_PLAIN(qkv_proj_norm_rope, T3, CT, CT, CT, CT, CT, CT, int64_t, double);
   ANIMA_PLAIN(proj_head_norm, Tensor, CT, CT, CT, int64_t, double);
   ANIMA_PLAIN(kv_proj_norm, T2, CT, CT, CT, int64_t, double);
+  ANIMA_ADD(residual_adaln, &residual_adaln_autograd);
+  ANIMA_ADD(adaln, &adaln_autograd);
+  ANIMA_ADD(gelu8, &gelu8_autograd);
+  ANIMA_ADD(lora_down8, &lora_down8_autograd);
+  ANIMA_PLAIN(residual_adaln_int8, T3, CT, CT, CT, CT, CT, CO, double, double);
+  ANIMA_PLAIN(adaln_bwd, T6, CO, CO, CT, CO, CO, CT, CO, CT, int64_t, double, bool);
+  ANIMA_PLAIN(rowquant_int8, T2, CT, bool);
+  ANIMA_PLAIN(int8_linear, Tensor, CT, CT, CT, CT);
+  ANIMA_PLAIN(gelu8_bwd, Tensor, CT, CT, CT);
+  ANIMA_PLAIN(lora_down8_bwd, T2, CT, CT, CT, CT, bool, bool);
   TORCH_CHECK(false, "no native kernels for ", ns, "::", name);
 }
 
