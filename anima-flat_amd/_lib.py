@@ -81,7 +81,8 @@ _PROTOTYPES: dict[str, tuple[object, list[object]]] = {
     "aa_int8_linear": (c_int, [c_void_p] * 5 + [_I64] * 3 + [c_int, c_void_p]),
     "aa_gelu8_fwd": (c_int, [c_void_p] * 4 + [_I64] * 2 + [c_int, c_void_p]),
     "aa_gelu8_bwd": (c_int, [c_void_p] * 4 + [_I64] * 2 + [c_int, c_void_p]),
-    "aa_lora8_fwd": (c_int, [c_void_p] * 5 + [_I64] * 3 + [c_int, c_void_p]),
+    "aa_lora8_fwd_workspace": (c_size_t, [_I64] * 3),
+    "aa_lora8_fwd": (c_int, [c_void_p] * 6 + [c_size_t] + [_I64] * 3 + [c_int, c_void_p]),
     "aa_lora8_bwd_workspace": (c_size_t, [_I64] * 3),
     "aa_lora8_bwd": (c_int, [c_void_p] * 6 + [c_void_p, c_size_t] + [_I64] * 3 + [c_int, c_void_p]),
 }

@@ -119,6 +119,9 @@ __global__ __launch_bounds__(kAdThreads) void adaln_fwd_kernel(AdFwd p) {
   int row = blockIdx.x * (kRows * p.rpw) + wave / WPR;
   int b = row / p.S, at = row - b * p.S;  // batch item and place in it
   int have = -1;
+  // bf16 modulation rows stay in registers from row to row; fp32 ones, twice as
+  // many, are read again (from L1: the workgroup's waves share them).
+  constexpr bool kHold = !kModF32;
   Mod8<kModF32> gate[NU], scale[NU], shift[NU];
   for (int it = 0; it < p.rpw && row < p.rows; ++it, row += kRows, at += kRows) {
     while (at >= p.S) {
@@ -134,7 +137,7 @@ __global__ __launch_bounds__(kAdThreads) void adaln_fwd_kernel(AdFwd p) {
         if (p.y) yr[i] = ld16(p.y + (int64_t)row * p.D + 8 * unit[i]);
       }
     }
-    if (b != have) {
+    if (kHold && b != have) {
       have = b;
 #pragma unroll
       for (int i = 0; i < NU; ++i) {
@@ -169,9 +172,10 @@ __global__ __launch_bounds__(kAdThreads) void adaln_fwd_kernel(AdFwd p) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) y[j] *= ry * (j < 4 ? w0[j & 3] : w1[j & 3]);
         }
+        if constexpr (!kHold) gate[i].load(p.gate, b * p.gs + 8 * unit[i]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) r[i][j] = fmaf(p.c * gate[i].get(j), y[j], r[i][j]);
-        st16(p.r + (int64_t)row * p.D + 8 * unit[i], pack8(r[i]));
+        st16_nt(p.r + (int64_t)row * p.D + 8 * unit[i], pack8(r[i]));
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) sum += r[i][j];
@@ -188,19 +192,24 @@ __global__ __launch_bounds__(kAdThreads) void adaln_fwd_kernel(AdFwd p) {
       }
     }
     const float rstd = 1.0f / sqrtf(share.sum(var) * inv_d + p.eps);
-    uint32_t top = 0;
+    float top = 0.f;
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
       if (!live[i]) continue;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        r[i][j] = fmaf(r[i][j] * rstd, 1.0f + scale[i].get(j), shift[i].get(j));
-        if constexpr (kInt8) top = max(top, mag_bits(r[i][j]));
+      if constexpr (!kHold) {
+        scale[i].load(p.scale, b * p.ss + 8 * unit[i]);
+        shift[i].load(p.shift, b * p.hs + 8 * unit[i]);
       }
-      if constexpr (!kInt8) st16(p.h + (int64_t)row * p.D + 8 * unit[i], pack8(r[i]));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) r[i][j] = fmaf(r[i][j] * rstd, 1.0f + scale[i].get(j), shift[i].get(j));
+      if constexpr (kInt8) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) top = max3abs_nan(top, r[i][j], r[i][j + 1]);
+      }
+      if constexpr (!kInt8) st16_nt(p.h + (int64_t)row * p.D + 8 * unit[i], pack8(r[i]));
     }
     if constexpr (kInt8) {
-      const RowScale rs = row_scale(share.umax(top));
+      const RowScale rs = row_scale(share.umax(mag_bits(top)));
 #pragma unroll
       for (int i = 0; i < NU; ++i)
         if (live[i])
@@ -236,7 +245,7 @@ struct AdBwd {
 // one row each in turn. NC > 0: sums over the chunk's rows stay in registers,
 // are added over the waves in LDS in a fixed order and leave as one partial
 // record, which colsum_kernel adds up.
-template <int NU, int WPR, bool kModF32, int NC>
+template <int NU, int WPR, bool kModF32, int NC, bool kPost>
 __global__ __launch_bounds__(kAdBThreads) void adaln_bwd_kernel(AdBwd p) {
   constexpr int kGroups = kAdBWaves / WPR;   // rows at a time
   constexpr int kWidth = NU * WPR * 64 * 8;  // columns a group holds (>= D)
@@ -259,33 +268,82 @@ __global__ __launch_bounds__(kAdBThreads) void adaln_bwd_kernel(AdBwd p) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) acc[v][i][j] = 0.f;
 
+  int unit[NU];
+  bool live[NU];
+#pragma unroll
+  for (int i = 0; i < NU; ++i) {
+    unit[i] = lane + 64 * (wsub + WPR * i);
+    live[i] = unit[i] < nunit;
+  }
+  struct Row {
+    f32x4 st;
+    u32x4 x[NU], y[NU], dh[NU], dr[NU];
+  };
+  auto load = [&](Row& t, int s) {
+    const int64_t row = row0 + min(s, last - 1);
+    t.st = ldf4(p.stats + 4 * row);
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+      const int64_t at = row * p.D + 8 * unit[i];
+      t.x[i] = t.y[i] = t.dh[i] = t.dr[i] = u32x4{0, 0, 0, 0};
+      if (live[i]) {
+        t.x[i] = ld16(p.x + at);
+        if (p.y) t.y[i] = ld16(p.y + at);
+        if (p.dh) t.dh[i] = ld16(p.dh + at);
+        if (p.dr) t.dr[i] = ld16(p.dr + at);
+      }
+    }
+  };
+  // c gate, 1 + scale and w of a lane's columns, from registers for all rows where
+  // a workgroup is alone on its CU (sums), else as they are needed.
+  constexpr bool kHold = NC > 0;
+  float hg[kHold ? NU : 1][8], hs[kHold ? NU : 1][8], hw[kHold && kPost ? NU : 1][8];
+  auto get_gate = [&](float (&v)[8], int i) {
+    Mod8<kModF32> m;
+    m.load(p.gate, b * p.gs + 8 * unit[i]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = p.c * m.get(j);
+  };
+  auto get_scale = [&](float (&v)[8], int i) {
+    Mod8<kModF32> m;
+    m.load(p.scale, b * p.ss + 8 * unit[i]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 1.0f + m.get(j);
+  };
+  auto get_w = [&](float (&v)[8], int i) {
+    const f32x4 w0 = ldf4(p.w + 8 * unit[i]), w1 = ldf4(p.w + 8 * unit[i] + 4);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < 4 ? w0[j & 3] : w1[j & 3];
+  };
+  if constexpr (kHold) {
+#pragma unroll
+    for (int i = 0; i < NU; ++i)
+      if (live[i]) {
+        get_scale(hs[i], i);
+        if (p.y) get_gate(hg[i], i);
+        if constexpr (kPost) get_w(hw[i], i);
+      }
+  }
   // Every wave of a row's group makes the same turns, and all groups as many
   // (the barriers of a shared row's sums): a group past its rows computes on
   // the last row and writes nothing.
   const int turns = (last - first + kGroups - 1) / kGroups;
+  Row next;
+  if constexpr (kHold) load(next, first + group);
   for (int it = 0; it < turns; ++it) {
     const int s = first + it * kGroups + group;
     const bool mine = s < last;
     if (WPR == 1 && !mine) break;
     const int64_t row = row0 + min(s, last - 1);
-    const f32x4 st = ldf4(p.stats + 4 * row);
-    const float mean = st[0], rstd = st[1], ry = st[2];
-    u32x4 rx[NU], rdy[NU], rdh[NU], rdr[NU];
-    int unit[NU];
-    bool live[NU];
-#pragma unroll
-    for (int i = 0; i < NU; ++i) {
-      unit[i] = lane + 64 * (wsub + WPR * i);
-      live[i] = unit[i] < nunit;
-      const int64_t at = row * p.D + 8 * unit[i];
-      rx[i] = rdy[i] = rdh[i] = rdr[i] = u32x4{0, 0, 0, 0};
-      if (live[i]) {
-        rx[i] = ld16(p.x + at);
-        if (p.y) rdy[i] = ld16(p.y + at);
-        if (p.dh) rdh[i] = ld16(p.dh + at);
-        if (p.dr) rdr[i] = ld16(p.dr + at);
-      }
+    Row cur;
+    if constexpr (kHold) {
+      cur = next;
+      if (it + 1 < turns) load(next, s + kGroups);
+    } else {
+      load(cur, s);
     }
+    const auto &rx = cur.x, &rdy = cur.y, &rdh = cur.dh, &rdr = cur.dr;
+    const float mean = cur.st[0], rstd = cur.st[1], ry = cur.st[2];
     // xh in place of r, and the two means.
     float xh[NU][8];
     float m1 = 0.f, m2 = 0.f;
@@ -293,47 +351,47 @@ __global__ __launch_bounds__(kAdBThreads) void adaln_bwd_kernel(AdBwd p) {
     for (int i = 0; i < NU; ++i) {
       unpack8(rx[i], xh[i]);
       if (!live[i]) continue;
+      float v[8];
       if (p.y) {
-        Mod8<kModF32> gate;
-        gate.load(p.gate, b * p.gs + 8 * unit[i]);
         float y[8];
         unpack8(rdy[i], y);
-        if (p.w) {
-          const f32x4 w0 = ldf4(p.w + 8 * unit[i]), w1 = ldf4(p.w + 8 * unit[i] + 4);
+        if constexpr (kPost) {
+          if constexpr (!kHold) get_w(v, i);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) y[j] *= ry * (j < 4 ? w0[j & 3] : w1[j & 3]);
+          for (int j = 0; j < 8; ++j) y[j] *= ry * (kHold ? hw[kHold ? i : 0][j] : v[j]);
         }
+        if constexpr (!kHold) get_gate(v, i);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) xh[i][j] = fmaf(p.c * gate.get(j), y[j], xh[i][j]);
+        for (int j = 0; j < 8; ++j) xh[i][j] = fmaf(kHold ? hg[kHold ? i : 0][j] : v[j], y[j], xh[i][j]);
       }
-      Mod8<kModF32> scale;
-      scale.load(p.scale, b * p.ss + 8 * unit[i]);
+      if constexpr (!kHold) get_scale(v, i);
       float dh[8];
       unpack8(rdh[i], dh);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         xh[i][j] = (xh[i][j] - mean) * rstd;
-        const float u = dh[j] * (1.0f + scale.get(j));
+        const float u = dh[j] * (kHold ? hs[kHold ? i : 0][j] : v[j]);
         m1 += u;
         m2 = fmaf(u, xh[i][j], m2);
       }
     }
     m1 = share.sum(m1) * inv_d;
     m2 = share.sum(m2) * inv_d;
+    // With a norm on y, dy waits for a third mean: dn w stays until then.
     float m3 = 0.f;
-    float d[NU][8];
+    float dnw[kPost ? NU : 1][8];
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
       if (!live[i]) continue;
-      Mod8<kModF32> scale;
-      scale.load(p.scale, b * p.ss + 8 * unit[i]);
-      float dh[8], dr[8];
+      float v[8];
+      if constexpr (!kHold) get_scale(v, i);
+      float dh[8], d[8];
       unpack8(rdh[i], dh);
-      unpack8(rdr[i], dr);
+      unpack8(rdr[i], d);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float u = dh[j] * (1.0f + scale.get(j));
-        d[i][j] = fmaf(rstd, u - m1 - xh[i][j] * m2, dr[j]);
+        const float u = dh[j] * (kHold ? hs[kHold ? i : 0][j] : v[j]);
+        d[j] = fmaf(rstd, u - m1 - xh[i][j] * m2, d[j]);
         if constexpr (NC > 0) {
           if (mine) {
             acc[0][i][j] = fmaf(dh[j], xh[i][j], acc[0][i][j]);
@@ -341,51 +399,49 @@ __global__ __launch_bounds__(kAdBThreads) void adaln_bwd_kernel(AdBwd p) {
           }
         }
       }
-      if (mine) st16(p.dx + row * p.D + 8 * unit[i], pack8(d[i]));
-      if (p.y) {
-        Mod8<kModF32> gate;
-        gate.load(p.gate, b * p.gs + 8 * unit[i]);
-        float y[8];
-        unpack8(rdy[i], y);
-        if (p.w) {
-          const f32x4 w0 = ldf4(p.w + 8 * unit[i]), w1 = ldf4(p.w + 8 * unit[i] + 4);
+      if (mine) st16_nt(p.dx + row * p.D + 8 * unit[i], pack8(d));
+      if (!p.y) continue;
+      if constexpr (!kHold) get_gate(v, i);
+      float y[8];
+      unpack8(rdy[i], y);
+      if constexpr (kPost) {
+        float w[8];
+        if constexpr (!kHold) get_w(w, i);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float w = j < 4 ? w0[j & 3] : w1[j & 3];
-            const float yh = y[j] * ry;
-            const float dn = p.c * gate.get(j) * d[i][j];
-            if constexpr (NC > 3) {
-              if (mine) {
-                acc[2][i][j] = fmaf(p.c * yh * w, d[i][j], acc[2][i][j]);
-                acc[3][i][j] = fmaf(dn, yh, acc[3][i][j]);
-              }
+        for (int j = 0; j < 8; ++j) {
+          const float wj = kHold ? hw[kHold ? i : 0][j] : w[j];
+          const float yh = y[j] * ry;
+          const float dn = (kHold ? hg[kHold ? i : 0][j] : v[j]) * d[j];
+          if constexpr (NC > 3) {
+            if (mine) {
+              acc[2][i][j] = fmaf(p.c * yh * wj, d[j], acc[2][i][j]);
+              acc[3][i][j] = fmaf(dn, yh, acc[3][i][j]);
             }
-            d[i][j] = dn * w;
-            m3 = fmaf(d[i][j], yh, m3);
           }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            if constexpr (NC > 2) {
-              if (mine) acc[2][i][j] = fmaf(p.c * y[j], d[i][j], acc[2][i][j]);
-            }
-            d[i][j] *= p.c * gate.get(j);
-          }
+          dnw[i][j] = dn * wj;
+          m3 = fmaf(dnw[i][j], yh, m3);
         }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if constexpr (NC > 2) {
+            if (mine) acc[2][i][j] = fmaf(p.c * y[j], d[j], acc[2][i][j]);
+          }
+          d[j] *= kHold ? hg[kHold ? i : 0][j] : v[j];
+        }
+        if (mine) st16_nt(p.dy + row * p.D + 8 * unit[i], pack8(d));
       }
     }
-    if (p.y) {
-      if (p.w) m3 = share.sum(m3) * inv_d;
+    if constexpr (kPost) {
+      m3 = share.sum(m3) * inv_d;
 #pragma unroll
       for (int i = 0; i < NU; ++i) {
         if (!live[i]) continue;
-        if (p.w) {
-          float y[8];
-          unpack8(rdy[i], y);
+        float y[8];
+        unpack8(rdy[i], y);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) d[i][j] = ry * (d[i][j] - y[j] * ry * m3);
-        }
-        if (mine) st16(p.dy + row * p.D + 8 * unit[i], pack8(d[i]));
+        for (int j = 0; j < 8; ++j) y[j] = ry * (dnw[i][j] - y[j] * ry * m3);
+        if (mine) st16_nt(p.dy + row * p.D + 8 * unit[i], pack8(y));
       }
     }
   }
@@ -424,12 +480,14 @@ struct ColSum {
   } out[4];
 };
 
-__global__ __launch_bounds__(256) void colsum_kernel(ColSum p) {
+constexpr int kCsParts = 16;  // waves of a workgroup, each with every 16th record
+
+__global__ __launch_bounds__(64 * kCsParts) void colsum_kernel(ColSum p) {
   const ColSum::Out o = p.out[blockIdx.y];
   const int b = blockIdx.z;
   if (b >= o.rows) return;  // whole workgroups
   const int col = blockIdx.x * 64 + (threadIdx.x & 63), part = threadIdx.x >> 6;
-  __shared__ float join[4][64];
+  __shared__ float join[kCsParts][64];
   const int c0 = o.rows == 1 ? 0 : b * p.chunks;
   const int n = o.rows == 1 ? p.B * p.chunks : p.chunks;
   float s = 0.f;
@@ -439,17 +497,19 @@ __global__ __launch_bounds__(256) void colsum_kernel(ColSum p) {
     // Four running sums: a chain of one would wait for each load's add.
     float t[4] = {0.f, 0.f, 0.f, 0.f};
     int c = part;
-    for (; c + 12 < n; c += 16)
+    for (; c + 3 * kCsParts < n; c += 4 * kCsParts)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) t[i] += at[(c + 4 * i) * step];
-    for (; c < n; c += 4) t[0] += at[c * step];
+      for (int i = 0; i < 4; ++i) t[i] += at[(c + kCsParts * i) * step];
+    for (; c < n; c += kCsParts) t[0] += at[c * step];
     s = (t[0] + t[1]) + (t[2] + t[3]);
   }
   join[part][threadIdx.x & 63] = s;
   __syncthreads();
   if (part == 0 && col < p.D) {
     const int l = threadIdx.x;
-    s = (join[0][l] + join[1][l]) + (join[2][l] + join[3][l]);
+    s = join[0][l];
+#pragma unroll
+    for (int i = 1; i < kCsParts; ++i) s += join[i][l];
     const int64_t at = (int64_t)b * p.D + col;
     if (o.f32) ((float*)o.out)[at] = s;
     else ((bf16*)o.out)[at] = (bf16)s;
@@ -466,27 +526,29 @@ static void launch_fwd(dim3 grid, hipStream_t st, const AdFwd& p, bool f32, bool
   else adaln_fwd_kernel<NU, WPR, false, false><<<grid, kAdThreads, 0, st>>>(p);
 }
 
-template <int NU, int WPR, int NC>
+template <int NU, int WPR, int NC, bool kPost>
 static void launch_bwd_nc(dim3 grid, hipStream_t st, const AdBwd& p, bool f32) {
-  if (f32) adaln_bwd_kernel<NU, WPR, true, NC><<<grid, kAdBThreads, 0, st>>>(p);
-  else adaln_bwd_kernel<NU, WPR, false, NC><<<grid, kAdBThreads, 0, st>>>(p);
+  if (f32) adaln_bwd_kernel<NU, WPR, true, NC, kPost><<<grid, kAdBThreads, 0, st>>>(p);
+  else adaln_bwd_kernel<NU, WPR, false, NC, kPost><<<grid, kAdBThreads, 0, st>>>(p);
 }
 template <int NU, int WPR>
-static void launch_bwd(dim3 grid, hipStream_t st, const AdBwd& p, int nc, bool f32) {
-  if (nc == 4) launch_bwd_nc<NU, WPR, 4>(grid, st, p, f32);
-  else if (nc == 3) launch_bwd_nc<NU, WPR, 3>(grid, st, p, f32);
-  else launch_bwd_nc<NU, WPR, 0>(grid, st, p, f32);
+static void launch_bwd(dim3 grid, hipStream_t st, const AdBwd& p, bool sums, bool f32) {
+  if (sums && p.w) launch_bwd_nc<NU, WPR, 4, true>(grid, st, p, f32);
+  else if (sums) launch_bwd_nc<NU, WPR, 3, false>(grid, st, p, f32);
+  else if (p.w) launch_bwd_nc<NU, WPR, 0, true>(grid, st, p, f32);
+  else launch_bwd_nc<NU, WPR, 0, false>(grid, st, p, f32);
 }
 
 // Chunks of rows per batch item in the backward: with column sums one
 // workgroup per CU (its partial record, NC D floats, is as much as 2 NC rows of
 // an input, so no more of them than fill the device), else four rows a wave.
-static int bwd_waves_per_row(int64_t D, bool sums) {
-  // A lane holds 16 columns of a row; 32 where no sums want registers, too.
-  return D <= 1024 || (D <= 2048 && !sums) ? 1 : D <= 2048 ? 2 : D <= 4096 ? 4 : 8;
+// wave_rows: a wave takes whole rows up to D = 2048 (32 columns a lane, else 16),
+// where neither sums nor a norm on y want the registers.
+static int bwd_waves_per_row(int64_t D, bool wave_rows) {
+  return D <= 1024 || (D <= 2048 && wave_rows) ? 1 : D <= 2048 ? 2 : D <= 4096 ? 4 : 8;
 }
-static int bwd_rows_per_chunk(int64_t B, int64_t S, int64_t D, bool sums) {
-  const int64_t groups = kAdBWaves / bwd_waves_per_row(D, sums);
+static int bwd_rows_per_chunk(int64_t B, int64_t S, int64_t D, bool sums, bool wave_rows) {
+  const int64_t groups = kAdBWaves / bwd_waves_per_row(D, wave_rows);
   const int64_t cus = std::max(1, device_cu_count());
   const int64_t per = sums ? (B * S + cus - 1) / cus : std::min<int64_t>(4 * groups, (B * S + 2 * cus - 1) / (2 * cus));
   return (int)std::min<int64_t>(S, std::max<int64_t>(1, (per + groups - 1) / groups) * groups);
@@ -575,7 +637,7 @@ extern "C" int aa_adaln_fwd(const aa_adaln_args* a, void* stream) {
 
 extern "C" size_t aa_adaln_bwd_workspace(int64_t B, int64_t S, int64_t D, int sums) {
   if (B <= 0 || S <= 0 || D <= 0 || !sums) return 0;
-  const int64_t rpc = bwd_rows_per_chunk(B, S, D, true);
+  const int64_t rpc = bwd_rows_per_chunk(B, S, D, true, false);
   return (size_t)(B * ((S + rpc - 1) / rpc) * 4 * D) * sizeof(float);
 }
 
@@ -622,19 +684,20 @@ extern "C" int aa_adaln_bwd(const aa_adaln_bwd_args* a, void* workspace, size_t 
   p.part = (float*)workspace;
   p.S = (int)a->S;
   p.D = (int)a->D;
-  p.rpc = bwd_rows_per_chunk(a->B, a->S, a->D, sums);
+  const bool wave_rows = !sums && !a->weight;
+  p.rpc = bwd_rows_per_chunk(a->B, a->S, a->D, sums, wave_rows);
   p.chunks = (p.S + p.rpc - 1) / p.rpc;
   p.c = a->branch_scale;
   const int nc = !sums ? 0 : a->weight ? 4 : 3;
   const dim3 grid((unsigned)(a->B * p.chunks));
   hipStream_t st = (hipStream_t)stream;
   const bool f32 = a->mod_dtype == AA_DTYPE_FP32;
-  if (p.D <= 512) launch_bwd<1, 1>(grid, st, p, nc, f32);
-  else if (p.D <= 1024) launch_bwd<2, 1>(grid, st, p, nc, f32);
-  else if (p.D <= 2048 && !sums) launch_bwd_nc<4, 1, 0>(grid, st, p, f32);
-  else if (p.D <= 2048) launch_bwd<2, 2>(grid, st, p, nc, f32);
-  else if (p.D <= 4096) launch_bwd<2, 4>(grid, st, p, nc, f32);
-  else launch_bwd<2, 8>(grid, st, p, nc, f32);
+  if (p.D <= 512) launch_bwd<1, 1>(grid, st, p, sums, f32);
+  else if (p.D <= 1024) launch_bwd<2, 1>(grid, st, p, sums, f32);
+  else if (p.D <= 2048 && wave_rows) launch_bwd_nc<4, 1, 0, false>(grid, st, p, f32);
+  else if (p.D <= 2048) launch_bwd<2, 2>(grid, st, p, sums, f32);
+  else if (p.D <= 4096) launch_bwd<2, 4>(grid, st, p, sums, f32);
+  else launch_bwd<2, 8>(grid, st, p, sums, f32);
   if (int rc = check_launch(what)) return rc;
   if (!sums) return AA_OK;
   ColSum c;
@@ -653,6 +716,6 @@ extern "C" int aa_adaln_bwd(const aa_adaln_bwd_args* a, void* workspace, size_t 
   add(a->dshift, 1, a->shift_rows, f32);
   add(a->dgate, 2, a->gate_rows, f32);
   add(a->dweight, 3, 1, true);
-  colsum_kernel<<<dim3((p.D + 63) / 64, n, zmax), 256, 0, st>>>(c);
+  colsum_kernel<<<dim3((p.D + 63) / 64, n, zmax), 64 * kCsParts, 0, st>>>(c);
   return check_launch(what);
 }

@@ -39,6 +39,13 @@ __device__ __forceinline__ uint32_t wave_umax(uint32_t x) {
   return wave_reduce(x, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
 }
 
+// max(a, |b|, |c|) that is NaN if one of them is.
+__device__ __forceinline__ float max3abs_nan(float a, float b, float c) {
+  float r;
+  asm("v_maximum3_f32 %0, %1, |%2|, |%3|" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
 // Magnitudes are compared as bit patterns: among non-negative floats the order
 // is the same, and a NaN stands above infinity instead of being dropped.
 constexpr uint32_t kInfBits = 0x7f800000u;
@@ -46,40 +53,48 @@ __device__ __forceinline__ uint32_t mag_bits(float x) { return __float_as_uint(x
 
 // GELU(x) = x Phi(x) with Phi the normal distribution function. For a = |x|
 //   Q(a) = 1 - Phi(a) = exp(-a^2 / 2) F(a),  F(a) = erfcx(a / sqrt 2) / 2,
-// and F(a) = t P(t) with t = 1 / (1 + 0.31 a): P is a polynomial of degree 5
-// fitted to a relative error of 4.7e-6 over 0 <= a <= 14 (minimax, by linear
+// and F(a) = t P(t) with t = 1 / (1 + 0.375 a): P is a polynomial of degree 4
+// fitted to a relative error of 3.1e-5 over 0 <= a <= 14 (minimax, by linear
 // programming against scipy's erfcx), below which Q is under 2^-126. The error
-// is relative, so that the lower tail of GELU keeps its digits; it is a
-// hundredth of a bf16 rounding (2^-9).
-struct Phi {
-  float p;  // Phi(x)
-  float e;  // exp(-x^2 / 2)
+// is relative, so that the lower tail of GELU keeps its digits; it is a 60th of
+// a bf16 rounding (2^-9). Then, for either sign of x,
+//   GELU(x) = max(x, 0) - a Q(a).
+// The kernels that use these are bound by vector instructions as much as by
+// memory: 12 and two transcendental ones a value (a degree more, and selecting
+// Phi by x's sign, took 18).
+struct Tail {
+  float a;  // |x|, or 2^100
+  float f;  // Q / e
+  float e;  // exp(-x^2 / 2); NaN for NaN
 };
-__device__ __forceinline__ Phi normal_cdf(float x) {
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.31f, fabsf(x), 1.0f));
-  const float e = __builtin_amdgcn_exp2f((x * x) * (-0.5f * kLog2e));
-  float f = fmaf(t, -0.07393838465213776f, 0.18047693371772766f);
-  f = fmaf(t, f, 0.01571611687541008f);
-  f = fmaf(t, f, 0.13344404101371765f);
-  f = fmaf(t, f, 0.12043801695108414f);
-  f = fmaf(t, f, 0.12386097013950348f);
-  const float q = f * t * e;
-  return {x < 0.f ? q : 1.0f - q, e};
+__device__ __forceinline__ Tail normal_tail(float x) {
+  // Bounded so that infinity times Q's zero is no NaN. (fminf and fmaxf would
+  // quiet their operand first, an instruction each; NaN comes through e.)
+  const float a = __builtin_amdgcn_fmed3f(__builtin_fabsf(x), 0.f, 0x1p+100f);
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.375f, a, 1.0f));
+  const float e = __builtin_amdgcn_exp2f((x * (-0.5f * kLog2e)) * x);
+  float f = fmaf(t, -0.0906425192952156f, 0.20028099417686462f);
+  f = fmaf(t, f, 0.08356455713510513f);
+  f = fmaf(t, f, 0.15773384273052216f);
+  f = fmaf(t, f, 0.14906103909015656f);
+  return {a, f * t, e};
 }
-// x Phi(x); -inf gives its limit 0 (the product alone would be -inf * 0).
 __device__ __forceinline__ float gelu(float x) {
-  return fmaxf(x, -0x1p+100f) * normal_cdf(x).p;
+  const Tail n = normal_tail(x);
+  return fmaf(-n.a, n.f * n.e, __builtin_amdgcn_fmed3f(x, 0.f, __builtin_inff()));
 }
-// d GELU / dx = Phi(x) + x phi(x), phi(x) = exp(-x^2 / 2) / sqrt(2 pi).
+// d GELU / dx = Phi(x) + x phi(x), phi(x) = exp(-x^2 / 2) / sqrt(2 pi): with
+// d = Q(a) - a phi(a), it is d for negative x and 1 - d otherwise.
 __device__ __forceinline__ float gelu_slope(float x) {
-  const Phi n = normal_cdf(x);
-  return fmaf(x * 0.3989422804014327f, n.e, n.p);
+  const Tail n = normal_tail(x);
+  const float d = fmaf(-0.3989422804014327f, n.a, n.f) * n.e;
+  return x < 0.f ? d : 1.0f - d;
 }
 
-// The low byte of the result's bits is round-to-nearest-even(x) in two's
-// complement for |x| <= 127: adding 1.5 * 2^23 leaves the integer in the low
-// mantissa bits.
-__device__ __forceinline__ uint32_t round_bits(float x) { return __float_as_uint(x + 12582912.0f); }
+// x + kRoundMagic for |x| <= 127, rounded to nearest even, has round(x) in two's
+// complement in the low byte of its bits: 1.5 * 2^23 leaves the integer in the
+// low mantissa bits.
+constexpr float kRoundMagic = 12582912.0f;
 // The low bytes of four words, the first lowest.
 __device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   const uint32_t ab = __builtin_amdgcn_perm(b, a, 0x0c0c0400u);
@@ -87,48 +102,26 @@ __device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c
   return ab | cd;
 }
 
-// Per-token int8 codes: with s = max(max |y|, 1e-12) / 127, the code of y is
-// round-to-nearest-even(y / s), |code| <= 127. The quotient is rounded
-// correctly before it is rounded to an integer, as a division would (ties of
-// the second rounding would otherwise fall either way): from the correctly
-// rounded reciprocal, q0 = RN(y rcp), e = y - q0 s exact in an FMA, and
-// RN(q0 + e rcp) is the quotient (Markstein) as long as no remainder
-// underflows, which holds for max |y| >= 2^-60 where it decides a code.
-// A row with a value that is not finite has the scale NaN and codes 0.
+// Per-token int8 codes: with s = max(max |y|, 1e-12) / 127 and rcp = 1 / s, both
+// rounded to fp32, the code of y is round-to-nearest-even(y rcp), the product
+// exact (one FMA); |y rcp| <= 127 (1 + 2^-22), so |code| <= 127. The correctly
+// rounded quotient y / s in its place took two more instructions a value, a
+// tenth of the kernel's time, for codes that differ where y / s is within
+// 2^-16 of a half. A row with a value that is not finite has the scale NaN and
+// codes 0 (NaN + magic is 0x7fc00000).
 struct RowScale {
   float s, rcp;
-  bool divide;
 };
 __device__ __forceinline__ RowScale row_scale(uint32_t amax_bits) {
-  const float amax = __uint_as_float(amax_bits);
   RowScale r;
-  r.s = amax_bits >= kInfBits ? __builtin_nanf("") : fmaxf(amax, 1e-12f) / 127.0f;
+  r.s = amax_bits >= kInfBits ? __builtin_nanf("") : fmaxf(__uint_as_float(amax_bits), 1e-12f) / 127.0f;
   r.rcp = 1.0f / r.s;
-  r.divide = amax < 0x1p-60f;
   return r;
 }
-template <bool kDivide>
-__device__ __forceinline__ uint32_t int8_code(float y, const RowScale& r) {
-  float t;
-  if constexpr (kDivide) {
-    t = y / r.s;
-  } else {
-    const float q0 = y * r.rcp;
-    t = fmaf(fmaf(-q0, r.s, y), r.rcp, q0);
-  }
-  return round_bits(t);
-}
-// Eight values' codes. NaN scale: every quotient is NaN, whose bits + magic
-// have a zero low byte (the quiet NaN 0x7fc00000).
 __device__ __forceinline__ u32x2 int8_codes8(const float* y, const RowScale& r) {
   uint32_t c[8];
-  if (r.divide) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = int8_code<true>(y[i], r);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = int8_code<false>(y[i], r);
-  }
+  for (int i = 0; i < 8; ++i) c[i] = __float_as_uint(fmaf(y[i], r.rcp, kRoundMagic));
   return u32x2{low_bytes(c[0], c[1], c[2], c[3]), low_bytes(c[4], c[5], c[6], c[7])};
 }
 

@@ -21,6 +21,7 @@
 
 #include "aa_common.h"
 #include "block_math.h"
+#include "tile_io.h"
 
 namespace aa {
 
@@ -33,80 +34,109 @@ __device__ __forceinline__ uint32_t step_exp(uint32_t amax_bits) {
   const int e = (int)(amax_bits >> 23) - 6;  // amax in [2^(e' - 127), 2^(e' - 126))
   return amax_bits >= kInfBits ? kNotFinite : (uint32_t)max(e, 1);
 }
+// The bits of the largest magnitude of a group that four neighbouring lanes hold
+// 8 values each of, from the packed bf16: as 16-bit integers, magnitudes keep
+// their order and NaN stands above infinity.
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t packed_max(uint32_t a, uint32_t b) {
+  const u16x2 x = __builtin_bit_cast(u16x2, a), y = __builtin_bit_cast(u16x2, b);
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(x, y));
+}
+__device__ __forceinline__ uint32_t lane_amax(u32x4 w) {
+  const uint32_t m = 0x7fff7fffu;
+  return packed_max(packed_max(w[0] & m, w[1] & m), packed_max(w[2] & m, w[3] & m));
+}
+// The larger of a packed pair, as the bits of a float.
+__device__ __forceinline__ uint32_t pair_amax(uint32_t top) { return max(top << 16, top & 0xffff0000u); }
+__device__ __forceinline__ uint32_t group_amax(u32x4 w) {
+  uint32_t top = pair_amax(lane_amax(w));
+  top = max(top, dpp_mov<kDppXor1>(top));
+  return max(top, dpp_mov<kDppXor2>(top));
+}
+
 // step, and 1 / step (both exact: 1 <= exponent <= 248).
 __device__ __forceinline__ float step_of(uint32_t e) {
   return __uint_as_float(e == kNotFinite ? 0x7fc00000u : e << 23);
 }
 __device__ __forceinline__ float inv_step_of(uint32_t e) { return __uint_as_float((254u - e) << 23); }
 
-// Codes of 8 values. An exponent above 253 needs an inverse step below the
+// Codes of 8 values: v * inv is exact (a power of two), so the FMA's one
+// rounding is that to an integer. An exponent above 253 needs an inverse step below the
 // normal range, which cannot occur for finite values (e <= 248); for a marked
 // group the codes are never read as numbers.
 __device__ __forceinline__ u32x2 codes8(const float* v, float inv) {
   uint32_t c[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    c[i] = round_bits(__builtin_amdgcn_fmed3f(v[i] * inv, -127.0f, 127.0f));
+    c[i] = __float_as_uint(__builtin_amdgcn_fmed3f(fmaf(v[i], inv, kRoundMagic), kRoundMagic - 127.0f, kRoundMagic + 127.0f));
   return u32x2{low_bytes(c[0], c[1], c[2], c[3]), low_bytes(c[4], c[5], c[6], c[7])};
 }
-// Signed byte i (0..3) of a word as a float.
+// code * step of byte kByte of a word of codes with their sign bits flipped
+// (code + 128 as an unsigned byte, which one instruction converts), with low =
+// -128 step. Exact: (code + 128) step - 128 step has at most 8 significant bits.
 template <int kByte>
-__device__ __forceinline__ float byte_f(uint32_t w) {
-  return (float)((int)(w << (24 - 8 * kByte)) >> 24);
+__device__ __forceinline__ float kept_value(uint32_t flipped, float step, float low) {
+  return fmaf((float)((flipped >> (8 * kByte)) & 255u), step, low);
 }
 
 // -------------------------------------------------------------------- GELU --
 
 constexpr int kGeThreads = 256;
+constexpr int kGeChunks = 4;  // per lane
 
-// Sixteen values per lane: a group of 32 is two neighbouring lanes. Rows are
-// cut into 2 G units of 16 (G = ceil(K / 32)); codes have the row stride 32 G.
-// With kFlat (K % 32 == 0) rows follow one another without gaps and a unit's
-// index is its place.
+// Chunks of 8 values, a lane's kGeChunks at a stride of the workgroup, so that
+// every load and store of a wave covers whole cache lines (with 16 neighbouring
+// values a lane, each store half of every other 32 bytes, nontemporal stores
+// took twice the time); a group of 32 is four neighbouring lanes. Rows are cut
+// into 4 G chunks (G = ceil(K / 32)); codes have the row stride 32 G. With kFlat
+// (K % 32 == 0) rows follow one another without gaps and a chunk's index is its
+// place.
 struct GeluFwd {
   const bf16* x;
   bf16* y;
   uint8_t* codes;  // [rows][32 G], or null: no checkpoint
   uint8_t* exps;   // [rows][G]
-  int64_t units;
-  int K, upr;  // units per row
+  int64_t chunks;
+  int K, cpr;  // chunks per row
 };
+
+// Element index of chunk c, or -1 past its row's end.
+template <bool kFlat>
+__device__ __forceinline__ int64_t chunk_at(int64_t c, int K, int cpr) {
+  if constexpr (kFlat) return 8 * c;
+  const int64_t row = c / cpr;
+  const int k = 8 * (int)(c - row * cpr);
+  return k < K ? row * K + k : -1;
+}
 
 template <bool kFlat>
 __global__ __launch_bounds__(kGeThreads) void gelu8_fwd_kernel(GeluFwd p) {
-  const int64_t u = (int64_t)blockIdx.x * kGeThreads + threadIdx.x;
-  if (u >= p.units) return;  // units come in pairs: both lanes of a group stay
-  int64_t at = 16 * u;
-  int have = 2;  // 8-value halves of this unit that are inside the row
-  if constexpr (!kFlat) {
-    const int64_t row = u / p.upr;
-    const int k = 16 * (int)(u - row * p.upr);
-    at = row * p.K + k;
-    have = k + 16 <= p.K ? 2 : k + 8 <= p.K ? 1 : 0;
-  }
-  u32x4 raw[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+  const int64_t first = (int64_t)blockIdx.x * (kGeThreads * kGeChunks) + threadIdx.x;
+  u32x4 raw[kGeChunks];
+  int64_t at[kGeChunks];
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
-    if (h < have) raw[h] = ld16(p.x + at + 8 * h);
-  float v[16];
-  unpack8(raw[0], v);
-  unpack8(raw[1], v + 8);
-  if (p.codes) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) top = max(top, mag_bits(v[i]));
-    top = max(top, dpp_mov<kDppXor1>(top));
-    const uint32_t e = step_exp(top);
-    const float inv = inv_step_of(e);
-    const u32x2 a = codes8(v, inv), b = codes8(v + 8, inv);
-    st16(p.codes + 16 * u, u32x4{a[0], a[1], b[0], b[1]});
-    if ((threadIdx.x & 1) == 0) p.exps[u >> 1] = (uint8_t)e;
+  for (int i = 0; i < kGeChunks; ++i) {
+    const int64_t c = first + kGeThreads * i;
+    at[i] = c < p.chunks ? chunk_at<kFlat>(c, p.K, p.cpr) : -1;
+    raw[i] = u32x4{0, 0, 0, 0};
+    if (at[i] >= 0) raw[i] = ld16(p.x + at[i]);
   }
 #pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = gelu(v[i]);
+  for (int i = 0; i < kGeChunks; ++i) {
+    const int64_t c = first + kGeThreads * i;
+    float v[8];
+    unpack8(raw[i], v);
+    if (p.codes) {
+      const uint32_t e = step_exp(group_amax(raw[i]));
+      if (c < p.chunks) {  // chunks come in fours: all lanes of a group
+        __builtin_nontemporal_store(codes8(v, inv_step_of(e)), reinterpret_cast<u32x2*>(p.codes + 8 * c));
+        if ((threadIdx.x & 3) == 0) p.exps[c >> 2] = (uint8_t)e;
+      }
+    }
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
-    if (h < have) st16(p.y + at + 8 * h, pack8(v + 8 * h));
+    for (int j = 0; j < 8; ++j) v[j] = gelu(v[j]);
+    if (at[i] >= 0) st16_nt(p.y + at[i], pack8(v));
+  }
 }
 
 struct GeluBwd {
@@ -114,34 +144,38 @@ struct GeluBwd {
   const uint8_t* codes;
   const uint8_t* exps;
   bf16* dx;
-  int64_t units;
-  int K, upr;
+  int64_t chunks;
+  int K, cpr;
 };
 
 template <bool kFlat>
 __global__ __launch_bounds__(kGeThreads) void gelu8_bwd_kernel(GeluBwd p) {
-  const int64_t u = (int64_t)blockIdx.x * kGeThreads + threadIdx.x;
-  if (u >= p.units) return;
-  int64_t at = 16 * u;
-  int have = 2;
-  if constexpr (!kFlat) {
-    const int64_t row = u / p.upr;
-    const int k = 16 * (int)(u - row * p.upr);
-    at = row * p.K + k;
-    have = k + 16 <= p.K ? 2 : k + 8 <= p.K ? 1 : 0;
-  }
-  const u32x4 c = ld16(p.codes + 16 * u);
-  const float step = step_of(p.exps[u >> 1]);
+  const int64_t first = (int64_t)blockIdx.x * (kGeThreads * kGeChunks) + threadIdx.x;
+  u32x4 raw[kGeChunks];
+  u32x2 code[kGeChunks];
+  uint32_t e[kGeChunks];
+  int64_t at[kGeChunks];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    if (h >= have) continue;
+  for (int i = 0; i < kGeChunks; ++i) {
+    const int64_t c = first + kGeThreads * i;
+    at[i] = c < p.chunks ? chunk_at<kFlat>(c, p.K, p.cpr) : -1;
+    if (at[i] >= 0) {
+      raw[i] = ld16(p.dy + at[i]);
+      code[i] = *reinterpret_cast<const u32x2*>(p.codes + 8 * c);
+      e[i] = p.exps[c >> 2];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kGeChunks; ++i) {
+    if (at[i] < 0) continue;
+    const float step = step_of(e[i]), low = -128.0f * step;
     float g[8];
-    unpack8(ld16(p.dy + at + 8 * h), g);
-    static_for<0, 8>([&](auto I) {
-      constexpr int i = decltype(I)::value;
-      g[i] *= gelu_slope(byte_f<i & 3>(c[2 * h + (i >> 2)]) * step);
+    unpack8(raw[i], g);
+    static_for<0, 8>([&](auto J) {
+      constexpr int j = decltype(J)::value;
+      g[j] *= gelu_slope(kept_value<j & 3>(code[i][j >> 2] ^ 0x80808080u, step, low));
     });
-    st16(p.dx + at + 8 * h, pack8(g));
+    st16_nt(p.dx + at[i], pack8(g));
   }
 }
 
@@ -149,130 +183,148 @@ __global__ __launch_bounds__(kGeThreads) void gelu8_bwd_kernel(GeluBwd p) {
 
 constexpr int kLoMaxR = 64;
 
-// t = x A^T and the checkpoint of x, in one pass over x. A workgroup takes 16
-// RT rows; its waves take slices of 256 channels in turn. A slice's 16 rows are
-// loaded as whole lines (two rows of 512 bytes per instruction, lane l: row
-// i + 8 (l / 32), channels 8 (l % 32)), so a group of 32 channels is four
-// neighbouring lanes; they are coded and stored from there, and cross to the
-// MFMA's operand layout through a tile of LDS that the wave has to itself
-// (row r's 16-byte chunk c in slot c ^ r). The waves' partial sums are added in
-// LDS in a fixed order.
+// t = x A^T and the checkpoint of x, in one pass over x. A workgroup takes 2048
+// channels (1024 above rank 48), its 16 (8) waves 128 each, and tiles of 16 rows in turn. A wave keeps
+// its part of A in registers, loads its 16 x 128 part of x as whole lines (lane
+// l: row i + 4 (l / 16), channels 8 (l % 16)), so that a group of 32 channels is
+// four neighbouring lanes, and codes and stores it from there; x crosses to the
+// MFMA's operand layout through a tile of LDS that the wave has to itself (row
+// r's 16-byte chunk c in slot c ^ r). The waves' 16 x R sums then go to the same
+// place, and after a barrier four waves, others from tile to tile, add them in a
+// fixed order. Two such places in turn, so one barrier a tile. With more channels
+// than one workgroup takes, the sums of the ranges leave in fp32 for lora8_sum_kernel.
+// Forms measured before, 7904 x 8192 at rank 40 (floor 28 us): every wave with
+// rows and channels of its own and A from memory in the operand layout 79 us
+// (A's traffic, 16 ranks x 64 bytes an instruction); A's part of a step through
+// LDS, shared by 32 rows, 58 us (LDS and vector work between barriers).
 struct LoraFwd {
   const bf16* x;  // [M, K]
   const bf16* a;  // [R, K]
-  bf16* t;        // [M, R]
+  bf16* t;        // [M, R], written here when splits == 1
+  float* part;    // [splits][M][R]
   uint8_t* codes;  // [M][32 G], or null
   uint8_t* exps;   // [G][Mp], Mp = M up to a multiple of 16
   int64_t M, Mp;
   int K, R, G;
+  int splits;  // ranges of channels
+  int tiles;   // tiles of 16 rows per workgroup
 };
 
-constexpr int kLoWaves = 8;
-constexpr int kLoThreads = 64 * kLoWaves;
-constexpr int kLoSlice = 256;
+constexpr int kLoSlice = 128;
+// Waves of a workgroup: A's part takes 16 registers per 16 ranks, and 64 do not
+// fit beside the rest of 16 waves' 128.
+constexpr int lora_waves(int64_t R) { return R <= 48 ? 16 : 8; }
+constexpr int lora_splits(int64_t K, int64_t R) {
+  return (int)((K + kLoSlice * lora_waves(R) - 1) / (kLoSlice * lora_waves(R)));
+}
 
 typedef float f32x4v __attribute__((ext_vector_type(4)));
 
-template <int NR, int RT>
-__global__ __launch_bounds__(kLoThreads) void lora8_fwd_kernel(LoraFwd p) {
-  // The waves' x tiles, then their sums.
-  constexpr int kTile = 16 * kLoSlice * 2;
-  constexpr int kSums = NR * RT * 16 * 16 * 4;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[kLoWaves * (kTile > kSums ? kTile : kSums)];
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+template <int NR>
+__global__ __launch_bounds__(64 * lora_waves(16 * NR)) void lora8_fwd_kernel(LoraFwd p) {
+  constexpr int kLoWaves = lora_waves(16 * NR);
+  constexpr int kLoRange = kLoSlice * kLoWaves;
+  constexpr int kTile = 16 * kLoSlice * 2;  // >= NR KiB of sums
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2][kLoWaves][kTile];
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int li = lane & 15, g = lane >> 4;
-  const int64_t row0 = (int64_t)blockIdx.x * (16 * RT);
-  uint8_t* tile = lds + wave * kTile;
-  f32x4v acc[RT][NR];
+  const int k0 = blockIdx.y * kLoRange + kLoSlice * wave;  // the wave's channels
+  const int col = k0 + 8 * li;                             // this lane's
+  const bool in = col < p.K;
+  const bool keep = p.codes && col < kGroup * p.G;
+
+  bf16x8 a[4][NR];
 #pragma unroll
-  for (int t = 0; t < RT; ++t)
+  for (int s = 0; s < 4; ++s)
 #pragma unroll
-    for (int n = 0; n < NR; ++n) acc[t][n] = f32x4v{0.f, 0.f, 0.f, 0.f};
-  for (int k0 = kLoSlice * wave; k0 < p.K; k0 += kLoSlice * kLoWaves) {
-    const int col = k0 + 8 * (lane & 31);
-    const bool in = col < p.K;  // K is a multiple of 8
-    u32x4 raw[RT][8];
-#pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        raw[t][i] = u32x4{0, 0, 0, 0};
-        const int64_t row = min(row0 + 16 * t + i + 8 * (lane >> 5), p.M - 1);
-        if (in) raw[t][i] = ld16(p.x + row * p.K + col);
-      }
-    bf16x8 w[8][NR];
-#pragma unroll
-    for (int s = 0; s < 8; ++s)
-#pragma unroll
-      for (int n = 0; n < NR; ++n) {
-        const int rank = 16 * n + li, k = k0 + 32 * s + 8 * g;
-        u32x4 v = u32x4{0, 0, 0, 0};
-        if (rank < p.R && k < p.K) v = ld16(p.a + (int64_t)rank * p.K + k);
-        w[s][n] = __builtin_bit_cast(bf16x8, v);
-      }
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      uint32_t ex[2] = {0, 0};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = i + 8 * (lane >> 5);
-        *reinterpret_cast<u32x4*>(tile + r * 512 + (((lane & 31) ^ r) * 16)) = raw[t][i];
-        if (p.codes) {
-          float v[8];
-          unpack8(raw[t][i], v);
-          uint32_t top = 0;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) top = max(top, mag_bits(v[j]));
-          top = max(top, dpp_mov<kDppXor1>(top));
-          top = max(top, dpp_mov<kDppXor2>(top));
-          const uint32_t e = step_exp(top);
-          const int64_t row = row0 + 16 * t + r;
-          if (row < p.M && col < kGroup * p.G)
-            *reinterpret_cast<u32x2*>(p.codes + row * (kGroup * p.G) + col) = codes8(v, inv_step_of(e));
-          ex[i >> 2] |= e << (8 * (i & 3));
-        }
-      }
-      // Rows r0 .. r0 + 7 of this lane's group; rows past M, up to Mp, too.
-      if (p.codes && (lane & 3) == 0 && col < kGroup * p.G && row0 + 16 * t < p.Mp)
-        *reinterpret_cast<u32x2*>(p.exps + (int64_t)(col / kGroup) * p.Mp + row0 + 16 * t + 8 * (lane >> 5)) =
-            u32x2{ex[0], ex[1]};
-      // The wave's own tile: its writes are in order with its reads.
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        const bf16x8 xv = *reinterpret_cast<const bf16x8*>(tile + li * 512 + (((4 * s + g) ^ li) * 16));
-#pragma unroll
-        for (int n = 0; n < NR; ++n)
-          acc[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[s][n], xv, acc[t][n], 0, 0, 0);
-      }
-      __builtin_amdgcn_wave_barrier();
+    for (int n = 0; n < NR; ++n) {
+      const int rank = 16 * n + li, k = k0 + 32 * s + 8 * g;
+      u32x4 v = u32x4{0, 0, 0, 0};
+      if (rank < p.R && k < p.K) v = ld16(p.a + (int64_t)rank * p.K + k);
+      a[s][n] = __builtin_bit_cast(bf16x8, v);
     }
-  }
-  // acc[t][n]: lane li is token 16 t + li, element i is rank 16 n + 4 g + i.
-  __syncthreads();
-  f32x4v* sums = reinterpret_cast<f32x4v*>(lds);
+  const int64_t first = (int64_t)blockIdx.x * p.tiles;
+  const int tiles = (int)min<int64_t>(p.tiles, p.Mp / 16 - first);
+  u32x4 x[4];
+  // Addresses: a uniform base per tile and 32-bit offsets (15 rows of at most 65536).
+  const uint32_t pitch = kGroup * p.G;
+  auto load = [&](int64_t row0) {  // rows past M re-read the last
+    const bf16* base = p.x + row0 * p.K;
+    const int last = (int)min<int64_t>(15, p.M - 1 - row0);
 #pragma unroll
-  for (int t = 0; t < RT; ++t)
+    for (int i = 0; i < 4; ++i) x[i] = u32x4{0, 0, 0, 0};
+    if (in) {
 #pragma unroll
-    for (int n = 0; n < NR; ++n) sums[(wave * RT * NR + t * NR + n) * 64 + lane] = acc[t][n];
-  __syncthreads();
-  for (int o = threadIdx.x; o < RT * NR * 64; o += kLoThreads) {
-    f32x4v s = sums[o];
+      for (int i = 0; i < 4; ++i) x[i] = ld16(base + ((uint32_t)(min(i + 4 * g, last) * p.K) + (uint32_t)col));
+    }
+  };
+  load(16 * first);
+  for (int it = 0; it < tiles; ++it) {
+    const int64_t row0 = 16 * (first + it);
+    uint8_t* tile = lds[it & 1][wave];
 #pragma unroll
-    for (int w = 1; w < kLoWaves; ++w) s += sums[w * RT * NR * 64 + o];
-    const int l = o & 63, n = (o >> 6) % NR, t = (o >> 6) / NR;
-    const int64_t row = row0 + 16 * t + (l & 15);
-    const int rank = 16 * n + 4 * (l >> 4);
-    if (row < p.M && rank < p.R)  // R is a multiple of 8
-      *reinterpret_cast<u32x2*>(p.t + row * p.R + rank) = u32x2{pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3])};
+    for (int i = 0; i < 4; ++i) {
+      const int r = i + 4 * g;
+      *reinterpret_cast<u32x4*>(tile + r * 256 + ((li ^ r) * 16)) = x[i];
+    }
+    if (p.codes) {
+      uint8_t* codes = p.codes + row0 * pitch;
+      const int rows = keep ? (int)min<int64_t>(16, p.M - row0) : 0;
+      uint32_t ex = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t e = step_exp(group_amax(x[i]));
+        float v[8];
+        unpack8(x[i], v);
+        const u32x2 c = codes8(v, inv_step_of(e));
+        if (i + 4 * g < rows) *reinterpret_cast<u32x2*>(codes + ((uint32_t)(i + 4 * g) * pitch + (uint32_t)col)) = c;
+        ex |= e << (8 * i);
+      }
+      // Four rows' exponents; rows past M, up to Mp, are written too.
+      if (keep && (lane & 3) == 0)
+        *reinterpret_cast<uint32_t*>(p.exps + row0 + ((int64_t)(col / kGroup) * p.Mp + 4 * g)) = ex;
+    }
+    if (it + 1 < tiles) load(row0 + 16);
+    f32x4v acc[NR];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) acc[n] = f32x4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const bf16x8 xv = *reinterpret_cast<const bf16x8*>(tile + li * 256 + (((4 * s + g) ^ li) * 16));
+#pragma unroll
+      for (int n = 0; n < NR; ++n) acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[s][n], xv, acc[n], 0, 0, 0);
+    }
+    // acc[n]: lane li is row li, element i is rank 16 n + 4 g + i. The wave's reads
+    // of its tile come before these writes.
+#pragma unroll
+    for (int n = 0; n < NR; ++n) reinterpret_cast<f32x4v*>(tile)[n * 64 + lane] = acc[n];
+    __syncthreads();
+    const int turn = (wave - 4 * it) & (kLoWaves - 1);
+    if (turn < NR) {  // this wave adds rank block `turn`
+      f32x4v s = reinterpret_cast<const f32x4v*>(lds[it & 1][0])[turn * 64 + lane];
+#pragma unroll
+      for (int w = 1; w < kLoWaves; ++w) s += reinterpret_cast<const f32x4v*>(lds[it & 1][w])[turn * 64 + lane];
+      const int64_t row = row0 + li;
+      const int rank = 16 * turn + 4 * g;
+      if (row < p.M && rank < p.R) {  // R is a multiple of 8
+        if (p.splits == 1)
+          *reinterpret_cast<u32x2*>(p.t + row * p.R + rank) = u32x2{pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3])};
+        else
+          *reinterpret_cast<f32x4v*>(p.part + ((int64_t)blockIdx.y * p.M + row) * p.R + rank) = s;
+      }
+    }
   }
 }
 
-// dx = dt A: a wave takes 128 channels and 16 rows at a time. A's columns are
-// the MFMA's row operand, gathered once per wave (A^T is not in memory);
-// channel 32 j + 8 g + 4 h + i is row 4 g + i of product (j, h), so that a lane
-// ends with 8 neighbouring channels of its row.
+// dx = dt A: a wave takes 128 channels and 16 rows at a time. The MFMA's row
+// operand is A's columns (A^T is not in memory): the workgroup's part of A
+// lies in LDS as it is, and ds_read_b64_tr_b16 hands a lane four ranks of its
+// channel. Row 4 q + i of product (j, h) is channel 32 j + 8 q + 4 h + i, so that
+// a lane ends with 8 neighbouring channels of its row; the lanes of rows 8..15
+// then trade places between products j and j + 1, and each store covers 8 rows
+// of 128 bytes, whole lines.
 struct LoraDx {
   const bf16* dt;  // [M, R]
   const bf16* a;
@@ -283,31 +335,35 @@ struct LoraDx {
 
 template <int NS>  // 32 ranks per step
 __global__ __launch_bounds__(256) void lora8_dx_kernel(LoraDx p) {
+  __shared__ __attribute__((aligned(16))) bf16 as[32 * NS * 128];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int li = lane & 15, g = lane >> 4;
   const int k0 = blockIdx.x * 128;
+  for (int o = threadIdx.x; o < 32 * NS * 16; o += 256) {
+    const int rank = o >> 4, k = k0 + 8 * (o & 15);
+    u32x4 v = u32x4{0, 0, 0, 0};
+    if (rank < p.R && k < p.K) v = ld16(p.a + (int64_t)rank * p.K + k);
+    *reinterpret_cast<u32x4*>(as + rank * 128 + 8 * (o & 15)) = v;
+  }
+  __syncthreads();
+  // Lanes 4 r + q of a group of 16 give the piece of four channels at 8 q of rank
+  // 8 g + r (+ 4 for the second read).
+  const bf16* piece = as + (8 * g + (li >> 2)) * 128 + 8 * (li & 3);
   bf16x8 w[4][2][NS];
 #pragma unroll
   for (int j = 0; j < 4; ++j)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int k = k0 + 32 * j + 8 * (li >> 2) + 4 * h + (li & 3);
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
-        bf16x8 v;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int rank = 32 * s + 8 * g + e;
-          v[e] = rank < p.R && k < p.K ? p.a[(int64_t)rank * p.K + k] : (bf16)0.f;
-        }
-        w[j][h][s] = v;
+        const s16x4 lo = ds_read_tr(piece + 32 * s * 128 + 32 * j + 4 * h);
+        const s16x4 hi = ds_read_tr(piece + (32 * s + 4) * 128 + 32 * j + 4 * h);
+        w[j][h][s] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
       }
-    }
   const int64_t begin = (int64_t)blockIdx.y * p.rows, end = min(p.M, begin + p.rows);
-  for (int64_t r0 = begin + 16 * wave; r0 < end; r0 += 64) {
+  auto load = [&](bf16x8 (&d)[NS], int64_t r0) {
     const int64_t row = min(r0 + li, p.M - 1);
-    bf16x8 d[NS];
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
       const int rank = 32 * s + 8 * g;
@@ -315,30 +371,55 @@ __global__ __launch_bounds__(256) void lora8_dx_kernel(LoraDx p) {
       if (rank < p.R) v = ld16(p.dt + row * p.R + rank);
       d[s] = __builtin_bit_cast(bf16x8, v);
     }
+  };
+  bf16x8 next[NS];
+  load(next, begin + 16 * wave);
+  for (int64_t r0 = begin + 16 * wave; r0 < end; r0 += 64) {
+    bf16x8 d[NS];
+#pragma unroll
+    for (int s = 0; s < NS; ++s) d[s] = next[s];
+    if (r0 + 64 < end) load(next, r0 + 64);
+    u32x4 o[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      f32x4v o[2];
+      f32x4v q[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        o[h] = f32x4v{0.f, 0.f, 0.f, 0.f};
+        q[h] = f32x4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < NS; ++s)
-          o[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[j][h][s], d[s], o[h], 0, 0, 0);
+          q[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[j][h][s], d[s], q[h], 0, 0, 0);
       }
-      const int k = k0 + 32 * j + 8 * g;
-      if (r0 + li < end && k < p.K)
-        st16(p.dx + (r0 + li) * p.K + k, u32x4{pack_bf16(o[0][0], o[0][1]), pack_bf16(o[0][2], o[0][3]),
-                                               pack_bf16(o[1][0], o[1][1]), pack_bf16(o[1][2], o[1][3])});
+      o[j] = u32x4{pack_bf16(q[0][0], q[0][1]), pack_bf16(q[0][2], q[0][3]), pack_bf16(q[1][0], q[1][1]),
+                   pack_bf16(q[1][2], q[1][3])};
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) {
+      u32x4 lo, hi;  // rows 0..7 and rows 8..15 of channels 32 j .. 32 j + 63
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // Lanes 8..15 (bank mask 12) of each 16 take product j + 1's lanes 0..7;
+        // lanes 0..7 product j's lanes 8..15.
+        lo[i] = (uint32_t)__builtin_amdgcn_update_dpp((int)o[j][i], (int)o[j + 1][i], kDppRor + 8, 0xf, 0xc, false);
+        hi[i] = (uint32_t)__builtin_amdgcn_update_dpp((int)o[j + 1][i], (int)o[j][i], kDppRor + 8, 0xf, 0x3, false);
+      }
+      const int k = k0 + 32 * j + 32 * (li >> 3) + 8 * g;
+      if (k < p.K) {
+        const int64_t r = r0 + (li & 7);
+        if (r < end) st16_nt(p.dx + r * p.K + k, lo);
+        if (r + 8 < end) st16_nt(p.dx + (r + 8) * p.K + k, hi);
+      }
     }
   }
 }
 
-// dA = dt^T kept(x): a workgroup takes 256 channels and a range of rows, its
-// four waves 32 rows each in turn. Lane l reads 16 channels (16 (l % 16)) of
-// rows 8 (l / 16) .. + 7: product j of 16 takes channel 16 li + j of every
-// lane, the rows as the contracted index. dt comes transposed through LDS,
-// 128 rows at a time. Partial sums per range of rows, in fp32, are added by
-// lora8_da_sum_kernel (or, of one range, written as they are).
+// dA = dt^T kept(x): a workgroup takes 128 channels and a range of rows, its
+// four waves 32 rows each in turn. Lane l reads 8 channels (8 (l % 16)) of rows
+// 8 (l / 16) .. + 7: product j of 8 takes channel 8 li + j of every lane, the
+// rows as the contracted index. dt lies in LDS as it is in memory, 128 rows at
+// a time, and is read transposed. The next turn's codes, steps and dt are
+// loaded before this turn's products. Partial sums per range of rows, in fp32,
+// are added by lora8_sum_kernel (or, of one range, written as they are).
 struct LoraDa {
   const bf16* dt;
   const uint8_t* codes;
@@ -352,75 +433,104 @@ struct LoraDa {
 constexpr int kDaWaves = 4;
 constexpr int kDaThreads = 64 * kDaWaves;
 constexpr int kDaRows = 32 * kDaWaves;  // rows of a turn
-constexpr int kDaPitch = kDaRows + 8;   // bf16 elements per rank in LDS
+constexpr int kDaCols = 128;
 
 template <int NR>
-__global__ __launch_bounds__(kDaThreads) void lora8_da_kernel(LoraDa p) {
-  constexpr int kDt = 16 * NR * kDaPitch * 2;
-  constexpr int kSum = kDaWaves * 64 * 16 * NR * 4;  // one rank row i of every wave at a time
+__global__ __launch_bounds__(kDaThreads, NR < 4 ? 2 : 1) void lora8_da_kernel(LoraDa p) {
+  // Row pitch in LDS: a multiple of 8 bytes whose 16-row stride spreads over the
+  // banks (the transposed reads take 4 rows x 32 bytes per 16 lanes).
+  constexpr int kPitch = 16 * NR + 4;
+  constexpr int kDt = kDaRows * kPitch * 2;
+  constexpr int kSum = kDaWaves * NR * 4 * kDaCols * 4;  // one element i of every wave at a time
   __shared__ __attribute__((aligned(16))) uint8_t lds[kDt > kSum ? kDt : kSum];
   bf16* dts = reinterpret_cast<bf16*>(lds);
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int li = lane & 15, g = lane >> 4;
-  const int col = blockIdx.x * 256 + 16 * li;
-  const int grp = min(col / kGroup, p.G - 1);
-  const bool in = col < kGroup * p.G;  // the codes' rows are padded to whole groups
+  // The codes' rows are padded to whole groups; channels past them read the last.
+  const int col = min(blockIdx.x * kDaCols + 8 * li, kGroup * p.G - 8);
+  const int grp = col / kGroup;
   const int64_t begin = (int64_t)blockIdx.y * p.rows, end = min(p.M, begin + p.rows);
-  f32x4v acc[16][NR];
+  f32x4v acc[8][NR];
 #pragma unroll
-  for (int j = 0; j < 16; ++j)
+  for (int j = 0; j < 8; ++j)
 #pragma unroll
     for (int n = 0; n < NR; ++n) acc[j][n] = f32x4v{0.f, 0.f, 0.f, 0.f};
+
+  constexpr int kPieces = kDaRows * 4 * NR / kDaThreads;  // 8-byte pieces of dt per thread
+  const uint32_t pitch = kGroup * p.G;
+  struct Turn {
+    u32x2 c[8];  // codes of this lane's 8 rows
+    u32x2 ex;    // their groups' exponents
+    u32x2 dt[kPieces];
+  } cur, next;
+  auto load = [&](Turn& t, int64_t r0) {
+    // Addresses: a uniform row base and 32-bit offsets in the turn's 128 rows.
+    const uint8_t* codes = p.codes + r0 * pitch;
+    const bf16* dt = p.dt + r0 * p.R;
+    const int last = (int)min<int64_t>(end - r0, kDaRows) - 1;
+    const int mine = 32 * wave + 8 * g;  // this lane's 8 rows
+    // Every load is in bounds and made: rows past the range re-read its last, and
+    // count nothing below; channels and ranks past theirs are not written.
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      t.c[e] = *reinterpret_cast<const u32x2*>(codes + ((uint32_t)min(mine + e, last) * pitch + (uint32_t)col));
+    t.ex = *reinterpret_cast<const u32x2*>(p.exps + (int64_t)grp * p.Mp + r0 + min(mine, last & ~7));
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int o = tid + kDaThreads * i, r = o / (4 * NR), rank = min(4 * (o % (4 * NR)), p.R - 4);
+      t.dt[i] = *reinterpret_cast<const u32x2*>(dt + (uint32_t)(min(r, last) * p.R + rank));
+    }
+    if (last < kDaRows - 1) {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i)
+        if ((tid + kDaThreads * i) / (4 * NR) > last) t.dt[i] = u32x2{0, 0};
+    }
+  };
+  if (begin < end) load(cur, begin);
   for (int64_t r0 = begin; r0 < end; r0 += kDaRows) {
-    const int64_t mine = r0 + 32 * wave + 8 * g;  // this lane's 8 rows
-    u32x4 c[8];
-    uint32_t ex[2] = {0, 0};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      c[e] = u32x4{0, 0, 0, 0};
-      if (in && mine + e < end) c[e] = ld16(p.codes + (mine + e) * (kGroup * p.G) + col);
-    }
-    if (mine < end) {
-      const u32x2 v = *reinterpret_cast<const u32x2*>(p.exps + (int64_t)grp * p.Mp + mine);
-      ex[0] = v[0];
-      ex[1] = v[1];
-    }
     __syncthreads();  // the turn before has read its dt
-    for (int o = tid; o < kDaRows * 2 * NR; o += kDaThreads) {
-      const int r = o / (2 * NR), rank = 8 * (o % (2 * NR));
-      u32x4 v = u32x4{0, 0, 0, 0};
-      if (r0 + r < end && rank < p.R) v = ld16(p.dt + (r0 + r) * p.R + rank);
-      const bf16x8 b = __builtin_bit_cast(bf16x8, v);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) dts[(rank + e) * kDaPitch + r] = b[e];
+    for (int i = 0; i < kPieces; ++i) {
+      const int o = tid + kDaThreads * i, r = o / (4 * NR), rank = 4 * (o % (4 * NR));
+      *reinterpret_cast<u32x2*>(dts + r * kPitch + rank) = cur.dt[i];
     }
     __syncthreads();
+    if (r0 + kDaRows < end) load(next, r0 + kDaRows);
+    // Lanes 4 r + q of a group of 16 give the piece of four ranks at 4 q of row
+    // 8 g + r (+ 4 for the second read); lane li receives rank li of four rows.
+    const bf16* piece = dts + (32 * wave + 8 * g + (li >> 2)) * kPitch + 4 * (li & 3);
+    bf16x8 d[NR];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      const s16x4 lo = ds_read_tr(piece + 16 * n);
+      const s16x4 hi = ds_read_tr(piece + 4 * kPitch + 16 * n);
+      d[n] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
     float step[8];
+    const int64_t left = end - r0 - (32 * wave + 8 * g);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       // Rows past the range count nothing, whatever their group's mark.
-      step[e] = mine + e < end ? step_of((ex[e >> 2] >> (8 * (e & 3))) & 255u) : 0.f;
+      step[e] = e < left ? step_of((cur.ex[e >> 2] >> (8 * (e & 3))) & 255u) : 0.f;
     }
-    bf16x8 d[NR];
-#pragma unroll
-    for (int n = 0; n < NR; ++n)
-      d[n] = *reinterpret_cast<const bf16x8*>(dts + (16 * n + li) * kDaPitch + 32 * wave + 8 * g);
-    static_for<0, 16>([&](auto J) {
+    static_for<0, 8>([&](auto J) {
       constexpr int j = decltype(J)::value;
       u32x4 v;
       static_for<0, 4>([&](auto E) {
         constexpr int e = 2 * decltype(E)::value;
-        v[e / 2] = pack_bf16(byte_f<j & 3>(c[e][j >> 2]) * step[e], byte_f<j & 3>(c[e + 1][j >> 2]) * step[e + 1]);
+        v[e / 2] = pack_bf16(kept_value<j & 3>(cur.c[e][j >> 2] ^ 0x80808080u, step[e], -128.0f * step[e]),
+                             kept_value<j & 3>(cur.c[e + 1][j >> 2] ^ 0x80808080u, step[e + 1], -128.0f * step[e + 1]));
       });
       const bf16x8 xv = __builtin_bit_cast(bf16x8, v);
 #pragma unroll
       for (int n = 0; n < NR; ++n) acc[j][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(d[n], xv, acc[j][n], 0, 0, 0);
     });
+    cur = next;
   }
-  // acc[j][n]: lane li is channel 16 li + j, element i is rank 16 n + 4 g + i.
-  // Added over the waves one element i at a time: sums[wave][n][g][256 channels].
+  // acc[j][n]: lane li is channel 8 li + j, element i is rank 16 n + 4 g + i.
+  // Added over the waves one element i at a time: sums[wave][n][g][channel].
   float* sums = reinterpret_cast<float*>(lds);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -428,19 +538,20 @@ __global__ __launch_bounds__(kDaThreads) void lora8_da_kernel(LoraDa p) {
 #pragma unroll
     for (int n = 0; n < NR; ++n)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<f32x4v*>(sums + ((wave * NR + n) * 4 + g) * 256 + 16 * li + 4 * q) =
+      for (int q = 0; q < 2; ++q)
+        *reinterpret_cast<f32x4v*>(sums + ((wave * NR + n) * 4 + g) * kDaCols + 8 * li + 4 * q) =
             f32x4v{acc[4 * q][n][i], acc[4 * q + 1][n][i], acc[4 * q + 2][n][i], acc[4 * q + 3][n][i]};
     __syncthreads();
-    const int k = blockIdx.x * 256 + tid;
+    const int at = tid & (kDaCols - 1), k = blockIdx.x * kDaCols + at;
     if (k < p.K) {
 #pragma unroll
-      for (int m = 0; m < NR * 4; ++m) {
-        const int rank = 16 * (m >> 2) + 4 * (m & 3) + i;
+      for (int m0 = 0; m0 < NR * 4; m0 += 2) {
+        const int m = m0 + (tid >> 7);  // rank 16 n + 4 g + i with m = 4 n + g
+        const int rank = 4 * m + i;
         if (rank >= p.R) continue;
         float s = 0.f;
 #pragma unroll
-        for (int w = 0; w < kDaWaves; ++w) s += sums[(w * NR * 4 + m) * 256 + tid];
+        for (int w = 0; w < kDaWaves; ++w) s += sums[(w * NR * 4 + m) * kDaCols + at];
         if (p.splits == 1) p.da[(int64_t)rank * p.K + k] = (bf16)s;
         else p.part[((int64_t)blockIdx.y * p.R + rank) * p.K + k] = s;
       }
@@ -448,23 +559,25 @@ __global__ __launch_bounds__(kDaThreads) void lora8_da_kernel(LoraDa p) {
   }
 }
 
-// Adds the ranges' partial sums in order, eight values per lane.
-__global__ __launch_bounds__(64) void lora8_da_sum_kernel(const float* part, bf16* da, int64_t n, int splits) {
+// Adds the ranges' partial sums of t or dA in order, four values per lane.
+__global__ __launch_bounds__(64) void lora8_sum_kernel(const float* part, bf16* out, int64_t n, int splits) {
   const int64_t at = ((int64_t)blockIdx.x * 64 + threadIdx.x) * 4;
-  if (at >= n) return;  // n = R K is a multiple of 64
+  if (at >= n) return;  // n, R times K or M, is a multiple of 8
   f32x4v s = f32x4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
   for (int i = 0; i < splits; ++i) s += *reinterpret_cast<const f32x4v*>(part + i * n + at);
-  *reinterpret_cast<u32x2*>(da + at) = u32x2{pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3])};
+  *reinterpret_cast<u32x2*>(out + at) = u32x2{pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3])};
 }
 
-// Ranges of rows of the dA product: enough workgroups for the device, but at
+// Ranges of rows of the dA product: one round of the workgroups that fit on the
+// CUs (registers: 4, 3, 2 and 1 a CU for ranks up to 16, 32, 48 and 64), but at
 // least 256 rows each (a partial sum is 4 R bytes a channel, 256 rows' codes
-// are 256).
-static int da_splits(int64_t M, int64_t K) {
+// are 256). With one and a half rounds 7904 x 8192 at rank 40 took 32 us, with
+// one XX.
+static int da_splits(int64_t M, int64_t K, int64_t R) {
   const int64_t cus = std::max(1, device_cu_count());
-  const int64_t tiles = (K + 255) / 256;
-  const int64_t want = (2 * cus + tiles - 1) / tiles;
+  const int64_t tiles = (K + kDaCols - 1) / kDaCols;
+  const int64_t want = std::max<int64_t>(1, (5 - (R + 15) / 16) * cus / tiles);
   return (int)std::clamp<int64_t>(std::min(want, (M + 255) / 256), 1, 65535);
 }
 
@@ -502,9 +615,9 @@ extern "C" int aa_gelu8_fwd(const void* x, void* y, void* codes, void* exps, int
   p.codes = (uint8_t*)codes;
   p.exps = (uint8_t*)exps;
   p.K = (int)K;
-  p.upr = 2 * (int)((K + kGroup - 1) / kGroup);
-  p.units = rows * p.upr;
-  const int64_t blocks = (p.units + kGeThreads - 1) / kGeThreads;
+  p.cpr = 4 * (int)((K + kGroup - 1) / kGroup);
+  p.chunks = rows * p.cpr;
+  const int64_t blocks = (p.chunks + kGeThreads * kGeChunks - 1) / (kGeThreads * kGeChunks);
   if (blocks > 0x7fffffff) return fail(AA_EUNSUPPORTED, "gelu8: too many values");
   hipStream_t st = (hipStream_t)stream;
   if (K % kGroup == 0) gelu8_fwd_kernel<true><<<dim3((unsigned)blocks), kGeThreads, 0, st>>>(p);
@@ -526,9 +639,9 @@ extern "C" int aa_gelu8_bwd(const void* dy, const void* codes, const void* exps,
   p.exps = (const uint8_t*)exps;
   p.dx = (bf16*)dx;
   p.K = (int)K;
-  p.upr = 2 * (int)((K + kGroup - 1) / kGroup);
-  p.units = rows * p.upr;
-  const int64_t blocks = (p.units + kGeThreads - 1) / kGeThreads;
+  p.cpr = 4 * (int)((K + kGroup - 1) / kGroup);
+  p.chunks = rows * p.cpr;
+  const int64_t blocks = (p.chunks + kGeThreads * kGeChunks - 1) / (kGeThreads * kGeChunks);
   if (blocks > 0x7fffffff) return fail(AA_EUNSUPPORTED, "gelu8_bwd: too many values");
   hipStream_t st = (hipStream_t)stream;
   if (K % kGroup == 0) gelu8_bwd_kernel<true><<<dim3((unsigned)blocks), kGeThreads, 0, st>>>(p);
@@ -536,29 +649,29 @@ extern "C" int aa_gelu8_bwd(const void* dy, const void* codes, const void* exps,
   return check_launch("gelu8_bwd");
 }
 
-template <int RT>
-static void launch_lora_fwd(dim3 grid, hipStream_t st, const LoraFwd& p) {
-  if (p.R <= 16) lora8_fwd_kernel<1, RT><<<grid, kLoThreads, 0, st>>>(p);
-  else if (p.R <= 32) lora8_fwd_kernel<2, RT><<<grid, kLoThreads, 0, st>>>(p);
-  else if constexpr (RT == 1) {
-    if (p.R <= 48) lora8_fwd_kernel<3, RT><<<grid, kLoThreads, 0, st>>>(p);
-    else lora8_fwd_kernel<4, RT><<<grid, kLoThreads, 0, st>>>(p);
-  }
+extern "C" size_t aa_lora8_fwd_workspace(int64_t M, int64_t K, int64_t R) {
+  if (M <= 0 || K <= 0 || R <= 0) return 0;
+  const int64_t splits = lora_splits(K, R);
+  return splits == 1 ? 0 : (size_t)(splits * M * R) * sizeof(float);
 }
 
-extern "C" int aa_lora8_fwd(const void* x, const void* a, void* t, void* codes, void* exps, int64_t M,
-                            int64_t K, int64_t R, int dtype, void* stream) {
+extern "C" int aa_lora8_fwd(const void* x, const void* a, void* t, void* codes, void* exps,
+                            void* workspace, size_t workspace_bytes, int64_t M, int64_t K, int64_t R,
+                            int dtype, void* stream) {
   clear_error();
   if (int rc = check_rows("lora8", M, K, dtype)) return rc;
   if (int rc = check_rank("lora8", R)) return rc;
   if (M == 0) return AA_OK;
   if (!x || !a || !t || (codes && !exps)) return fail(AA_EINVAL, "lora8: null pointer");
-  if (!aligned16(x) || !aligned16(a) || !aligned16(t) || !aligned16(codes) || !aligned16(exps))
-    return fail(AA_EINVAL, "lora8: pointers must be 16-byte aligned");
+  for (const void* q : {x, a, (const void*)t, (const void*)codes, (const void*)exps, (const void*)workspace})
+    if (!aligned16(q)) return fail(AA_EINVAL, "lora8: pointers must be 16-byte aligned");
+  const size_t need = aa_lora8_fwd_workspace(M, K, R);
+  if (need && (!workspace || workspace_bytes < need)) return fail(AA_EINVAL, "lora8: workspace too small");
   LoraFwd p;
   p.x = (const bf16*)x;
   p.a = (const bf16*)a;
   p.t = (bf16*)t;
+  p.part = (float*)workspace;
   p.codes = (uint8_t*)codes;
   p.exps = (uint8_t*)exps;
   p.M = M;
@@ -566,16 +679,27 @@ extern "C" int aa_lora8_fwd(const void* x, const void* a, void* t, void* codes, 
   p.K = (int)K;
   p.R = (int)R;
   p.G = (int)((K + kGroup - 1) / kGroup);
+  p.splits = lora_splits(K, R);
+  // One workgroup a CU (16 waves, 128 KiB of LDS), each with its share of the tiles.
   const int64_t cus = std::max(1, device_cu_count());
+  const int64_t tiles = p.Mp / 16, groups = std::clamp<int64_t>(cus / p.splits, 1, tiles);
+  p.tiles = (int)((tiles + groups - 1) / groups);
   hipStream_t st = (hipStream_t)stream;
-  if (M >= 32 * cus && R <= 32) launch_lora_fwd<2>(dim3((unsigned)((M + 31) / 32)), st, p);
-  else launch_lora_fwd<1>(dim3((unsigned)((M + 15) / 16)), st, p);
+  const dim3 grid((unsigned)((tiles + p.tiles - 1) / p.tiles), (unsigned)p.splits);
+  if (R <= 16) lora8_fwd_kernel<1><<<grid, 64 * lora_waves(16 * 1), 0, st>>>(p);
+  else if (R <= 32) lora8_fwd_kernel<2><<<grid, 64 * lora_waves(16 * 2), 0, st>>>(p);
+  else if (R <= 48) lora8_fwd_kernel<3><<<grid, 64 * lora_waves(16 * 3), 0, st>>>(p);
+  else lora8_fwd_kernel<4><<<grid, 64 * lora_waves(16 * 4), 0, st>>>(p);
+  if (int rc = check_launch("lora8")) return rc;
+  if (p.splits == 1) return AA_OK;
+  const int64_t n = M * R;
+  lora8_sum_kernel<<<dim3((unsigned)((n / 4 + 63) / 64)), 64, 0, st>>>(p.part, p.t, n, p.splits);
   return check_launch("lora8");
 }
 
 extern "C" size_t aa_lora8_bwd_workspace(int64_t M, int64_t K, int64_t R) {
   if (M <= 0 || K <= 0 || R <= 0) return 0;
-  const int64_t splits = da_splits(M, K);
+  const int64_t splits = da_splits(M, K, R);
   return splits == 1 ? 0 : (size_t)(splits * R * K) * sizeof(float);
 }
 
@@ -602,8 +726,10 @@ extern "C" int aa_lora8_bwd(const void* dt, const void* a, const void* codes, co
     p.K = (int)K;
     p.R = (int)R;
     const int64_t tiles = (K + 127) / 128;
+    // Two to four workgroups a CU, each with at least 128 rows to spend the
+    // reading of its part of A on.
     const int64_t per = (M * tiles + 4 * cus - 1) / (4 * cus);
-    p.rows = (int)((std::clamp<int64_t>(per, std::max<int64_t>(64, (M + 65534) / 65535), 1 << 20) + 63) / 64 * 64);
+    p.rows = (int)((std::clamp<int64_t>(per, std::max<int64_t>(128, (M + 65534) / 65535), 1 << 20) + 63) / 64 * 64);
     const dim3 grid((unsigned)tiles, (unsigned)((M + p.rows - 1) / p.rows));
     if (R <= 32) lora8_dx_kernel<1><<<grid, 256, 0, st>>>(p);
     else lora8_dx_kernel<2><<<grid, 256, 0, st>>>(p);
@@ -621,10 +747,10 @@ extern "C" int aa_lora8_bwd(const void* dt, const void* a, const void* codes, co
   p.K = (int)K;
   p.R = (int)R;
   p.G = (int)((K + kGroup - 1) / kGroup);
-  p.splits = da_splits(M, K);
+  p.splits = da_splits(M, K, R);
   // Ranges of whole turns' rows; the last ones may be empty and write zeros.
   p.rows = (int)(((M + p.splits - 1) / p.splits + kDaRows - 1) / kDaRows * kDaRows);
-  const dim3 grid((unsigned)((K + 255) / 256), (unsigned)p.splits);
+  const dim3 grid((unsigned)((K + kDaCols - 1) / kDaCols), (unsigned)p.splits);
   if (R <= 16) lora8_da_kernel<1><<<grid, kDaThreads, 0, st>>>(p);
   else if (R <= 32) lora8_da_kernel<2><<<grid, kDaThreads, 0, st>>>(p);
   else if (R <= 48) lora8_da_kernel<3><<<grid, kDaThreads, 0, st>>>(p);
@@ -632,6 +758,6 @@ extern "C" int aa_lora8_bwd(const void* dt, const void* a, const void* codes, co
   if (int rc = check_launch("lora8_bwd")) return rc;
   if (p.splits == 1) return AA_OK;
   const int64_t n = R * K;
-  lora8_da_sum_kernel<<<dim3((unsigned)((n / 4 + 63) / 64)), 64, 0, st>>>(p.part, p.da, n, p.splits);
+  lora8_sum_kernel<<<dim3((unsigned)((n / 4 + 63) / 64)), 64, 0, st>>>(p.part, p.da, n, p.splits);
   return check_launch("lora8_bwd");
 }

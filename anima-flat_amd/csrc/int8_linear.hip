@@ -52,19 +52,19 @@ __global__ __launch_bounds__(kQ8Threads) void rowquant_int8_kernel(const bf16* _
       for (int w = 0; w < U / 8; ++w) raw[p][w] = ld16(xr + U * (lane + 64 * p) + 8 * w);
     }
   float v[NU][U];
-  uint32_t top = 0;
+  float top = 0.f;
 #pragma unroll
   for (int p = 0; p < NU; ++p)
     if (lane + 64 * p < nunit) {
 #pragma unroll
       for (int w = 0; w < U / 8; ++w) unpack8(raw[p][w], &v[p][8 * w]);
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
+      for (int i = 0; i < U; ++i)
         if constexpr (kGelu) v[p][i] = gelu(v[p][i]);
-        top = max(top, mag_bits(v[p][i]));
-      }
+#pragma unroll
+      for (int i = 0; i < U; i += 2) top = max3abs_nan(top, v[p][i], v[p][i + 1]);
     }
-  const RowScale rs = row_scale(wave_umax(top));
+  const RowScale rs = row_scale(wave_umax(mag_bits(top)));
 #pragma unroll
   for (int p = 0; p < NU; ++p)
     if (lane + 64 * p < nunit) {
@@ -72,7 +72,7 @@ __global__ __launch_bounds__(kQ8Threads) void rowquant_int8_kernel(const bf16* _
       const u32x2 a = int8_codes8(&v[p][0], rs);
       if constexpr (U == 16) {
         const u32x2 b = int8_codes8(&v[p][8], rs);
-        st16(to, u32x4{a[0], a[1], b[0], b[1]});
+        st16_nt(to, u32x4{a[0], a[1], b[0], b[1]});
       } else {
         *reinterpret_cast<u32x2*>(to) = a;
       }
@@ -289,7 +289,7 @@ __global__ __launch_bounds__(T::kThreads) void int8_linear_kernel(I8Params p) {
     if (col < ncols) {
       bf16* out = p.y + row0 * p.N + nt * T::kNT + col;
       for (int r = grp; r < nrows; r += T::kThreads / 16)
-        st16(out + (int64_t)r * p.N, *reinterpret_cast<const u32x4*>(lds + r * 256 + ((j ^ (r & 15)) * 16)));
+        st16_nt(out + (int64_t)r * p.N, *reinterpret_cast<const u32x4*>(lds + r * 256 + ((j ^ (r & 15)) * 16)));
     }
   }
 }

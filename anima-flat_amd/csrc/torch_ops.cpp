@@ -641,8 +641,12 @@ T3 lora_down8(const Tensor& x, const Tensor& a, bool keep) {
     const int64_t rows = x.size(0) * x.size(1), K = x.size(2), R = a.size(0);
     Tensor t = at::empty({x.size(0), x.size(1), R}, x.options()), codes, exps;
     kept(x, keep, (K + 31) / 32, (rows + 15) / 16 * 16, &codes, &exps);
+    const size_t bytes = aa_lora8_fwd_workspace(rows, K, R);
+    Tensor ws;
+    if (bytes) ws = at::empty({(int64_t)bytes / 4}, x.options().dtype(at::kFloat));
     if (launched(aa_lora8_fwd(x.data_ptr(), a.data_ptr(), t.data_ptr(), keep ? codes.data_ptr() : nullptr,
-                              keep ? exps.data_ptr() : nullptr, rows, K, R, AA_DTYPE_BF16, stream_of(x)),
+                              keep ? exps.data_ptr() : nullptr, bytes ? ws.data_ptr() : nullptr, bytes, rows, K, R,
+                              AA_DTYPE_BF16, stream_of(x)),
                  "lora_down8"))
       return {t, codes, exps};
   }

@@ -37,9 +37,47 @@ def _mod_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else 0
 
 
+def _check_arguments(x, y, gate, scale, shift, weight) -> None:
+    tensors = [t for t in (x, y, gate, scale, shift, weight) if t is not None]
+    if not x.is_meta:
+        _check(*tensors)
+    if any(t.device != x.device for t in tensors):
+        raise ValueError("all tensors must be on one device")
+    if x.ndim != 3 or x.shape[2] == 0:
+        raise ValueError("x must be [B, S, D]")
+    B, _, D = x.shape
+    if D % 8 or D > MAX_D:
+        raise ValueError(f"D must be a multiple of 8 and at most {MAX_D}")
+    if y is not None and y.shape != x.shape:
+        raise ValueError("y must have x's shape")
+    if any(t is not None and t.dtype != torch.bfloat16 for t in (x, y)):
+        raise ValueError("unsupported dtype of x or y: only bfloat16 is implemented")
+    for name, t in (("gate", gate), ("scale", scale), ("shift", shift)):
+        if t is None:
+            continue
+        if t.ndim != 2 or t.shape[1] != D or t.shape[0] not in (1, B):
+            raise ValueError(f"{name} must be [B, D], [B, 1, D], [1, D] or [D]")
+        if t.dtype not in (torch.bfloat16, torch.float32) or t.dtype != scale.dtype:
+            raise ValueError(f"{name} must be bfloat16 or float32, as the other modulations")
+    if weight is not None and (weight.shape != x.shape[2:] or weight.dtype not in (torch.bfloat16, torch.float32)):
+        raise ValueError("weight must be [D], bfloat16 or float32")
+
+
+def _readable(t: torch.Tensor | None) -> torch.Tensor | None:
+    """Modulation rows that the kernels read in place, or a copy."""
+    if t is None:
+        return None
+    unit = 16 // t.element_size()
+    if t.stride(1) != 1 or (t.shape[0] > 1 and (t.stride(0) % unit or t.stride(0) < t.shape[1])):
+        t = t.contiguous()
+    return aligned(t)
+
+
 def _forward(x, y, gate, scale, shift, weight, eps, branch_scale, want_stats, int8):
+    _check_arguments(x, y, gate, scale, shift, weight)
     B, S, D = x.shape
-    x, y, gate, scale, shift = (None if t is None else aligned(t) for t in (x, y, gate, scale, shift))
+    x, y = (None if t is None else aligned(t.contiguous()) for t in (x, y))
+    gate, scale, shift = (_readable(t) for t in (gate, scale, shift))
     r = torch.empty_like(x) if y is not None else None
     h = q = qs = None
     if int8:
@@ -64,8 +102,8 @@ def _forward(x, y, gate, scale, shift, weight, eps, branch_scale, want_stats, in
 def _backward(dr, dh, x, y, gate, scale, weight, stats, shift_rows, branch_scale, mods):
     """(dx, dy, dgate, dscale, dshift, dweight); what is not computed has no elements."""
     B, S, D = x.shape
-    dr, dh = (None if t is None else aligned(t.contiguous()) for t in (dr, dh))
-    x, y, gate, scale = (None if t is None else aligned(t) for t in (x, y, gate, scale))
+    dr, dh, x, y = (None if t is None else aligned(t.contiguous()) for t in (dr, dh, x, y))
+    gate, scale = _readable(gate), _readable(scale)
     dx = torch.empty_like(x)
     dy = torch.empty_like(x) if y is not None else x.new_empty(0)
     dgate, dscale, dshift, dweight = (x.new_empty(0) for _ in range(4))
@@ -116,8 +154,9 @@ def _residual_adaln(
 
 @_residual_adaln.register_fake
 def _(x, y, gate, scale, shift, weight, eps, branch_scale, want_stats):
+    _check_arguments(x, y, gate, scale, shift, weight)
     rows = x.shape[0] * x.shape[1] if want_stats else 0
-    return torch.empty_like(x), torch.empty_like(x), x.new_empty((rows, 4), dtype=torch.float32)
+    return x.new_empty(x.shape), x.new_empty(x.shape), x.new_empty((rows, 4), dtype=torch.float32)
 
 
 @custom_op("anima_flat_amd::adaln", mutates_args=())
@@ -130,8 +169,9 @@ def _adaln(
 
 @_adaln.register_fake
 def _(x, scale, shift, eps, want_stats):
+    _check_arguments(x, None, None, scale, shift, None)
     rows = x.shape[0] * x.shape[1] if want_stats else 0
-    return torch.empty_like(x), x.new_empty((rows, 4), dtype=torch.float32)
+    return x.new_empty(x.shape), x.new_empty((rows, 4), dtype=torch.float32)
 
 
 @custom_op("anima_flat_amd::residual_adaln_int8", mutates_args=())
@@ -145,8 +185,9 @@ def _residual_adaln_int8(
 
 @_residual_adaln_int8.register_fake
 def _(x, y, gate, scale, shift, weight, eps, branch_scale):
+    _check_arguments(x, y, gate, scale, shift, weight)
     rows = x.shape[0] * x.shape[1]
-    return torch.empty_like(x), torch.empty_like(x, dtype=torch.int8), x.new_empty((rows, 1), dtype=torch.float32)
+    return x.new_empty(x.shape), x.new_empty(x.shape, dtype=torch.int8), x.new_empty((rows, 1), dtype=torch.float32)
 
 
 @custom_op("anima_flat_amd::adaln_bwd", mutates_args=())
@@ -162,8 +203,8 @@ def _adaln_bwd(
 def _(dr, dh, x, y, gate, scale, weight, stats, shift_rows, branch_scale, mods):
     D = x.shape[2]
     return (
-        torch.empty_like(x),
-        torch.empty_like(x) if y is not None else x.new_empty(0),
+        x.new_empty(x.shape),
+        x.new_empty(x.shape) if y is not None else x.new_empty(0),
         gate.new_empty(gate.shape) if mods and y is not None else x.new_empty(0),
         scale.new_empty(scale.shape) if mods else x.new_empty(0),
         scale.new_empty((shift_rows, D)) if mods else x.new_empty(0),
@@ -223,50 +264,26 @@ torch.library.register_autograd("anima_flat_amd::adaln", _adaln_backward, setup_
 
 
 # -------------------------------------------------------------- public API --
+#
+# Checks are made once: by the native kernels, which hand what they do not take to the ops'
+# Python functions, and by these and the fakes through _check_arguments.
 
 
-def _rows(t: torch.Tensor, x: torch.Tensor, name: str) -> torch.Tensor:
-    """A modulation as [1 or B, D] rows with unit stride that the kernel can read."""
-    B, _, D = x.shape
+def _rows2(t: torch.Tensor) -> torch.Tensor:
+    """A modulation `[B, 1, D]` or `[D]` as rows; anything else as it is, for the checks."""
     if t.ndim == 3 and t.shape[1] == 1:
-        t = t[:, 0]
-    if t.ndim == 1:
-        t = t[None]
-    if t.ndim != 2 or t.shape[1] != D or t.shape[0] not in (1, B):
-        raise ValueError(f"{name} must be [B, D], [B, 1, D], [1, D] or [D]")
-    if t.dtype not in (torch.bfloat16, torch.float32):
-        raise ValueError(f"{name} must be bfloat16 or float32")
-    unit = 16 // t.element_size()
-    if t.stride(1) != 1 or (t.shape[0] > 1 and (t.stride(0) % unit or t.stride(0) < D)):
-        t = t.contiguous()
-    return t
+        return t[:, 0]
+    return t[None] if t.ndim == 1 else t
 
 
-def _tokens(x: torch.Tensor, name: str) -> torch.Tensor:
-    if x.ndim != 3 or x.shape[2] == 0:
-        raise ValueError(f"{name} must be [B, S, D]")
-    if x.dtype != torch.bfloat16:
-        raise ValueError(f"unsupported dtype {x.dtype}: only bfloat16 is implemented")
-    if x.shape[2] % 8 or x.shape[2] > MAX_D:
-        raise ValueError(f"D must be a multiple of 8 and at most {MAX_D}")
-    return x.contiguous()
-
-
-def _arguments(x, y, gate, scale, shift, weight):
-    tensors = [t for t in (x, y, gate, scale, shift, weight) if t is not None]
-    _check(*tensors)
-    if any(t.device != x.device for t in tensors):
-        raise ValueError("all tensors must be on one device")
-    if y is not None and y.shape != x.shape:
-        raise ValueError("y must have x's shape")
-    if weight is not None and (weight.shape != x.shape[2:] or weight.dtype not in (torch.bfloat16, torch.float32)):
-        raise ValueError("weight must be [D], bfloat16 or float32")
-    x = _tokens(x, "x")
-    y = None if y is None else _tokens(y, "y")
-    mods = [None if t is None else _rows(t, x, n) for t, n in ((gate, "gate"), (scale, "scale"), (shift, "shift"))]
-    if len({t.dtype for t in mods if t is not None}) > 1:
-        mods = [None if t is None else t.float() for t in mods]
-    return x, y, *mods, None if weight is None else weight.contiguous()
+def _modulation(*mods: torch.Tensor) -> list[torch.Tensor]:
+    """Modulations as rows of one dtype."""
+    mods = [t if t.ndim == 2 else _rows2(t) for t in mods]
+    if any(t.dtype != mods[0].dtype for t in mods):
+        if any(t.dtype not in (torch.bfloat16, torch.float32) for t in mods):
+            raise ValueError("gate, scale and shift must be bfloat16 or float32")
+        mods = [t.float() for t in mods]
+    return mods
 
 
 def _wants_grad(*ts) -> bool:
@@ -294,7 +311,7 @@ def residual_adaln(x, y, gate, scale, shift, weight=None, eps=1e-6, branch_scale
     Raises:
         ValueError: If a tensor is not on CUDA, or its shape or dtype is not supported.
     """
-    x, y, gate, scale, shift, weight = _arguments(x, y, gate, scale, shift, weight)
+    gate, scale, shift = _modulation(gate, scale, shift)
     stats = _wants_grad(x, y, gate, scale, shift, weight)
     r, h, _ = _residual_adaln(x, y, gate, scale, shift, weight, eps, branch_scale, stats)
     return r, h
@@ -302,7 +319,7 @@ def residual_adaln(x, y, gate, scale, shift, weight=None, eps=1e-6, branch_scale
 
 def adaln(x, scale, shift, eps=1e-6):
     """`LayerNorm(x) * (1 + scale) + shift`, arguments as for `residual_adaln`."""
-    x, _, _, scale, shift, _ = _arguments(x, None, None, scale, shift, None)
+    scale, shift = _modulation(scale, shift)
     return _adaln(x, scale, shift, eps, _wants_grad(x, scale, shift))[0]
 
 
@@ -314,7 +331,7 @@ def residual_adaln_int8(x, y, gate, scale, shift, weight=None, eps=1e-6, branch_
         `h ~ q * s`, rounded from the fp32 h. A token with a value that is not finite has
         the scale NaN.
     """
-    x, y, gate, scale, shift, weight = _arguments(x, y, gate, scale, shift, weight)
+    gate, scale, shift = _modulation(gate, scale, shift)
     if _wants_grad(x, y, gate, scale, shift, weight):
         raise RuntimeError("residual_adaln_int8 has no backward: use residual_adaln for training")
     return _residual_adaln_int8(x, y, gate, scale, shift, weight, eps, branch_scale)

@@ -26,6 +26,31 @@ MAX_RANK = 64
 MAX_K = 65536
 
 
+# Checks are made once: by the native kernels, which hand what they do not take to the ops'
+# Python functions, and by these and the fakes through _check_tokens and _check_adapter.
+
+
+def _check_tokens(x: torch.Tensor) -> None:
+    if not x.is_meta:
+        _check(x)
+    if x.ndim != 3 or x.shape[2] == 0:
+        raise ValueError("x must be [B, S, K]")
+    if x.dtype != torch.bfloat16:
+        raise ValueError(f"unsupported dtype {x.dtype}: only bfloat16 is implemented")
+    if x.shape[2] % 8 or x.shape[2] > MAX_K:
+        raise ValueError(f"K must be a multiple of 8 and at most {MAX_K}")
+
+
+def _check_adapter(x: torch.Tensor, a: torch.Tensor) -> None:
+    if not x.is_meta:
+        _check(x, a)
+    _check_tokens(x)
+    if a.ndim != 2 or a.shape[1] != x.shape[2] or a.dtype != x.dtype or a.device != x.device:
+        raise ValueError("a must be [R, K] of x's dtype and device")
+    if a.shape[0] % 8 or not 0 < a.shape[0] <= MAX_RANK:
+        raise ValueError(f"the rank must be a multiple of 8 and at most {MAX_RANK}")
+
+
 def _groups(K: int) -> int:
     return -(-K // GROUP)
 
@@ -46,8 +71,9 @@ def _ptr(t: torch.Tensor):
 
 @custom_op("anima_flat_amd::gelu8", mutates_args=())
 def _gelu8(x: torch.Tensor, keep: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    _check_tokens(x)
     B, S, K = x.shape
-    x = aligned(x)
+    x = aligned(x.contiguous())
     y = torch.empty_like(x)
     codes, exps = _kept(x, keep, (B * S, _groups(K)))
     with torch.cuda.device(x.device):
@@ -62,8 +88,9 @@ def _gelu8(x: torch.Tensor, keep: bool) -> tuple[torch.Tensor, torch.Tensor, tor
 
 @_gelu8.register_fake
 def _(x, keep):
+    _check_tokens(x)
     B, S, K = x.shape
-    return torch.empty_like(x), *_kept(x, keep, (B * S, _groups(K)))
+    return x.new_empty(x.shape), *_kept(x, keep, (B * S, _groups(K)))
 
 
 @custom_op("anima_flat_amd::gelu8_bwd", mutates_args=())
@@ -107,15 +134,19 @@ torch.library.register_autograd("anima_flat_amd::gelu8", _gelu8_backward, setup_
 
 @custom_op("anima_flat_amd::lora_down8", mutates_args=())
 def _lora_down8(x: torch.Tensor, a: torch.Tensor, keep: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    _check_adapter(x, a)
     B, S, K = x.shape
     R = a.shape[0]
-    x, a = aligned(x), aligned(a)
+    x, a = aligned(x.contiguous()), aligned(a.contiguous())
     t = x.new_empty((B, S, R))
     codes, exps = _kept(x, keep, (_groups(K), -(-B * S // 16) * 16))
     with torch.cuda.device(x.device):
+        ws_bytes = _lib.lib().aa_lora8_fwd_workspace(B * S, K, R)
+        ws = torch.empty(ws_bytes // 4, dtype=torch.float32, device=x.device) if ws_bytes else None
         _lib.check(
             _lib.lib().aa_lora8_fwd(
-                _ptr(x), _ptr(a), _ptr(t), _ptr(codes), _ptr(exps), B * S, K, R, _lib.dtype_code(x), _lib.stream(x)
+                _ptr(x), _ptr(a), _ptr(t), _ptr(codes), _ptr(exps), _lib.ptr(ws), ws_bytes, B * S, K, R,
+                _lib.dtype_code(x), _lib.stream(x),
             ),
             "lora_down8",
         )
@@ -124,6 +155,7 @@ def _lora_down8(x: torch.Tensor, a: torch.Tensor, keep: bool) -> tuple[torch.Ten
 
 @_lora_down8.register_fake
 def _(x, a, keep):
+    _check_adapter(x, a)
     B, S, K = x.shape
     return x.new_empty((B, S, a.shape[0])), *_kept(x, keep, (_groups(K), -(-B * S // 16) * 16))
 
@@ -134,9 +166,9 @@ def _lora_down8_bwd(
 ) -> tuple[torch.Tensor, torch.Tensor]:
     B, S, R = dt.shape
     K = a.shape[1]
-    dt, a = aligned(dt.contiguous()), aligned(a)
+    dt, a = aligned(dt.contiguous()), aligned(a.contiguous())
     dx = dt.new_empty((B, S, K) if need_x else 0)
-    da = torch.empty_like(a) if need_a else dt.new_empty(0)
+    da = dt.new_empty(a.shape if need_a else 0)
     if B * S == 0:
         return dx, da.zero_()
     with torch.cuda.device(dt.device):
@@ -155,7 +187,7 @@ def _lora_down8_bwd(
 @_lora_down8_bwd.register_fake
 def _(dt, a, codes, exps, need_x, need_a):
     B, S, _ = dt.shape
-    return dt.new_empty((B, S, a.shape[1]) if need_x else 0), torch.empty_like(a) if need_a else dt.new_empty(0)
+    return dt.new_empty((B, S, a.shape[1]) if need_x else 0), dt.new_empty(a.shape if need_a else 0)
 
 
 def _lora_down8_setup(ctx, inputs, output):
@@ -183,17 +215,6 @@ torch.library.register_autograd(
 # -------------------------------------------------------------- public API --
 
 
-def _tokens(x: torch.Tensor) -> torch.Tensor:
-    _check(x)
-    if x.ndim != 3 or x.shape[2] == 0:
-        raise ValueError("x must be [B, S, K]")
-    if x.dtype != torch.bfloat16:
-        raise ValueError(f"unsupported dtype {x.dtype}: only bfloat16 is implemented")
-    if x.shape[2] % 8 or x.shape[2] > MAX_K:
-        raise ValueError(f"K must be a multiple of 8 and at most {MAX_K}")
-    return x.contiguous()
-
-
 def gelu8(x: torch.Tensor) -> torch.Tensor:
     """GELU (erf form) whose backward reads an 8-bit copy of its input.
 
@@ -207,8 +228,7 @@ def gelu8(x: torch.Tensor) -> torch.Tensor:
     Raises:
         ValueError: If `x` is not on CUDA, or its shape or dtype is not supported.
     """
-    x = _tokens(x)
-    return _gelu8(x, torch.is_grad_enabled() and x.requires_grad)[0]
+    return _gelu8(x, x.requires_grad and torch.is_grad_enabled())[0]
 
 
 def lora_down8(x: torch.Tensor, a: torch.Tensor) -> torch.Tensor:
@@ -226,10 +246,4 @@ def lora_down8(x: torch.Tensor, a: torch.Tensor) -> torch.Tensor:
     Raises:
         ValueError: If a tensor is not on CUDA, or a shape or dtype is not supported.
     """
-    _check(x, a)
-    x = _tokens(x)
-    if a.ndim != 2 or a.shape[1] != x.shape[2] or a.dtype != x.dtype or a.device != x.device:
-        raise ValueError("a must be [R, K] of x's dtype and device")
-    if a.shape[0] % 8 or not 0 < a.shape[0] <= MAX_RANK:
-        raise ValueError(f"the rank must be a multiple of 8 and at most {MAX_RANK}")
-    return _lora_down8(x, a.contiguous(), torch.is_grad_enabled() and a.requires_grad)[0]
+    return _lora_down8(x, a, a.requires_grad and torch.is_grad_enabled())[0]

@@ -19,10 +19,24 @@ from .. import _lib
 from .common import _check, aligned, custom_op
 
 
+# Checks are made once: by the native kernels, which hand what they do not take to the ops'
+# Python functions, and by these and the fakes through _check_tokens and _check_product.
+
+
+def _check_tokens(x: torch.Tensor) -> None:
+    if not x.is_meta:
+        _check(x)
+    if x.ndim != 3:
+        raise ValueError("x must be [B, S, K]")
+    if x.dtype != torch.bfloat16:
+        raise ValueError(f"unsupported dtype {x.dtype}: only bfloat16 is implemented")
+
+
 @custom_op("anima_flat_amd::rowquant_int8", mutates_args=())
 def _rowquant_int8(x: torch.Tensor, gelu: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    _check_tokens(x)
     B, S, K = x.shape
-    x = aligned(x)
+    x = aligned(x.contiguous())
     q = torch.empty(B, S, K, dtype=torch.int8, device=x.device)
     s = torch.empty(B * S, 1, dtype=torch.float32, device=x.device)
     with torch.cuda.device(x.device):
@@ -37,8 +51,9 @@ def _rowquant_int8(x: torch.Tensor, gelu: bool) -> tuple[torch.Tensor, torch.Ten
 
 @_rowquant_int8.register_fake
 def _(x, gelu):
+    _check_tokens(x)
     B, S, _ = x.shape
-    return torch.empty_like(x, dtype=torch.int8), x.new_empty((B * S, 1), dtype=torch.float32)
+    return x.new_empty(x.shape, dtype=torch.int8), x.new_empty((B * S, 1), dtype=torch.float32)
 
 
 def rowquant_int8(x: torch.Tensor, gelu: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
@@ -50,19 +65,16 @@ def rowquant_int8(x: torch.Tensor, gelu: bool = False) -> tuple[torch.Tensor, to
 
     Returns:
         `(q, s)`: int8 tokens `[B, S, K]`, `s = max(max|y|, 1e-12) / 127` as float32
-        `[B * S, 1]`, `q = round(y / s)` to nearest even. A token with a value that is not
+        `[B * S, 1]`, `q = round(y * (1 / s))` to nearest even. A token with a value that is not
         finite has the scale NaN and codes 0.
 
     Raises:
         ValueError: If `x` is not on CUDA, or its dtype / K is not supported.
         RuntimeError: If `x` requires grad (there is no backward).
     """
-    _check(x)
-    if x.ndim != 3:
-        raise ValueError("x must be [B, S, K]")
-    if torch.is_grad_enabled() and x.requires_grad:
+    if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("rowquant_int8 has no backward")
-    return _rowquant_int8(x.contiguous(), gelu)
+    return _rowquant_int8(x, gelu)
 
 
 def quantize_weight(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -74,13 +86,30 @@ def quantize_weight(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     return q[0], s[:, 0]
 
 
+def _check_product(q, s, weight, weight_scale) -> None:
+    if not q.is_meta:
+        _check(q, s, weight, weight_scale)
+    if q.ndim != 3 or q.dtype != torch.int8:
+        raise ValueError("q must be int8 [B, S, K]")
+    if weight.ndim != 2 or weight.dtype != torch.int8 or weight.shape[1] != q.shape[2]:
+        raise ValueError("weight must be int8 [N, K]")
+    if s.dtype != torch.float32 or s.numel() != q.shape[0] * q.shape[1]:
+        raise ValueError("s must be float32 with one scale per token")
+    if weight_scale.dtype != torch.float32 or weight_scale.numel() != weight.shape[0]:
+        raise ValueError("weight_scale must be float32 with one scale per output channel")
+    if any(t.device != q.device for t in (s, weight, weight_scale)):
+        raise ValueError("all tensors must be on one device")
+
+
 @custom_op("anima_flat_amd::int8_linear", mutates_args=())
 def _int8_linear(
     q: torch.Tensor, s: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor
 ) -> torch.Tensor:
+    _check_product(q, s, weight, weight_scale)
     B, S, K = q.shape
     N = weight.shape[0]
-    q, weight = aligned(q), aligned(weight)
+    q, weight = aligned(q.contiguous()), aligned(weight.contiguous())
+    s, weight_scale = s.contiguous(), weight_scale.contiguous()
     y = torch.empty(B, S, N, dtype=torch.bfloat16, device=q.device)
     with torch.cuda.device(q.device):
         _lib.check(
@@ -95,6 +124,7 @@ def _int8_linear(
 
 @_int8_linear.register_fake
 def _(q, s, weight, weight_scale):
+    _check_product(q, s, weight, weight_scale)
     return q.new_empty((q.shape[0], q.shape[1], weight.shape[0]), dtype=torch.bfloat16)
 
 
@@ -116,17 +146,6 @@ def int8_linear(
     Raises:
         ValueError: If a tensor is not on CUDA, or a shape or dtype is not supported.
     """
-    _check(q, s, weight, weight_scale)
-    if q.ndim != 3 or q.dtype != torch.int8:
-        raise ValueError("q must be int8 [B, S, K]")
-    if weight.ndim != 2 or weight.dtype != torch.int8 or weight.shape[1] != q.shape[2]:
-        raise ValueError("weight must be int8 [N, K]")
-    if s.dtype != torch.float32 or s.numel() != q.shape[0] * q.shape[1]:
-        raise ValueError("s must be float32 with one scale per token")
-    if weight_scale.dtype != torch.float32 or weight_scale.numel() != weight.shape[0]:
-        raise ValueError("weight_scale must be float32 with one scale per output channel")
-    if any(t.device != q.device for t in (s, weight, weight_scale)):
-        raise ValueError("all tensors must be on one device")
-    if torch.is_grad_enabled() and (s.requires_grad or weight_scale.requires_grad):
+    if (s.requires_grad or weight_scale.requires_grad) and torch.is_grad_enabled():
         raise RuntimeError("int8_linear has no backward")
-    return _int8_linear(q.contiguous(), s.contiguous(), weight.contiguous(), weight_scale.contiguous())
+    return _int8_linear(q, s, weight, weight_scale)

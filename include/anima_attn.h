@@ -370,8 +370,8 @@ typedef struct aa_adaln_args {
  * n = y, or y * rsqrt(mean(y^2) + eps) * weight; r = x + branch_scale * gate * n
  * (r = x without y); h = (r - mean(r)) * rsqrt(var(r) + eps) * (1 + scale) + shift,
  * per token over D channels, all in fp32; r and h are rounded to bf16 once each
- * (h is that of the fp32 r). With q: s = max(max|h|, 1e-12) / 127 and
- * q = round-to-nearest-even(h / s) per token; a token with a value that is not
+ * (h is that of the fp32 r). With q: s = max(max|h|, 1e-12) / 127 and q as
+ * aa_rowquant_int8 makes them, of the fp32 h; a token with a value that is not
  * finite has the scale NaN.
  * x, y, r, h, q contiguous; D a multiple of 8, at most 8192; 16-byte aligned
  * pointers and modulation rows.
@@ -424,7 +424,7 @@ int aa_adaln_bwd(const aa_adaln_bwd_args* args, void* workspace, size_t workspac
 /*
  * Per-row int8 quantisation of x [rows, K] bf16 (contiguous): y = x or GELU(x)
  * (gelu != 0), s[row] = max(max|y|, 1e-12) / 127 (float), q = round-to-nearest-
- * even(y / s) (int8 [rows, K]). A row with a value that is not finite has the
+ * even(y * (1 / s)), 1 / s rounded to float, the product exact (int8 [rows, K]). A row with a value that is not finite has the
  * scale NaN and codes 0. K a multiple of 8 and at most 8192; x 16-byte and q
  * 8-byte aligned.
  */
@@ -469,10 +469,13 @@ int aa_gelu8_bwd(const void* dy, const void* codes, const void* exps, void* dx, 
  * R a multiple of 8, at most 64; K a multiple of 8, at most 65536; all pointers
  * 16-byte aligned.
  */
-int aa_lora8_fwd(const void* x, const void* a, void* t, void* codes, void* exps, int64_t M,
-                 int64_t K, int64_t R, int dtype, void* stream);
+int aa_lora8_fwd(const void* x, const void* a, void* t, void* codes, void* exps,
+                 void* workspace, size_t workspace_bytes, int64_t M, int64_t K, int64_t R,
+                 int dtype, void* stream);
 
-/* Bytes of workspace aa_lora8_bwd needs on the current device for da. */
+/* Bytes of workspace aa_lora8_fwd and aa_lora8_bwd (for da) need on the current
+ * device, 16-byte aligned: fp32 partial sums of ranges of channels and rows. */
+size_t aa_lora8_fwd_workspace(int64_t M, int64_t K, int64_t R);
 size_t aa_lora8_bwd_workspace(int64_t M, int64_t K, int64_t R);
 
 /*

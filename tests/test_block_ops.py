@@ -136,8 +136,8 @@ def test_other_refusals(lib):
     assert lib.aa_gelu8_bwd(FAKE, None, FAKE, FAKE, 4, 64, 0, None) == bad
     assert lib.aa_gelu8_bwd(FAKE + 2, FAKE, FAKE, FAKE, 4, 64, 0, None) == bad
 
-    def lora(x=FAKE, a=FAKE, t=FAKE, c=FAKE, e=FAKE, M=4, K=64, R=16, dtype=0):
-        return lib.aa_lora8_fwd(x, a, t, c, e, M, K, R, dtype, None)
+    def lora(x=FAKE, a=FAKE, t=FAKE, c=FAKE, e=FAKE, ws=None, n=0, M=4, K=64, R=16, dtype=0):
+        return lib.aa_lora8_fwd(x, a, t, c, e, ws, n, M, K, R, dtype, None)
 
     assert lora(dtype=1) == no and lora(R=12) == no and lora(R=72) == no and lora(R=0) == no and lora(K=4) == no
     assert lora(e=None) == bad and lora(a=FAKE + 2) == bad and lora(M=0, x=None) == 0

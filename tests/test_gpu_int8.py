@@ -50,7 +50,7 @@ def test_rowquant_ties(int8):
 
 
 def test_rowquant_gelu(int8):
-    """GELU's float32 error (at most 6e-6, relative) moves the scale by as much and a code by
+    """GELU's float32 error (the fit's 3.1e-5 and a few roundings, relative) moves the scale by as much and a code by
     one step where the quotient is that near a tie."""
     g = gen(3)
     x = bf(g, 2, 40, 1032, scale=3.0)
@@ -58,8 +58,8 @@ def test_rowquant_gelu(int8):
     y = ref.gelu(x.double())
     want = y.abs().amax(-1, keepdim=True) / 127
     sd = s.view(2, 40, 1).double()
-    assert ((sd - want).abs() <= 6e-6 * want).all()
-    within(q.double() * sd, y, sd * (0.5 + 2e-5) + 6e-6 * y.abs(), "q s")
+    assert ((sd - want).abs() <= 3.3e-5 * want).all()
+    within(q.double() * sd, y, sd * (0.5 + 2e-5) + 3.3e-5 * y.abs(), "q s")
 
 
 def test_rowquant_not_finite(int8):
