@@ -71,9 +71,16 @@ __device__ __forceinline__ u32x2 codes8(const float* v, float inv) {
     c[i] = __float_as_uint(__builtin_amdgcn_fmed3f(fmaf(v[i], inv, kRoundMagic), kRoundMagic - 127.0f, kRoundMagic + 127.0f));
   return u32x2{low_bytes(c[0], c[1], c[2], c[3]), low_bytes(c[4], c[5], c[6], c[7])};
 }
-// code * step of byte kByte of a word of codes with their sign bits flipped
-// (code + 128 as an unsigned byte, which one instruction converts), with low =
-// -128 step. Exact: (code + 128) step - 128 step has at most 8 significant bits.
+// Four codes + 128 as unsigned bytes, which one instruction each converts. The
+// empty asm keeps the flip on the word: left alone, the compiler flips every byte
+// by itself.
+__device__ __forceinline__ uint32_t flip_signs(uint32_t w) {
+  w ^= 0x80808080u;
+  asm("" : "+v"(w));
+  return w;
+}
+// code * step of byte kByte of flip_signs(codes), with low = -128 step. Exact:
+// (code + 128) step - 128 step has at most 8 significant bits.
 template <int kByte>
 __device__ __forceinline__ float kept_value(uint32_t flipped, float step, float low) {
   return fmaf((float)((flipped >> (8 * kByte)) & 255u), step, low);
@@ -171,9 +178,10 @@ __global__ __launch_bounds__(kGeThreads) void gelu8_bwd_kernel(GeluBwd p) {
     const float step = step_of(e[i]), low = -128.0f * step;
     float g[8];
     unpack8(raw[i], g);
+    const uint32_t c[2] = {flip_signs(code[i][0]), flip_signs(code[i][1])};
     static_for<0, 8>([&](auto J) {
       constexpr int j = decltype(J)::value;
-      g[j] *= gelu_slope(kept_value<j & 3>(code[i][j >> 2] ^ 0x80808080u, step, low));
+      g[j] *= gelu_slope(kept_value<j & 3>(c[j >> 2], step, low));
     });
     st16_nt(p.dx + at[i], pack8(g));
   }
@@ -318,7 +326,22 @@ __global__ __launch_bounds__(64 * lora_waves(16 * NR)) void lora8_fwd_kernel(Lor
   }
 }
 
-// dx = dt A: a wave takes 128 channels and 16 rows at a time. The MFMA's row
+// Workgroups of a tiles x groups grid (tiles along the channels), numbered so
+// that an XCD (blocks go to the 8 in turn) takes whole runs of tiles of a few
+// groups of rows. With the tiles in turn over the XCDs, an XCD wrote or read only
+// every eighth piece of each row, and with rows of a power of two of bytes
+// those lie in 2 to 4 of its L2's 16 channels.
+static unsigned grid_blocks(int64_t n) { return (unsigned)((n + 7) / 8 * 8); }
+__device__ __forceinline__ bool grid_place(int tiles, int groups, int* tile, int* group) {
+  const int n = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
+  *group = n / tiles;
+  *tile = n - *group * tiles;
+  return *group < groups;
+}
+
+// dx = dt A: a workgroup takes 512 channels, its four waves 128 each, and 16 rows
+// at a time, so that it writes 1 KiB of each row (the waves on 16 rows each of
+// 128 channels wrote at 3.9 TB/s, 32 us at 7904 x 8192). The MFMA's row
 // operand is A's columns (A^T is not in memory): the workgroup's part of A
 // lies in LDS as it is, and ds_read_b64_tr_b16 hands a lane four ranks of its
 // channel. Row 4 q + i of product (j, h) is channel 32 j + 8 q + 4 h + i, so that
@@ -331,37 +354,49 @@ struct LoraDx {
   bf16* dx;
   int64_t M;
   int K, R, rows;  // rows per workgroup
+  int tiles, groups;
 };
 
+constexpr int kDxCols = 512;
+
 template <int NS>  // 32 ranks per step
-__global__ __launch_bounds__(256) void lora8_dx_kernel(LoraDx p) {
-  __shared__ __attribute__((aligned(16))) bf16 as[32 * NS * 128];
+__global__ __launch_bounds__(256, 4) void lora8_dx_kernel(LoraDx p) {
+  // Each wave's 128 channels of 32 ranks at a time, 256 bytes a rank.
+  __shared__ __attribute__((aligned(16))) bf16 lds[4][32 * 128];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int li = lane & 15, g = lane >> 4;
-  const int k0 = blockIdx.x * 128;
-  for (int o = threadIdx.x; o < 32 * NS * 16; o += 256) {
-    const int rank = o >> 4, k = k0 + 8 * (o & 15);
-    u32x4 v = u32x4{0, 0, 0, 0};
-    if (rank < p.R && k < p.K) v = ld16(p.a + (int64_t)rank * p.K + k);
-    *reinterpret_cast<u32x4*>(as + rank * 128 + 8 * (o & 15)) = v;
-  }
-  __syncthreads();
+  int bx, by;
+  if (!grid_place(p.tiles, p.groups, &bx, &by)) return;
+  const int k0 = bx * kDxCols + 128 * wave;
+  bf16* as = lds[wave];
   // Lanes 4 r + q of a group of 16 give the piece of four channels at 8 q of rank
   // 8 g + r (+ 4 for the second read).
   const bf16* piece = as + (8 * g + (li >> 2)) * 128 + 8 * (li & 3);
   bf16x8 w[4][2][NS];
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int s = 0; s < NS; ++s) {
+    u32x4 v[8];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int i = 0; i < 8; ++i) {
+      const int rank = 32 * s + 4 * i + g, k = k0 + 8 * li;
+      v[i] = u32x4{0, 0, 0, 0};
+      if (rank < p.R && k < p.K) v[i] = ld16(p.a + (int64_t)rank * p.K + k);
+    }
 #pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        const s16x4 lo = ds_read_tr(piece + 32 * s * 128 + 32 * j + 4 * h);
-        const s16x4 hi = ds_read_tr(piece + (32 * s + 4) * 128 + 32 * j + 4 * h);
+    for (int i = 0; i < 8; ++i) *reinterpret_cast<u32x4*>(as + (4 * i + g) * 128 + 8 * li) = v[i];
+    __builtin_amdgcn_wave_barrier();  // the wave's own part: its writes are in order with its reads
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const s16x4 lo = ds_read_tr(piece + 32 * j + 4 * h);
+        const s16x4 hi = ds_read_tr(piece + 4 * 128 + 32 * j + 4 * h);
         w[j][h][s] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
       }
-  const int64_t begin = (int64_t)blockIdx.y * p.rows, end = min(p.M, begin + p.rows);
+    __builtin_amdgcn_wave_barrier();
+  }
+  const int64_t begin = (int64_t)by * p.rows, end = min(p.M, begin + p.rows);
   auto load = [&](bf16x8 (&d)[NS], int64_t r0) {
     const int64_t row = min(r0 + li, p.M - 1);
 #pragma unroll
@@ -373,12 +408,12 @@ __global__ __launch_bounds__(256) void lora8_dx_kernel(LoraDx p) {
     }
   };
   bf16x8 next[NS];
-  load(next, begin + 16 * wave);
-  for (int64_t r0 = begin + 16 * wave; r0 < end; r0 += 64) {
+  load(next, begin);
+  for (int64_t r0 = begin; r0 < end; r0 += 16) {
     bf16x8 d[NS];
 #pragma unroll
     for (int s = 0; s < NS; ++s) d[s] = next[s];
-    if (r0 + 64 < end) load(next, r0 + 64);
+    if (r0 + 16 < end) load(next, r0 + 16);
     u32x4 o[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -417,7 +452,7 @@ __global__ __launch_bounds__(256) void lora8_dx_kernel(LoraDx p) {
 // four waves 32 rows each in turn. Lane l reads 8 channels (8 (l % 16)) of rows
 // 8 (l / 16) .. + 7: product j of 8 takes channel 8 li + j of every lane, the
 // rows as the contracted index. dt lies in LDS as it is in memory, 128 rows at
-// a time, and is read transposed. The next turn's codes, steps and dt are
+// a time, and is read transposed. The codes, steps and dt of two turns ahead are
 // loaded before this turn's products. Partial sums per range of rows, in fp32,
 // are added by lora8_sum_kernel (or, of one range, written as they are).
 struct LoraDa {
@@ -440,7 +475,7 @@ __global__ __launch_bounds__(kDaThreads, NR < 4 ? 2 : 1) void lora8_da_kernel(Lo
   // Row pitch in LDS: a multiple of 8 bytes whose 16-row stride spreads over the
   // banks (the transposed reads take 4 rows x 32 bytes per 16 lanes).
   constexpr int kPitch = 16 * NR + 4;
-  constexpr int kDt = kDaRows * kPitch * 2;
+  constexpr int kDt = 2 * kDaRows * kPitch * 2;  // two turns' dt
   constexpr int kSum = kDaWaves * NR * 4 * kDaCols * 4;  // one element i of every wave at a time
   __shared__ __attribute__((aligned(16))) uint8_t lds[kDt > kSum ? kDt : kSum];
   bf16* dts = reinterpret_cast<bf16*>(lds);
@@ -449,9 +484,11 @@ __global__ __launch_bounds__(kDaThreads, NR < 4 ? 2 : 1) void lora8_da_kernel(Lo
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int li = lane & 15, g = lane >> 4;
   // The codes' rows are padded to whole groups; channels past them read the last.
-  const int col = min(blockIdx.x * kDaCols + 8 * li, kGroup * p.G - 8);
+  int bx, by;
+  if (!grid_place((p.K + kDaCols - 1) / kDaCols, p.splits, &bx, &by)) return;
+  const int col = min(bx * kDaCols + 8 * li, kGroup * p.G - 8);
   const int grp = col / kGroup;
-  const int64_t begin = (int64_t)blockIdx.y * p.rows, end = min(p.M, begin + p.rows);
+  const int64_t begin = (int64_t)by * p.rows, end = min(p.M, begin + p.rows);
   f32x4v acc[8][NR];
 #pragma unroll
   for (int j = 0; j < 8; ++j)
@@ -460,11 +497,12 @@ __global__ __launch_bounds__(kDaThreads, NR < 4 ? 2 : 1) void lora8_da_kernel(Lo
 
   constexpr int kPieces = kDaRows * 4 * NR / kDaThreads;  // 8-byte pieces of dt per thread
   const uint32_t pitch = kGroup * p.G;
+  const uint32_t whole = (uint32_t)(32 * wave + 8 * g) * pitch + (uint32_t)col;  // of this lane's first row
   struct Turn {
     u32x2 c[8];  // codes of this lane's 8 rows
     u32x2 ex;    // their groups' exponents
     u32x2 dt[kPieces];
-  } cur, next;
+  } cur, next, after;
   auto load = [&](Turn& t, int64_t r0) {
     // Addresses: a uniform row base and 32-bit offsets in the turn's 128 rows.
     const uint8_t* codes = p.codes + r0 * pitch;
@@ -473,9 +511,14 @@ __global__ __launch_bounds__(kDaThreads, NR < 4 ? 2 : 1) void lora8_da_kernel(Lo
     const int mine = 32 * wave + 8 * g;  // this lane's 8 rows
     // Every load is in bounds and made: rows past the range re-read its last, and
     // count nothing below; channels and ranks past theirs are not written.
+    if (last == kDaRows - 1) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      t.c[e] = *reinterpret_cast<const u32x2*>(codes + ((uint32_t)min(mine + e, last) * pitch + (uint32_t)col));
+      for (int e = 0; e < 8; ++e) t.c[e] = *reinterpret_cast<const u32x2*>(codes + (int64_t)e * pitch + whole);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        t.c[e] = *reinterpret_cast<const u32x2*>(codes + ((uint32_t)min(mine + e, last) * pitch + (uint32_t)col));
+    }
     t.ex = *reinterpret_cast<const u32x2*>(p.exps + (int64_t)grp * p.Mp + r0 + min(mine, last & ~7));
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
@@ -489,18 +532,22 @@ __global__ __launch_bounds__(kDaThreads, NR < 4 ? 2 : 1) void lora8_da_kernel(Lo
     }
   };
   if (begin < end) load(cur, begin);
+  if (begin + kDaRows < end) load(next, begin + kDaRows);
+  bf16* mydt = dts;
   for (int64_t r0 = begin; r0 < end; r0 += kDaRows) {
-    __syncthreads();  // the turn before has read its dt
+    if (r0 + 2 * kDaRows < end) load(after, r0 + 2 * kDaRows);
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       const int o = tid + kDaThreads * i, r = o / (4 * NR), rank = 4 * (o % (4 * NR));
-      *reinterpret_cast<u32x2*>(dts + r * kPitch + rank) = cur.dt[i];
+      *reinterpret_cast<u32x2*>(mydt + r * kPitch + rank) = cur.dt[i];
     }
+    // One barrier a turn: these places are written again two turns on, behind the
+    // next turn's barrier, which every wave reaches after its reads here.
     __syncthreads();
-    if (r0 + kDaRows < end) load(next, r0 + kDaRows);
     // Lanes 4 r + q of a group of 16 give the piece of four ranks at 4 q of row
     // 8 g + r (+ 4 for the second read); lane li receives rank li of four rows.
-    const bf16* piece = dts + (32 * wave + 8 * g + (li >> 2)) * kPitch + 4 * (li & 3);
+    const bf16* piece = mydt + (32 * wave + 8 * g + (li >> 2)) * kPitch + 4 * (li & 3);
+    mydt = mydt == dts ? dts + kDaRows * kPitch : dts;
     bf16x8 d[NR];
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
@@ -508,26 +555,35 @@ __global__ __launch_bounds__(kDaThreads, NR < 4 ? 2 : 1) void lora8_da_kernel(Lo
       const s16x4 hi = ds_read_tr(piece + 4 * kPitch + 16 * n);
       d[n] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
-    float step[8];
-    const int64_t left = end - r0 - (32 * wave + 8 * g);
+    float step[8], low[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) step[e] = step_of((cur.ex[e >> 2] >> (8 * (e & 3))) & 255u);
+    if (r0 + kDaRows > end) {  // rows past the range count nothing, whatever their group's mark
+      const int left = (int)(end - r0) - (32 * wave + 8 * g);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) step[e] = e < left ? step[e] : 0.f;
+    }
+    uint32_t code[8][2];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      // Rows past the range count nothing, whatever their group's mark.
-      step[e] = e < left ? step_of((cur.ex[e >> 2] >> (8 * (e & 3))) & 255u) : 0.f;
+      low[e] = -128.0f * step[e];
+      code[e][0] = flip_signs(cur.c[e][0]);
+      code[e][1] = flip_signs(cur.c[e][1]);
     }
     static_for<0, 8>([&](auto J) {
       constexpr int j = decltype(J)::value;
       u32x4 v;
       static_for<0, 4>([&](auto E) {
         constexpr int e = 2 * decltype(E)::value;
-        v[e / 2] = pack_bf16(kept_value<j & 3>(cur.c[e][j >> 2] ^ 0x80808080u, step[e], -128.0f * step[e]),
-                             kept_value<j & 3>(cur.c[e + 1][j >> 2] ^ 0x80808080u, step[e + 1], -128.0f * step[e + 1]));
+        v[e / 2] = pack_bf16(kept_value<j & 3>(code[e][j >> 2], step[e], low[e]),
+                             kept_value<j & 3>(code[e + 1][j >> 2], step[e + 1], low[e + 1]));
       });
       const bf16x8 xv = __builtin_bit_cast(bf16x8, v);
 #pragma unroll
       for (int n = 0; n < NR; ++n) acc[j][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(d[n], xv, acc[j][n], 0, 0, 0);
     });
     cur = next;
+    next = after;
   }
   // acc[j][n]: lane li is channel 8 li + j, element i is rank 16 n + 4 g + i.
   // Added over the waves one element i at a time: sums[wave][n][g][channel].
@@ -542,7 +598,7 @@ __global__ __launch_bounds__(kDaThreads, NR < 4 ? 2 : 1) void lora8_da_kernel(Lo
         *reinterpret_cast<f32x4v*>(sums + ((wave * NR + n) * 4 + g) * kDaCols + 8 * li + 4 * q) =
             f32x4v{acc[4 * q][n][i], acc[4 * q + 1][n][i], acc[4 * q + 2][n][i], acc[4 * q + 3][n][i]};
     __syncthreads();
-    const int at = tid & (kDaCols - 1), k = blockIdx.x * kDaCols + at;
+    const int at = tid & (kDaCols - 1), k = bx * kDaCols + at;
     if (k < p.K) {
 #pragma unroll
       for (int m0 = 0; m0 < NR * 4; m0 += 2) {
@@ -553,7 +609,7 @@ __global__ __launch_bounds__(kDaThreads, NR < 4 ? 2 : 1) void lora8_da_kernel(Lo
 #pragma unroll
         for (int w = 0; w < kDaWaves; ++w) s += sums[(w * NR * 4 + m) * kDaCols + at];
         if (p.splits == 1) p.da[(int64_t)rank * p.K + k] = (bf16)s;
-        else p.part[((int64_t)blockIdx.y * p.R + rank) * p.K + k] = s;
+        else p.part[((int64_t)by * p.R + rank) * p.K + k] = s;
       }
     }
   }
@@ -725,12 +781,14 @@ extern "C" int aa_lora8_bwd(const void* dt, const void* a, const void* codes, co
     p.M = M;
     p.K = (int)K;
     p.R = (int)R;
-    const int64_t tiles = (K + 127) / 128;
-    // Two to four workgroups a CU, each with at least 128 rows to spend the
-    // reading of its part of A on.
+    const int64_t tiles = (K + kDxCols - 1) / kDxCols;
+    // Up to four workgroups a CU, each with at least 32 rows to spend the reading
+    // of its part of A on.
     const int64_t per = (M * tiles + 4 * cus - 1) / (4 * cus);
-    p.rows = (int)((std::clamp<int64_t>(per, std::max<int64_t>(128, (M + 65534) / 65535), 1 << 20) + 63) / 64 * 64);
-    const dim3 grid((unsigned)tiles, (unsigned)((M + p.rows - 1) / p.rows));
+    p.rows = (int)((std::clamp<int64_t>(per, std::max<int64_t>(32, (M + 65534) / 65535), 1 << 20) + 15) / 16 * 16);
+    p.tiles = (int)tiles;
+    p.groups = (int)((M + p.rows - 1) / p.rows);
+    const dim3 grid(grid_blocks(tiles * p.groups));
     if (R <= 32) lora8_dx_kernel<1><<<grid, 256, 0, st>>>(p);
     else lora8_dx_kernel<2><<<grid, 256, 0, st>>>(p);
     if (int rc = check_launch("lora8_bwd")) return rc;
@@ -750,7 +808,7 @@ extern "C" int aa_lora8_bwd(const void* dt, const void* a, const void* codes, co
   p.splits = da_splits(M, K, R);
   // Ranges of whole turns' rows; the last ones may be empty and write zeros.
   p.rows = (int)(((M + p.splits - 1) / p.splits + kDaRows - 1) / kDaRows * kDaRows);
-  const dim3 grid((unsigned)((K + kDaCols - 1) / kDaCols), (unsigned)p.splits);
+  const dim3 grid(grid_blocks((K + kDaCols - 1) / kDaCols * p.splits));
   if (R <= 16) lora8_da_kernel<1><<<grid, kDaThreads, 0, st>>>(p);
   else if (R <= 32) lora8_da_kernel<2><<<grid, kDaThreads, 0, st>>>(p);
   else if (R <= 48) lora8_da_kernel<3><<<grid, kDaThreads, 0, st>>>(p);

@@ -119,7 +119,6 @@ struct I8Tile {
   static_assert(kRingBytes <= 160 * 1024 && MT * 256 <= kRingBytes, "LDS");
   static_assert(NT % 128 == 0 && 128 % WN == 0 || WN == 128, "128-channel sections");
 };
-using I8TileA = I8Tile<256, 256, 128, 2>;  // 128 KiB ring
 using I8TileC = I8Tile<128, 128, 64, 2>;   // 64 KiB ring, two workgroups per CU
 using I8TileD = I8Tile<128, 128, 64, 4>;   // 128 KiB ring
 
@@ -289,8 +288,221 @@ __global__ __launch_bounds__(T::kThreads) void int8_linear_kernel(I8Params p) {
     if (col < ncols) {
       bf16* out = p.y + row0 * p.N + nt * T::kNT + col;
       for (int r = grp; r < nrows; r += T::kThreads / 16)
-        st16_nt(out + (int64_t)r * p.N, *reinterpret_cast<const u32x4*>(lds + r * 256 + ((j ^ (r & 15)) * 16)));
+        st16(out + (int64_t)r * p.N, *reinterpret_cast<const u32x4*>(lds + r * 256 + ((j ^ (r & 15)) * 16)));
     }
+  }
+}
+
+// The large tile: 256 tokens x 256 channels, one wave per SIMD, each with 128 x
+// 128 outputs in 256 accumulator registers. Per 32 bytes of K a wave reads 8
+// operands for 16 MFMAs (the 64 x 128 waves of the tiles above: 6 for 8), which
+// halves the LDS reads that two waves per SIMD could not hide behind each
+// other's MFMAs.
+// A stage is four k-steps of 16 slots: an MFMA, and in the first eight an
+// operand read of the k-step after it, in the others a DMA of a stage ahead.
+// The ring holds three stages of X and two of W, 32 KiB each. The one barrier
+// stands before the last k-step of stage s, whose operands are read by then: it
+// publishes stage s + 1 (whose first operands are read in that k-step) and frees
+// stage s's places, for W of s + 2 (its DMA goes out behind the barrier) and X of
+// s + 3 (in the k-step after; it may be in flight still at the next barrier).
+// K % 128 != 0: the first stage is the short one; its lanes past the rest load
+// zeros.
+__device__ const u32x4 kZeroChunk = {0, 0, 0, 0};
+
+constexpr int kBigTile = 256;
+constexpr int kBigThreads = 256;
+constexpr int kBigPart = kBigTile * kIK;  // bytes of X or W per stage
+
+struct NoDma {
+  template <class I>
+  __device__ void operator()(I) const {}
+};
+
+__global__ __launch_bounds__(kBigThreads, 1) void int8_linear_big_kernel(I8Params p) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[5 * kBigPart];  // X's three, W's two
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int ntn = (p.N + kBigTile - 1) / kBigTile;
+  const int total = p.mtiles * ntn;
+  const int L = xcd_remap(blockIdx.x, total);
+  const int group = L / (kIGroupM * ntn);
+  const int within = L - group * kIGroupM * ntn;
+  const int gm = min(kIGroupM, p.mtiles - group * kIGroupM);
+  const int mt = group * kIGroupM + within % gm;
+  const int nt = within / gm;
+  const int64_t row0 = (int64_t)mt * kBigTile;
+  const int nrows = (int)min<int64_t>(kBigTile, p.M - row0);
+  const int ncols = min(kBigTile, p.N - kBigTile * nt);
+
+  // The scales of token and channel `tid` of the tile, for the epilogue.
+  const float xscale = p.xs[row0 + min(tid, nrows - 1)];
+  const float wscale = p.ws[(int64_t)nt * kBigTile + min(tid, ncols - 1)];
+
+  // DMA: 32 blocks of 8 rows x 128 bytes of each matrix; wave w moves blocks 8 w ..
+  // 8 w + 7 of both, lane roles as above. Per block its first row's address,
+  // per lane the byte offset from there.
+  const int drow = lane >> 3;
+  const int chunk0 = (lane & 7) ^ drow, chunk1 = chunk0 ^ 1;  // even and odd blocks
+  const int nk = (p.K + kIK - 1) / kIK;
+  const int rest = p.K - (nk - 1) * kIK;  // bytes of the first stage, 16 .. 128
+  const uint8_t* xbase[8];
+  const uint8_t* wbase[8];
+  uint32_t xoff[8], woff[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t chunk = 16 * ((i & 1) ? chunk1 : chunk0);
+    const int x0 = min(8 * (wave * 8 + i), nrows - 1), w0 = min(8 * (wave * 8 + i), ncols - 1);
+    xbase[i] = p.x + (row0 + x0) * p.K;
+    wbase[i] = p.w + ((int64_t)nt * kBigTile + w0) * p.K;
+    xoff[i] = (uint32_t)(min(drow, nrows - 1 - x0) * p.K) + chunk;
+    woff[i] = (uint32_t)(min(drow, ncols - 1 - w0) * p.K) + chunk;
+  }
+  const uint32_t ring = lds_addr(lds);
+  const uint32_t mine = ring + (uint32_t)wave * 8192u;
+  // Block I of this wave's share of a stage s >= 1, X to the place at byte `at`.
+  auto issue_x = [&](auto I, int s, uint32_t at) {
+    constexpr int i = decltype(I)::value;
+    dma16_sva_off<0, 1024 * i>(xbase[i] + (rest + (s - 1) * kIK), xoff[i], mine + at);
+  };
+  auto issue_w = [&](auto I, int s) {
+    constexpr int i = decltype(I)::value;
+    dma16_sva_off<0, 1024 * i>(wbase[i] + (rest + (s - 1) * kIK), woff[i], mine + (uint32_t)(3 + (s & 1)) * kBigPart);
+  };
+  static_for<0, 8>([&](auto I) {
+    constexpr int i = decltype(I)::value;
+    const bool in = 16 * ((i & 1) ? chunk1 : chunk0) < rest;
+    dma16_a(in ? xbase[i] + xoff[i] : (const uint8_t*)&kZeroChunk, mine + 1024u * i);
+    dma16_a(in ? wbase[i] + woff[i] : (const uint8_t*)&kZeroChunk, mine + 3u * kBigPart + 1024u * i);
+  });
+  if (nk > 1) {
+    static_for<0, 8>([&](auto I) { issue_x(I, 1, kBigPart); });
+    static_for<0, 8>([&](auto I) { issue_w(I, 1); });
+  }
+
+  const int wm = wave & 1;   // tokens 128 wm ..
+  const int wn = wave >> 1;  // channels 128 wn ..
+  const int li = lane & 31, hh = lane >> 5;
+  const uint32_t kbase = (li >> 3) * 1024 + (li & 7) * 128 + (hh ^ (li & 7) ^ ((li >> 3) & 1)) * 16;
+  // Operand addresses of k-step kk: these ^ 32 kk (the ring and its parts are
+  // aligned to 1 KiB, bits 4 to 6 are the slot's), blocks of 32 rows at + 4096.
+  const uint32_t xa = ring + wm * 16384 + kbase;
+  const uint32_t wa = ring + 3u * kBigPart + wn * 16384 + kbase;
+
+  i32x16 acc[4][4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[c][t][e] = 0;
+
+  struct Ops {
+    i32x4 v[8];  // four channel blocks, four token blocks
+  } o0, o1;
+  auto read = [&](auto J, Ops& o, uint32_t x, uint32_t w) {
+    constexpr int j = decltype(J)::value;
+    o.v[j] = __builtin_bit_cast(i32x4, lds_ld16((j < 4 ? w : x) + 4096u * (j & 3)));
+  };
+  // 16 MFMAs on `cur`, beside them the operands of the next k-step to `next` and
+  // eight DMAs: a read and a DMA in turn (four waves' DMAs back to back would hold
+  // up their MFMAs: the CU's load path takes one per ~11 cycles), or the reads in
+  // the first slots where none go out.
+  auto kstep = [&](const Ops& cur, Ops& next, uint32_t x, uint32_t w, auto has_next, auto dma) {
+    constexpr int kStride = std::is_same_v<decltype(dma), NoDma> ? 1 : 2;
+    static_for<0, 16>([&](auto J) {
+      constexpr int j = decltype(J)::value;
+      acc[j >> 2][j & 3] = mfma_i8(cur.v[j >> 2], cur.v[4 + (j & 3)], acc[j >> 2][j & 3]);
+      if constexpr (j % kStride == 0 && j / kStride < 8 && decltype(has_next)::value) {
+        // Channel block 0 and the token blocks first: the next k-step's first four MFMAs.
+        constexpr int order[8] = {0, 4, 5, 6, 7, 1, 2, 3};
+        read(std::integral_constant<int, order[j / kStride]>{}, next, x, w);
+      }
+      if constexpr (kStride == 2 && j % 2 == 1) dma(std::integral_constant<int, j / 2>{});
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  const NoDma none;
+  // This wave's DMAs of stage 0 are done (stage 1's may be in flight); the barrier
+  // publishes every wave's.
+  if (nk > 1) asm volatile("s_waitcnt vmcnt(16)\n\ts_barrier" ::: "memory");
+  else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+  static_for<0, 8>([&](auto J) { read(J, o0, xa, wa); });
+
+  // Places of X in the ring: of this stage, the next, and the one after, in
+  // which X of stage s + 2 is sent for in this stage's first k-step.
+  uint32_t px0 = 0, px1 = kBigPart, px2 = 2 * kBigPart;
+  // left: stages after this one, as far as it matters (0, 1, 2).
+  auto stage = [&](int s, auto left) {
+    constexpr int kLeft = decltype(left)::value;
+    const uint32_t x = xa + px0, w = wa + (uint32_t)(s & 1) * kBigPart;
+    if constexpr (kLeft >= 2)
+      kstep(o0, o1, x ^ 32u, w ^ 32u, std::true_type{}, [&](auto I) { issue_x(I, s + 2, px2); });
+    else
+      kstep(o0, o1, x ^ 32u, w ^ 32u, std::true_type{}, none);
+    kstep(o1, o0, x ^ 64u, w ^ 64u, std::true_type{}, none);
+    kstep(o0, o1, x ^ 96u, w ^ 96u, std::true_type{}, none);
+    if constexpr (kLeft >= 1) {
+      // Every read of stage s has arrived, and this wave's DMAs of stage s + 1: only
+      // X of s + 2 came after them.
+      if constexpr (kLeft >= 2) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      const uint32_t x1 = xa + px1, w1 = wa + (uint32_t)((s + 1) & 1) * kBigPart;
+      if constexpr (kLeft >= 2)
+        kstep(o1, o0, x1, w1, std::true_type{}, [&](auto I) { issue_w(I, s + 2); });
+      else
+        kstep(o1, o0, x1, w1, std::true_type{}, none);
+      const uint32_t t = px0;
+      px0 = px1;
+      px1 = px2;
+      px2 = t;
+    } else {
+      kstep(o1, o0, x, w, std::false_type{}, none);
+    }
+  };
+  int s = 0;
+  for (; s + 2 < nk; ++s) stage(s, std::integral_constant<int, 2>{});
+  if (s + 1 < nk) stage(s++, std::integral_constant<int, 1>{});
+  stage(s, std::integral_constant<int, 0>{});
+
+  // acc[c][t]: lane li is token 128 wm + 32 t + li, element e channel 128 wn + 32 c
+  // + 8 (e / 4) + 4 hh + e % 4. Each wave stages its 128 x 128 as 256-byte rows
+  // in a quarter of the ring, chunk ch of row r in slot ch ^ (r & 15), and
+  // stores them as whole lines.
+  float* scales = reinterpret_cast<float*>(lds + 4 * 32768);
+  __syncthreads();  // the last operands of every wave are read
+  scales[tid] = xscale;
+  scales[256 + tid] = wscale;
+  __syncthreads();
+  uint8_t* out = lds + wave * 32768;
+  const int wcols = ncols - 128 * wn, wrows = nrows - 128 * wm;  // what there is of them
+  if (wcols <= 0 || wrows <= 0) return;
+  float rs[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) rs[t] = scales[128 * wm + 32 * t + li];
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+#pragma unroll
+    for (int e4 = 0; e4 < 4; ++e4) {
+      const f32x4 w = *reinterpret_cast<const f32x4*>(scales + 256 + 128 * wn + 32 * c + 8 * e4 + 4 * hh);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int r = 32 * t + li;
+        const i32x16& v = acc[c][t];
+        u32x2 b;
+        b[0] = pack_bf16((float)v[4 * e4] * rs[t] * w[0], (float)v[4 * e4 + 1] * rs[t] * w[1]);
+        b[1] = pack_bf16((float)v[4 * e4 + 2] * rs[t] * w[2], (float)v[4 * e4 + 3] * rs[t] * w[3]);
+        *reinterpret_cast<u32x2*>(out + r * 256 + (((4 * c + e4) ^ (r & 15)) * 16) + 8 * hh) = b;
+      }
+    }
+  // The wave's own rows: its writes are in order with its reads.
+  __builtin_amdgcn_wave_barrier();
+  const int j = lane & 15;
+  bf16* y = p.y + (row0 + 128 * wm) * p.N + nt * kBigTile + 128 * wn + 8 * j;
+  if (8 * j < wcols) {
+#pragma unroll 8
+    for (int r = lane >> 4; r < wrows && r < 128; r += 4)
+      st16(y + (int64_t)r * p.N, *reinterpret_cast<const u32x4*>(out + r * 256 + ((j ^ (r & 15)) * 16)));
   }
 }
 
@@ -386,6 +598,9 @@ extern "C" int aa_rowquant_int8(const void* x, int64_t rows, int64_t K, int gelu
   return check_launch("rowquant_int8");
 }
 
+// A round of small tiles against one of large tiles: one a CU, and two a CU.
+constexpr double kSmallAlone = 0.38, kSmallPair = 0.62;
+
 extern "C" int aa_int8_linear(const void* q, const float* s, const void* weight, const float* weight_scale,
                               void* y, int64_t M, int64_t N, int64_t K, int dtype, void* stream) {
   clear_error();
@@ -416,17 +631,43 @@ extern "C" int aa_int8_linear(const void* q, const float* s, const void* weight,
     return check_launch("int8_linear");
   }
   const int64_t cus = std::max(1, device_cu_count());
-  const auto tiles = [&](int64_t mt, int64_t nt) { return (M + mt - 1) / mt * ((N + nt - 1) / nt); };
-  // Whole rounds of workgroups over the CUs times a round's relative time.
-  const double big = (double)((tiles(256, 256) + cus - 1) / cus) * 1.93;
-  const double small = (double)((tiles(128, 128) + 2 * cus - 1) / (2 * cus)) * 1.24;
-  const bool use_big = big <= small;
-  const int64_t mt = use_big ? 256 : 128;
-  const int64_t total = use_big ? tiles(256, 256) : tiles(128, 128);
-  if (total > 0x7fffffff) return fail(AA_EUNSUPPORTED, "int8_linear: too many tokens");
-  p.mtiles = (int)((M + mt - 1) / mt);
-  if (use_big) int8_linear_kernel<I8TileA><<<dim3((unsigned)total), I8TileA::kThreads, 0, st>>>(p);
-  else if (total <= cus) int8_linear_kernel<I8TileD><<<dim3((unsigned)total), I8TileD::kThreads, 0, st>>>(p);
-  else int8_linear_kernel<I8TileC><<<dim3((unsigned)total), I8TileC::kThreads, 0, st>>>(p);
+  const int64_t ntn = (N + kBigTile - 1) / kBigTile, mtn = (M + kBigTile - 1) / kBigTile;
+  const auto small_tiles = [&](int64_t rows) { return (rows + 127) / 128 * ((N + 127) / 128); };
+  // Time of the small tiles over `rows` tokens, in rounds of large tiles: XX
+  const auto small_time = [&](int64_t rows) {
+    const int64_t t = small_tiles(rows);
+    return t <= cus ? kSmallAlone : (double)((t + 2 * cus - 1) / (2 * cus)) * kSmallPair;
+  };
+  // Tokens for the large tiles: all, or what fills whole rounds of them (the rest
+  // goes to small tiles, in a launch of its own), or none.
+  const int64_t whole = mtn * ntn / cus * cus / ntn * kBigTile;
+  int64_t big = 0;
+  double best = small_time(M);
+  for (const int64_t rows : {std::min(M, whole), M}) {
+    if (rows <= 0) continue;
+    const int64_t t = (rows + kBigTile - 1) / kBigTile * ntn;
+    const double time = (double)((t + cus - 1) / cus) + (rows < M ? small_time(M - rows) : 0.0);
+    if (time < best) {
+      best = time;
+      big = rows;
+    }
+  }
+  if (small_tiles(M) > 0x7fffffff) return fail(AA_EUNSUPPORTED, "int8_linear: too many tokens");
+  if (big > 0) {
+    p.M = big;
+    p.mtiles = (int)((big + kBigTile - 1) / kBigTile);
+    int8_linear_big_kernel<<<dim3((unsigned)(p.mtiles * ntn)), kBigThreads, 0, st>>>(p);
+    if (int rc = check_launch("int8_linear")) return rc;
+    p.x += big * K;
+    p.xs += big;
+    p.y += big * N;
+  }
+  if (big < M) {
+    p.M = M - big;
+    p.mtiles = (int)((p.M + 127) / 128);
+    const int64_t t = small_tiles(p.M);
+    if (t <= cus && K >= 4096) int8_linear_kernel<I8TileD><<<dim3((unsigned)t), I8TileD::kThreads, 0, st>>>(p);
+    else int8_linear_kernel<I8TileC><<<dim3((unsigned)t), I8TileC::kThreads, 0, st>>>(p);
+  }
   return check_launch("int8_linear");
 }
