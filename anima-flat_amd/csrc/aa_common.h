@@ -137,6 +137,10 @@ int check_launch(const char* what);
 // Compute units of the current device; 0 if it cannot be queried.
 int device_cu_count();
 
+// Whether a launch of `blocks` workgroups of `threads` stays below the 2^32 work
+// items of one grid dimension.
+inline bool grid_fits(int64_t blocks, int64_t threads) { return blocks * threads <= int64_t{0xffffffff}; }
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 }  // namespace aa

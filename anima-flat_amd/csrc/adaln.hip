@@ -624,7 +624,9 @@ extern "C" int aa_adaln_fwd(const aa_adaln_args* a, void* stream) {
   const int64_t cus = std::max(1, device_cu_count());
   p.rpw = (int)std::clamp<int64_t>(p.rows / (cus * 4 * rows_at_once), 1, 4);
   const int64_t per = (int64_t)rows_at_once * p.rpw;
-  const dim3 grid((unsigned)((p.rows + per - 1) / per));
+  const int64_t blocks = (p.rows + per - 1) / per;
+  if (!grid_fits(blocks, kAdThreads)) return fail(AA_EUNSUPPORTED, "adaln: too many tokens");
+  const dim3 grid((unsigned)blocks);
   hipStream_t st = (hipStream_t)stream;
   const bool f32 = a->mod_dtype == AA_DTYPE_FP32, int8 = a->q != nullptr;
   if (p.D <= 512) launch_fwd<1, 1>(grid, st, p, f32, int8);
@@ -689,6 +691,7 @@ extern "C" int aa_adaln_bwd(const aa_adaln_bwd_args* a, void* workspace, size_t 
   p.chunks = (p.S + p.rpc - 1) / p.rpc;
   p.c = a->branch_scale;
   const int nc = !sums ? 0 : a->weight ? 4 : 3;
+  if (!grid_fits(a->B * p.chunks, kAdBThreads)) return fail(AA_EUNSUPPORTED, "adaln_bwd: too many tokens");
   const dim3 grid((unsigned)(a->B * p.chunks));
   hipStream_t st = (hipStream_t)stream;
   const bool f32 = a->mod_dtype == AA_DTYPE_FP32;

@@ -339,15 +339,15 @@ __device__ __forceinline__ bool grid_place(int tiles, int groups, int* tile, int
   return *group < groups;
 }
 
-// dx = dt A: a workgroup takes 512 channels, its four waves 128 each, and 16 rows
-// at a time, so that it writes 1 KiB of each row (the waves on 16 rows each of
-// 128 channels wrote at 3.9 TB/s, 32 us at 7904 x 8192). The MFMA's row
-// operand is A's columns (A^T is not in memory): the workgroup's part of A
-// lies in LDS as it is, and ds_read_b64_tr_b16 hands a lane four ranks of its
-// channel. Row 4 q + i of product (j, h) is channel 32 j + 8 q + 4 h + i, so that
-// a lane ends with 8 neighbouring channels of its row; the lanes of rows 8..15
-// then trade places between products j and j + 1, and each store covers 8 rows
-// of 128 bytes, whole lines.
+// dx = dt A: a workgroup takes 512 channels, its four waves 128 each, and 128 rows
+// of dt in LDS at a time. Product j of 8 takes channel 8 li + j of every lane as
+// its column (A's rows are loaded as 256-byte pieces, eight ranks' 8 channels a
+// lane, and transposed in registers) and 16 rows of dt, so that a lane ends with
+// 8 neighbouring channels of rows 4 g .. 4 g + 3 and the 16 lanes of a quarter
+// wave store 256 bytes of one row. With dt's rows along the lanes instead, the
+// quarter waves of a store spread over 8 rows, four times as many pieces of
+// lines: the CU's address unit was busy 80% of the time, 33 us at 7904 x 8192
+// and rank 40 against 28.5 (4.6 TB/s of writes; a fill of that size reaches 6.2).
 struct LoraDx {
   const bf16* dt;  // [M, R]
   const bf16* a;
@@ -358,91 +358,72 @@ struct LoraDx {
 };
 
 constexpr int kDxCols = 512;
+constexpr int kDxRows = 128;
 
 template <int NS>  // 32 ranks per step
-__global__ __launch_bounds__(256, 4) void lora8_dx_kernel(LoraDx p) {
-  // Each wave's 128 channels of 32 ranks at a time, 256 bytes a rank.
-  __shared__ __attribute__((aligned(16))) bf16 lds[4][32 * 128];
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+__global__ __launch_bounds__(256) void lora8_dx_kernel(LoraDx p) {
+  // dt's rows, 16-byte chunk c (8 ranks) of row r at slot c ^ (r & (4 NS - 1)).
+  __shared__ __attribute__((aligned(16))) bf16 dts[kDxRows * 32 * NS];
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int li = lane & 15, g = lane >> 4;
   int bx, by;
   if (!grid_place(p.tiles, p.groups, &bx, &by)) return;
-  const int k0 = bx * kDxCols + 128 * wave;
-  bf16* as = lds[wave];
-  // Lanes 4 r + q of a group of 16 give the piece of four channels at 8 q of rank
-  // 8 g + r (+ 4 for the second read).
-  const bf16* piece = as + (8 * g + (li >> 2)) * 128 + 8 * (li & 3);
-  bf16x8 w[4][2][NS];
+  const int k = bx * kDxCols + 128 * wave + 8 * li;  // this lane's channels
+  const bool in = k < p.K;
+  bf16x8 w[8][NS];
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
     u32x4 v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int rank = 32 * s + 4 * i + g, k = k0 + 8 * li;
-      v[i] = u32x4{0, 0, 0, 0};
-      if (rank < p.R && k < p.K) v[i] = ld16(p.a + (int64_t)rank * p.K + k);
+    for (int e = 0; e < 8; ++e) {
+      const int rank = 32 * s + 8 * g + e;
+      v[e] = u32x4{0, 0, 0, 0};
+      if (rank < p.R && in) v[e] = ld16(p.a + (int64_t)rank * p.K + k);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) *reinterpret_cast<u32x4*>(as + (4 * i + g) * 128 + 8 * li) = v[i];
-    __builtin_amdgcn_wave_barrier();  // the wave's own part: its writes are in order with its reads
+    for (int j = 0; j < 8; ++j) {
+      u32x4 t;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const s16x4 lo = ds_read_tr(piece + 32 * j + 4 * h);
-        const s16x4 hi = ds_read_tr(piece + 4 * 128 + 32 * j + 4 * h);
-        w[j][h][s] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-      }
-    __builtin_amdgcn_wave_barrier();
+      for (int e = 0; e < 8; e += 2)  // the bf16 j of ranks e and e + 1
+        t[e / 2] = __builtin_amdgcn_perm(v[e + 1][j / 2], v[e][j / 2], (j & 1) ? 0x07060302u : 0x05040100u);
+      w[j][s] = __builtin_bit_cast(bf16x8, t);
+    }
   }
   const int64_t begin = (int64_t)by * p.rows, end = min(p.M, begin + p.rows);
-  auto load = [&](bf16x8 (&d)[NS], int64_t r0) {
-    const int64_t row = min(r0 + li, p.M - 1);
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      const int rank = 32 * s + 8 * g;
+  for (int64_t c0 = begin; c0 < end; c0 += kDxRows) {
+    const int rows = (int)min<int64_t>(kDxRows, end - c0);
+    __syncthreads();  // the rows before have been read
+    for (int o = tid; o < kDxRows * 4 * NS; o += 256) {
+      const int r = o / (4 * NS), c = o % (4 * NS);
       u32x4 v = u32x4{0, 0, 0, 0};
-      if (rank < p.R) v = ld16(p.dt + row * p.R + rank);
-      d[s] = __builtin_bit_cast(bf16x8, v);
+      if (r < rows && 8 * c < p.R) v = ld16(p.dt + (c0 + r) * p.R + 8 * c);
+      *reinterpret_cast<u32x4*>(dts + (r * 4 * NS + (c ^ (r & (4 * NS - 1)))) * 8) = v;
     }
-  };
-  bf16x8 next[NS];
-  load(next, begin);
-  for (int64_t r0 = begin; r0 < end; r0 += 16) {
-    bf16x8 d[NS];
+    __syncthreads();
+    for (int r0 = 0; r0 < rows; r0 += 16) {
+      bf16x8 d[NS];
 #pragma unroll
-    for (int s = 0; s < NS; ++s) d[s] = next[s];
-    if (r0 + 16 < end) load(next, r0 + 16);
-    u32x4 o[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      f32x4v q[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        q[h] = f32x4v{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < NS; ++s)
-          q[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[j][h][s], d[s], q[h], 0, 0, 0);
+      for (int s = 0; s < NS; ++s) {
+        const int r = r0 + li, c = 4 * s + g;
+        d[s] = *reinterpret_cast<const bf16x8*>(dts + (r * 4 * NS + (c ^ (r & (4 * NS - 1)))) * 8);
       }
-      o[j] = u32x4{pack_bf16(q[0][0], q[0][1]), pack_bf16(q[0][2], q[0][3]), pack_bf16(q[1][0], q[1][1]),
-                   pack_bf16(q[1][2], q[1][3])};
-    }
+      f32x4v q[8];
 #pragma unroll
-    for (int j = 0; j < 4; j += 2) {
-      u32x4 lo, hi;  // rows 0..7 and rows 8..15 of channels 32 j .. 32 j + 63
+      for (int j = 0; j < 8; ++j) {
+        q[j] = f32x4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // Lanes 8..15 (bank mask 12) of each 16 take product j + 1's lanes 0..7;
-        // lanes 0..7 product j's lanes 8..15.
-        lo[i] = (uint32_t)__builtin_amdgcn_update_dpp((int)o[j][i], (int)o[j + 1][i], kDppRor + 8, 0xf, 0xc, false);
-        hi[i] = (uint32_t)__builtin_amdgcn_update_dpp((int)o[j + 1][i], (int)o[j][i], kDppRor + 8, 0xf, 0x3, false);
+        for (int s = 0; s < NS; ++s) q[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(d[s], w[j][s], q[j], 0, 0, 0);
       }
-      const int k = k0 + 32 * j + 32 * (li >> 3) + 8 * g;
-      if (k < p.K) {
-        const int64_t r = r0 + (li & 7);
-        if (r < end) st16_nt(p.dx + r * p.K + k, lo);
-        if (r + 8 < end) st16_nt(p.dx + (r + 8) * p.K + k, hi);
+      // q[j]: lane li is channel 8 li + j, element i is row 4 g + i.
+      if (in) {
+        bf16* out = p.dx + (c0 + r0 + 4 * g) * p.K + k;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (r0 + 4 * g + i < rows)
+            st16_nt(out + (int64_t)i * p.K, u32x4{pack_bf16(q[0][i], q[1][i]), pack_bf16(q[2][i], q[3][i]),
+                                                  pack_bf16(q[4][i], q[5][i]), pack_bf16(q[6][i], q[7][i])});
       }
     }
   }
@@ -629,7 +610,7 @@ __global__ __launch_bounds__(64) void lora8_sum_kernel(const float* part, bf16* 
 // CUs (registers: 4, 3, 2 and 1 a CU for ranks up to 16, 32, 48 and 64), but at
 // least 256 rows each (a partial sum is 4 R bytes a channel, 256 rows' codes
 // are 256). With one and a half rounds 7904 x 8192 at rank 40 took 32 us, with
-// one XX.
+// one 26.
 static int da_splits(int64_t M, int64_t K, int64_t R) {
   const int64_t cus = std::max(1, device_cu_count());
   const int64_t tiles = (K + kDaCols - 1) / kDaCols;
@@ -674,7 +655,7 @@ extern "C" int aa_gelu8_fwd(const void* x, void* y, void* codes, void* exps, int
   p.cpr = 4 * (int)((K + kGroup - 1) / kGroup);
   p.chunks = rows * p.cpr;
   const int64_t blocks = (p.chunks + kGeThreads * kGeChunks - 1) / (kGeThreads * kGeChunks);
-  if (blocks > 0x7fffffff) return fail(AA_EUNSUPPORTED, "gelu8: too many values");
+  if (!grid_fits(blocks, kGeThreads)) return fail(AA_EUNSUPPORTED, "gelu8: too many values");
   hipStream_t st = (hipStream_t)stream;
   if (K % kGroup == 0) gelu8_fwd_kernel<true><<<dim3((unsigned)blocks), kGeThreads, 0, st>>>(p);
   else gelu8_fwd_kernel<false><<<dim3((unsigned)blocks), kGeThreads, 0, st>>>(p);
@@ -698,7 +679,7 @@ extern "C" int aa_gelu8_bwd(const void* dy, const void* codes, const void* exps,
   p.cpr = 4 * (int)((K + kGroup - 1) / kGroup);
   p.chunks = rows * p.cpr;
   const int64_t blocks = (p.chunks + kGeThreads * kGeChunks - 1) / (kGeThreads * kGeChunks);
-  if (blocks > 0x7fffffff) return fail(AA_EUNSUPPORTED, "gelu8_bwd: too many values");
+  if (!grid_fits(blocks, kGeThreads)) return fail(AA_EUNSUPPORTED, "gelu8_bwd: too many values");
   hipStream_t st = (hipStream_t)stream;
   if (K % kGroup == 0) gelu8_bwd_kernel<true><<<dim3((unsigned)blocks), kGeThreads, 0, st>>>(p);
   else gelu8_bwd_kernel<false><<<dim3((unsigned)blocks), kGeThreads, 0, st>>>(p);
@@ -782,10 +763,10 @@ extern "C" int aa_lora8_bwd(const void* dt, const void* a, const void* codes, co
     p.K = (int)K;
     p.R = (int)R;
     const int64_t tiles = (K + kDxCols - 1) / kDxCols;
-    // Up to four workgroups a CU, each with at least 32 rows to spend the reading
-    // of its part of A on.
-    const int64_t per = (M * tiles + 4 * cus - 1) / (4 * cus);
-    p.rows = (int)((std::clamp<int64_t>(per, std::max<int64_t>(32, (M + 65534) / 65535), 1 << 20) + 15) / 16 * 16);
+    // One round of the three workgroups that fit on a CU, each with at least 32
+    // rows to spend the reading of its part of A on.
+    const int64_t per = (M * tiles + 3 * cus - 1) / (3 * cus);
+    p.rows = (int)((std::clamp<int64_t>(per, 32, 1 << 20) + 15) / 16 * 16);
     p.tiles = (int)tiles;
     p.groups = (int)((M + p.rows - 1) / p.rows);
     const dim3 grid(grid_blocks(tiles * p.groups));

@@ -506,53 +506,102 @@ __global__ __launch_bounds__(kBigThreads, 1) void int8_linear_big_kernel(I8Param
   }
 }
 
-// Few tokens: a workgroup takes 16 output channels, its four waves a quarter of
-// K each (64-byte steps in turn), TT tiles of 16 tokens. Operands go from
-// memory to registers: in v_mfma_i32_16x16x64_i8 lane l holds 16 bytes of row
-// l % 16 (a channel's weights, a token) at chunk l / 16 of the 64. The waves'
-// int32 sums are added in LDS.
-template <int TT>
+// Few tokens (M <= 8 XB): bound by reading the weights once. A workgroup takes 16
+// channels; its four waves take 128 bytes of K in turn, each through a ring of
+// LDS of its own, so nothing waits for another wave until the sums: per step two
+// DMAs of 8 channels x 128 bytes and XB of 8 tokens, kDepth steps ahead. 8192 x
+// 8192 weights: 14.8 us for 2 tokens, 14.9 for 16, 16.0 for 32, 20.8 for 64 (the
+// 128 x 128 tiles: 32). Operands straight from memory (16 rows x 16 bytes per quarter
+// wave, four times as many pieces of lines as a DMA's two rows x 128): 16.2,
+// 18.6, 25.2, 39.0; 32 channels a workgroup: 19.5, 20.1, 20.7, 23.1. In v_mfma_i32_16x16x64_i8 lane l holds 16 bytes of row l % 16 (a
+// channel, a token) at chunk l / 16 of the 64. The waves' int32 sums are added
+// in LDS.
+template <int XB>
+struct Skinny {
+  static constexpr int kTT = (XB + 1) / 2;         // token tiles of 16
+  static constexpr int kBlocks = 2 + XB;      // DMAs per step
+  static constexpr int kDepth = 20 / kBlocks;      // two workgroups a CU
+  static constexpr int kWaveBytes = kDepth * kBlocks * 1024;
+  static constexpr int kSums = 4 * kTT * 1024;
+  static constexpr int kLds = 4 * kWaveBytes > kSums ? 4 * kWaveBytes : kSums;
+};
+
+template <int XB>
 __global__ __launch_bounds__(256) void int8_skinny_kernel(I8Params p) {
-  __shared__ i32x4 part[4][TT][64];
+  using T = Skinny<XB>;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[T::kLds];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int li = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * 16;
   const int M = (int)p.M;
-  const uint8_t* w = p.w + (int64_t)min(n0 + li, p.N - 1) * p.K + 16 * g;
-  const uint8_t* x[TT];
+  // DMA roles as above: row lane >> 3 of a block, chunk (lane & 7) ^ row ^ parity.
+  const int drow = lane >> 3;
+  const uint8_t* src[T::kBlocks];
 #pragma unroll
-  for (int t = 0; t < TT; ++t) x[t] = p.x + (int64_t)min(16 * t + li, M - 1) * p.K + 16 * g;
-  i32x4 acc[TT];
-#pragma unroll
-  for (int t = 0; t < TT; ++t) acc[t] = i32x4{0, 0, 0, 0};
-  constexpr int kDepth = TT <= 2 ? 8 : 4;  // steps whose loads go out together
-  for (int k0 = 64 * wave; k0 < p.K; k0 += 256 * kDepth) {
-    i32x4 a[kDepth], b[kDepth][TT];
-#pragma unroll
-    for (int d = 0; d < kDepth; ++d) {
-      const int k = k0 + 256 * d;
-      const bool in = k + 16 * g < p.K;  // K is a multiple of 16
-      a[d] = i32x4{0, 0, 0, 0};
-      if (in) a[d] = *reinterpret_cast<const i32x4*>(w + k);
-#pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        b[d][t] = i32x4{0, 0, 0, 0};
-        if (in) b[d][t] = *reinterpret_cast<const i32x4*>(x[t] + k);
-      }
-    }
-#pragma unroll
-    for (int d = 0; d < kDepth; ++d)
-#pragma unroll
-      for (int t = 0; t < TT; ++t)
-        acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[d], b[d][t], acc[t], 0, 0, 0);
+  for (int i = 0; i < T::kBlocks; ++i) {
+    const bool is_w = i < 2;
+    const int b = is_w ? i : i - 2;
+    const int64_t row = is_w ? min(n0 + 8 * b + drow, p.N - 1) : min(8 * b + drow, M - 1);
+    src[i] = (is_w ? p.w : p.x) + row * p.K;
   }
+  const int c0 = 16 * ((lane & 7) ^ drow), c1 = c0 ^ 16;  // bytes of even and odd blocks' chunks
+  const uint32_t ring = lds_addr(lds) + (uint32_t)wave * T::kWaveBytes;
+  const int nk = (p.K + kIK - 1) / kIK;
+  const int n = (nk - wave + 3) / 4;  // this wave's steps
+  auto issue = [&](int i) {
+    const int k0 = (wave + 4 * i) * kIK;
+    const uint32_t dst = ring + (uint32_t)(i % T::kDepth) * (T::kBlocks * 1024u);
 #pragma unroll
-  for (int t = 0; t < TT; ++t) part[wave][t][lane] = acc[t];
+    for (int j = 0; j < T::kBlocks; ++j) {
+      const int k = k0 + ((j & 1) ? c1 : c0);
+      // Past the row's end: zeros (K is a multiple of 16).
+      dma16_a(k < p.K ? src[j] + k : (const uint8_t*)&kZeroChunk, dst + 1024u * j);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < T::kDepth; ++i)
+    if (i < n) issue(i);
+
+  i32x4 acc[T::kTT];
+#pragma unroll
+  for (int t = 0; t < T::kTT; ++t) acc[t] = i32x4{0, 0, 0, 0};
+  // Row li of a tile at chunk g: block li >> 3 (a tile of 8 tokens has one; its rows
+  // 8 to 15 are no tokens).
+  const int half = li >> 3;
+  const uint32_t at_w = half * 1024 + (li & 7) * 128 + (g ^ (li & 7) ^ half) * 16;
+  const uint32_t at_x = XB == 1 ? (li & 7) * 128 + (g ^ (li & 7)) * 16 : at_w;
+  for (int i = 0; i < n; ++i) {
+    if (i + T::kDepth <= n) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((T::kDepth - 1) * T::kBlocks) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const uint32_t slot = ring + (uint32_t)(i % T::kDepth) * (T::kBlocks * 1024u);
+    i32x4 a[2], b[2][T::kTT];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {  // chunks 4 h + g: bit 6 of the address
+      a[h] = __builtin_bit_cast(i32x4, lds_ld16((slot + at_w) ^ (64u * h)));
+#pragma unroll
+      for (int t = 0; t < T::kTT; ++t)
+        b[h][t] = __builtin_bit_cast(i32x4, lds_ld16((slot + 2048u + 2048u * t + at_x) ^ (64u * h)));
+    }
+    // The reads are back before the step kDepth on takes their place.
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (i + T::kDepth < n) issue(i + T::kDepth);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int t = 0; t < T::kTT; ++t)
+        acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[h], b[h][t], acc[t], 0, 0, 0);
+  }
+  __syncthreads();  // every wave is done with its ring
+  i32x4* part = reinterpret_cast<i32x4*>(lds);
+#pragma unroll
+  for (int t = 0; t < T::kTT; ++t) part[(wave * T::kTT + t) * 64 + lane] = acc[t];
   __syncthreads();
-  // Wave t of the first TT adds tile t: token 16 t + li, channels 4 g .. 4 g + 3.
-  for (int t = wave; t < TT; t += 4) {
-    const i32x4 s = part[0][t][lane] + part[1][t][lane] + part[2][t][lane] + part[3][t][lane];
+  // Tile t: token 16 t + li, channels 4 g .. 4 g + 3.
+  for (int t = wave; t < T::kTT; t += 4) {
+    i32x4 s = part[t * 64 + lane];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) s += part[(w * T::kTT + t) * 64 + lane];
     const int tok = 16 * t + li, ch = n0 + 4 * g;
     if (tok < M && ch < p.N) {
       const float rs = p.xs[tok];
@@ -575,7 +624,8 @@ extern "C" int aa_rowquant_int8(const void* x, int64_t rows, int64_t K, int gelu
   if (rows < 0 || K <= 0) return fail(AA_EINVAL, "rowquant_int8: bad rows/K");
   if (K % 8 != 0 || K > kQ8MaxK)
     return fail(AA_EUNSUPPORTED, "rowquant_int8: K must be a multiple of 8 and at most 8192");
-  if (rows > 0x7fffff00) return fail(AA_EUNSUPPORTED, "rowquant_int8: too many rows");
+  if (rows > 0x7fffff00 || !grid_fits((rows + kQ8Rows - 1) / kQ8Rows, kQ8Threads))
+    return fail(AA_EUNSUPPORTED, "rowquant_int8: too many rows");
   if (rows == 0) return AA_OK;
   if (!x || !q || !s) return fail(AA_EINVAL, "rowquant_int8: null pointer");
   if (!aligned16(x) || ((uintptr_t)q & 7u) != 0)
@@ -625,15 +675,18 @@ extern "C" int aa_int8_linear(const void* q, const float* s, const void* weight,
   hipStream_t st = (hipStream_t)stream;
   if (M <= 64) {
     const dim3 grid((unsigned)((N + 15) / 16));
-    if (M <= 16) int8_skinny_kernel<1><<<grid, 256, 0, st>>>(p);
-    else if (M <= 32) int8_skinny_kernel<2><<<grid, 256, 0, st>>>(p);
-    else int8_skinny_kernel<4><<<grid, 256, 0, st>>>(p);
+    if (M <= 8) int8_skinny_kernel<1><<<grid, 256, 0, st>>>(p);
+    else if (M <= 16) int8_skinny_kernel<2><<<grid, 256, 0, st>>>(p);
+    else if (M <= 32) int8_skinny_kernel<4><<<grid, 256, 0, st>>>(p);
+    else int8_skinny_kernel<8><<<grid, 256, 0, st>>>(p);
     return check_launch("int8_linear");
   }
   const int64_t cus = std::max(1, device_cu_count());
   const int64_t ntn = (N + kBigTile - 1) / kBigTile, mtn = (M + kBigTile - 1) / kBigTile;
   const auto small_tiles = [&](int64_t rows) { return (rows + 127) / 128 * ((N + 127) / 128); };
-  // Time of the small tiles over `rows` tokens, in rounds of large tiles: XX
+  // Time of the small tiles over `rows` tokens, in rounds of large tiles. Measured:
+  // a round of large tiles 37.5 us at K = 2048 and 109 at 8192; of small ones, one
+  // a CU 14.4 and 40.4, two a CU 20 to 23.5 and 67.7.
   const auto small_time = [&](int64_t rows) {
     const int64_t t = small_tiles(rows);
     return t <= cus ? kSmallAlone : (double)((t + 2 * cus - 1) / (2 * cus)) * kSmallPair;
@@ -652,7 +705,7 @@ extern "C" int aa_int8_linear(const void* q, const float* s, const void* weight,
       big = rows;
     }
   }
-  if (small_tiles(M) > 0x7fffffff) return fail(AA_EUNSUPPORTED, "int8_linear: too many tokens");
+  if (!grid_fits(small_tiles(M), 256)) return fail(AA_EUNSUPPORTED, "int8_linear: too many tokens");
   if (big > 0) {
     p.M = big;
     p.mtiles = (int)((big + kBigTile - 1) / kBigTile);
@@ -666,7 +719,9 @@ extern "C" int aa_int8_linear(const void* q, const float* s, const void* weight,
     p.M = M - big;
     p.mtiles = (int)((p.M + 127) / 128);
     const int64_t t = small_tiles(p.M);
-    if (t <= cus && K >= 4096) int8_linear_kernel<I8TileD><<<dim3((unsigned)t), I8TileD::kThreads, 0, st>>>(p);
+    // One workgroup a CU: the deeper ring, for weights that are not in a cache (666 x
+    // 1024 x 4096: 11.4 -> 9.4 us; where they are, 8.8 against 9.4).
+    if (t <= cus) int8_linear_kernel<I8TileD><<<dim3((unsigned)t), I8TileD::kThreads, 0, st>>>(p);
     else int8_linear_kernel<I8TileC><<<dim3((unsigned)t), I8TileC::kThreads, 0, st>>>(p);
   }
   return check_launch("int8_linear");

@@ -160,6 +160,16 @@ def test_gradients(adaln, B, S, D, kind):
     _check_gradients(t, names, _gradients(adaln, t, names, dr, dh), dr, dh)
 
 
+def test_weight_in_bf16(adaln):
+    """Widened for the kernel; its gradient comes back in bf16."""
+    t = _inputs(2, 21, 264, 31, post=True)
+    t["weight"] = t["weight"].to(BF)
+    names = ["x", "y", "gate", "scale", "shift", "weight"]
+    g = gen(32)
+    dr, dh = bf(g, 2, 21, 264), bf(g, 2, 21, 264)
+    _check_gradients(t, names, _gradients(adaln, t, names, dr, dh), dr, dh)
+
+
 @pytest.mark.parametrize("which", ["r", "h"])
 def test_one_output_used(adaln, which):
     """The gradient of the other output is None inside: it counts as zero."""

@@ -112,6 +112,17 @@ def test_product(int8, M, K, N):
     _check_product(*args, int8.int8_linear(*args))
 
 
+# Whole rounds of the 256 x 256 tiles (256 of them on 256 CUs), partial ones in both directions,
+# one to four stages of K with rests, and tokens left over for the small tiles.
+@pytest.mark.parametrize("M,K,N", [
+    (8192, 16, 2048), (8100, 112, 2040), (8192, 128, 2048), (8100, 144, 2040), (8192, 256, 2048), (8065, 400, 1800),
+    (8192, 512, 2048), (18000, 528, 2040), (16385, 2048, 2048), (260, 1040, 65544),
+])
+def test_large_product(int8, M, K, N):
+    args = _product(int8, M, K, N, M + K + N, full=True)
+    _check_product(*args, int8.int8_linear(*args))
+
+
 def test_largest_sums(int8):
     """All codes at -128 or 127, K at its most: 65536 products of up to 2^14."""
     for M in (3, 130):
