@@ -1,4 +1,4 @@
-// Device arithmetic shared by the block's operators (adaln.hip, int8_rows.hip,
+// Device arithmetic shared by the block's operators (adaln.hip, int8_linear.hip,
 // ckpt8.hip): wave reductions in the vector ALU, GELU, 8-bit encodings.
 #pragma once
 

@@ -414,7 +414,9 @@ int64_t mod_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : 0; }
 
 bool adaln_ready(const Tensor& x, const Tensor* y, const Tensor* gate, const Tensor& scale, const OptT& weight) {
   return rows_ready(x, x) && (!y || (rows_ready(*y, x) && y->sizes() == x.sizes() && gate && mod_ready(*gate, x, scale))) &&
-         mod_ready(scale, x, scale) && (!weight || (weight->numel() == x.size(2) && on_gpu(*weight, x)));
+         mod_ready(scale, x, scale) &&
+         (!weight || (weight->dim() == 1 && weight->size(0) == x.size(2) && on_gpu(*weight, x) &&
+                      (weight->scalar_type() == at::kFloat || weight->scalar_type() == at::kBFloat16)));
 }
 
 // fp32 weight that lives until the launch.
@@ -611,7 +613,7 @@ T3 gelu8(const Tensor& x, bool keep) {
 // A checkpoint of `rows` rows of K channels, with exponents of n elements.
 bool kept_ready(const Tensor& codes, const Tensor& exps, const Tensor& like, int64_t rows, int64_t K, int64_t n) {
   return codes.scalar_type() == at::kChar && exps.scalar_type() == at::kByte && on_gpu(codes, like) && on_gpu(exps, like) &&
-         codes.numel() == rows * ((K + 31) / 32 * 32) && exps.numel() == n && codes.is_contiguous() && exps.is_contiguous() &&
+         codes.numel() == rows * ((K + 31) / 32 * 32) && exps.numel() == n && codes.dim() == 2 && exps.dim() == 2 && codes.is_contiguous() && exps.is_contiguous() &&
          aligned16(codes) && aligned16(exps);
 }
 
@@ -867,6 +869,31 @@ Tensor head_norm_autograd(CT x, CT w, int64_t heads, double eps) {
   return HeadNorm::apply(x, w, heads, eps);
 }
 
+// Whether the gradient of t goes to a leaf (t itself, or through casts and views)
+// whose accumulator lives already, made by an eager graph on the default stream.
+bool leaf_on_default_stream(const Tensor& t) {
+  if (!t.defined() || !t.requires_grad()) return false;
+  std::shared_ptr<torch::autograd::Node> node =
+      t.grad_fn() ? t.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(t);
+  while (node && node->num_outputs() == 1) node = node->next_edge(0).function;
+  if (!node || node->num_outputs() != 0) return false;
+  const auto stream = node->stream();
+  return stream && stream->device_type() == c10::DeviceType::CUDA &&
+         *stream == c10::hip::getDefaultHIPStreamMasqueradingAsCUDA(stream->device_index()).unwrap();
+}
+// The backward of a captured forward would make the default stream wait for captured
+// work in such a place, which it cannot join: that ends the capture, and the process
+// with it. (Any other stream joins the capture.)
+template <class... T>
+void check_capture(const Tensor& x, const T&... more) {
+  const hipStream_t stream = (hipStream_t)stream_of(x);
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (!stream || hipStreamIsCapturing(stream, &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+  TORCH_CHECK(!(leaf_on_default_stream(x) || ... || leaf_on_default_stream(more)),
+              "a forward with gradients is being captured while an eager graph of the same leaves lives: "
+              "its accumulators are on the default stream, which cannot join the capture; end that graph first");
+}
+
 // The statistics and 8-bit copies, which have no derivative, are handed past
 // the node as the LSE is.
 struct ResidualAdaln : torch::autograd::Function<ResidualAdaln> {
@@ -907,6 +934,7 @@ T3 residual_adaln_autograd(CT x, CT y, CT gate, CT scale, CT shift, CO weight, d
                            bool want_stats) {
   if (!needs_grad(x, y, gate, scale, shift, weight))
     return op_residual_adaln().below(x, y, gate, scale, shift, weight, eps, branch_scale, want_stats);
+  check_capture(x, y, gate, scale, shift, weight.value_or(Tensor()));
   const bool mods = gate.requires_grad() || scale.requires_grad() || shift.requires_grad() ||
                     (weight && weight->requires_grad());
   Tensor stats;
@@ -943,6 +971,7 @@ struct Adaln : torch::autograd::Function<Adaln> {
 
 T2 adaln_autograd(CT x, CT scale, CT shift, double eps, bool want_stats) {
   if (!needs_grad(x, scale, shift)) return op_adaln().below(x, scale, shift, eps, want_stats);
+  check_capture(x, scale, shift);
   Tensor stats;
   Tensor h = Adaln::apply(x, scale, shift, eps, scale.requires_grad() || shift.requires_grad(), &stats);
   return {h, stats};
@@ -968,6 +997,7 @@ struct Gelu8 : torch::autograd::Function<Gelu8> {
 
 T3 gelu8_autograd(CT x, bool keep) {
   if (!needs_grad(x)) return op_gelu8().below(x, keep);
+  check_capture(x);
   Tensor codes, exps;
   Tensor y = Gelu8::apply(x, &codes, &exps);
   return {y, codes, exps};
@@ -998,6 +1028,7 @@ struct LoraDown8 : torch::autograd::Function<LoraDown8> {
 
 T3 lora_down8_autograd(CT x, CT a, bool keep) {
   if (!needs_grad(x, a)) return op_lora_down8().below(x, a, keep);
+  check_capture(x, a);
   Tensor codes, exps;
   Tensor t = LoraDown8::apply(x, a, x.requires_grad(), a.requires_grad(), &codes, &exps);
   return {t, codes, exps};

@@ -101,7 +101,15 @@ def _forward(x, y, gate, scale, shift, weight, eps, branch_scale, want_stats, in
 
 def _backward(dr, dh, x, y, gate, scale, weight, stats, shift_rows, branch_scale, mods):
     """(dx, dy, dgate, dscale, dshift, dweight); what is not computed has no elements."""
+    _check_arguments(x, y, gate, scale, None, weight)
     B, S, D = x.shape
+    for t in (dr, dh):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype or t.device != x.device):
+            raise ValueError("gradients must have the outputs' shape, dtype and device")
+    if stats.shape != (B * S, 4) or stats.dtype != torch.float32 or stats.device != x.device or not stats.is_contiguous():
+        raise ValueError("stats must be those of the forward")
+    if (y is None) != (gate is None) or shift_rows not in (1, B):
+        raise ValueError("y and gate belong together, and shift has 1 or B rows")
     dr, dh, x, y = (None if t is None else aligned(t.contiguous()) for t in (dr, dh, x, y))
     gate, scale = _readable(gate), _readable(scale)
     dx = torch.empty_like(x)
@@ -306,7 +314,8 @@ def residual_adaln(x, y, gate, scale, shift, weight=None, eps=1e-6, branch_scale
     Returns:
         `(r, h)`: `r = x + branch_scale * gate * y` (y normed with `weight`) and
         `h = LayerNorm(r) * (1 + scale) + shift`, both bfloat16 `[B, S, D]`. Differentiable
-        in every tensor.
+        in every tensor, once (no second derivatives); in modulations and weight for at most
+        65535 batch items.
 
     Raises:
         ValueError: If a tensor is not on CUDA, or its shape or dtype is not supported.

@@ -62,6 +62,14 @@ def _kept(x: torch.Tensor, keep: bool, exps_shape: tuple[int, int]) -> tuple[tor
     return codes, exps
 
 
+def _check_kept(g: torch.Tensor, codes: torch.Tensor, exps: torch.Tensor, K: int, exps_shape: tuple[int, int]) -> None:
+    """The copy that the forward of [B, S, K] tokens made, for a gradient of [B, S, ...]."""
+    rows = g.shape[0] * g.shape[1]
+    for t, shape, dtype in ((codes, (rows, GROUP * _groups(K)), torch.int8), (exps, exps_shape, torch.uint8)):
+        if t.shape != shape or t.dtype != dtype or t.device != g.device or not t.is_contiguous():
+            raise ValueError("codes and exps must be those of the forward")
+
+
 def _ptr(t: torch.Tensor):
     return t.data_ptr() if t.numel() else None
 
@@ -95,7 +103,9 @@ def _(x, keep):
 
 @custom_op("anima_flat_amd::gelu8_bwd", mutates_args=())
 def _gelu8_bwd(dy: torch.Tensor, codes: torch.Tensor, exps: torch.Tensor) -> torch.Tensor:
+    _check_tokens(dy)
     B, S, K = dy.shape
+    _check_kept(dy, codes, exps, K, (B * S, _groups(K)))
     dy = aligned(dy.contiguous())
     dx = torch.empty_like(dy)
     with torch.cuda.device(dy.device):
@@ -164,8 +174,13 @@ def _(x, a, keep):
 def _lora_down8_bwd(
     dt: torch.Tensor, a: torch.Tensor, codes: torch.Tensor, exps: torch.Tensor, need_x: bool, need_a: bool
 ) -> tuple[torch.Tensor, torch.Tensor]:
-    B, S, R = dt.shape
-    K = a.shape[1]
+    _check(dt, a)
+    if dt.ndim != 3 or a.ndim != 2 or dt.shape[2] != a.shape[0] or any(t.dtype != torch.bfloat16 for t in (dt, a)):
+        raise ValueError("dt must be bfloat16 [B, S, R] and a bfloat16 [R, K]")
+    B, S, _ = dt.shape
+    R, K = a.shape
+    if need_a:
+        _check_kept(dt, codes, exps, K, (_groups(K), -(-B * S // 16) * 16))
     dt, a = aligned(dt.contiguous()), aligned(a.contiguous())
     dx = dt.new_empty((B, S, K) if need_x else 0)
     da = dt.new_empty(a.shape if need_a else 0)

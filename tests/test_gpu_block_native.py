@@ -147,3 +147,86 @@ def test_no_gradient_through_int8(mods):
             call()
         with torch.no_grad():
             call()
+
+
+def test_refusals_on_the_gpu(mods):
+    """What the native kernels do not take is refused as the fakes refuse it, before any launch."""
+    adaln, int8, ckpt8 = mods
+
+    def t(*shape, dtype=BF):
+        return torch.zeros(*shape, dtype=dtype, device="cuda")
+
+    x, m = t(2, 5, 64), t(2, 64)
+    cases = [
+        (f, args, says) for f in (adaln.residual_adaln, adaln.residual_adaln_int8) for args, says in (
+            ((x.half(), x.half(), m, m, m), "only bfloat16"),
+            ((x, t(2, 5, 72), m, m, m), "x's shape"),
+            ((x, x.cpu(), m, m, m), "CUDA tensors"),
+            ((x[0], x[0], m, m, m), "must be .B, S, D"),
+            ((t(2, 5, 60), t(2, 5, 60), t(2, 60), t(2, 60), t(2, 60)), "multiple of 8"),
+            ((t(1, 2, 8200), t(1, 2, 8200), t(8200), t(8200), t(8200)), "at most 8192"),
+            ((x, x, t(3, 64), m, m), "gate must be"),
+            ((x, x, m, t(2, 5, 64), m), "scale must be"),
+            ((x, x, m, m, t(2, 32)), "shift must be"),
+            ((x, x, m, m, m.half()), "must be bfloat16 or float32"),
+            ((x, x, m, m, m, t(32)), "weight must be"),
+            ((x, x, m, m, m, t(1, 64)), "weight must be"),
+            ((x, x, m, m, m, t(64).half()), "weight must be"),
+            ((x, x, m, m, m, t(64).double()), "weight must be"),
+        )
+    ]
+    q, s, w, ws = t(2, 5, 64, dtype=torch.int8), t(10, 1, dtype=torch.float32), t(8, 64, dtype=torch.int8), t(8, dtype=torch.float32)
+    cases += [(int8.int8_linear, args, says) for args, says in (
+        ((x, s, w, ws), "q must be"), ((q[0], s, w, ws), "q must be"), ((q, s[:9], w, ws), "s must be"),
+        ((q, s.half(), w, ws), "s must be"), ((q, s, w[:, :48], ws), "weight must be"),
+        ((q, s, w.float(), ws), "weight must be"), ((q, s, w, ws[:4]), "weight_scale must be"),
+        ((q, s, w, ws.double()), "weight_scale must be"), ((q, s, w, ws.cpu()), "CUDA tensors"),
+        ((q[..., :24], s, w[:, :24], ws), "multiple of 16"), ((q, s, w[:4], ws[:4]), "multiple of 8"),
+    )]
+    cases += [
+        (int8.rowquant_int8, (m,), "B, S, K"), (int8.rowquant_int8, (x.half(),), "only bfloat16"),
+        (int8.rowquant_int8, (t(1, 1, 12),), "multiple of 8"), (int8.rowquant_int8, (t(1, 1, 8200),), "at most 8192"),
+        (ckpt8.gelu8, (x.float(),), "only bfloat16"), (ckpt8.gelu8, (x[0],), "B, S, K"),
+        (ckpt8.gelu8, (t(1, 1, 12),), "multiple of 8"), (ckpt8.gelu8, (t(1, 1, 65544),), "at most 65536"),
+    ] + [(ckpt8.lora_down8, (x, a), says) for a, says in (
+        (t(12, 64), "rank"), (t(72, 64), "rank"), (t(0, 64), "rank"), (t(8, 72), "a must be"),
+        (t(8, 64).float(), "a must be"), (t(8, 64).cpu(), "CUDA tensors"),
+    )]
+    for call, args, says in cases:
+        with pytest.raises(ValueError, match=says):
+            call(*args)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_inference_mode(mods, name):
+    run = _calls(mods)[name]
+    x = bf(gen(12), 1, 40, 256)
+    want = run(x)
+    with torch.inference_mode():
+        assert torch.equal(run(x), want)
+    assert torch.equal(run(x), want)
+
+
+def test_backward_refuses_what_is_not_the_forwards(mods):
+    """The backward ops take only statistics and copies of the sizes that their forward makes."""
+    ops = torch.ops.anima_flat_amd
+    cases = _cases()
+
+    def refused(name, args, *changes):
+        for at, value in changes:
+            changed = list(args)
+            changed[at] = value
+            with pytest.raises(ValueError):
+                getattr(ops, name)(*changed)
+
+    args = cases["adaln_bwd"][0]
+    dr, x, stats = args[0], args[2], args[7]
+    refused("adaln_bwd", args, (0, dr[:1]), (0, dr.float()), (1, dr[..., :256]), (3, None), (4, None), (7, stats[:-1]),
+            (7, stats.half()), (7, stats.cpu()), (8, 3), (2, x[:1]))
+    dy, codes, exps = cases["gelu8_bwd"][0]
+    refused("gelu8_bwd", (dy, codes, exps), (0, dy.float()), (0, dy[:1]), (1, codes[:-1]), (1, codes.cpu()), (2, exps[:, :-1]),
+            (2, exps.float()))
+    args = cases["lora_down8_bwd"][0]
+    dt, a, codes, exps = args[:4]
+    refused("lora_down8_bwd", args, (0, dt.float()), (0, dt[..., :8]), (0, dt[:1]), (1, a[:8]), (1, a.cpu()), (2, codes[:-1]),
+            (3, exps[:-1]))

@@ -249,3 +249,33 @@ def test_two_norms_of_one_stream(mods):
     assert (h.float() - h2.float()).abs().max() < 0.05  # of the fp32 r, of the bf16 r
     dx, dr = torch.autograd.grad([h, h2], [x, r], [torch.ones_like(h), torch.ones_like(h)])
     assert torch.isfinite(dx.float()).all() and torch.isfinite(dr.float()).all()
+
+
+def test_capture_beside_a_live_graph(mods):
+    """A captured forward with gradients is refused while an eager graph of its leaves lives on
+    the default stream (whose accumulators could not join the capture), and taken after it."""
+    adaln, _, ckpt8 = mods
+    g = gen(61)
+    x, a, m = bf(g, 1, 40, 64).requires_grad_(True), torch.randn(8, 64, generator=g).cuda().requires_grad_(True), bf(g, 1, 64)
+    dt = bf(g, 1, 40, 8)
+    steps = [
+        lambda: torch.autograd.grad(adaln.residual_adaln(x, x, m, m, m)[1], [x], x.detach()),
+        lambda: torch.autograd.grad(adaln.adaln(x, m, m), [x], x.detach()),
+        lambda: torch.autograd.grad(ckpt8.gelu8(x), [x], x.detach()),
+        lambda: torch.autograd.grad(ckpt8.lora_down8(x.detach(), a.to(BF)), [a], dt),
+    ]
+    want = [[t.clone() for t in step()] for step in steps]
+    live = x.float() * 2, a.to(BF)
+    for step in steps:
+        with pytest.raises(RuntimeError, match="eager graph of the same leaves"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                step()
+        torch.cuda.synchronize()
+    del live
+    for step, first in zip(steps, want):
+        graph, out = _captured(step)
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(out, first))
+            assert all(torch.equal(p, q) for p, q in zip(step(), first))
