@@ -332,8 +332,11 @@ __global__ __launch_bounds__(64 * lora_waves(16 * NR)) void lora8_fwd_kernel(Lor
 // every eighth piece of each row, and with rows of a power of two of bytes
 // those lie in 2 to 4 of its L2's 16 channels.
 static unsigned grid_blocks(int64_t n) { return (unsigned)((n + 7) / 8 * 8); }
-__device__ __forceinline__ bool grid_place(int tiles, int groups, int* tile, int* group) {
-  const int n = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
+struct Block {
+  int at, of;  // this workgroup among those of its work
+};
+__device__ __forceinline__ bool grid_place(Block b, int tiles, int groups, int* tile, int* group) {
+  const int n = (b.at & 7) * (b.of >> 3) + (b.at >> 3);
   *group = n / tiles;
   *tile = n - *group * tiles;
   return *group < groups;
@@ -360,16 +363,19 @@ struct LoraDx {
 constexpr int kDxCols = 512;
 constexpr int kDxRows = 128;
 
+template <int NS>
+constexpr int dx_lds() { return kDxRows * 32 * NS * 2; }
+
 template <int NS>  // 32 ranks per step
-__global__ __launch_bounds__(256) void lora8_dx_kernel(LoraDx p) {
+__device__ __forceinline__ void lora8_dx(const LoraDx& p, uint8_t* lds, Block block) {
   // dt's rows, 16-byte chunk c (8 ranks) of row r at slot c ^ (r & (4 NS - 1)).
-  __shared__ __attribute__((aligned(16))) bf16 dts[kDxRows * 32 * NS];
+  bf16* dts = reinterpret_cast<bf16*>(lds);
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int li = lane & 15, g = lane >> 4;
   int bx, by;
-  if (!grid_place(p.tiles, p.groups, &bx, &by)) return;
+  if (!grid_place(block, p.tiles, p.groups, &bx, &by)) return;
   const int k = bx * kDxCols + 128 * wave + 8 * li;  // this lane's channels
   const bool in = k < p.K;
   bf16x8 w[8][NS];
@@ -451,14 +457,17 @@ constexpr int kDaThreads = 64 * kDaWaves;
 constexpr int kDaRows = 32 * kDaWaves;  // rows of a turn
 constexpr int kDaCols = 128;
 
+// Row pitch in LDS: a multiple of 8 bytes whose 16-row stride spreads over the
+// banks (the transposed reads take 4 rows x 32 bytes per 16 lanes).
+constexpr int da_pitch(int NR) { return 16 * NR + 4; }
 template <int NR>
-__global__ __launch_bounds__(kDaThreads, NR < 4 ? 2 : 1) void lora8_da_kernel(LoraDa p) {
-  // Row pitch in LDS: a multiple of 8 bytes whose 16-row stride spreads over the
-  // banks (the transposed reads take 4 rows x 32 bytes per 16 lanes).
-  constexpr int kPitch = 16 * NR + 4;
-  constexpr int kDt = 2 * kDaRows * kPitch * 2;  // two turns' dt
-  constexpr int kSum = kDaWaves * NR * 4 * kDaCols * 4;  // one element i of every wave at a time
-  __shared__ __attribute__((aligned(16))) uint8_t lds[kDt > kSum ? kDt : kSum];
+constexpr int da_lds() {  // two turns' dt, or one element i of every wave's sums
+  return std::max(2 * kDaRows * da_pitch(NR) * 2, kDaWaves * NR * 4 * kDaCols * 4);
+}
+
+template <int NR>
+__device__ __forceinline__ void lora8_da(const LoraDa& p, uint8_t* lds, Block block) {
+  constexpr int kPitch = da_pitch(NR);
   bf16* dts = reinterpret_cast<bf16*>(lds);
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -466,7 +475,7 @@ __global__ __launch_bounds__(kDaThreads, NR < 4 ? 2 : 1) void lora8_da_kernel(Lo
   const int li = lane & 15, g = lane >> 4;
   // The codes' rows are padded to whole groups; channels past them read the last.
   int bx, by;
-  if (!grid_place((p.K + kDaCols - 1) / kDaCols, p.splits, &bx, &by)) return;
+  if (!grid_place(block, (p.K + kDaCols - 1) / kDaCols, p.splits, &bx, &by)) return;
   const int col = min(bx * kDaCols + 8 * li, kGroup * p.G - 8);
   const int grp = col / kGroup;
   const int64_t begin = (int64_t)by * p.rows, end = min(p.M, begin + p.rows);
@@ -596,6 +605,34 @@ __global__ __launch_bounds__(kDaThreads, NR < 4 ? 2 : 1) void lora8_da_kernel(Lo
   }
 }
 
+template <int NS>
+__global__ __launch_bounds__(256) void lora8_dx_kernel(LoraDx p) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[dx_lds<NS>()];
+  lora8_dx<NS>(p, lds, {(int)blockIdx.x, (int)gridDim.x});
+}
+template <int NR>
+__global__ __launch_bounds__(kDaThreads, NR < 4 ? 2 : 1) void lora8_da_kernel(LoraDa p) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[da_lds<NR>()];
+  lora8_da<NR>(p, lds, {(int)blockIdx.x, (int)gridDim.x});
+}
+// Both in one launch, eight workgroups (one an XCD) of each in turn: dx is bound by
+// its stores and dA by the vector instructions that unpack the codes, so that a CU
+// with workgroups of both does better than one after the other. 7904 x 8192, one
+// launch against two: rank 16 39 against 49 us, rank 32 45 against 51, rank 40 52
+// against 56. Above rank 48 dA's registers leave a CU one workgroup, of either
+// (rank 64: 84 against 64), and two launches are made.
+template <int NR>
+__global__ __launch_bounds__(kDaThreads, 2) void lora8_both_kernel(LoraDx x, LoraDa a, int nx, int na) {
+  constexpr int NS = (NR + 1) / 2;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[std::max(dx_lds<NS>(), da_lds<NR>())];
+  const int u = blockIdx.x >> 3, xcd = blockIdx.x & 7;
+  const int pairs = min(nx, na) >> 3;  // units of eight of each
+  const bool dx = u < 2 * pairs ? (u & 1) == 0 : nx > na;
+  const int at = 8 * (u < 2 * pairs ? u >> 1 : u - pairs) + xcd;
+  if (dx) lora8_dx<NS>(x, lds, {at, nx});
+  else lora8_da<NR>(a, lds, {at, na});
+}
+
 // Adds the ranges' partial sums of t or dA in order, four values per lane.
 __global__ __launch_bounds__(64) void lora8_sum_kernel(const float* part, bf16* out, int64_t n, int splits) {
   const int64_t at = ((int64_t)blockIdx.x * 64 + threadIdx.x) * 4;
@@ -606,15 +643,14 @@ __global__ __launch_bounds__(64) void lora8_sum_kernel(const float* part, bf16* 
   *reinterpret_cast<u32x2*>(out + at) = u32x2{pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3])};
 }
 
-// Ranges of rows of the dA product: one round of the workgroups that fit on the
-// CUs (registers: 4, 3, 2 and 1 a CU for ranks up to 16, 32, 48 and 64), but at
-// least 256 rows each (a partial sum is 4 R bytes a channel, 256 rows' codes
-// are 256). With one and a half rounds 7904 x 8192 at rank 40 took 32 us, with
-// one 26.
+// Ranges of rows of the dA product: two workgroups a CU (one above rank 48, where no
+// more fit), but at least 256 rows each (a partial sum is 4 R bytes a channel, 256
+// rows' codes are 256). 7904 x 8192, one, two and four a CU: rank 16 28, 24 and 27
+// us; rank 40 35, 31 and, two at a time, 32.
 static int da_splits(int64_t M, int64_t K, int64_t R) {
   const int64_t cus = std::max(1, device_cu_count());
   const int64_t tiles = (K + kDaCols - 1) / kDaCols;
-  const int64_t want = std::max<int64_t>(1, (5 - (R + 15) / 16) * cus / tiles);
+  const int64_t want = std::max<int64_t>(1, (R <= 48 ? 2 : 1) * cus / tiles);
   return (int)std::clamp<int64_t>(std::min(want, (M + 255) / 256), 1, 65535);
 }
 
@@ -754,47 +790,59 @@ extern "C" int aa_lora8_bwd(const void* dt, const void* a, const void* codes, co
   if (need && (!workspace || workspace_bytes < need)) return fail(AA_EINVAL, "lora8_bwd: workspace too small");
   hipStream_t st = (hipStream_t)stream;
   const int64_t cus = std::max(1, device_cu_count());
+  LoraDx x;
+  LoraDa p;
+  unsigned nx = 0, na = 0;
   if (dx) {
-    LoraDx p;
+    x.dt = (const bf16*)dt;
+    x.a = (const bf16*)a;
+    x.dx = (bf16*)dx;
+    x.M = M;
+    x.K = (int)K;
+    x.R = (int)R;
+    const int64_t tiles = (K + kDxCols - 1) / kDxCols;
+    // Two workgroups a CU (one to six: within 3 us of each other at 7904 x 8192), each
+    // with at least 32 rows to spend the reading of its part of A on.
+    const int64_t per = (M * tiles + 2 * cus - 1) / (2 * cus);
+    x.rows = (int)((std::clamp<int64_t>(per, 32, 1 << 20) + 15) / 16 * 16);
+    x.tiles = (int)tiles;
+    x.groups = (int)((M + x.rows - 1) / x.rows);
+    nx = grid_blocks(tiles * x.groups);
+  }
+  if (da) {
     p.dt = (const bf16*)dt;
-    p.a = (const bf16*)a;
-    p.dx = (bf16*)dx;
+    p.codes = (const uint8_t*)codes;
+    p.exps = (const uint8_t*)exps;
+    p.part = (float*)workspace;
+    p.da = (bf16*)da;
     p.M = M;
+    p.Mp = (M + 15) / 16 * 16;
     p.K = (int)K;
     p.R = (int)R;
-    const int64_t tiles = (K + kDxCols - 1) / kDxCols;
-    // One round of the three workgroups that fit on a CU, each with at least 32
-    // rows to spend the reading of its part of A on.
-    const int64_t per = (M * tiles + 3 * cus - 1) / (3 * cus);
-    p.rows = (int)((std::clamp<int64_t>(per, 32, 1 << 20) + 15) / 16 * 16);
-    p.tiles = (int)tiles;
-    p.groups = (int)((M + p.rows - 1) / p.rows);
-    const dim3 grid(grid_blocks(tiles * p.groups));
-    if (R <= 32) lora8_dx_kernel<1><<<grid, 256, 0, st>>>(p);
-    else lora8_dx_kernel<2><<<grid, 256, 0, st>>>(p);
-    if (int rc = check_launch("lora8_bwd")) return rc;
+    p.G = (int)((K + kGroup - 1) / kGroup);
+    p.splits = da_splits(M, K, R);
+    // Ranges of whole turns' rows; the last ones may be empty and write zeros.
+    p.rows = (int)(((M + p.splits - 1) / p.splits + kDaRows - 1) / kDaRows * kDaRows);
+    na = grid_blocks((K + kDaCols - 1) / kDaCols * p.splits);
   }
-  if (!da) return AA_OK;
-  LoraDa p;
-  p.dt = (const bf16*)dt;
-  p.codes = (const uint8_t*)codes;
-  p.exps = (const uint8_t*)exps;
-  p.part = (float*)workspace;
-  p.da = (bf16*)da;
-  p.M = M;
-  p.Mp = (M + 15) / 16 * 16;
-  p.K = (int)K;
-  p.R = (int)R;
-  p.G = (int)((K + kGroup - 1) / kGroup);
-  p.splits = da_splits(M, K, R);
-  // Ranges of whole turns' rows; the last ones may be empty and write zeros.
-  p.rows = (int)(((M + p.splits - 1) / p.splits + kDaRows - 1) / kDaRows * kDaRows);
-  const dim3 grid(grid_blocks((K + kDaCols - 1) / kDaCols * p.splits));
-  if (R <= 16) lora8_da_kernel<1><<<grid, kDaThreads, 0, st>>>(p);
-  else if (R <= 32) lora8_da_kernel<2><<<grid, kDaThreads, 0, st>>>(p);
-  else if (R <= 48) lora8_da_kernel<3><<<grid, kDaThreads, 0, st>>>(p);
-  else lora8_da_kernel<4><<<grid, kDaThreads, 0, st>>>(p);
+  const bool both = nx && na && R <= 48;
+  if (both) {
+    if (R <= 16) lora8_both_kernel<1><<<nx + na, kDaThreads, 0, st>>>(x, p, nx, na);
+    else if (R <= 32) lora8_both_kernel<2><<<nx + na, kDaThreads, 0, st>>>(x, p, nx, na);
+    else lora8_both_kernel<3><<<nx + na, kDaThreads, 0, st>>>(x, p, nx, na);
+  }
+  if (nx && !both) {
+    if (R <= 32) lora8_dx_kernel<1><<<nx, 256, 0, st>>>(x);
+    else lora8_dx_kernel<2><<<nx, 256, 0, st>>>(x);
+  }
+  if (na && !both) {
+    if (R <= 16) lora8_da_kernel<1><<<na, kDaThreads, 0, st>>>(p);
+    else if (R <= 32) lora8_da_kernel<2><<<na, kDaThreads, 0, st>>>(p);
+    else if (R <= 48) lora8_da_kernel<3><<<na, kDaThreads, 0, st>>>(p);
+    else lora8_da_kernel<4><<<na, kDaThreads, 0, st>>>(p);
+  }
   if (int rc = check_launch("lora8_bwd")) return rc;
+  if (!da) return AA_OK;
   if (p.splits == 1) return AA_OK;
   const int64_t n = R * K;
   lora8_sum_kernel<<<dim3((unsigned)((n / 4 + 63) / 64)), 64, 0, st>>>(p.part, p.da, n, p.splits);
