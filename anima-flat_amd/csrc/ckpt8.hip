@@ -13,9 +13,11 @@
 // read back as NaN. 33/32 bytes a value against bf16's 2.
 //
 // gelu8: y = GELU(x) in bf16 from x itself; dx = dy GELU'(kept x). HBM bound:
-//   2 + 2 + 33/32 bytes a value forward, 33/32 + 2 + 2 backward.
+//   2 + 2 + 33/32 bytes a value forward, 33/32 + 2 + 2 backward. 4096 x 8192: 33 and
+//   34 us, 5.1 and 5.0 TB/s, a copy's rate.
 // lora_down8: t = x A^T for A [R, K], R <= 64; dx = dt A; dA = dt^T kept(x).
-//   HBM bound: 2 + 33/32 bytes a value forward, 2 (dx) + 33/32 (dA) backward.
+//   HBM bound: 2 + 33/32 bytes a value forward, 2 (dx) + 33/32 (dA) backward, the
+//   latter beside the vector instructions that unpack the codes.
 #include <algorithm>
 #include <type_traits>
 
@@ -204,7 +206,8 @@ constexpr int kLoMaxR = 64;
 // Forms measured before, 7904 x 8192 at rank 40 (floor 28 us): every wave with
 // rows and channels of its own and A from memory in the operand layout 79 us
 // (A's traffic, 16 ranks x 64 bytes an instruction); A's part of a step through
-// LDS, shared by 32 rows, 58 us (LDS and vector work between barriers).
+// LDS, shared by 32 rows, 58 us (LDS and vector work between barriers). This one: 42
+// (38 at rank 16; 196 MB: 4.7 and 5.2 TB/s, a copy's rate 5.1).
 struct LoraFwd {
   const bf16* x;  // [M, K]
   const bf16* a;  // [R, K]
@@ -350,7 +353,8 @@ __device__ __forceinline__ bool grid_place(Block b, int tiles, int groups, int* 
 // wave store 256 bytes of one row. With dt's rows along the lanes instead, the
 // quarter waves of a store spread over 8 rows, four times as many pieces of
 // lines: the CU's address unit was busy 80% of the time, 33 us at 7904 x 8192
-// and rank 40 against 28.5 (4.6 TB/s of writes; a fill of that size reaches 6.2).
+// and rank 40 against 25.5 to 28 (4.6 to 5.1 TB/s of writes; a fill of that size
+// reaches 6.2).
 struct LoraDx {
   const bf16* dt;  // [M, R]
   const bf16* a;
@@ -441,7 +445,11 @@ __device__ __forceinline__ void lora8_dx(const LoraDx& p, uint8_t* lds, Block bl
 // rows as the contracted index. dt lies in LDS as it is in memory, 128 rows at
 // a time, and is read transposed. The codes, steps and dt of two turns ahead are
 // loaded before this turn's products. Partial sums per range of rows, in fp32,
-// are added by lora8_sum_kernel (or, of one range, written as they are).
+// are added by lora8_sum_kernel (or, of one range, written as they are). Bound by
+// vector instructions: per 8 codes 8 conversions, 8 FMAs and 4 packs, with the rest
+// of a turn 2.5 times a read of the codes at the memory's rate (7904 x 8192: 22 us at
+// rank 16, 24 at 32, 28 at 40, 37 at 64; 67 MB in 13). Three sets of a turn's
+// registers in turn, copied, and pointers per lane: 24, 26, 31, 39.
 struct LoraDa {
   const bf16* dt;
   const uint8_t* codes;
@@ -487,69 +495,62 @@ __device__ __forceinline__ void lora8_da(const LoraDa& p, uint8_t* lds, Block bl
 
   constexpr int kPieces = kDaRows * 4 * NR / kDaThreads;  // 8-byte pieces of dt per thread
   const uint32_t pitch = kGroup * p.G;
-  const uint32_t whole = (uint32_t)(32 * wave + 8 * g) * pitch + (uint32_t)col;  // of this lane's first row
   struct Turn {
     u32x2 c[8];  // codes of this lane's 8 rows
     u32x2 ex;    // their groups' exponents
     u32x2 dt[kPieces];
-  } cur, next, after;
+  } even, odd;
+  const int mine = 32 * wave + 8 * g;  // this lane's 8 rows
+  uint32_t piece[kPieces];  // bytes of dt, in a whole turn
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    const int o = tid + kDaThreads * i;
+    piece[i] = 2u * (uint32_t)(o / (4 * NR) * p.R + min(4 * (o % (4 * NR)), p.R - 4));
+  }
+  const uint32_t whole = (uint32_t)mine * pitch + (uint32_t)col;  // of this lane's first row
   auto load = [&](Turn& t, int64_t r0) {
-    // Addresses: a uniform row base and 32-bit offsets in the turn's 128 rows.
+    // Addresses: a uniform row base and 32-bit offsets in the turn's 128 rows. (The
+    // empty asm keeps r0 in a scalar register: left alone, the compiler carries a
+    // pointer per lane and load through the loop, 60 registers.)
+    asm("" : "+s"(r0));
     const uint8_t* codes = p.codes + r0 * pitch;
-    const bf16* dt = p.dt + r0 * p.R;
-    const int last = (int)min<int64_t>(end - r0, kDaRows) - 1;
-    const int mine = 32 * wave + 8 * g;  // this lane's 8 rows
+    const uint8_t* exps = p.exps + (int64_t)grp * p.Mp + r0;
+    const uint8_t* dt = reinterpret_cast<const uint8_t*>(p.dt + r0 * p.R);
     // Every load is in bounds and made: rows past the range re-read its last, and
     // count nothing below; channels and ranks past theirs are not written.
-    if (last == kDaRows - 1) {
+    if (end - r0 >= kDaRows) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) t.c[e] = *reinterpret_cast<const u32x2*>(codes + (int64_t)e * pitch + whole);
+      t.ex = *reinterpret_cast<const u32x2*>(exps + mine);
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) t.dt[i] = *reinterpret_cast<const u32x2*>(dt + piece[i]);
     } else {
+      const int last = (int)(end - r0) - 1;
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         t.c[e] = *reinterpret_cast<const u32x2*>(codes + ((uint32_t)min(mine + e, last) * pitch + (uint32_t)col));
-    }
-    t.ex = *reinterpret_cast<const u32x2*>(p.exps + (int64_t)grp * p.Mp + r0 + min(mine, last & ~7));
+      t.ex = *reinterpret_cast<const u32x2*>(exps + min(mine, last & ~7));
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int o = tid + kDaThreads * i, r = o / (4 * NR), rank = min(4 * (o % (4 * NR)), p.R - 4);
-      t.dt[i] = *reinterpret_cast<const u32x2*>(dt + (uint32_t)(min(r, last) * p.R + rank));
-    }
-    if (last < kDaRows - 1) {
-#pragma unroll
-      for (int i = 0; i < kPieces; ++i)
-        if ((tid + kDaThreads * i) / (4 * NR) > last) t.dt[i] = u32x2{0, 0};
+      for (int i = 0; i < kPieces; ++i) {
+        const int r = (tid + kDaThreads * i) / (4 * NR);
+        const u32x2 v = *reinterpret_cast<const u32x2*>(dt + (piece[i] - 2u * (uint32_t)(max(r - last, 0) * p.R)));
+        t.dt[i] = r <= last ? v : u32x2{0, 0};
+      }
     }
   };
-  if (begin < end) load(cur, begin);
-  if (begin + kDaRows < end) load(next, begin + kDaRows);
-  bf16* mydt = dts;
-  for (int64_t r0 = begin; r0 < end; r0 += kDaRows) {
-    if (r0 + 2 * kDaRows < end) load(after, r0 + 2 * kDaRows);
+  // One turn of t's rows from r0; t is free for the turn after the next as soon as its
+  // codes and steps are unpacked and its dt is in LDS.
+  auto turn = [&](Turn& t, int64_t r0, bf16* mydt) {
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       const int o = tid + kDaThreads * i, r = o / (4 * NR), rank = 4 * (o % (4 * NR));
-      *reinterpret_cast<u32x2*>(mydt + r * kPitch + rank) = cur.dt[i];
-    }
-    // One barrier a turn: these places are written again two turns on, behind the
-    // next turn's barrier, which every wave reaches after its reads here.
-    __syncthreads();
-    // Lanes 4 r + q of a group of 16 give the piece of four ranks at 4 q of row
-    // 8 g + r (+ 4 for the second read); lane li receives rank li of four rows.
-    const bf16* piece = mydt + (32 * wave + 8 * g + (li >> 2)) * kPitch + 4 * (li & 3);
-    mydt = mydt == dts ? dts + kDaRows * kPitch : dts;
-    bf16x8 d[NR];
-#pragma unroll
-    for (int n = 0; n < NR; ++n) {
-      const s16x4 lo = ds_read_tr(piece + 16 * n);
-      const s16x4 hi = ds_read_tr(piece + 4 * kPitch + 16 * n);
-      d[n] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+      *reinterpret_cast<u32x2*>(mydt + r * kPitch + rank) = t.dt[i];
     }
     float step[8], low[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) step[e] = step_of((cur.ex[e >> 2] >> (8 * (e & 3))) & 255u);
+    for (int e = 0; e < 8; ++e) step[e] = step_of((t.ex[e >> 2] >> (8 * (e & 3))) & 255u);
     if (r0 + kDaRows > end) {  // rows past the range count nothing, whatever their group's mark
-      const int left = (int)(end - r0) - (32 * wave + 8 * g);
+      const int left = (int)(end - r0) - mine;
 #pragma unroll
       for (int e = 0; e < 8; ++e) step[e] = e < left ? step[e] : 0.f;
     }
@@ -557,8 +558,22 @@ __device__ __forceinline__ void lora8_da(const LoraDa& p, uint8_t* lds, Block bl
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       low[e] = -128.0f * step[e];
-      code[e][0] = flip_signs(cur.c[e][0]);
-      code[e][1] = flip_signs(cur.c[e][1]);
+      code[e][0] = flip_signs(t.c[e][0]);
+      code[e][1] = flip_signs(t.c[e][1]);
+    }
+    if (r0 + 2 * kDaRows < end) load(t, r0 + 2 * kDaRows);
+    // One barrier a turn: these places are written again two turns on, behind the
+    // next turn's barrier, which every wave reaches after its reads here.
+    __syncthreads();
+    // Lanes 4 r + q of a group of 16 give the piece of four ranks at 4 q of row
+    // 8 g + r (+ 4 for the second read); lane li receives rank li of four rows.
+    const bf16* from = mydt + (mine + (li >> 2)) * kPitch + 4 * (li & 3);
+    bf16x8 d[NR];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      const s16x4 lo = ds_read_tr(from + 16 * n);
+      const s16x4 hi = ds_read_tr(from + 4 * kPitch + 16 * n);
+      d[n] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
     static_for<0, 8>([&](auto J) {
       constexpr int j = decltype(J)::value;
@@ -572,8 +587,12 @@ __device__ __forceinline__ void lora8_da(const LoraDa& p, uint8_t* lds, Block bl
 #pragma unroll
       for (int n = 0; n < NR; ++n) acc[j][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(d[n], xv, acc[j][n], 0, 0, 0);
     });
-    cur = next;
-    next = after;
+  };
+  if (begin < end) load(even, begin);
+  if (begin + kDaRows < end) load(odd, begin + kDaRows);
+  for (int64_t r0 = begin; r0 < end; r0 += 2 * kDaRows) {
+    turn(even, r0, dts);
+    if (r0 + kDaRows < end) turn(odd, r0 + kDaRows, dts + kDaRows * kPitch);
   }
   // acc[j][n]: lane li is channel 8 li + j, element i is rank 16 n + 4 g + i.
   // Added over the waves one element i at a time: sums[wave][n][g][channel].
@@ -618,9 +637,9 @@ __global__ __launch_bounds__(kDaThreads, NR < 4 ? 2 : 1) void lora8_da_kernel(Lo
 // Both in one launch, eight workgroups (one an XCD) of each in turn: dx is bound by
 // its stores and dA by the vector instructions that unpack the codes, so that a CU
 // with workgroups of both does better than one after the other. 7904 x 8192, one
-// launch against two: rank 16 39 against 49 us, rank 32 45 against 51, rank 40 52
-// against 56. Above rank 48 dA's registers leave a CU one workgroup, of either
-// (rank 64: 84 against 64), and two launches are made.
+// launch against two: rank 16 37 against 48 us (128 MB out and 67 in: 5.3 TB/s), rank
+// 32 41 against 48, rank 40 46 to 48 against 54. Above rank 48 dA's registers leave a
+// CU one workgroup, of either (rank 64: 84 against 62), and two launches are made.
 template <int NR>
 __global__ __launch_bounds__(kDaThreads, 2) void lora8_both_kernel(LoraDx x, LoraDa a, int nx, int na) {
   constexpr int NS = (NR + 1) / 2;
@@ -645,8 +664,9 @@ __global__ __launch_bounds__(64) void lora8_sum_kernel(const float* part, bf16* 
 
 // Ranges of rows of the dA product: two workgroups a CU (one above rank 48, where no
 // more fit), but at least 256 rows each (a partial sum is 4 R bytes a channel, 256
-// rows' codes are 256). 7904 x 8192, one, two and four a CU: rank 16 28, 24 and 27
-// us; rank 40 35, 31 and, two at a time, 32.
+// rows' codes are 256). 7904 x 8192 with an earlier form of the loop, one, two and
+// four a CU: rank 16 28, 24 and 27 us; rank 40 35, 31 and (two at a time) 32; rank
+// 64, one and two: 39 and 47.
 static int da_splits(int64_t M, int64_t K, int64_t R) {
   const int64_t cus = std::max(1, device_cu_count());
   const int64_t tiles = (K + kDaCols - 1) / kDaCols;
