@@ -1,7 +1,7 @@
 // Tokens to int8 with a scale per token, and the product of such tokens with
 // int8 weights that have a scale per output channel:
 //
-//   s[t] = max(max_k |x[t, k]|, 1e-12) / 127, q[t, k] = round(x[t, k] / s[t])
+//   s[t] = max(max_k |x[t, k]|, 1e-12) / 127, q[t, k] = round(x[t, k] (1 / s[t]))
 //   y[t, n] = s[t] ws[n] sum_k q[t, k] wq[n, k]
 //
 // The sum is exact: int8 MFMA accumulates in int32, and K <= 65536 products of
@@ -13,6 +13,7 @@
 // v_mfma_i32_32x32x32_i8 is 16 bytes per lane, as bf16's is, with twice the K,
 // so LDS blocks, XOR, DMA and k-steps are the same in bytes, at twice the
 // operations per MFMA cycle.
+// Many tokens (int8_linear_big_kernel): 256 x 256 tiles, for whole rounds of them.
 // Few tokens (int8_skinny_kernel, M <= 64): bound by reading the weights once.
 #include <algorithm>
 #include <type_traits>
@@ -33,7 +34,10 @@ constexpr int kQ8Rows = kQ8Threads / 64;  // one wave per row
 constexpr int kQ8MaxK = 8192;
 
 // One wave per row, the row in registers between its one read and the store of
-// its codes: unit lane + 64 p of U values (16 where K allows 16-byte stores).
+// its codes: unit lane + 64 p of U values (16 where K allows 16-byte stores). HBM
+// bound, 3 bytes a value; with GELU as much by its vector instructions (block_math.h).
+// 18432 x 8192 with GELU 95 to 107 us (453 MB: 4.2 to 4.8 TB/s; a copy 5.1), 131 with
+// a division per value, a polynomial a degree longer and plain stores.
 template <int NU, int U, bool kGelu>
 __global__ __launch_bounds__(kQ8Threads) void rowquant_int8_kernel(const bf16* __restrict__ x,
                                                                    uint8_t* __restrict__ q,
@@ -307,6 +311,14 @@ __global__ __launch_bounds__(T::kThreads) void int8_linear_kernel(I8Params p) {
 // s + 3 (in the k-step after; it may be in flight still at the next barrier).
 // K % 128 != 0: the first stage is the short one; its lanes past the rest load
 // zeros.
+// One workgroup a CU takes its tiles in turn. The next tile's first two stages are
+// sent for behind the last operand reads of this one, ahead of its epilogue, whose
+// stores then run beside the next tile's first two stages: 16384 x 8192 x 2048 (M,
+// N, K; four rounds) 265 -> 252 us, two rounds 76.7 -> 75.7 and 261 -> 258.
+// Bound by the power limit: at 16384 x 8192 x 2048 the matrix pipe is busy for 82% of
+// a CU's cycles, at a clock of 1.67 GHz. 4096 x 8192 x 2048 73 to 78 us (1.82 POPS),
+// 7904 x 6144 x 2048 102 to 106 (1.91), 18432 x 2048 x 8192 258 (2.40); two waves per
+// SIMD of 64 x 128 each, per wave two barriers a stage: 76, 102 and 319.
 __device__ const u32x4 kZeroChunk = {0, 0, 0, 0};
 
 constexpr int kBigTile = 256;
@@ -323,41 +335,19 @@ __global__ __launch_bounds__(kBigThreads, 1) void int8_linear_big_kernel(I8Param
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave & 1;   // tokens 128 wm ..
+  const int wn = wave >> 1;  // channels 128 wn ..
   const int ntn = (p.N + kBigTile - 1) / kBigTile;
   const int total = p.mtiles * ntn;
-  const int L = xcd_remap(blockIdx.x, total);
-  const int group = L / (kIGroupM * ntn);
-  const int within = L - group * kIGroupM * ntn;
-  const int gm = min(kIGroupM, p.mtiles - group * kIGroupM);
-  const int mt = group * kIGroupM + within % gm;
-  const int nt = within / gm;
-  const int64_t row0 = (int64_t)mt * kBigTile;
-  const int nrows = (int)min<int64_t>(kBigTile, p.M - row0);
-  const int ncols = min(kBigTile, p.N - kBigTile * nt);
-
-  // The scales of token and channel `tid` of the tile, for the epilogue.
-  const float xscale = p.xs[row0 + min(tid, nrows - 1)];
-  const float wscale = p.ws[(int64_t)nt * kBigTile + min(tid, ncols - 1)];
+  const int nk = (p.K + kIK - 1) / kIK;
+  const int rest = p.K - (nk - 1) * kIK;  // bytes of the first stage, 16 .. 128
 
   // DMA: 32 blocks of 8 rows x 128 bytes of each matrix; wave w moves blocks 8 w ..
   // 8 w + 7 of both, lane roles as above. Per block its first row's address,
   // per lane the byte offset from there.
-  const int drow = lane >> 3;
-  const int chunk0 = (lane & 7) ^ drow, chunk1 = chunk0 ^ 1;  // even and odd blocks
-  const int nk = (p.K + kIK - 1) / kIK;
-  const int rest = p.K - (nk - 1) * kIK;  // bytes of the first stage, 16 .. 128
   const uint8_t* xbase[8];
   const uint8_t* wbase[8];
   uint32_t xoff[8], woff[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t chunk = 16 * ((i & 1) ? chunk1 : chunk0);
-    const int x0 = min(8 * (wave * 8 + i), nrows - 1), w0 = min(8 * (wave * 8 + i), ncols - 1);
-    xbase[i] = p.x + (row0 + x0) * p.K;
-    wbase[i] = p.w + ((int64_t)nt * kBigTile + w0) * p.K;
-    xoff[i] = (uint32_t)(min(drow, nrows - 1 - x0) * p.K) + chunk;
-    woff[i] = (uint32_t)(min(drow, ncols - 1 - w0) * p.K) + chunk;
-  }
   const uint32_t ring = lds_addr(lds);
   const uint32_t mine = ring + (uint32_t)wave * 8192u;
   // Block I of this wave's share of a stage s >= 1, X to the place at byte `at`.
@@ -369,19 +359,56 @@ __global__ __launch_bounds__(kBigThreads, 1) void int8_linear_big_kernel(I8Param
     constexpr int i = decltype(I)::value;
     dma16_sva_off<0, 1024 * i>(wbase[i] + (rest + (s - 1) * kIK), woff[i], mine + (uint32_t)(3 + (s & 1)) * kBigPart);
   };
-  static_for<0, 8>([&](auto I) {
-    constexpr int i = decltype(I)::value;
-    const bool in = 16 * ((i & 1) ? chunk1 : chunk0) < rest;
-    dma16_a(in ? xbase[i] + xoff[i] : (const uint8_t*)&kZeroChunk, mine + 1024u * i);
-    dma16_a(in ? wbase[i] + woff[i] : (const uint8_t*)&kZeroChunk, mine + 3u * kBigPart + 1024u * i);
-  });
-  if (nk > 1) {
+  // Tile `n` of the work order: its place, and its first two stages sent for.
+  struct Tile {
+    int64_t row0;
+    int nt, nrows, ncols;
+    float scale[4];  // of tokens and channels lane and lane + 64 of this wave's
+  } next;
+  // (The empty asm here and below keeps what follows from the lane where it is used:
+  // computed once, ahead of the tiles, it would not leave room for the sums.)
+  auto start = [&](int n) {
+    int l = lane;
+    asm volatile("" : "+v"(l));
+    const int drow = l >> 3;
+    const int chunk0 = (l & 7) ^ drow, chunk1 = chunk0 ^ 1;  // even and odd blocks
+    const int L = xcd_remap(n, total);
+    const int group = L / (kIGroupM * ntn);
+    const int within = L - group * kIGroupM * ntn;
+    const int gm = min(kIGroupM, p.mtiles - group * kIGroupM);
+    const int mt = group * kIGroupM + within % gm;
+    const int nt = within / gm;
+    const int64_t row0 = (int64_t)mt * kBigTile;
+    const int nrows = (int)min<int64_t>(kBigTile, p.M - row0);
+    const int ncols = min(kBigTile, p.N - kBigTile * nt);
+    next.row0 = row0;
+    next.nt = nt;
+    next.nrows = nrows;
+    next.ncols = ncols;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      next.scale[h] = p.xs[row0 + min(128 * wm + 64 * h + l, nrows - 1)];
+      next.scale[2 + h] = p.ws[(int64_t)nt * kBigTile + min(128 * wn + 64 * h + l, ncols - 1)];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t chunk = 16 * ((i & 1) ? chunk1 : chunk0);
+      const int x0 = min(8 * (wave * 8 + i), nrows - 1), w0 = min(8 * (wave * 8 + i), ncols - 1);
+      xbase[i] = p.x + (row0 + x0) * p.K;
+      wbase[i] = p.w + ((int64_t)nt * kBigTile + w0) * p.K;
+      xoff[i] = (uint32_t)(min(drow, nrows - 1 - x0) * p.K) + chunk;
+      woff[i] = (uint32_t)(min(drow, ncols - 1 - w0) * p.K) + chunk;
+    }
+    static_for<0, 8>([&](auto I) {
+      constexpr int i = decltype(I)::value;
+      const bool in = 16 * ((i & 1) ? chunk1 : chunk0) < rest;
+      dma16_a(in ? xbase[i] + xoff[i] : (const uint8_t*)&kZeroChunk, mine + 1024u * i);
+      dma16_a(in ? wbase[i] + woff[i] : (const uint8_t*)&kZeroChunk, mine + 3u * kBigPart + 1024u * i);
+    });
     static_for<0, 8>([&](auto I) { issue_x(I, 1, kBigPart); });
     static_for<0, 8>([&](auto I) { issue_w(I, 1); });
-  }
+  };
 
-  const int wm = wave & 1;   // tokens 128 wm ..
-  const int wn = wave >> 1;  // channels 128 wn ..
   const int li = lane & 31, hh = lane >> 5;
   const uint32_t kbase = (li >> 3) * 1024 + (li & 7) * 128 + (hh ^ (li & 7) ^ ((li >> 3) & 1)) * 16;
   // Operand addresses of k-step kk: these ^ 32 kk (the ring and its parts are
@@ -390,13 +417,6 @@ __global__ __launch_bounds__(kBigThreads, 1) void int8_linear_big_kernel(I8Param
   const uint32_t wa = ring + 3u * kBigPart + wn * 16384 + kbase;
 
   i32x16 acc[4][4];
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[c][t][e] = 0;
-
   struct Ops {
     i32x4 v[8];  // four channel blocks, four token blocks
   } o0, o1;
@@ -408,11 +428,12 @@ __global__ __launch_bounds__(kBigThreads, 1) void int8_linear_big_kernel(I8Param
   // eight DMAs: a read and a DMA in turn (four waves' DMAs back to back would hold
   // up their MFMAs: the CU's load path takes one per ~11 cycles), or the reads in
   // the first slots where none go out.
-  auto kstep = [&](const Ops& cur, Ops& next, uint32_t x, uint32_t w, auto has_next, auto dma) {
+  auto kstep = [&](const Ops& cur, Ops& next, uint32_t x, uint32_t w, auto has_next, auto dma, auto fresh) {
     constexpr int kStride = std::is_same_v<decltype(dma), NoDma> ? 1 : 2;
     static_for<0, 16>([&](auto J) {
       constexpr int j = decltype(J)::value;
-      acc[j >> 2][j & 3] = mfma_i8(cur.v[j >> 2], cur.v[4 + (j & 3)], acc[j >> 2][j & 3]);
+      if constexpr (decltype(fresh)::value) acc[j >> 2][j & 3] = mfma_i8(cur.v[j >> 2], cur.v[4 + (j & 3)], i32x16{});
+      else acc[j >> 2][j & 3] = mfma_i8(cur.v[j >> 2], cur.v[4 + (j & 3)], acc[j >> 2][j & 3]);
       if constexpr (j % kStride == 0 && j / kStride < 8 && decltype(has_next)::value) {
         // Channel block 0 and the token blocks first: the next k-step's first four MFMAs.
         constexpr int order[8] = {0, 4, 5, 6, 7, 1, 2, 3};
@@ -423,86 +444,126 @@ __global__ __launch_bounds__(kBigThreads, 1) void int8_linear_big_kernel(I8Param
     });
   };
   const NoDma none;
-  // This wave's DMAs of stage 0 are done (stage 1's may be in flight); the barrier
-  // publishes every wave's.
-  if (nk > 1) asm volatile("s_waitcnt vmcnt(16)\n\ts_barrier" ::: "memory");
-  else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-  static_for<0, 8>([&](auto J) { read(J, o0, xa, wa); });
-
   // Places of X in the ring: of this stage, the next, and the one after, in
   // which X of stage s + 2 is sent for in this stage's first k-step.
-  uint32_t px0 = 0, px1 = kBigPart, px2 = 2 * kBigPart;
-  // left: stages after this one, as far as it matters (0, 1, 2).
-  auto stage = [&](int s, auto left) {
+  uint32_t px0, px1, px2;
+  // The 32 stores of the tile before, made after this tile's first two stages were
+  // sent for, may be in flight until the end of its second stage.
+  bool stores = false;
+  // left: stages after this one, as far as it matters (0, 1, 2). first: the tile's
+  // first stage, whose first products start the sums.
+  constexpr std::true_type kYes;
+  constexpr std::false_type kNo;
+  auto stage = [&](int s, auto left, auto first) {
     constexpr int kLeft = decltype(left)::value;
     const uint32_t x = xa + px0, w = wa + (uint32_t)(s & 1) * kBigPart;
     if constexpr (kLeft >= 2)
-      kstep(o0, o1, x ^ 32u, w ^ 32u, std::true_type{}, [&](auto I) { issue_x(I, s + 2, px2); });
+      kstep(o0, o1, x ^ 32u, w ^ 32u, kYes, [&](auto I) { issue_x(I, s + 2, px2); }, first);
     else
-      kstep(o0, o1, x ^ 32u, w ^ 32u, std::true_type{}, none);
-    kstep(o1, o0, x ^ 64u, w ^ 64u, std::true_type{}, none);
-    kstep(o0, o1, x ^ 96u, w ^ 96u, std::true_type{}, none);
+      kstep(o0, o1, x ^ 32u, w ^ 32u, kYes, none, first);
+    kstep(o1, o0, x ^ 64u, w ^ 64u, kYes, none, kNo);
+    kstep(o0, o1, x ^ 96u, w ^ 96u, kYes, none, kNo);
     if constexpr (kLeft >= 1) {
       // Every read of stage s has arrived, and this wave's DMAs of stage s + 1: only
-      // X of s + 2 came after them.
-      if constexpr (kLeft >= 2) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      // X of s + 2 came after them (and, in the first stage, the stores).
+      if constexpr (kLeft >= 2) {
+        if (decltype(first)::value && stores) asm volatile("s_waitcnt vmcnt(40) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      } else {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      }
       const uint32_t x1 = xa + px1, w1 = wa + (uint32_t)((s + 1) & 1) * kBigPart;
       if constexpr (kLeft >= 2)
-        kstep(o1, o0, x1, w1, std::true_type{}, [&](auto I) { issue_w(I, s + 2); });
+        kstep(o1, o0, x1, w1, kYes, [&](auto I) { issue_w(I, s + 2); }, kNo);
       else
-        kstep(o1, o0, x1, w1, std::true_type{}, none);
+        kstep(o1, o0, x1, w1, kYes, none, kNo);
       const uint32_t t = px0;
       px0 = px1;
       px1 = px2;
       px2 = t;
     } else {
-      kstep(o1, o0, x, w, std::false_type{}, none);
+      // Every wave's reads have arrived: the ring is free behind this barrier.
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      kstep(o1, o0, x, w, kNo, none, kNo);
     }
   };
-  int s = 0;
-  for (; s + 2 < nk; ++s) stage(s, std::integral_constant<int, 2>{});
-  if (s + 1 < nk) stage(s++, std::integral_constant<int, 1>{});
-  stage(s, std::integral_constant<int, 0>{});
 
-  // acc[c][t]: lane li is token 128 wm + 32 t + li, element e channel 128 wn + 32 c
-  // + 8 (e / 4) + 4 hh + e % 4. Each wave stages its 128 x 128 as 256-byte rows
-  // in a quarter of the ring, chunk ch of row r in slot ch ^ (r & 15), and
-  // stores them as whole lines.
-  float* scales = reinterpret_cast<float*>(lds + 4 * 32768);
-  __syncthreads();  // the last operands of every wave are read
-  scales[tid] = xscale;
-  scales[256 + tid] = wscale;
-  __syncthreads();
-  uint8_t* out = lds + wave * 32768;
-  const int wcols = ncols - 128 * wn, wrows = nrows - 128 * wm;  // what there is of them
-  if (wcols <= 0 || wrows <= 0) return;
-  float rs[4];
+  int n = blockIdx.x;
+  start(n);
+  for (;;) {
+    const Tile tile = next;
+    // This wave's DMAs of stage 0 are done (stage 1's, and the stores of the tile
+    // before, may be in flight); the barrier publishes every wave's.
+    if (stores) asm volatile("s_waitcnt vmcnt(48)\n\ts_barrier" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(16)\n\ts_barrier" ::: "memory");
+    static_for<0, 8>([&](auto J) { read(J, o0, xa, wa); });
+    px0 = 0, px1 = kBigPart, px2 = 2 * kBigPart;
+    stage(0, std::integral_constant<int, 2>{}, kYes);
+    int s = 1;
+    for (; s + 2 < nk; ++s) stage(s, std::integral_constant<int, 2>{}, kNo);
+    stage(s++, std::integral_constant<int, 1>{}, kNo);
+    stage(s, std::integral_constant<int, 0>{}, kNo);
+    n += gridDim.x;
+    const bool more = n < total;
+    if (more) start(n);
+
+    // acc[c][t]: lane li is token 128 wm + 32 t + li, element e channel 128 wn + 32 c
+    // + 8 (e / 4) + 4 hh + e % 4. The scales and then 16 tokens at a time go through
+    // this wave's 8 KiB of X's third place (the next tile's stages are under way to
+    // the others, and this wave's own DMAs are the first to write here): 256-byte
+    // rows, chunk ch of row r in slot ch ^ r, stored as whole lines. A wave's LDS
+    // accesses are in order.
+    int l = lane, N = p.N;
+    asm volatile("" : "+v"(l), "+s"(N));
+    const int li = l & 31, hh = l >> 5;
+    uint8_t* out = lds + 2 * kBigPart + wave * 8192;
+    float* scales = reinterpret_cast<float*>(out);
 #pragma unroll
-  for (int t = 0; t < 4; ++t) rs[t] = scales[128 * wm + 32 * t + li];
+    for (int h = 0; h < 4; ++h) scales[64 * h + l] = tile.scale[h];
+    __builtin_amdgcn_wave_barrier();
+    float rs[4];
+    f32x4 ws[4][4];
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
+    for (int t = 0; t < 4; ++t) rs[t] = scales[32 * t + li];
 #pragma unroll
-    for (int e4 = 0; e4 < 4; ++e4) {
-      const f32x4 w = *reinterpret_cast<const f32x4*>(scales + 256 + 128 * wn + 32 * c + 8 * e4 + 4 * hh);
+    for (int c = 0; c < 4; ++c)
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int r = 32 * t + li;
-        const i32x16& v = acc[c][t];
-        u32x2 b;
-        b[0] = pack_bf16((float)v[4 * e4] * rs[t] * w[0], (float)v[4 * e4 + 1] * rs[t] * w[1]);
-        b[1] = pack_bf16((float)v[4 * e4 + 2] * rs[t] * w[2], (float)v[4 * e4 + 3] * rs[t] * w[3]);
-        *reinterpret_cast<u32x2*>(out + r * 256 + (((4 * c + e4) ^ (r & 15)) * 16) + 8 * hh) = b;
+      for (int e4 = 0; e4 < 4; ++e4) ws[c][e4] = *reinterpret_cast<const f32x4*>(scales + 128 + 32 * c + 8 * e4 + 4 * hh);
+    const int wcols = tile.ncols - 128 * wn, wrows = tile.nrows - 128 * wm;  // what there is of the wave's
+    const int j = l & 15, q = l >> 4;
+    bf16* y = p.y + (tile.row0 + 128 * wm) * N + (int64_t)tile.nt * kBigTile + 128 * wn + 8 * j;
+    static_for<0, 4>([&](auto T) {
+      constexpr int t = decltype(T)::value;
+      // The sums stay in accumulator registers until their turn.
+#pragma unroll
+      for (int c = 0; c < 4; ++c) asm volatile("" : "+a"(acc[c][t]));
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4) {
+          const i32x16& v = acc[c][t];
+          const f32x4 w = ws[c][e4];
+          u32x2 b;
+          b[0] = pack_bf16((float)v[4 * e4] * rs[t] * w[0], (float)v[4 * e4 + 1] * rs[t] * w[1]);
+          b[1] = pack_bf16((float)v[4 * e4 + 2] * rs[t] * w[2], (float)v[4 * e4 + 3] * rs[t] * w[3]);
+          *reinterpret_cast<u32x2*>(out + li * 256 + (((4 * c + e4) ^ (li & 15)) * 16) + 8 * hh) = b;
+        }
+      __builtin_amdgcn_sched_barrier(0);
+      u32x4 row[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = q + 4 * i;
+        row[i] = *reinterpret_cast<const u32x4*>(out + r * 256 + ((j ^ (r & 15)) * 16));
       }
-    }
-  // The wave's own rows: its writes are in order with its reads.
-  __builtin_amdgcn_wave_barrier();
-  const int j = lane & 15;
-  bf16* y = p.y + (row0 + 128 * wm) * p.N + nt * kBigTile + 128 * wn + 8 * j;
-  if (8 * j < wcols) {
-#pragma unroll 8
-    for (int r = lane >> 4; r < wrows && r < 128; r += 4)
-      st16(y + (int64_t)r * p.N, *reinterpret_cast<const u32x4*>(out + r * 256 + ((j ^ (r & 15)) * 16)));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = 32 * t + q + 4 * i;
+        if (8 * j < wcols && r < wrows) st16(y + (int64_t)r * N, row[i]);
+      }
+    });
+    if (!more) return;
+    stores = tile.nrows == kBigTile && tile.ncols == kBigTile;  // 32 of them, in every wave
   }
 }
 
@@ -510,12 +571,12 @@ __global__ __launch_bounds__(kBigThreads, 1) void int8_linear_big_kernel(I8Param
 // channels; its four waves take 128 bytes of K in turn, each through a ring of
 // LDS of its own, so nothing waits for another wave until the sums: per step two
 // DMAs of 8 channels x 128 bytes and XB of 8 tokens, kDepth steps ahead. 8192 x
-// 8192 weights: 14.8 us for 2 tokens, 14.9 for 16, 16.0 for 32, 20.8 for 64 (the
-// 128 x 128 tiles: 32). Operands straight from memory (16 rows x 16 bytes per quarter
-// wave, four times as many pieces of lines as a DMA's two rows x 128): 16.2,
-// 18.6, 25.2, 39.0; 32 channels a workgroup: 19.5, 20.1, 20.7, 23.1. In v_mfma_i32_16x16x64_i8 lane l holds 16 bytes of row l % 16 (a
-// channel, a token) at chunk l / 16 of the 64. The waves' int32 sums are added
-// in LDS.
+// 8192 weights: 14.8 us for 2 tokens (67 MB: 4.5 TB/s), 14.9 for 16, 16.0 for 32,
+// 20.8 for 64 (the 128 x 128 tiles: 32). Operands straight from memory (16 rows x 16
+// bytes per quarter wave, four times as many pieces of lines as a DMA's two rows x
+// 128): 16.2, 18.6, 25.2, 39.0; 32 channels a workgroup: 19.5, 20.1, 20.7, 23.1. In
+// v_mfma_i32_16x16x64_i8 lane l holds 16 bytes of row l % 16 (a channel, a token) at
+// chunk l / 16 of the 64. The waves' int32 sums are added in LDS.
 template <int XB>
 struct Skinny {
   static constexpr int kTT = (XB + 1) / 2;         // token tiles of 16
@@ -697,7 +758,7 @@ extern "C" int aa_int8_linear(const void* q, const float* s, const void* weight,
   int64_t big = 0;
   double best = small_time(M);
   for (const int64_t rows : {std::min(M, whole), M}) {
-    if (rows <= 0) continue;
+    if (rows <= 0 || K <= 2 * kIK) continue;  // the large tiles' ring takes three stages or more
     const int64_t t = (rows + kBigTile - 1) / kBigTile * ntn;
     const double time = (double)((t + cus - 1) / cus) + (rows < M ? small_time(M - rows) : 0.0);
     if (time < best) {
@@ -709,7 +770,8 @@ extern "C" int aa_int8_linear(const void* q, const float* s, const void* weight,
   if (big > 0) {
     p.M = big;
     p.mtiles = (int)((big + kBigTile - 1) / kBigTile);
-    int8_linear_big_kernel<<<dim3((unsigned)(p.mtiles * ntn)), kBigThreads, 0, st>>>(p);
+    const int64_t t = p.mtiles * ntn;
+    int8_linear_big_kernel<<<dim3((unsigned)std::min(t, cus)), kBigThreads, 0, st>>>(p);
     if (int rc = check_launch("int8_linear")) return rc;
     p.x += big * K;
     p.xs += big;
