@@ -117,6 +117,8 @@ def test_product(int8, M, K, N):
 @pytest.mark.parametrize("M,K,N", [
     (8192, 16, 2048), (8100, 112, 2040), (8192, 128, 2048), (8100, 144, 2040), (8192, 256, 2048), (8065, 400, 1800),
     (8192, 512, 2048), (18000, 528, 2040), (16385, 2048, 2048), (260, 1040, 65544),
+    # Several tiles in turn, whole ones (whose stores the next tile's waits count) and partial ones.
+    (16384, 272, 2048), (24576, 384, 2048), (33000, 400, 1000), (24576, 528, 2056),
 ])
 def test_large_product(int8, M, K, N):
     args = _product(int8, M, K, N, M + K + N, full=True)
