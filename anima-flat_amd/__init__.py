@@ -19,6 +19,13 @@ Opt-in modules, not imported here (import them explicitly):
                  proj_head_norm, kv_proj_norm; ops anima_flat_amd::qkv_proj_norm_rope /
                  proj_head_norm / kv_proj_norm): the GEMM + norm pairs of src/model.py:308-316,
                  :324 and :256-258 in one kernel each; no single counterpart in the reference.
+  kernels.adaln  the block's modulated norms with gate and residual, forward and backward, and
+                 with int8 tokens out (residual_adaln, adaln, residual_adaln_int8): what
+                 src/kernels/adaln.py does between two sublayers, under ops of its own.
+  kernels.int8   int8 products with a scale per token and per output channel (rowquant_int8,
+                 quantize_weight, int8_linear), inference; the reference's are FP8.
+  kernels.ckpt8  training with activations kept in 8 bits (gelu8, lora_down8); no counterpart
+                 in the reference.
 
 Every op is registered through kernels.common.custom_op, which raises if the name is already
 registered in the process (torch.library would otherwise re-bind it silently). Ops this package

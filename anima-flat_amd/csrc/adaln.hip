@@ -537,12 +537,12 @@ static void launch_bwd_nc(dim3 grid, hipStream_t st, const AdBwd& p, bool f32) {
   if (f32) adaln_bwd_kernel<NU, WPR, true, NC, kPost><<<grid, kAdBThreads, 0, st>>>(p);
   else adaln_bwd_kernel<NU, WPR, false, NC, kPost><<<grid, kAdBThreads, 0, st>>>(p);
 }
-template <int NU, int WPR>
+template <int NU, int WPR, bool kPlain = true>
 static void launch_bwd(dim3 grid, hipStream_t st, const AdBwd& p, bool sums, bool f32) {
   if (sums && p.w) launch_bwd_nc<NU, WPR, 4, true>(grid, st, p, f32);
   else if (sums) launch_bwd_nc<NU, WPR, 3, false>(grid, st, p, f32);
   else if (p.w) launch_bwd_nc<NU, WPR, 0, true>(grid, st, p, f32);
-  else launch_bwd_nc<NU, WPR, 0, false>(grid, st, p, f32);
+  else if constexpr (kPlain) launch_bwd_nc<NU, WPR, 0, false>(grid, st, p, f32);
 }
 
 // Chunks of rows per batch item in the backward: with column sums one
@@ -704,7 +704,7 @@ extern "C" int aa_adaln_bwd(const aa_adaln_bwd_args* a, void* workspace, size_t 
   if (p.D <= 512) launch_bwd<1, 1>(grid, st, p, sums, f32);
   else if (p.D <= 1024) launch_bwd<2, 1>(grid, st, p, sums, f32);
   else if (p.D <= 2048 && wave_rows) launch_bwd_nc<4, 1, 0, false>(grid, st, p, f32);
-  else if (p.D <= 2048) launch_bwd<2, 2>(grid, st, p, sums, f32);
+  else if (p.D <= 2048) launch_bwd<2, 2, false>(grid, st, p, sums, f32);
   else if (p.D <= 4096) launch_bwd<2, 4>(grid, st, p, sums, f32);
   else launch_bwd<2, 8>(grid, st, p, sums, f32);
   if (int rc = check_launch(what)) return rc;
