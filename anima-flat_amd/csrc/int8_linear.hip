@@ -14,7 +14,8 @@
 // so LDS blocks, XOR, DMA and k-steps are the same in bytes, at twice the
 // operations per MFMA cycle.
 // Many tokens (int8_linear_big_kernel): 256 x 256 tiles, for whole rounds of them.
-// Few tokens (int8_skinny_kernel, M <= 64): bound by reading the weights once.
+// Some tokens (int8_mid_kernel): 64 x 64 tiles with K split over the waves.
+// Few tokens (int8_skinny_kernel, up to 64): bound by reading the weights once.
 #include <algorithm>
 #include <type_traits>
 
@@ -579,6 +580,7 @@ __global__ __launch_bounds__(kBigThreads, 1) void int8_linear_big_kernel(I8Param
 // 128): 16.2, 18.6, 25.2, 39.0; 32 channels a workgroup: 19.5, 20.1, 20.7, 23.1. In
 // v_mfma_i32_16x16x64_i8 lane l holds 16 bytes of row l % 16 (a channel, a token) at
 // chunk l / 16 of the 64. The waves' int32 sums are added in LDS.
+constexpr int kSkinnyRows = 64;
 template <int XB>
 struct Skinny {
   static constexpr int kTT = (XB + 1) / 2;         // token tiles of 16
@@ -676,6 +678,134 @@ __global__ __launch_bounds__(256) void int8_skinny_kernel(I8Params p) {
   }
 }
 
+// Too few tokens or channels to fill the device with 128 x 128 tiles: 64 x 64 ones,
+// whose four waves take 128 bytes of K in turn, each all 64 x 64 outputs, through 16 KiB
+// of LDS of its own (8 blocks of X and of W), so that a quarter of the steps stand one
+// behind another and nothing waits for another wave until the sums, which are added in
+// LDS, in int32: exact. Bound by latency: a step's operands are read into registers, the
+// next step's DMAs go out, and the products run beside them and beside the CU's other
+// workgroup. 333 tokens, N x K = 2048 x 2048: 6.5 us (the 128 x 128 tiles 10.9), 4096 x
+// 1024 7.1 (7.8), 1024 x 4096 8.0 (17.4), 2048 x 8192 15 (32); with two steps' LDS, one
+// workgroup a CU: 6.8, 9.2, 8.5, 15. More than two workgroups a CU lose: 1500 tokens,
+// 2048 x 2048 15.8 against 12.4.
+constexpr int kMidTile = 64;
+constexpr int kMidBlocks = 2 * kMidTile / 8;  // DMAs per step
+constexpr int kMidStep = kMidBlocks * 1024;   // bytes
+
+__global__ __launch_bounds__(256) void int8_mid_kernel(I8Params p) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kMidStep];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ntn = (p.N + kMidTile - 1) / kMidTile;
+  const int L = xcd_remap(blockIdx.x, p.mtiles * ntn);
+  const int group = L / (kIGroupM * ntn);
+  const int within = L - group * kIGroupM * ntn;
+  const int gm = min(kIGroupM, p.mtiles - group * kIGroupM);
+  const int64_t row0 = (int64_t)(group * kIGroupM + within % gm) * kMidTile;
+  const int n0 = within / gm * kMidTile;
+  const int nrows = (int)min<int64_t>(kMidTile, p.M - row0), ncols = min(kMidTile, p.N - n0);
+  // DMA roles as above; rows past the last re-read it.
+  const int drow = lane >> 3;
+  const uint32_t c0 = 16 * ((lane & 7) ^ drow), c1 = c0 ^ 16;  // bytes of even and odd blocks' chunks
+  const uint8_t* base[kMidBlocks];
+  uint32_t off[kMidBlocks];
+#pragma unroll
+  for (int i = 0; i < kMidBlocks; ++i) {
+    const bool is_x = i < kMidBlocks / 2;
+    const int last = (is_x ? nrows : ncols) - 1, b0 = min(8 * (is_x ? i : i - kMidBlocks / 2), last);
+    base[i] = is_x ? p.x + (row0 + b0) * p.K : p.w + (int64_t)(n0 + b0) * p.K;
+    off[i] = (uint32_t)(min(drow, last - b0) * p.K) + ((i & 1) ? c1 : c0);
+  }
+  const uint32_t mine = lds_addr(lds) + (uint32_t)wave * kMidStep;
+  const int nk = (p.K + kIK - 1) / kIK;
+  const int n = (nk - wave + 3) / 4;  // this wave's steps
+  auto issue = [&](int i) {
+    const int k0 = (wave + 4 * i) * kIK;
+    if (k0 + kIK <= p.K) {
+      static_for<0, kMidBlocks>([&](auto I) {
+        constexpr int j = decltype(I)::value;
+        dma16_sva_off<0, 1024 * j>(base[j] + k0, off[j], mine);
+      });
+    } else {  // past the row's end: zeros
+#pragma unroll
+      for (int j = 0; j < kMidBlocks; ++j) {
+        const int k = k0 + (int)((j & 1) ? c1 : c0);
+        dma16_a(k < p.K ? base[j] + k0 + off[j] : (const uint8_t*)&kZeroChunk, mine + 1024u * j);
+      }
+    }
+  };
+  if (n > 0) issue(0);
+
+  const int li = lane & 31, hh = lane >> 5;
+  const uint32_t kbase = (li >> 3) * 1024 + (li & 7) * 128 + (hh ^ (li & 7) ^ ((li >> 3) & 1)) * 16;
+  i32x16 acc[2][2];
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[c][t][e] = 0;
+  for (int i = 0; i < n; ++i) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const uint32_t at = mine + kbase;
+    i32x4 a[4][2], b[4][2];
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        b[kk][h] = __builtin_bit_cast(i32x4, lds_ld16((at ^ (32u * kk)) + 4096u * h));
+        a[kk][h] = __builtin_bit_cast(i32x4, lds_ld16((at ^ (32u * kk)) + 8192u + 4096u * h));
+      }
+    // The reads are back before the next step takes their place.
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (i + 1 < n) issue(i + 1);
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) acc[c][t] = mfma_i8(a[kk][c], b[kk][t], acc[c][t]);
+  }
+  // acc[c][t]: lane li is token 32 t + li, element e channel 32 c + 8 (e / 4) + 4 hh +
+  // e % 4. Each wave's sums as 256-byte rows of int32 in its own LDS, 16-byte chunk ch
+  // of row r in slot ch ^ (r & 15); then wave w adds rows 16 w .. + 15.
+  uint8_t* sums = lds + wave * kMidStep;
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4) {
+        const int r = 32 * t + li;
+        const i32x16& v = acc[c][t];
+        *reinterpret_cast<i32x4*>(sums + r * 256 + (((8 * c + 2 * e4 + hh) ^ (r & 15)) * 16)) =
+            i32x4{v[4 * e4], v[4 * e4 + 1], v[4 * e4 + 2], v[4 * e4 + 3]};
+      }
+  __syncthreads();
+  const int j = lane & 7;  // channels 8 j .. 8 j + 7
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = 16 * wave + 8 * i + (lane >> 3);
+    i32x4 s[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        s[h] += *reinterpret_cast<const i32x4*>(lds + w * kMidStep + r * 256 + (((2 * j + h) ^ (r & 15)) * 16));
+    if (r < nrows && 8 * j < ncols) {
+      const float rs = p.xs[row0 + r];
+      const float* ws = p.ws + n0 + 8 * j;
+      u32x4 v;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          v[2 * h + e] = pack_bf16((float)s[h][2 * e] * rs * ws[4 * h + 2 * e], (float)s[h][2 * e + 1] * rs * ws[4 * h + 2 * e + 1]);
+      st16(p.y + (row0 + r) * p.N + n0 + 8 * j, v);
+    }
+  }
+}
+
 }  // namespace aa
 
 using namespace aa;
@@ -711,8 +841,11 @@ extern "C" int aa_rowquant_int8(const void* x, int64_t rows, int64_t K, int gelu
   return check_launch("rowquant_int8");
 }
 
-// A round of small tiles against one of large tiles: one a CU, and two a CU.
-constexpr double kSmallAlone = 0.38, kSmallPair = 0.62;
+// Times of what stands beside the large tiles, in rounds of those (37.5 us at K = 2048,
+// 109 at 8192). Measured: up to 64 tokens 4 and 9 us; 64 x 64 tiles, one or two a CU,
+// 6.2 and 10 at K = 2048, 11 to 15 and 27 at 8192; 128 x 128 tiles, one or two a CU, 14.4
+// and 20 to 23.5 at K = 2048, 40 and 68 at 8192.
+constexpr double kFewTime = 0.1, kMidAlone = 0.16, kMidPair = 0.26, kSmallAlone = 0.38, kSmallPair = 0.62;
 
 extern "C" int aa_int8_linear(const void* q, const float* s, const void* weight, const float* weight_scale,
                               void* y, int64_t M, int64_t N, int64_t K, int dtype, void* stream) {
@@ -736,53 +869,52 @@ extern "C" int aa_int8_linear(const void* q, const float* s, const void* weight,
   p.N = (int)N;
   p.K = (int)K;
   hipStream_t st = (hipStream_t)stream;
-  if (M <= 64) {
-    const dim3 grid((unsigned)((N + 15) / 16));
-    if (M <= 8) int8_skinny_kernel<1><<<grid, 256, 0, st>>>(p);
-    else if (M <= 16) int8_skinny_kernel<2><<<grid, 256, 0, st>>>(p);
-    else if (M <= 32) int8_skinny_kernel<4><<<grid, 256, 0, st>>>(p);
-    else int8_skinny_kernel<8><<<grid, 256, 0, st>>>(p);
-    return check_launch("int8_linear");
-  }
   const int64_t cus = std::max(1, device_cu_count());
-  const int64_t ntn = (N + kBigTile - 1) / kBigTile, mtn = (M + kBigTile - 1) / kBigTile;
-  const auto small_tiles = [&](int64_t rows) { return (rows + 127) / 128 * ((N + 127) / 128); };
-  // Time of the small tiles over `rows` tokens, in rounds of large tiles. Measured:
-  // a round of large tiles 37.5 us at K = 2048 and 109 at 8192; of small ones, one
-  // a CU 14.4 and 40.4, two a CU 20 to 23.5 and 67.7.
-  const auto small_time = [&](int64_t rows) {
-    const int64_t t = small_tiles(rows);
+  const auto tiles = [&](int64_t rows, int64_t size) { return (rows + size - 1) / size * ((N + size - 1) / size); };
+  const auto time_without_large = [&](int64_t rows) {
+    if (rows <= kSkinnyRows) return kFewTime;
+    if (tiles(rows, kMidTile) <= 2 * cus) return tiles(rows, kMidTile) <= cus ? kMidAlone : kMidPair;
+    const int64_t t = tiles(rows, 128);
     return t <= cus ? kSmallAlone : (double)((t + 2 * cus - 1) / (2 * cus)) * kSmallPair;
   };
   // Tokens for the large tiles: all, or what fills whole rounds of them (the rest
-  // goes to small tiles, in a launch of its own), or none.
+  // goes in a launch of its own), or none.
+  const int64_t ntn = (N + kBigTile - 1) / kBigTile, mtn = (M + kBigTile - 1) / kBigTile;
   const int64_t whole = mtn * ntn / cus * cus / ntn * kBigTile;
   int64_t big = 0;
-  double best = small_time(M);
+  double best = time_without_large(M);
   for (const int64_t rows : {std::min(M, whole), M}) {
     if (rows <= 0 || K <= 2 * kIK) continue;  // the large tiles' ring takes three stages or more
-    const int64_t t = (rows + kBigTile - 1) / kBigTile * ntn;
-    const double time = (double)((t + cus - 1) / cus) + (rows < M ? small_time(M - rows) : 0.0);
+    const double time = (double)((tiles(rows, kBigTile) + cus - 1) / cus) + (rows < M ? time_without_large(M - rows) : 0.0);
     if (time < best) {
       best = time;
       big = rows;
     }
   }
-  if (!grid_fits(small_tiles(M), 256)) return fail(AA_EUNSUPPORTED, "int8_linear: too many tokens");
+  if (!grid_fits(tiles(M, 128), 256)) return fail(AA_EUNSUPPORTED, "int8_linear: too many tokens");
   if (big > 0) {
     p.M = big;
     p.mtiles = (int)((big + kBigTile - 1) / kBigTile);
-    const int64_t t = p.mtiles * ntn;
-    int8_linear_big_kernel<<<dim3((unsigned)std::min(t, cus)), kBigThreads, 0, st>>>(p);
+    int8_linear_big_kernel<<<dim3((unsigned)std::min(tiles(big, kBigTile), cus)), kBigThreads, 0, st>>>(p);
     if (int rc = check_launch("int8_linear")) return rc;
     p.x += big * K;
     p.xs += big;
     p.y += big * N;
-  }
-  if (big < M) {
     p.M = M - big;
+  }
+  if (p.M == 0) return AA_OK;
+  if (p.M <= kSkinnyRows) {
+    const dim3 grid((unsigned)((N + 15) / 16));
+    if (p.M <= 8) int8_skinny_kernel<1><<<grid, 256, 0, st>>>(p);
+    else if (p.M <= 16) int8_skinny_kernel<2><<<grid, 256, 0, st>>>(p);
+    else if (p.M <= 32) int8_skinny_kernel<4><<<grid, 256, 0, st>>>(p);
+    else int8_skinny_kernel<8><<<grid, 256, 0, st>>>(p);
+  } else if (tiles(p.M, kMidTile) <= 2 * cus) {
+    p.mtiles = (int)((p.M + kMidTile - 1) / kMidTile);
+    int8_mid_kernel<<<dim3((unsigned)tiles(p.M, kMidTile)), 256, 0, st>>>(p);
+  } else {
     p.mtiles = (int)((p.M + 127) / 128);
-    const int64_t t = small_tiles(p.M);
+    const int64_t t = tiles(p.M, 128);
     // One workgroup a CU: the deeper ring, for weights that are not in a cache (666 x
     // 1024 x 4096: 11.4 -> 9.4 us; where they are, 8.8 against 9.4).
     if (t <= cus) int8_linear_kernel<I8TileD><<<dim3((unsigned)t), I8TileD::kThreads, 0, st>>>(p);

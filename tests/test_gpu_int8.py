@@ -125,6 +125,17 @@ def test_large_product(int8, M, K, N):
     _check_product(*args, int8.int8_linear(*args))
 
 
+# 64 x 64 tiles with K split over the waves: one to five steps (some waves without any), rests of
+# K, partial tiles both ways, one and two workgroups a CU; and rests of the large tiles.
+@pytest.mark.parametrize("M,K,N", [
+    (65, 16, 8), (65, 128, 64), (70, 144, 72), (128, 256, 128), (100, 400, 200), (333, 512, 520), (200, 640, 6144),
+    (333, 4112, 2040), (666, 8192, 2048), (1000, 65536, 64), (8193, 512, 2048), (8192 + 100, 512, 2048),
+])
+def test_middle_product(int8, M, K, N):
+    args = _product(int8, M, K, N, M + K + N, full=True)
+    _check_product(*args, int8.int8_linear(*args))
+
+
 def test_largest_sums(int8):
     """All codes at -128 or 127, K at its most: 65536 products of up to 2^14."""
     for M in (3, 130):
