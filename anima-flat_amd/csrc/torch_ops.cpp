@@ -513,9 +513,12 @@ T6 adaln_bwd(const OptT& dr_, const OptT& dh_, const Tensor& x, const OptT& y, c
   }
   const Tensor w = f32_or_none(weight);
   if (w.defined() && !aligned16(w)) return slow();
-  const auto none = [&] { return at::empty({0}, x.options()); };
-  Tensor dx = at::empty(x.sizes(), x.options()), dy = y ? at::empty(x.sizes(), x.options()) : none();
-  Tensor dgate = none(), dscale = none(), dshift = none(), dweight = none();
+  // One tensor without elements stands for all that is not computed (an allocation each
+  // would be a fifth of the call's host time).
+  Tensor none;
+  if (!y || !mods || !weight) none = at::empty({0}, x.options());
+  Tensor dx = at::empty(x.sizes(), x.options()), dy = y ? at::empty(x.sizes(), x.options()) : none;
+  Tensor dgate = none, dscale = none, dshift = none, dweight = none;
   if (mods) {
     dscale = at::empty(scale.sizes(), scale.options());
     dshift = at::empty({shift_rows, D}, scale.options());

@@ -285,7 +285,8 @@ def _rows2(t: torch.Tensor) -> torch.Tensor:
 
 
 def _modulation(*mods: torch.Tensor) -> list[torch.Tensor]:
-    """Modulations as rows of one dtype."""
+    """Modulations as rows of one dtype. (The callers leave out what is so already: in a small
+    call this and _wants_grad would be a tenth of the host's time.)"""
     mods = [t if t.ndim == 2 else _rows2(t) for t in mods]
     if any(t.dtype != mods[0].dtype for t in mods):
         if any(t.dtype not in (torch.bfloat16, torch.float32) for t in mods):
@@ -294,8 +295,11 @@ def _modulation(*mods: torch.Tensor) -> list[torch.Tensor]:
     return mods
 
 
-def _wants_grad(*ts) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+def _wants_grad(x, y, gate, scale, shift, weight) -> bool:
+    return torch.is_grad_enabled() and (
+        x.requires_grad or y.requires_grad or gate.requires_grad or scale.requires_grad or shift.requires_grad
+        or (weight is not None and weight.requires_grad)
+    )
 
 
 def residual_adaln(x, y, gate, scale, shift, weight=None, eps=1e-6, branch_scale=1.0):
@@ -320,7 +324,8 @@ def residual_adaln(x, y, gate, scale, shift, weight=None, eps=1e-6, branch_scale
     Raises:
         ValueError: If a tensor is not on CUDA, or its shape or dtype is not supported.
     """
-    gate, scale, shift = _modulation(gate, scale, shift)
+    if not (gate.ndim == scale.ndim == shift.ndim == 2 and gate.dtype == scale.dtype == shift.dtype):
+        gate, scale, shift = _modulation(gate, scale, shift)
     stats = _wants_grad(x, y, gate, scale, shift, weight)
     r, h, _ = _residual_adaln(x, y, gate, scale, shift, weight, eps, branch_scale, stats)
     return r, h
@@ -328,8 +333,10 @@ def residual_adaln(x, y, gate, scale, shift, weight=None, eps=1e-6, branch_scale
 
 def adaln(x, scale, shift, eps=1e-6):
     """`LayerNorm(x) * (1 + scale) + shift`, arguments as for `residual_adaln`."""
-    scale, shift = _modulation(scale, shift)
-    return _adaln(x, scale, shift, eps, _wants_grad(x, scale, shift))[0]
+    if not (scale.ndim == shift.ndim == 2 and scale.dtype == shift.dtype):
+        scale, shift = _modulation(scale, shift)
+    stats = torch.is_grad_enabled() and (x.requires_grad or scale.requires_grad or shift.requires_grad)
+    return _adaln(x, scale, shift, eps, stats)[0]
 
 
 def residual_adaln_int8(x, y, gate, scale, shift, weight=None, eps=1e-6, branch_scale=1.0):
@@ -340,7 +347,8 @@ def residual_adaln_int8(x, y, gate, scale, shift, weight=None, eps=1e-6, branch_
         `h ~ q * s`, rounded from the fp32 h. A token with a value that is not finite has
         the scale NaN.
     """
-    gate, scale, shift = _modulation(gate, scale, shift)
+    if not (gate.ndim == scale.ndim == shift.ndim == 2 and gate.dtype == scale.dtype == shift.dtype):
+        gate, scale, shift = _modulation(gate, scale, shift)
     if _wants_grad(x, y, gate, scale, shift, weight):
         raise RuntimeError("residual_adaln_int8 has no backward: use residual_adaln for training")
     return _residual_adaln_int8(x, y, gate, scale, shift, weight, eps, branch_scale)
