@@ -91,6 +91,26 @@ __device__ __forceinline__ float gelu_slope(float x) {
   return x < 0.f ? d : 1.0f - d;
 }
 
+// GELU for 8-bit codes whose step is at least 1e-12 / 127: log2 Q(a) is a polynomial of
+// degree 8 up to a = 9 (minimax, by linear programming against scipy's log_ndtr: 6e-6 of
+// Q, 1.4e-5 with fp32 rounding), where a Q is under 2e-18, far below half a step, and
+// stays there. One transcendental instruction and 11 others a value against the two and
+// 12 above: the row quantiser is bound by them. NaN comes through the maximum.
+__device__ __forceinline__ float gelu_coarse(float x) {
+  const float a = __builtin_amdgcn_fmed3f(__builtin_fabsf(x), 0.f, 9.0f);
+  float p = fmaf(a, 7.462385553935746e-08f, -3.6554802136379294e-06f);
+  p = fmaf(p, a, 7.943361561046913e-05f);
+  p = fmaf(p, a, -0.001020022202283144f);
+  p = fmaf(p, a, 0.008750777691602707f);
+  p = fmaf(p, a, -0.05430452153086662f);
+  p = fmaf(p, a, -0.4582415819168091f);
+  p = fmaf(p, a, -1.1512950658798218f);
+  p = fmaf(p, a, -0.999996542930603f);
+  float top;
+  asm("v_maximum3_f32 %0, %1, 0, 0" : "=v"(top) : "v"(x));
+  return fmaf(-a, __builtin_amdgcn_exp2f(p), top);
+}
+
 // x + kRoundMagic for |x| <= 127, rounded to nearest even, has round(x) in two's
 // complement in the low byte of its bits: 1.5 * 2^23 leaves the integer in the
 // low mantissa bits.

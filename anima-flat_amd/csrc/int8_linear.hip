@@ -37,8 +37,9 @@ constexpr int kQ8MaxK = 8192;
 // One wave per row, the row in registers between its one read and the store of
 // its codes: unit lane + 64 p of U values (16 where K allows 16-byte stores). HBM
 // bound, 3 bytes a value; with GELU as much by its vector instructions (block_math.h).
-// 18432 x 8192 with GELU 95 to 107 us (453 MB: 4.2 to 4.8 TB/s; a copy 5.1), 131 with
-// a division per value, a polynomial a degree longer and plain stores.
+// 18432 x 8192 with GELU 84 to 97 us (453 MB: 4.7 to 5.4 TB/s; a copy 5.1); with the
+// GELU of two transcendental instructions 95 to 107, vector instructions issued in all
+// of a CU's cycles; with a division per value and plain stores 131.
 template <int NU, int U, bool kGelu>
 __global__ __launch_bounds__(kQ8Threads) void rowquant_int8_kernel(const bf16* __restrict__ x,
                                                                    uint8_t* __restrict__ q,
@@ -65,7 +66,7 @@ __global__ __launch_bounds__(kQ8Threads) void rowquant_int8_kernel(const bf16* _
       for (int w = 0; w < U / 8; ++w) unpack8(raw[p][w], &v[p][8 * w]);
 #pragma unroll
       for (int i = 0; i < U; ++i)
-        if constexpr (kGelu) v[p][i] = gelu(v[p][i]);
+        if constexpr (kGelu) v[p][i] = gelu_coarse(v[p][i]);
 #pragma unroll
       for (int i = 0; i < U; i += 2) top = max3abs_nan(top, v[p][i], v[p][i + 1]);
     }

@@ -50,7 +50,7 @@ def test_rowquant_ties(int8):
 
 
 def test_rowquant_gelu(int8):
-    """GELU's float32 error (the fit's 3.1e-5 and a few roundings, relative) moves the scale by as much and a code by
+    """GELU's float32 error (under 3.1e-5 with a few roundings, relative) moves the scale by as much and a code by
     one step where the quotient is that near a tie."""
     g = gen(3)
     x = bf(g, 2, 40, 1032, scale=3.0)
@@ -60,6 +60,26 @@ def test_rowquant_gelu(int8):
     sd = s.view(2, 40, 1).double()
     assert ((sd - want).abs() <= 3.3e-5 * want).all()
     within(q.double() * sd, y, sd * (0.5 + 2e-5) + 3.3e-5 * y.abs(), "q s")
+
+
+def test_rowquant_gelu_tails(int8):
+    """Far negative values (GELU's tail, -0 at -inf) and rows of nothing else; +inf and NaN."""
+    x = torch.linspace(-13, 13, 512, device="cuda").repeat(6, 1)
+    x[0, ::7] = -float("inf")
+    x[1] = -12.0
+    x[2] = torch.linspace(-9.5, -6, 512)
+    x[3, 5] = float("inf")
+    x[4, 6] = float("nan")
+    x = x.to(BF)[None]
+    q, s = int8.rowquant_int8(x, gelu=True)
+    assert torch.isnan(s[:, 0]).tolist() == [False, False, False, True, True, False]
+    assert (q[0, [1, 3, 4]] == 0).all() and (q[0, 0, ::7] == 0).all()
+    keep = [0, 1, 2, 5]
+    y = ref.gelu(x.double().clamp(min=-1e3))[0, keep]  # the formula has 0 * inf at -inf
+    want = y.abs().amax(-1, keepdim=True).clamp(min=1e-12) / 127
+    sd = s[keep].double()
+    assert ((sd - want).abs() <= 3.3e-5 * want).all()
+    within(q[0, keep].double() * sd, y, sd * (0.5 + 2e-5) + 3.3e-5 * y.abs(), "q s")
 
 
 def test_rowquant_not_finite(int8):
