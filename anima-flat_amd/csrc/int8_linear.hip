@@ -322,7 +322,8 @@ __global__ __launch_bounds__(T::kThreads) void int8_linear_kernel(I8Params p) {
 // N, K; four rounds) 265 -> 252 us, two rounds 76.7 -> 75.7 and 261 -> 258.
 // At K = 8192 the matrix pipe is busy for 79% of a CU's cycles, at a clock of 1.55 GHz:
 // the power limit. At K = 2048 60% at 1.6 GHz: some 15000 cycles a tile go by outside
-// the main loop's 33000, most of them the stores of all CUs at once (33 MB a round).
+// the main loop's 33000: the epilogue's 1200 vector instructions a lane, the next tile's
+// addresses and first DMAs, and the stores of all CUs at once (33 MB a round).
 // 4096 x 8192 x 2048 73 to 78 us (1.82 POPS), 7904 x 6144 x 2048 98 to 106 (1.95),
 // 18432 x 2048 x 8192 258 (2.40, with the rest rows' launch); two waves per
 // SIMD of 64 x 128 each, per wave two barriers a stage: 76, 102 and 319.
