@@ -122,20 +122,27 @@ __device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c
   return ab | cd;
 }
 
-// Per-token int8 codes: with s = max(max |y|, 1e-12) / 127 and rcp = 1 / s, both
-// rounded to fp32, the code of y is round-to-nearest-even(y rcp), the product
-// exact (one FMA); |y rcp| <= 127 (1 + 2^-22), so |code| <= 127. The correctly
-// rounded quotient y / s in its place took two more instructions a value, a
-// tenth of the kernel's time, for codes that differ where y / s is within
-// 2^-16 of a half. A row with a value that is not finite has the scale NaN and
-// codes 0 (NaN + magic is 0x7fc00000).
+// Per-token int8 codes: with m = max(max |y|, 1e-12) the scale is m / 127, rounded to
+// fp32, and the code of y is round-to-nearest-even(127 y / m): from one FMA with the
+// row's rcp, 127 / m rounded up to fp32, whose product with y is exact in it.
+// For a bf16 y that is the rule's code in exact arithmetic, ties included. 127 y / m is
+// either a tie or 2^-17 away from one, relatively (8-bit mantissas), far more than rcp's
+// 2^-23. Ties are y = +-m / 2, 63.5, where the rounding up leaves a product of at
+// least that, so 64, the even one; and rows with 127 in m, where rcp is a power of
+// two and exact. (With 1 / s rounded either way instead, half of the values at m / 2,
+// up to 0.1% of a row, got 63.) An fp32 y's code is the rule's unless its quotient is
+// within 2^-16 of a half. |y rcp| <= 127 (1 + 2^-22), so |code| <= 127. A row with a
+// value that is not finite has the scale NaN and codes 0 (NaN + magic is 0x7fc00000).
 struct RowScale {
   float s, rcp;
 };
 __device__ __forceinline__ RowScale row_scale(uint32_t amax_bits) {
+  const float m = fmaxf(__uint_as_float(amax_bits), 1e-12f);
   RowScale r;
-  r.s = amax_bits >= kInfBits ? __builtin_nanf("") : fmaxf(__uint_as_float(amax_bits), 1e-12f) / 127.0f;
-  r.rcp = 1.0f / r.s;
+  r.s = m / 127.0f;
+  r.rcp = 127.0f / m;  // rounded to nearest: the FMA's sign says which way
+  if (fmaf(r.rcp, m, -127.0f) < 0.f) r.rcp = __uint_as_float(__float_as_uint(r.rcp) + 1u);
+  if (amax_bits >= kInfBits) r.s = r.rcp = __builtin_nanf("");
   return r;
 }
 __device__ __forceinline__ u32x2 int8_codes8(const float* y, const RowScale& r) {

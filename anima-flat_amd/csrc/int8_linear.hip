@@ -1,7 +1,7 @@
 // Tokens to int8 with a scale per token, and the product of such tokens with
 // int8 weights that have a scale per output channel:
 //
-//   s[t] = max(max_k |x[t, k]|, 1e-12) / 127, q[t, k] = round(x[t, k] (1 / s[t]))
+//   s[t] = max(max_k |x[t, k]|, 1e-12) / 127, q[t, k] = round(x[t, k] / s[t])
 //   y[t, n] = s[t] ws[n] sum_k q[t, k] wq[n, k]
 //
 // The sum is exact: int8 MFMA accumulates in int32, and K <= 65536 products of

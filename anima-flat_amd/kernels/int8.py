@@ -64,9 +64,9 @@ def rowquant_int8(x: torch.Tensor, gelu: bool = False) -> tuple[torch.Tensor, to
         gelu: Apply GELU (erf form) before quantizing.
 
     Returns:
-        `(q, s)`: int8 tokens `[B, S, K]`, `s = max(max|y|, 1e-12) / 127` as float32
-        `[B * S, 1]`, `q = round(y * (1 / s))` to nearest even. A token with a value that is not
-        finite has the scale NaN and codes 0.
+        `(q, s)`: int8 tokens `[B, S, K]`, `q = round(127 * y / m)` to nearest even with the
+        token's `m = max(max|y|, 1e-12)`, and `s = m / 127` as float32 `[B * S, 1]`. A token with a
+        value that is not finite has the scale NaN and codes 0.
 
     Raises:
         ValueError: If `x` is not on CUDA, or its dtype / K is not supported.

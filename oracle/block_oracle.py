@@ -35,15 +35,16 @@ def residual_adaln(x, y, gate, scale, shift, weight=None, eps=1e-6, branch_scale
 
 
 def int8_rows(y32):
-    """Codes (int8) and scales (float32 [rows]) of float32 rows: the scale and its reciprocal
-    rounded to float32, their product with a value (exact in float64) to an integer. On the
+    """Codes (int8) and scales (float32 [rows]) of float32 rows: the scale rounded to float32, the
+    code 127 y / max in float64 (127 y exact, and a tie's quotient too) to an integer. On the
     CPU: torch's GPU division by a constant multiplies by a rounded reciprocal."""
     dev, y32 = y32.device, y32.cpu()
     amax = y32.abs().amax(-1)
-    s = amax.clamp_min(1e-12) / 127
+    m = amax.clamp_min(1e-12)
+    s = m / 127
     bad = ~torch.isfinite(y32).all(-1)
     s = torch.where(bad, torch.full_like(s, math.nan), s)
-    q = torch.round(y32.double() * (1 / s).double().unsqueeze(-1))
+    q = torch.round(127 * y32.double() / m.double().unsqueeze(-1))
     return torch.where(bad.unsqueeze(-1), torch.zeros_like(q), q).to(dev, torch.int8), s.reshape(-1).to(dev)
 
 

@@ -289,3 +289,26 @@ def test_oracle_checkpoint():
     # A tie and the clamp at the largest magnitude: 1.9921875 / 2^-6 = 127.5.
     v = torch.tensor([[1.9921875, -1.9921875, 0.5 / 64, 1.5 / 64]]).to(BF)
     assert ref.checkpoint(v)[0][0, :4].tolist() == [127, -127, 0, 2]
+
+
+def test_int8_rule_for_every_bf16_value():
+    """The quantiser's arithmetic (an exact product with 127 / max rounded up to float32, then to
+    an integer) gives the oracle's codes for each bf16 mantissa of the largest value and every
+    smaller value, ties included."""
+    bits = torch.arange(0x7F80, dtype=torch.int32)
+    values = (bits << 16).view(torch.float32)  # finite and not negative
+    for e in (-39, -30, 0, 40, 110):
+        for m in (128 + torch.arange(128.0)) * 2.0 ** (e - 7):
+            y = values[(values <= m) & (values >= m * 2.0**-11)]
+            rcp = 127 / m
+            if rcp.double() * m.double() < 127:
+                rcp = torch.nextafter(rcp, torch.tensor(math.inf))
+            q, s = ref.int8_rows(y[None])
+            assert torch.equal(torch.round(y.double() * rcp.double()).to(torch.int8), q[0]) and s == m / 127
+    y = values[values <= 1e-12]
+    m = torch.tensor(1e-12)
+    rcp = 127 / m
+    rcp = rcp if rcp.double() * m.double() >= 127 else torch.nextafter(rcp, torch.tensor(math.inf))
+    assert torch.equal(torch.round(y.double() * rcp.double()).to(torch.int8), ref.int8_rows(y[None])[0][0])
+    half = torch.tensor([[255.0, 127.5, -127.5, 1.0]])
+    assert ref.int8_rows(half)[0].tolist() == [[127, 64, -64, 0]]
