@@ -53,15 +53,14 @@ __device__ __forceinline__ uint32_t mag_bits(float x) { return __float_as_uint(x
 
 // GELU(x) = x Phi(x) with Phi the normal distribution function. For a = |x|
 //   Q(a) = 1 - Phi(a) = exp(-a^2 / 2) F(a),  F(a) = erfcx(a / sqrt 2) / 2,
-// and F(a) = t P(t) with t = 1 / (1 + 0.375 a): P is a polynomial of degree 4
-// fitted to a relative error of 3.1e-5 over 0 <= a <= 14 (minimax, by linear
-// programming against scipy's erfcx), below which Q is under 2^-126. The error
-// is relative, so that the lower tail of GELU keeps its digits; it is a 60th of
-// a bf16 rounding (2^-9). Then, for either sign of x,
+// and F(a) = t P(t) with t = 1 / (1 + 0.3625 a): P is a polynomial of degree 6
+// fitted to a relative error of 7.7e-7 over 0 <= a <= 14 (minimax, by linear
+// programming against scipy's erfcx), below which Q is under 2^-126; 1.0e-6 with
+// fp32 rounding. The error is relative, so that the lower tail of GELU keeps its
+// digits. Then, for either sign of x,
 //   GELU(x) = max(x, 0) - a Q(a).
-// The kernels that use these are bound by vector instructions as much as by
-// memory: 12 and two transcendental ones a value (a degree more, and selecting
-// Phi by x's sign, took 18).
+// 14 vector instructions and two transcendental ones a value. Degree 4 (3.1e-5, 12
+// instructions) moved 1% of the results to the other side of a bf16 rounding.
 struct Tail {
   float a;  // |x|, or 2^100
   float f;  // Q / e
@@ -71,12 +70,14 @@ __device__ __forceinline__ Tail normal_tail(float x) {
   // Bounded so that infinity times Q's zero is no NaN. (fminf and fmaxf would
   // quiet their operand first, an instruction each; NaN comes through e.)
   const float a = __builtin_amdgcn_fmed3f(__builtin_fabsf(x), 0.f, 0x1p+100f);
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.375f, a, 1.0f));
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.3625f, a, 1.0f));
   const float e = __builtin_amdgcn_exp2f((x * (-0.5f * kLog2e)) * x);
-  float f = fmaf(t, -0.0906425192952156f, 0.20028099417686462f);
-  f = fmaf(t, f, 0.08356455713510513f);
-  f = fmaf(t, f, 0.15773384273052216f);
-  f = fmaf(t, f, 0.14906103909015656f);
+  float f = fmaf(t, 0.04806283116340637f, -0.17974217236042023f);
+  f = fmaf(t, f, 0.17510363459587097f);
+  f = fmaf(t, f, 0.029682673513889313f);
+  f = fmaf(t, f, 0.13925662636756897f);
+  f = fmaf(t, f, 0.14293640851974487f);
+  f = fmaf(t, f, 0.14470037817955017f);
   return {a, f * t, e};
 }
 __device__ __forceinline__ float gelu(float x) {
