@@ -73,19 +73,21 @@ __device__ __forceinline__ u32x2 codes8(const float* v, float inv) {
     c[i] = __float_as_uint(__builtin_amdgcn_fmed3f(fmaf(v[i], inv, kRoundMagic), kRoundMagic - 127.0f, kRoundMagic + 127.0f));
   return u32x2{low_bytes(c[0], c[1], c[2], c[3]), low_bytes(c[4], c[5], c[6], c[7])};
 }
-// Four codes + 128 as unsigned bytes, which one instruction each converts. The
-// empty asm keeps the flip on the word: left alone, the compiler flips every byte
-// by itself.
-__device__ __forceinline__ uint32_t flip_signs(uint32_t w) {
-  w ^= 0x80808080u;
+// 127 less each of four codes, as unsigned bytes, which one instruction each converts:
+// all but a byte's sign flipped. The empty asm keeps that on the word: left alone, the
+// compiler flips every byte by itself.
+__device__ __forceinline__ uint32_t below_top(uint32_t w) {
+  w ^= 0x7f7f7f7fu;
   asm("" : "+v"(w));
   return w;
 }
-// code * step of byte kByte of flip_signs(codes), with low = -128 step. Exact:
-// (code + 128) step - 128 step has at most 8 significant bits.
+// The value of a code of 127: finite for every step (128 of the largest, 2^121, are not).
+__device__ __forceinline__ float top_of(float step) { return 127.0f * step; }
+// code * step of byte kByte of below_top(codes), with top = top_of(step): 127 step -
+// (127 - code) step, exact in the FMA since code * step has at most 7 significant bits.
 template <int kByte>
-__device__ __forceinline__ float kept_value(uint32_t flipped, float step, float low) {
-  return fmaf((float)((flipped >> (8 * kByte)) & 255u), step, low);
+__device__ __forceinline__ float kept_value(uint32_t below, float step, float top) {
+  return fmaf((float)((below >> (8 * kByte)) & 255u), -step, top);
 }
 
 // -------------------------------------------------------------------- GELU --
@@ -177,13 +179,13 @@ __global__ __launch_bounds__(kGeThreads) void gelu8_bwd_kernel(GeluBwd p) {
 #pragma unroll
   for (int i = 0; i < kGeChunks; ++i) {
     if (at[i] < 0) continue;
-    const float step = step_of(e[i]), low = -128.0f * step;
+    const float step = step_of(e[i]), top = top_of(step);
     float g[8];
     unpack8(raw[i], g);
-    const uint32_t c[2] = {flip_signs(code[i][0]), flip_signs(code[i][1])};
+    const uint32_t c[2] = {below_top(code[i][0]), below_top(code[i][1])};
     static_for<0, 8>([&](auto J) {
       constexpr int j = decltype(J)::value;
-      g[j] *= gelu_slope(kept_value<j & 3>(c[j >> 2], step, low));
+      g[j] *= gelu_slope(kept_value<j & 3>(c[j >> 2], step, top));
     });
     st16_nt(p.dx + at[i], pack8(g));
   }
@@ -546,7 +548,7 @@ __device__ __forceinline__ void lora8_da(const LoraDa& p, uint8_t* lds, Block bl
       const int o = tid + kDaThreads * i, r = o / (4 * NR), rank = 4 * (o % (4 * NR));
       *reinterpret_cast<u32x2*>(mydt + r * kPitch + rank) = t.dt[i];
     }
-    float step[8], low[8];
+    float step[8], top[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) step[e] = step_of((t.ex[e >> 2] >> (8 * (e & 3))) & 255u);
     if (r0 + kDaRows > end) {  // rows past the range count nothing, whatever their group's mark
@@ -557,9 +559,9 @@ __device__ __forceinline__ void lora8_da(const LoraDa& p, uint8_t* lds, Block bl
     uint32_t code[8][2];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      low[e] = -128.0f * step[e];
-      code[e][0] = flip_signs(t.c[e][0]);
-      code[e][1] = flip_signs(t.c[e][1]);
+      top[e] = top_of(step[e]);
+      code[e][0] = below_top(t.c[e][0]);
+      code[e][1] = below_top(t.c[e][1]);
     }
     if (r0 + 2 * kDaRows < end) load(t, r0 + 2 * kDaRows);
     // One barrier a turn: these places are written again two turns on, behind the
@@ -580,8 +582,8 @@ __device__ __forceinline__ void lora8_da(const LoraDa& p, uint8_t* lds, Block bl
       u32x4 v;
       static_for<0, 4>([&](auto E) {
         constexpr int e = 2 * decltype(E)::value;
-        v[e / 2] = pack_bf16(kept_value<j & 3>(code[e][j >> 2], step[e], low[e]),
-                             kept_value<j & 3>(code[e + 1][j >> 2], step[e + 1], low[e + 1]));
+        v[e / 2] = pack_bf16(kept_value<j & 3>(code[e][j >> 2], step[e], top[e]),
+                             kept_value<j & 3>(code[e + 1][j >> 2], step[e + 1], top[e + 1]));
       });
       const bf16x8 xv = __builtin_bit_cast(bf16x8, v);
 #pragma unroll
