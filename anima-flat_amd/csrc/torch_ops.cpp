@@ -613,11 +613,14 @@ T3 gelu8(const Tensor& x, bool keep) {
   return python_impl<T3>("gelu8", x, keep);
 }
 
-// A checkpoint of `rows` rows of K channels, with exponents of n elements.
-bool kept_ready(const Tensor& codes, const Tensor& exps, const Tensor& like, int64_t rows, int64_t K, int64_t n) {
-  return codes.scalar_type() == at::kChar && exps.scalar_type() == at::kByte && on_gpu(codes, like) && on_gpu(exps, like) &&
-         codes.numel() == rows * ((K + 31) / 32 * 32) && exps.numel() == n && codes.dim() == 2 && exps.dim() == 2 && codes.is_contiguous() && exps.is_contiguous() &&
-         aligned16(codes) && aligned16(exps);
+// The copy that the forward of `rows` rows of K channels made, with exponents [e0, e1].
+bool kept_ready(const Tensor& codes, const Tensor& exps, const Tensor& like, int64_t rows, int64_t K, int64_t e0,
+                int64_t e1) {
+  const auto is = [&](const Tensor& t, at::ScalarType dtype, int64_t n0, int64_t n1) {
+    return t.scalar_type() == dtype && on_gpu(t, like) && t.dim() == 2 && t.size(0) == n0 && t.size(1) == n1 &&
+           t.is_contiguous() && aligned16(t);
+  };
+  return is(codes, at::kChar, rows, (K + 31) / 32 * 32) && is(exps, at::kByte, e0, e1);
 }
 
 Tensor gelu8_bwd(const Tensor& dy_, const Tensor& codes, const Tensor& exps) {
@@ -625,7 +628,7 @@ Tensor gelu8_bwd(const Tensor& dy_, const Tensor& codes, const Tensor& exps) {
     const c10::DeviceGuard guard(dy_.device());
     const Tensor dy = dy_.contiguous();
     const int64_t rows = dy.size(0) * dy.size(1), K = dy.size(2);
-    if (aligned16(dy) && kept_ready(codes, exps, dy, rows, K, rows * ((K + 31) / 32))) {
+    if (aligned16(dy) && kept_ready(codes, exps, dy, rows, K, rows, (K + 31) / 32)) {
       Tensor dx = at::empty(dy.sizes(), dy.options());
       if (launched(aa_gelu8_bwd(dy.data_ptr(), codes.data_ptr(), exps.data_ptr(), dx.data_ptr(), rows, K,
                                 AA_DTYPE_BF16, stream_of(dy)),
@@ -664,7 +667,7 @@ T2 lora_down8_bwd(const Tensor& dt_, const Tensor& a, const Tensor& codes, const
     const Tensor dt = dt_.contiguous();
     const int64_t rows = dt.size(0) * dt.size(1), R = a.size(0), K = a.size(1);
     if (aligned16(dt) &&
-        (!need_a || kept_ready(codes, exps, dt, rows, K, (K + 31) / 32 * ((rows + 15) / 16 * 16)))) {
+        (!need_a || kept_ready(codes, exps, dt, rows, K, (K + 31) / 32, (rows + 15) / 16 * 16))) {
       Tensor dx = need_x ? at::empty({dt.size(0), dt.size(1), K}, dt.options()) : at::empty({0}, dt.options());
       Tensor da = need_a ? at::empty({R, K}, dt.options()) : at::empty({0}, dt.options());
       const size_t bytes = need_a ? aa_lora8_bwd_workspace(rows, K, R) : 0;
