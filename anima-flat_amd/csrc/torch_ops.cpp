@@ -500,7 +500,8 @@ T6 adaln_bwd(const OptT& dr_, const OptT& dh_, const Tensor& x, const OptT& y, c
   };
   if (!adaln_ready(x, y ? &*y : nullptr, gate ? &*gate : nullptr, scale, weight)) return slow();
   const int64_t B = x.size(0), S = x.size(1), D = x.size(2);
-  if (stats.scalar_type() != at::kFloat || stats.numel() != 4 * B * S || !stats.is_contiguous() || !on_gpu(stats, x) ||
+  if (stats.scalar_type() != at::kFloat || stats.dim() != 2 || stats.size(0) != B * S || stats.size(1) != 4 ||
+      !stats.is_contiguous() || !on_gpu(stats, x) || y.has_value() != gate.has_value() ||
       (shift_rows != 1 && shift_rows != B))
     return slow();
   const c10::DeviceGuard guard(x.device());
