@@ -21,11 +21,13 @@
 #include <algorithm>
 #include <cmath>
 #include <functional>
+#include <initializer_list>
 #include <map>
 #include <memory>
 #include <optional>
 #include <string>
 #include <tuple>
+#include <unordered_set>
 #include <utility>
 #include <vector>
 
@@ -876,17 +878,32 @@ Tensor head_norm_autograd(CT x, CT w, int64_t heads, double eps) {
   return HeadNorm::apply(x, w, heads, eps);
 }
 
-// Whether the gradient of t goes to a leaf (t itself, or through casts and views)
-// whose accumulator lives already, made by an eager graph on the default stream.
-bool leaf_on_default_stream(const Tensor& t) {
-  if (!t.defined() || !t.requires_grad()) return false;
-  std::shared_ptr<torch::autograd::Node> node =
-      t.grad_fn() ? t.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(t);
-  while (node && node->num_outputs() == 1) node = node->next_edge(0).function;
-  if (!node || node->num_outputs() != 0) return false;
-  const auto stream = node->stream();
-  return stream && stream->device_type() == c10::DeviceType::CUDA &&
-         *stream == c10::hip::getDefaultHIPStreamMasqueradingAsCUDA(stream->device_index()).unwrap();
+// Whether a node that the gradient of one of `inputs` goes to, or on to, was made by an
+// eager graph on the default stream: a live accumulator of a leaf, or an operation
+// ahead of this one. Every edge is followed; this runs in captures only.
+bool reaches_default_stream(std::initializer_list<Tensor> inputs) {
+  using torch::autograd::Node;
+  std::vector<std::shared_ptr<Node>> roots;  // keep all nodes behind them alive
+  std::vector<Node*> todo;
+  std::unordered_set<Node*> seen;
+  const auto add = [&](Node* node) {
+    if (node && seen.insert(node).second) todo.push_back(node);
+  };
+  for (const Tensor& t : inputs) {
+    if (!t.defined() || !t.requires_grad()) continue;
+    roots.push_back(t.grad_fn() ? t.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(t));
+    add(roots.back().get());
+  }
+  while (!todo.empty()) {
+    Node* node = todo.back();
+    todo.pop_back();
+    const auto stream = node->stream();
+    if (stream && stream->device_type() == c10::DeviceType::CUDA &&
+        *stream == c10::hip::getDefaultHIPStreamMasqueradingAsCUDA(stream->device_index()).unwrap())
+      return true;
+    for (const auto& edge : node->next_edges()) add(edge.function.get());
+  }
+  return false;
 }
 // The backward of a captured forward would make the default stream wait for captured
 // work in such a place, which it cannot join: that ends the capture, and the process
@@ -896,9 +913,9 @@ void check_capture(const Tensor& x, const T&... more) {
   const hipStream_t stream = (hipStream_t)stream_of(x);
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
   if (!stream || hipStreamIsCapturing(stream, &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
-  TORCH_CHECK(!(leaf_on_default_stream(x) || ... || leaf_on_default_stream(more)),
+  TORCH_CHECK(!reaches_default_stream({x, more...}),
               "a forward with gradients is being captured while an eager graph of the same leaves lives: "
-              "its accumulators are on the default stream, which cannot join the capture; end that graph first");
+              "its nodes are on the default stream, which cannot join the capture; end that graph first");
 }
 
 // The statistics and 8-bit copies, which have no derivative, are handed past
