@@ -23,7 +23,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from .common import _check, aligned, custom_op
+from .common import _check, aligned, custom_op, refuse_captured_training
 from .rope import _f32
 
 MAX_D = 8192
@@ -221,6 +221,7 @@ def _(dr, dh, x, y, gate, scale, weight, stats, shift_rows, branch_scale, mods):
 
 
 def _residual_adaln_setup(ctx, inputs, output):
+    refuse_captured_training("residual_adaln")
     x, y, gate, scale, shift, weight, _, ctx.branch_scale, want_stats = inputs
     if not want_stats:
         raise RuntimeError("residual_adaln: a call that needs gradients keeps its statistics (want_stats)")
@@ -249,6 +250,7 @@ torch.library.register_autograd(
 
 
 def _adaln_setup(ctx, inputs, output):
+    refuse_captured_training("adaln")
     x, scale, shift, _, want_stats = inputs
     if not want_stats:
         raise RuntimeError("adaln: a call that needs gradients keeps its statistics (want_stats)")

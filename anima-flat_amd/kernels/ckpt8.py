@@ -19,7 +19,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from .common import _check, aligned, custom_op
+from .common import _check, aligned, custom_op, refuse_captured_training
 
 GROUP = 32
 MAX_RANK = 64
@@ -124,6 +124,7 @@ def _(dy, codes, exps):
 
 
 def _gelu8_setup(ctx, inputs, output):
+    refuse_captured_training("gelu8")
     if not inputs[1]:
         raise RuntimeError("gelu8: a call that needs gradients keeps its input (keep)")
     ctx.set_materialize_grads(False)
@@ -206,6 +207,7 @@ def _(dt, a, codes, exps, need_x, need_a):
 
 
 def _lora_down8_setup(ctx, inputs, output):
+    refuse_captured_training("lora_down8")
     _, a, keep = inputs
     if ctx.needs_input_grad[1] and not keep:
         raise RuntimeError("lora_down8: a call that needs a's gradient keeps its input (keep)")

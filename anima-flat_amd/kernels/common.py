@@ -31,6 +31,18 @@ def aligned(t: torch.Tensor) -> torch.Tensor:
     return t.clone() if t.data_ptr() % 16 else t
 
 
+def refuse_captured_training(name: str) -> None:
+    """For the autograd setups of the block's ops, which record a call only where the native
+    kernels do not: those look through the graph for an eager one that lives on the default
+    stream (its backward would end the capture, and the process); a node's stream is not to be
+    had from Python, so here every captured call with gradients is refused."""
+    if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(
+            f"{name}: a forward with gradients can be captured only with the torch extension (_anima_torch.so), "
+            "which checks that no eager graph of the same leaves lives; capture it under no_grad, or build it"
+        )
+
+
 def is_registered(qualname: str) -> bool:
     """True if the torch.library op `ns::name` exists in this process."""
     ns, name = qualname.split("::", 1)
