@@ -96,6 +96,9 @@ static void launch_rowquant(dim3 grid, hipStream_t st, const bf16* x, uint8_t* q
 // ----------------------------------------------------------------- product --
 
 constexpr int kIK = 128;      // bytes of K per stage
+// Rows of LDS of the kernels that choose k-steps by bits 5 and 6 of an address: their
+// offsets alone decide these only if the array starts at a row of 128 bytes.
+constexpr int kRowsAlign = 1024;
 constexpr int kIGroupM = 4;   // token tiles per work-order group
 
 struct I8Params {
@@ -339,7 +342,7 @@ struct NoDma {
 };
 
 __global__ __launch_bounds__(kBigThreads, 1) void int8_linear_big_kernel(I8Params p) {
-  __shared__ __attribute__((aligned(16))) uint8_t lds[5 * kBigPart];  // X's three, W's two
+  __shared__ __attribute__((aligned(kRowsAlign))) uint8_t lds[5 * kBigPart];  // X's three, W's two
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -599,7 +602,7 @@ struct Skinny {
 template <int XB>
 __global__ __launch_bounds__(256) void int8_skinny_kernel(I8Params p) {
   using T = Skinny<XB>;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[T::kLds];
+  __shared__ __attribute__((aligned(kRowsAlign))) uint8_t lds[T::kLds];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int li = lane & 15, g = lane >> 4;
@@ -698,7 +701,7 @@ constexpr int kMidBlocks = 2 * kMidTile / 8;  // DMAs per step
 constexpr int kMidStep = kMidBlocks * 1024;   // bytes
 
 __global__ __launch_bounds__(256) void int8_mid_kernel(I8Params p) {
-  __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kMidStep];
+  __shared__ __attribute__((aligned(kRowsAlign))) uint8_t lds[4 * kMidStep];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ntn = (p.N + kMidTile - 1) / kMidTile;
