@@ -425,6 +425,14 @@ bool adaln_ready(const Tensor& x, const Tensor* y, const Tensor* gate, const Ten
 Tensor f32_or_none(const OptT& weight) { return weight ? f32(*weight) : Tensor(); }
 float* float_ptr(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
 
+// A tensor without elements, with x's type and a storage of its own (no two outputs of an op
+// may share one), for what is not computed. (Through the dispatcher each would be a twentieth
+// of the backward's host time.)
+Tensor no_elements(const Tensor& x) {
+  c10::Storage none(c10::Storage::use_byte_size_t(), 0, at::DataPtr(nullptr, x.device()), nullptr, false);
+  return at::detail::make_tensor<c10::TensorImpl>(std::move(none), c10::DispatchKeySet(c10::DispatchKey::CUDA), x.dtype());
+}
+
 bool adaln_forward(const Tensor& x, const Tensor* y, const Tensor* gate, const Tensor& scale, const Tensor& shift,
                    const OptT& weight, double eps, double branch_scale, Tensor* r, Tensor* h, Tensor* q,
                    Tensor* qs, Tensor* stats) {
@@ -516,18 +524,12 @@ T6 adaln_bwd(const OptT& dr_, const OptT& dh_, const Tensor& x, const OptT& y, c
   }
   const Tensor w = f32_or_none(weight);
   if (w.defined() && !aligned16(w)) return slow();
-  // One tensor without elements stands for all that is not computed (an allocation each
-  // would be a fifth of the call's host time).
-  Tensor none;
-  if (!y || !mods || !weight) none = at::empty({0}, x.options());
-  Tensor dx = at::empty(x.sizes(), x.options()), dy = y ? at::empty(x.sizes(), x.options()) : none;
-  Tensor dgate = none, dscale = none, dshift = none, dweight = none;
-  if (mods) {
-    dscale = at::empty(scale.sizes(), scale.options());
-    dshift = at::empty({shift_rows, D}, scale.options());
-    if (y) dgate = at::empty(gate->sizes(), gate->options());
-    if (weight) dweight = at::empty({D}, x.options().dtype(at::kFloat));
-  }
+  Tensor dx = at::empty(x.sizes(), x.options());
+  Tensor dy = y ? at::empty(x.sizes(), x.options()) : no_elements(x);
+  Tensor dgate = mods && y ? at::empty(gate->sizes(), gate->options()) : no_elements(x);
+  Tensor dscale = mods ? at::empty(scale.sizes(), scale.options()) : no_elements(x);
+  Tensor dshift = mods ? at::empty({shift_rows, D}, scale.options()) : no_elements(x);
+  Tensor dweight = mods && weight ? at::empty({D}, x.options().dtype(at::kFloat)) : no_elements(x);
   const auto ptr = [](const Tensor& t) { return t.numel() ? t.data_ptr() : nullptr; };
   aa_adaln_bwd_args a = {};
   a.dr = dr.defined() ? dr.data_ptr() : nullptr;
