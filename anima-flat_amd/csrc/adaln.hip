@@ -24,8 +24,8 @@
 // with sums <= 1024) or of two, four or eight, so it is read once, the variance is
 // taken about the mean without a second read, and no barrier stands between loads
 // and stores of a wave's own row. Measured at D = 2048 (a copy: 5.1 TB/s): forward
-// 8192 tokens 20 to 22 us (6.1 to 6.7 TB/s; with plain in place of nontemporal stores
-// 22 to 25), 4096 tokens 12; int8 7904 tokens 21 to 24 (4.7 to 5.4); backward 4096
+// 8192 tokens 21 to 22 us (6.1 to 6.3 TB/s; with plain in place of nontemporal stores
+// 22 to 25), 4096 tokens 12; int8 7904 tokens 23 to 25 (4.5 to 4.9); backward 4096
 // tokens 18 (5.5 TB/s; the registers of the norm's form at two waves a SIMD: 26).
 // Backward with all gradients, 3 x 1001 tokens of 1544 17.4 (3.2 TB/s, a round of one
 // workgroup a CU, held modulation and the next row ahead; without these two 21), and

@@ -37,9 +37,9 @@ constexpr int kQ8MaxK = 8192;
 // One wave per row, the row in registers between its one read and the store of
 // its codes: unit lane + 64 p of U values (16 where K allows 16-byte stores). HBM
 // bound, 3 bytes a value; with GELU as much by its vector instructions (block_math.h).
-// 18432 x 8192 with GELU 84 to 97 us (453 MB: 4.7 to 5.4 TB/s; a copy 5.1); with the
-// GELU of two transcendental instructions 95 to 107, vector instructions issued in all
-// of a CU's cycles; with a division per value and plain stores 131.
+// 18432 x 8192 with GELU 84 to 97 us (453 MB: 4.7 to 5.4 TB/s; a copy 5.1), vector
+// instructions issued in 97% of a CU's cycles, 17 a value; with the GELU of two
+// transcendental instructions 95 to 107; with a division per value and plain stores 131.
 template <int NU, int U, bool kGelu>
 __global__ __launch_bounds__(kQ8Threads) void rowquant_int8_kernel(const bf16* __restrict__ x,
                                                                    uint8_t* __restrict__ q,
@@ -327,9 +327,10 @@ __global__ __launch_bounds__(T::kThreads) void int8_linear_kernel(I8Params p) {
 // the power limit. At K = 2048 60% at 1.6 GHz: some 15000 cycles a tile go by outside
 // the main loop's 33000: the epilogue's 1200 vector instructions a lane, the next tile's
 // addresses and first DMAs, and the stores of all CUs at once (33 MB a round).
-// 4096 x 8192 x 2048 73 to 78 us (1.82 POPS), 7904 x 6144 x 2048 98 to 106 (1.95),
-// 18432 x 2048 x 8192 258 (2.40, with the rest rows' launch); two waves per
-// SIMD of 64 x 128 each, per wave two barriers a stage: 76, 102 and 319.
+// 4096 x 8192 x 2048 64 to 68 us (2.0 to 2.15 POPS), 7904 x 6144 x 2048 92 to 95 (2.1),
+// 18432 x 2048 x 8192 245 to 265 (2.3 to 2.5, with the rest rows' launch). Two waves per SIMD of
+// 64 x 128 each, per wave two barriers a stage, 76, 102 and 319 where this form took 73 to
+// 78, 98 to 106 and 258 (another box, random codes).
 __device__ const u32x4 kZeroChunk = {0, 0, 0, 0};
 
 constexpr int kBigTile = 256;
@@ -854,7 +855,8 @@ extern "C" int aa_rowquant_int8(const void* x, int64_t rows, int64_t K, int gelu
 // Times of what stands beside the large tiles, in rounds of those (37.5 us at K = 2048,
 // 109 at 8192). Measured: up to 64 tokens 4 and 9 us; 64 x 64 tiles, one or two a CU,
 // 6.2 and 10 at K = 2048, 11 to 15 and 27 at 8192; 128 x 128 tiles, one or two a CU, 14.4
-// and 20 to 23.5 at K = 2048, 40 and 68 at 8192.
+// and 20 to 23.5 at K = 2048, 40 and 68 at 8192. Below K = 2048 a launch's fixed part weighs
+// more in all of them: 64 x 64 tiles two a CU 5.6 at K = 512, 128 x 128 one a CU 6.9 (8.9 at 1024).
 constexpr double kFewTime = 0.1, kMidAlone = 0.16, kMidPair = 0.26, kSmallAlone = 0.38, kSmallPair = 0.62;
 
 extern "C" int aa_int8_linear(const void* q, const float* s, const void* weight, const float* weight_scale,

@@ -425,8 +425,8 @@ int aa_adaln_bwd(const aa_adaln_bwd_args* args, void* workspace, size_t workspac
  * Per-row int8 quantisation of x [rows, K] bf16 (contiguous): y = x or GELU(x)
  * (gelu != 0; erf form, to 3e-5 relative or 2e-18), s[row] = max(max|y|, 1e-12)
  * / 127 (float), q = round-to-nearest-even(127 y / max(max|y|, 1e-12)) (int8
- * [rows, K]): without GELU as in exact arithmetic, after it but for quotients
- * within float's error of a tie. A row with a value that is not finite has the
+ * [rows, K]): without GELU as in exact arithmetic, after it but for quotients as
+ * near a tie as GELU's error. A row with a value that is not finite has the
  * scale NaN and codes 0. K a multiple of 8 and at most 8192; x 16-byte and q 8-byte
  * aligned.
  */
