@@ -12,7 +12,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import threading
-from ctypes import Structure, c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p
+from ctypes import Structure, c_char_p, c_double, c_float, c_int, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
 import torch
@@ -85,6 +85,8 @@ _PROTOTYPES: dict[str, tuple[object, list[object]]] = {
     "aa_lora8_fwd": (c_int, [c_void_p] * 6 + [c_size_t] + [_I64] * 3 + [c_int, c_void_p]),
     "aa_lora8_bwd_workspace": (c_size_t, [_I64] * 3),
     "aa_lora8_bwd": (c_int, [c_void_p] * 6 + [c_void_p, c_size_t] + [_I64] * 3 + [c_int, c_void_p]),
+    "aa_rotary_tables": (c_int, [c_void_p, c_void_p]),
+    "aa_rotary": (c_int, [c_void_p, c_void_p]),
 }
 
 EXPORTED = tuple(_PROTOTYPES)
@@ -208,6 +210,51 @@ class AdalnBwdArgs(Structure):
     ]
 
 
+class RotaryTablesArgs(Structure):
+    """Mirror of aa_rotary_tables_args."""
+
+    _fields_ = [
+        ("positions", c_void_p),
+        ("cos", c_void_p),
+        ("sin", c_void_p),
+        ("rows", c_int64),
+        ("axes", c_int64),
+        ("dims", c_int64 * 4),
+        ("theta", c_double * 4),
+        ("scale", c_double * 4),
+        ("original", c_double),
+        ("scaling", c_int),
+        ("position_type", c_int),
+    ]
+
+
+class RotaryArgs(Structure):
+    """Mirror of aa_rotary_args."""
+
+    _fields_ = [
+        ("q", c_void_p),
+        ("k", c_void_p),
+        ("q_out", c_void_p),
+        ("k_out", c_void_p),
+        ("cos", c_void_p),
+        ("sin", c_void_p),
+        ("q_stride", c_int64 * 3),
+        ("k_stride", c_int64 * 3),
+        ("q_out_stride", c_int64 * 3),
+        ("k_out_stride", c_int64 * 3),
+        ("table_stride", c_int64),
+        ("B", c_int64),
+        ("S", c_int64),
+        ("H", c_int64),
+        ("Hk", c_int64),
+        ("hd", c_int64),
+        ("part", c_int64),
+        ("interleaved", c_int),
+        ("inverse", c_int),
+        ("dtype", c_int),
+    ]
+
+
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 on_load: list = []  # called, in order, once the library is loaded
@@ -324,6 +371,8 @@ __all__ = [
     "AttnFwdArgs",
     "EXPORTED",
     "LIB_PATH",
+    "RotaryArgs",
+    "RotaryTablesArgs",
     "available",
     "bshd_strides",
     "c_strides",

@@ -35,6 +35,9 @@ NATIVE_BLOCK_OPS = frozenset("anima_flat_amd::" + name for name in (
     "gelu8", "gelu8_bwd", "lora_down8", "lora_down8_bwd",
 ))
 
+# Rotary positions and sparse attention (kernels.rotary, kernels.sparse).
+NATIVE_SPARSE_OPS = frozenset("anima_flat_amd::" + name for name in ("rotary_tables", "rotary"))
+
 _ext = None
 _missing = False
 
@@ -85,7 +88,7 @@ def _load():
 
 def attach(qualname: str, impl) -> None:
     """Give op `qualname` its native kernels, if it has any."""
-    if qualname in NATIVE_OPS or qualname in NATIVE_BLOCK_OPS:
+    if qualname in NATIVE_OPS or qualname in NATIVE_BLOCK_OPS or qualname in NATIVE_SPARSE_OPS:
         ext = _load()
         if ext is not None:
             ext.attach(qualname, impl)

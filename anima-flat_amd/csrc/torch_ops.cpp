@@ -689,6 +689,106 @@ T2 lora_down8_bwd(const Tensor& dt_, const Tensor& a, const Tensor& codes, const
   return python_impl<T2>("lora_down8_bwd", dt_, a, codes, exps, need_x, need_a);
 }
 
+// ------------------------------------------------------- rotary positions --
+
+using Ints = at::IntArrayRef;
+using Doubles = at::ArrayRef<double>;
+
+T2 rotary_tables(const Tensor& positions, Ints dims, Doubles theta, Doubles scale, int64_t scaling, double original) {
+  const int64_t axes = (int64_t)dims.size();
+  int type = -1;
+  switch (positions.scalar_type()) {
+    case at::kInt: type = AA_POSITION_INT32; break;
+    case at::kLong: type = AA_POSITION_INT64; break;
+    case at::kFloat: type = AA_POSITION_FP32; break;
+    case at::kDouble: type = AA_POSITION_FP64; break;
+    default: break;
+  }
+  int64_t values = 0;
+  for (const int64_t d : dims) values += d;
+  if (type >= 0 && axes >= 1 && axes <= 4 && (int64_t)theta.size() == axes && (int64_t)scale.size() == axes &&
+      positions.dim() >= 2 && positions.size(-1) == axes && positions.is_contiguous() && positions.numel() > 0 &&
+      values >= 2 && values <= 512) {
+    const c10::DeviceGuard guard(positions.device());
+    std::vector<int64_t> shape(positions.sizes().begin(), positions.sizes().end());
+    shape.back() = values / 2;
+    const auto fopt = positions.options().dtype(at::kFloat);
+    Tensor cos = at::empty(shape, fopt), sin = at::empty(shape, fopt);
+    aa_rotary_tables_args a = {};
+    a.positions = positions.data_ptr();
+    a.cos = cos.data_ptr<float>();
+    a.sin = sin.data_ptr<float>();
+    a.rows = positions.numel() / axes;
+    a.axes = axes;
+    for (int64_t i = 0; i < axes; ++i) {
+      a.dims[i] = dims[i];
+      a.theta[i] = theta[i];
+      a.scale[i] = scale[i];
+    }
+    a.original = original;
+    a.scaling = (int)scaling;
+    a.position_type = type;
+    if (launched(aa_rotary_tables(&a, stream_of(positions)), "rotary_tables")) return {cos, sin};
+  }
+  return python_impl<T2>("rotary_tables", positions, dims.vec(), theta.vec(), scale.vec(), scaling, original);
+}
+
+int rotary_dtype(const Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return AA_DTYPE_BF16;
+    case at::kHalf: return AA_DTYPE_FP16;
+    case at::kFloat: return AA_DTYPE_FP32;
+    default: return -1;
+  }
+}
+
+// [B, S, H, hd] heads that the turn reads in place.
+bool heads_ready(const Tensor& t, const Tensor& like) {
+  if (t.dim() != 4 || t.scalar_type() != like.scalar_type() || !t.is_cuda() || !on_gpu(t, like) || t.numel() == 0) return false;
+  const int64_t unit = 16 / t.element_size();
+  return t.stride(3) == 1 && t.stride(0) % unit == 0 && t.stride(1) % unit == 0 && t.stride(2) % unit == 0 && aligned16(t);
+}
+
+T2 rotary(const Tensor& q, const OptT& k_, const Tensor& cos, const Tensor& sin, bool interleaved, bool inverse) {
+  const Tensor* k = k_ && k_->defined() ? &*k_ : nullptr;
+  const int dtype = rotary_dtype(q);
+  if (dtype >= 0 && heads_ready(q, q) &&
+      (!k || (heads_ready(*k, q) && k->size(0) == q.size(0) && k->size(1) == q.size(1) && k->size(3) == q.size(3))) &&
+      (cos.dim() == 2 || (cos.dim() == 3 && (cos.size(0) == 1 || cos.size(0) == q.size(0)))) &&
+      cos.size(-2) == q.size(1) && sin.sizes() == cos.sizes() && cos.scalar_type() == at::kFloat &&
+      sin.scalar_type() == at::kFloat && on_gpu(cos, q) && on_gpu(sin, q) && cos.is_contiguous() &&
+      sin.is_contiguous() && aligned16(cos) && aligned16(sin)) {
+    const c10::DeviceGuard guard(q.device());
+    Tensor qo = at::empty(q.sizes(), q.options());
+    Tensor ko = k ? at::empty(k->sizes(), q.options()) : at::empty({0}, q.options());
+    aa_rotary_args a = {};
+    a.q = q.data_ptr();
+    a.q_out = qo.data_ptr();
+    set_strides(a.q_stride, q);
+    set_strides(a.q_out_stride, qo);
+    if (k) {
+      a.k = k->data_ptr();
+      a.k_out = ko.data_ptr();
+      set_strides(a.k_stride, *k);
+      set_strides(a.k_out_stride, ko);
+      a.Hk = k->size(2);
+    }
+    a.cos = cos.data_ptr<float>();
+    a.sin = sin.data_ptr<float>();
+    a.table_stride = cos.dim() == 3 && cos.size(0) > 1 ? cos.stride(0) : 0;
+    a.B = q.size(0);
+    a.S = q.size(1);
+    a.H = q.size(2);
+    a.hd = q.size(3);
+    a.part = 2 * cos.size(-1);
+    a.interleaved = interleaved;
+    a.inverse = inverse;
+    a.dtype = dtype;
+    if (launched(aa_rotary(&a, stream_of(q)), "rotary")) return {qo, ko};
+  }
+  return python_impl<T2>("rotary", q, k_, cos, sin, interleaved, inverse);
+}
+
 // ----------------------------------------------------------------- autograd --
 
 // The dispatcher's handle of one op, called below or above autograd.
@@ -737,6 +837,8 @@ ANIMA_OP(op_gelu8, "anima_flat_amd::gelu8", T3, CT, bool)
 ANIMA_OP(op_gelu8_bwd, "anima_flat_amd::gelu8_bwd", Tensor, CT, CT, CT)
 ANIMA_OP(op_lora_down8, "anima_flat_amd::lora_down8", T3, CT, CT, bool)
 ANIMA_OP(op_lora_down8_bwd, "anima_flat_amd::lora_down8_bwd", T2, CT, CT, CT, CT, bool, bool)
+ANIMA_OP(op_rotary_tables, "anima_flat_amd::rotary_tables", T2, CT, Ints, Doubles, Doubles, int64_t, double)
+ANIMA_OP(op_rotary, "anima_flat_amd::rotary", T2, CT, CO, CT, CT, bool, bool)
 #undef ANIMA_OP
 
 // Whether a call is recorded for the backward; no op here has a forward-mode
@@ -1061,6 +1163,43 @@ T3 lora_down8_autograd(CT x, CT a, bool keep) {
   return {t, codes, exps};
 }
 
+// Both outputs are linear in q and k: a backward of the backward is another turn.
+struct Rotary : torch::autograd::Function<Rotary> {
+  static constexpr bool is_traceable = true;
+  static variable_list forward(AutogradContext* ctx, CT q, CO k, CT cos, CT sin, bool interleaved, bool inverse) {
+    auto [qo, ko] = op_rotary().below(q, k, cos, sin, interleaved, inverse);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({cos, sin});
+    ctx->saved_data["pair"] = k.has_value() && k->defined();
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["inverse"] = inverse;
+    return {qo, ko};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    variable_list out(6);
+    const variable_list s = ctx->get_saved_variables();
+    const bool interleaved = ctx->saved_data["interleaved"].toBool(), inverse = !ctx->saved_data["inverse"].toBool();
+    const bool key = ctx->saved_data["pair"].toBool() && g[1].defined();
+    if (g[0].defined()) {
+      auto [dq, dk] = op_rotary()(g[0], key ? OptT(g[1]) : OptT(), s[0], s[1], interleaved, inverse);
+      out[0] = dq;
+      if (key) out[1] = dk;
+    } else if (key) {
+      out[1] = std::get<0>(op_rotary()(g[1], OptT(), s[0], s[1], interleaved, inverse));
+    }
+    return out;
+  }
+};
+
+T2 rotary_autograd(CT q, CO k, CT cos, CT sin, bool interleaved, bool inverse) {
+  if (!needs_grad(q, k, cos, sin)) return op_rotary().below(q, k, cos, sin, interleaved, inverse);
+  TORCH_CHECK(!cos.requires_grad() && !sin.requires_grad(), "rotary: the tables have no gradient");
+  check_capture(q, k.value_or(Tensor()));
+  T2 r;
+  from_list(Rotary::apply(q, k, cos, sin, interleaved, inverse), r);
+  return r;
+}
+
 // ------------------------------------------------------------- registration --
 
 // Registrations live as long as the process, as torch.library's do.
@@ -1108,6 +1247,8 @@ void add_kernels(const std::string& ns, const std::string& name) {
   ANIMA_PLAIN(int8_linear, Tensor, CT, CT, CT, CT);
   ANIMA_PLAIN(gelu8_bwd, Tensor, CT, CT, CT);
   ANIMA_PLAIN(lora_down8_bwd, T2, CT, CT, CT, CT, bool, bool);
+  ANIMA_ADD(rotary, &rotary_autograd);
+  ANIMA_PLAIN(rotary_tables, T2, CT, Ints, Doubles, Doubles, int64_t, double);
   TORCH_CHECK(false, "no native kernels for ", ns, "::", name);
 }
 

@@ -52,8 +52,8 @@ enum {
 
 enum {
   AA_DTYPE_BF16 = 0,
-  AA_DTYPE_FP16 = 1, /* reserved: rejected with AA_EUNSUPPORTED */
-  AA_DTYPE_FP32 = 2, /* modulation rows of aa_adaln_fwd / _bwd only */
+  AA_DTYPE_FP16 = 1, /* aa_rotary only */
+  AA_DTYPE_FP32 = 2, /* aa_rotary, and modulation rows of aa_adaln_fwd / _bwd, only */
 };
 
 /* ABI version of the loaded library (AA_ABI_VERSION when built from this header). */
@@ -487,6 +487,66 @@ size_t aa_lora8_bwd_workspace(int64_t M, int64_t K, int64_t R);
 int aa_lora8_bwd(const void* dt, const void* a, const void* codes, const void* exps, void* dx,
                  void* da, void* workspace, size_t workspace_bytes, int64_t M, int64_t K,
                  int64_t R, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Rotary positions                                                          */
+/* ------------------------------------------------------------------------ */
+
+enum { AA_POSITION_INT32 = 0, AA_POSITION_INT64 = 1, AA_POSITION_FP32 = 2, AA_POSITION_FP64 = 3 };
+enum { AA_SCALING_NTK = 0, AA_SCALING_LINEAR = 1, AA_SCALING_YARN = 2 };
+
+typedef struct aa_rotary_tables_args {
+  const void* positions; /* [rows, axes] of position_type */
+  float* cos;            /* [rows, pairs], pairs = sum(dims) / 2 */
+  float* sin;
+  int64_t rows, axes;    /* 1 to 4 axes */
+  int64_t dims[4];       /* values of a head that turn with each axis: even, 2 to 512 together */
+  double theta[4];       /* base of each axis' frequencies */
+  double scale[4];       /* >= 1: how much longer the axis is than in training */
+  double original;       /* AA_SCALING_YARN: the trained length */
+  int scaling;
+  int position_type;
+} aa_rotary_tables_args;
+
+/*
+ * cos and sin of positions[t, axis(i)] * f_i, the angle in 64 bits; f_i =
+ * theta^(-2 i / d) for pair i of an axis of d dims, and for a scale s:
+ *   AA_SCALING_NTK     theta s^(d / (d - 2)) in theta's place (d > 2);
+ *   AA_SCALING_LINEAR  f_i / s;
+ *   AA_SCALING_YARN    f_i (g + (1 - g) / s), g = (original f_i / (2 pi) - 1) / 31
+ *                      clamped to 0 .. 1, and both tables times 0.1 ln(max s) + 1.
+ * The angle is exact to 2^-52 of itself: positions up to 10^8 are told apart.
+ * Generalises src/model.py:51-84 (rope_tables), whose tables at 1 x 1 to h x w
+ * are AA_SCALING_NTK's of axes (t, y, x).
+ */
+int aa_rotary_tables(const aa_rotary_tables_args* args, void* stream);
+
+typedef struct aa_rotary_args {
+  const void* q;           /* [B, S, H, hd] */
+  const void* k;           /* [B, S, Hk, hd]; unused when Hk == 0 */
+  void* q_out;             /* [B, S, H, hd], no memory shared with the inputs */
+  void* k_out;
+  const float* cos;        /* [S, part / 2] contiguous, batch item b's at b * table_stride */
+  const float* sin;
+  int64_t q_stride[3];     /* batch, token, head strides in elements, head-dim stride 1 */
+  int64_t k_stride[3];
+  int64_t q_out_stride[3];
+  int64_t k_out_stride[3];
+  int64_t table_stride;    /* 0: one table for all batch items; else S * part / 2 or more */
+  int64_t B, S, H, Hk, hd;
+  int64_t part;            /* values of a head that are turned; the others are copied */
+  int interleaved;         /* pairs (2 i, 2 i + 1), not (i, i + part / 2) */
+  int inverse;             /* by minus the angles: the backward */
+  int dtype;               /* AA_DTYPE_BF16, AA_DTYPE_FP16 or AA_DTYPE_FP32 */
+} aa_rotary_args;
+
+/*
+ * (a, b) -> (a cos - b sin, b cos + a sin) for every pair of the first `part`
+ * values of every head, in fp32, rounded once. hd a multiple of 8, at most 512;
+ * pointers 16-byte aligned, strides multiples of 16 bytes.
+ * Stands beside src/kernels/rope.py:61-143, whose turn is fused with its norm.
+ */
+int aa_rotary(const aa_rotary_args* args, void* stream);
 
 #ifdef __cplusplus
 }
