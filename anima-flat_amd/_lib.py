@@ -87,6 +87,12 @@ _PROTOTYPES: dict[str, tuple[object, list[object]]] = {
     "aa_lora8_bwd": (c_int, [c_void_p] * 6 + [c_void_p, c_size_t] + [_I64] * 3 + [c_int, c_void_p]),
     "aa_rotary_tables": (c_int, [c_void_p, c_void_p]),
     "aa_rotary": (c_int, [c_void_p, c_void_p]),
+    "aa_block_select_workspace": (c_size_t, [_I64] * 5),
+    "aa_block_select": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
+    "aa_sparse_fwd_workspace": (c_size_t, [_I64] * 4),
+    "aa_sparse_fwd": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
+    "aa_sparse_bwd_workspace": (c_size_t, [_I64] * 4),
+    "aa_sparse_bwd": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
 }
 
 EXPORTED = tuple(_PROTOTYPES)
@@ -255,6 +261,91 @@ class RotaryArgs(Structure):
     ]
 
 
+class BlockSelectArgs(Structure):
+    """Mirror of aa_block_select_args."""
+
+    _fields_ = [
+        ("q", c_void_p),
+        ("k", c_void_p),
+        ("seqused_k", c_void_p),
+        ("blocks", c_void_p),
+        ("q_stride", c_int64 * 3),
+        ("k_stride", c_int64 * 3),
+        ("B", c_int64),
+        ("Sq", c_int64),
+        ("Sk", c_int64),
+        ("H", c_int64),
+        ("Hk", c_int64),
+        ("hd", c_int64),
+        ("count", c_int64),
+        ("dtype", c_int),
+    ]
+
+
+class SparseFwdArgs(Structure):
+    """Mirror of aa_sparse_fwd_args."""
+
+    _fields_ = [
+        ("q", c_void_p),
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("out", c_void_p),
+        ("rest", c_void_p),
+        ("lse", c_void_p),
+        ("seqused_k", c_void_p),
+        ("blocks", c_void_p),
+        ("q_stride", c_int64 * 3),
+        ("k_stride", c_int64 * 3),
+        ("v_stride", c_int64 * 3),
+        ("out_stride", c_int64 * 3),
+        ("B", c_int64),
+        ("Sq", c_int64),
+        ("Sk", c_int64),
+        ("H", c_int64),
+        ("Hk", c_int64),
+        ("hd", c_int64),
+        ("count", c_int64),
+        ("softmax_scale", c_float),
+        ("dtype", c_int),
+    ]
+
+
+class SparseBwdArgs(Structure):
+    """Mirror of aa_sparse_bwd_args."""
+
+    _fields_ = [
+        ("dout", c_void_p),
+        ("q", c_void_p),
+        ("k", c_void_p),
+        ("v", c_void_p),
+        ("out", c_void_p),
+        ("rest", c_void_p),
+        ("lse", c_void_p),
+        ("seqused_k", c_void_p),
+        ("blocks", c_void_p),
+        ("dq", c_void_p),
+        ("dk", c_void_p),
+        ("dv", c_void_p),
+        ("dout_stride", c_int64 * 3),
+        ("q_stride", c_int64 * 3),
+        ("k_stride", c_int64 * 3),
+        ("v_stride", c_int64 * 3),
+        ("out_stride", c_int64 * 3),
+        ("dq_stride", c_int64 * 3),
+        ("dk_stride", c_int64 * 3),
+        ("dv_stride", c_int64 * 3),
+        ("B", c_int64),
+        ("Sq", c_int64),
+        ("Sk", c_int64),
+        ("H", c_int64),
+        ("Hk", c_int64),
+        ("hd", c_int64),
+        ("count", c_int64),
+        ("softmax_scale", c_float),
+        ("dtype", c_int),
+    ]
+
+
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 on_load: list = []  # called, in order, once the library is loaded
@@ -369,10 +460,13 @@ __all__ = [
     "AdalnBwdArgs",
     "AttnBwdArgs",
     "AttnFwdArgs",
+    "BlockSelectArgs",
     "EXPORTED",
     "LIB_PATH",
     "RotaryArgs",
     "RotaryTablesArgs",
+    "SparseBwdArgs",
+    "SparseFwdArgs",
     "available",
     "bshd_strides",
     "c_strides",

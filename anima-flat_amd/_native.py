@@ -36,7 +36,9 @@ NATIVE_BLOCK_OPS = frozenset("anima_flat_amd::" + name for name in (
 ))
 
 # Rotary positions and sparse attention (kernels.rotary, kernels.sparse).
-NATIVE_SPARSE_OPS = frozenset("anima_flat_amd::" + name for name in ("rotary_tables", "rotary"))
+NATIVE_SPARSE_OPS = frozenset("anima_flat_amd::" + name for name in (
+    "rotary_tables", "rotary", "select_blocks", "sparse_fwd", "sparse_bwd",
+))
 
 _ext = None
 _missing = False

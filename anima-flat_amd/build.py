@@ -29,7 +29,8 @@ LIB_PATH = HERE / LIB_NAME
 SOURCES = (
     "abi.hip", "prologue.hip", "ctx_scale.hip", "context.hip", "rowquant.hip", "attn_fwd.hip",
     "attn_fwd_pp.hip", "attn_fwd_ks.hip", "attn_fwd_d384.hip", "attn_bwd.hip", "attn_bwd_dq_ks.hip",
-    "attn_bwd_dkdv.hip", "qkv_proj.hip", "adaln.hip", "int8_linear.hip", "ckpt8.hip", "rotary.hip",
+    "attn_bwd_dkdv.hip", "qkv_proj.hip", "adaln.hip", "int8_linear.hip", "ckpt8.hip", "rotary.hip", "sparse_select.hip",
+    "sparse_fwd.hip", "sparse_bwd.hip",
 )
 ARCH = "gfx950"
 # The measurement's MFMA-rate calibration (bench.py), a library of its own so
@@ -69,6 +70,8 @@ SOURCE_FLAGS: dict[str, list[str]] = {
     "attn_fwd_ks.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "attn_bwd_dq_ks.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "attn_bwd_dkdv.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "sparse_fwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "sparse_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 

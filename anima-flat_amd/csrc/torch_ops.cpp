@@ -789,6 +789,139 @@ T2 rotary(const Tensor& q, const OptT& k_, const Tensor& cos, const Tensor& sin,
   return python_impl<T2>("rotary", q, k_, cos, sin, interleaved, inverse);
 }
 
+// -------------------------------------------- attention over selected blocks --
+
+// q [B, Sq, H, 128] and k, v [B, Sk, Hk, 128] (v may be null) that the kernels read in place.
+bool grouped_ready(const Tensor& q, const Tensor& k, const Tensor* v, const OptT& seqused) {
+  if (q.dim() != 4 || k.dim() != 4 || q.size(3) != 128 || k.size(3) != 128 || k.size(0) != q.size(0) ||
+      k.size(2) == 0 || q.size(2) % k.size(2) || !bf16_on(q, q) || !bf16_on(k, q) || q.numel() == 0 ||
+      k.numel() == 0 || !kernel_ready(q) || !kernel_ready(k))
+    return false;
+  if (v && (!v->sizes().equals(k.sizes()) || !bf16_on(*v, q) || !kernel_ready(*v))) return false;
+  return !seqused || !seqused->defined() || lengths_ready(*seqused, q, at::kInt);
+}
+
+bool blocks_ready(const Tensor& blocks, const Tensor& q) {
+  return blocks.dim() == 4 && blocks.size(0) == q.size(0) && blocks.size(1) == q.size(2) &&
+         blocks.size(2) == (q.size(1) + 63) / 64 && blocks.size(3) > 0 && blocks.scalar_type() == at::kInt &&
+         on_gpu(blocks, q) && blocks.is_contiguous();
+}
+
+const int32_t* lengths_ptr(const OptT& t) { return t && t->defined() ? t->data_ptr<int32_t>() : nullptr; }
+
+// Workspace of `bytes` that lives until the launch.
+Tensor workspace(size_t bytes, const Tensor& like) {
+  return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor();
+}
+void* workspace_ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+template <class Args>
+void set_sizes(Args& a, const Tensor& q, const Tensor& k, int64_t count) {
+  a.B = q.size(0);
+  a.Sq = q.size(1);
+  a.Sk = k.size(1);
+  a.H = q.size(2);
+  a.Hk = k.size(2);
+  a.hd = 128;
+  a.count = count;
+  a.dtype = AA_DTYPE_BF16;
+}
+
+Tensor select_blocks(const Tensor& q, const Tensor& k, int64_t count, const OptT& seqused) {
+  if (grouped_ready(q, k, nullptr, seqused) && count >= 1 && count <= 4096) {
+    const c10::DeviceGuard guard(q.device());
+    Tensor blocks = at::empty({q.size(0), q.size(2), (q.size(1) + 63) / 64, count}, q.options().dtype(at::kInt));
+    aa_block_select_args a = {};
+    a.q = q.data_ptr();
+    a.k = k.data_ptr();
+    a.seqused_k = lengths_ptr(seqused);
+    a.blocks = blocks.data_ptr<int32_t>();
+    set_strides(a.q_stride, q);
+    set_strides(a.k_stride, k);
+    set_sizes(a, q, k, count);
+    const size_t bytes = aa_block_select_workspace(a.B, a.Sq, a.Sk, a.H, a.Hk);
+    const Tensor ws = workspace(bytes, q);
+    if (launched(aa_block_select(&a, workspace_ptr(ws), bytes, stream_of(q)), "select_blocks")) return blocks;
+  }
+  return python_impl<Tensor>("select_blocks", q, k, count, seqused);
+}
+
+T3 sparse_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& blocks, const OptT& seqused, bool keep) {
+  if (grouped_ready(q, k, &v, seqused) && blocks_ready(blocks, q)) {
+    const c10::DeviceGuard guard(q.device());
+    Tensor out = at::empty(q.sizes(), q.options()), lse, rest;
+    if (keep) {
+      lse = at::empty({q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
+      rest = at::empty(q.sizes(), q.options());
+    } else {
+      lse = at::empty({0}, q.options().dtype(at::kFloat));
+      rest = no_elements(q);
+    }
+    aa_sparse_fwd_args a = {};
+    a.q = q.data_ptr();
+    a.k = k.data_ptr();
+    a.v = v.data_ptr();
+    a.out = out.data_ptr();
+    a.rest = keep ? rest.data_ptr() : nullptr;
+    a.lse = keep ? lse.data_ptr<float>() : nullptr;
+    a.seqused_k = lengths_ptr(seqused);
+    a.blocks = blocks.data_ptr<int32_t>();
+    set_strides(a.q_stride, q);
+    set_strides(a.k_stride, k);
+    set_strides(a.v_stride, v);
+    set_strides(a.out_stride, out);
+    set_sizes(a, q, k, blocks.size(3));
+    a.softmax_scale = (float)(1.0 / std::sqrt(128.0));
+    const size_t bytes = aa_sparse_fwd_workspace(a.B, a.Sq, a.H, a.count);
+    const Tensor ws = workspace(bytes, q);
+    if (launched(aa_sparse_fwd(&a, workspace_ptr(ws), bytes, stream_of(q)), "sparse_attention")) return {out, lse, rest};
+  }
+  return python_impl<T3>("sparse_fwd", q, k, v, blocks, seqused, keep);
+}
+
+T3 sparse_bwd(const Tensor& dout_, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out,
+              const Tensor& rest, const Tensor& lse, const Tensor& blocks, const OptT& seqused) {
+  const auto slow = [&] { return python_impl<T3>("sparse_bwd", dout_, q, k, v, out, rest, lse, blocks, seqused); };
+  if (!grouped_ready(q, k, &v, seqused) || !blocks_ready(blocks, q)) return slow();
+  for (const Tensor* t : {&dout_, &out, &rest})
+    if (!t->sizes().equals(q.sizes()) || !bf16_on(*t, q)) return slow();
+  if (!out.is_contiguous() || !rest.is_contiguous() || !aligned16(out) || !aligned16(rest)) return slow();
+  if (lse.dim() != 3 || lse.size(0) != q.size(0) || lse.size(1) != q.size(2) || lse.size(2) != q.size(1) ||
+      lse.scalar_type() != at::kFloat || !on_gpu(lse, q) || !lse.is_contiguous())
+    return slow();
+  const c10::DeviceGuard guard(q.device());
+  const Tensor dout = kernel_ready(dout_) ? dout_ : dout_.contiguous();
+  if (!kernel_ready(dout)) return slow();
+  Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(v.sizes(), v.options());
+  aa_sparse_bwd_args a = {};
+  a.dout = dout.data_ptr();
+  a.q = q.data_ptr();
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  a.out = out.data_ptr();
+  a.rest = rest.data_ptr();
+  a.lse = lse.data_ptr<float>();
+  a.seqused_k = lengths_ptr(seqused);
+  a.blocks = blocks.data_ptr<int32_t>();
+  a.dq = dq.data_ptr();
+  a.dk = dk.data_ptr();
+  a.dv = dv.data_ptr();
+  set_strides(a.dout_stride, dout);
+  set_strides(a.q_stride, q);
+  set_strides(a.k_stride, k);
+  set_strides(a.v_stride, v);
+  set_strides(a.out_stride, out);
+  set_strides(a.dq_stride, dq);
+  set_strides(a.dk_stride, dk);
+  set_strides(a.dv_stride, dv);
+  set_sizes(a, q, k, blocks.size(3));
+  a.softmax_scale = (float)(1.0 / std::sqrt(128.0));
+  const size_t bytes = aa_sparse_bwd_workspace(a.B, a.Sq, a.Sk, a.H);
+  const Tensor ws = workspace(bytes, q);
+  if (!launched(aa_sparse_bwd(&a, workspace_ptr(ws), bytes, stream_of(q)), "sparse_attention backward")) return slow();
+  return {dq, dk, dv};
+}
+
 // ----------------------------------------------------------------- autograd --
 
 // The dispatcher's handle of one op, called below or above autograd.
@@ -839,6 +972,9 @@ ANIMA_OP(op_lora_down8, "anima_flat_amd::lora_down8", T3, CT, CT, bool)
 ANIMA_OP(op_lora_down8_bwd, "anima_flat_amd::lora_down8_bwd", T2, CT, CT, CT, CT, bool, bool)
 ANIMA_OP(op_rotary_tables, "anima_flat_amd::rotary_tables", T2, CT, Ints, Doubles, Doubles, int64_t, double)
 ANIMA_OP(op_rotary, "anima_flat_amd::rotary", T2, CT, CO, CT, CT, bool, bool)
+ANIMA_OP(op_select_blocks, "anima_flat_amd::select_blocks", Tensor, CT, CT, int64_t, CO)
+ANIMA_OP(op_sparse_fwd, "anima_flat_amd::sparse_fwd", T3, CT, CT, CT, CT, CO, bool)
+ANIMA_OP(op_sparse_bwd, "anima_flat_amd::sparse_bwd", T3, CT, CT, CT, CT, CT, CT, CT, CT, CO)
 #undef ANIMA_OP
 
 // Whether a call is recorded for the backward; no op here has a forward-mode
@@ -1200,6 +1336,33 @@ T2 rotary_autograd(CT q, CO k, CT cos, CT sin, bool interleaved, bool inverse) {
   return r;
 }
 
+struct SparseFwd : torch::autograd::Function<SparseFwd> {
+  static constexpr bool is_traceable = true;
+  static Tensor forward(AutogradContext* ctx, CT q, CT k, CT v, CT blocks, CO seqused, Tensor* lse, Tensor* rest) {
+    Tensor out;
+    std::tie(out, *lse, *rest) = op_sparse_fwd().below(q, k, v, blocks, seqused, true);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({q, k, v, out, *rest, *lse, blocks, seqused.value_or(Tensor())});
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    variable_list grads(7);
+    if (!g[0].defined()) return grads;
+    const variable_list s = ctx->get_saved_variables();
+    const T3 r = op_sparse_bwd()(g[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7].defined() ? OptT(s[7]) : OptT());
+    std::tie(grads[0], grads[1], grads[2]) = r;
+    return grads;
+  }
+};
+
+T3 sparse_fwd_autograd(CT q, CT k, CT v, CT blocks, CO seqused, bool keep) {
+  if (!needs_grad(q, k, v)) return op_sparse_fwd().below(q, k, v, blocks, seqused, keep);
+  check_capture(q, k, v);
+  Tensor lse, rest;
+  Tensor out = SparseFwd::apply(q, k, v, blocks, seqused, &lse, &rest);
+  return {out, lse, rest};
+}
+
 // ------------------------------------------------------------- registration --
 
 // Registrations live as long as the process, as torch.library's do.
@@ -1249,6 +1412,9 @@ void add_kernels(const std::string& ns, const std::string& name) {
   ANIMA_PLAIN(lora_down8_bwd, T2, CT, CT, CT, CT, bool, bool);
   ANIMA_ADD(rotary, &rotary_autograd);
   ANIMA_PLAIN(rotary_tables, T2, CT, Ints, Doubles, Doubles, int64_t, double);
+  ANIMA_ADD(sparse_fwd, &sparse_fwd_autograd);
+  ANIMA_PLAIN(select_blocks, Tensor, CT, CT, int64_t, CO);
+  ANIMA_PLAIN(sparse_bwd, T3, CT, CT, CT, CT, CT, CT, CT, CT, CO);
   TORCH_CHECK(false, "no native kernels for ", ns, "::", name);
 }
 

@@ -548,6 +548,113 @@ typedef struct aa_rotary_args {
  */
 int aa_rotary(const aa_rotary_args* args, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* Attention over selected blocks                                            */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * Blocks: 64 consecutive queries, 64 consecutive keys, the last of either may be
+ * shorter. A list of key blocks for each block of queries: int32 [B, H, nq,
+ * count] contiguous, nq = ceil(Sq / 64). Entries below 0 or past the last block
+ * with a key are no blocks; a block that is named twice counts once; a list
+ * without blocks gives out = 0 and lse = -inf. q has H heads, k and v Hk: head h
+ * of q reads head h / (H / Hk).
+ */
+typedef struct aa_block_select_args {
+  const void* q;            /* [B, Sq, H, hd] */
+  const void* k;            /* [B, Sk, Hk, hd]; may be NULL when Sk == 0 */
+  const int32_t* seqused_k; /* [B] keys that count, or NULL (all Sk) */
+  int32_t* blocks;          /* [B, H, nq, count] */
+  int64_t q_stride[3];      /* batch, seq, head strides in elements */
+  int64_t k_stride[3];
+  int64_t B, Sq, Sk, H, Hk, hd;
+  int64_t count;            /* 1 to 4096 */
+  int dtype;
+} aa_block_select_args;
+
+/* Bytes of workspace aa_block_select needs: the blocks' means, in 64 bits. */
+size_t aa_block_select_workspace(int64_t B, int64_t Sq, int64_t Sk, int64_t H, int64_t Hk);
+
+/*
+ * For each block of queries the `count` key blocks with the largest product of
+ * mean query and mean key (both over the rows there are), ties to the lower
+ * index, NaN before everything; in ascending order, -1 behind them where fewer
+ * blocks hold a key. Means and products are fp64. Sk at most 262144.
+ * No counterpart in the reference.
+ */
+int aa_block_select(const aa_block_select_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+typedef struct aa_sparse_fwd_args {
+  const void* q;            /* [B, Sq, H, hd] */
+  const void* k;            /* [B, Sk, Hk, hd]; k, v may be NULL when Sk == 0 */
+  const void* v;
+  void* out;                /* [B, Sq, H, hd] */
+  void* rest;               /* what out's rounding left out, laid out as out, or NULL */
+  float* lse;               /* [B, H, Sq] contiguous, or NULL */
+  const int32_t* seqused_k; /* [B], or NULL */
+  const int32_t* blocks;    /* [B, H, nq, count] */
+  int64_t q_stride[3];
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t out_stride[3];
+  int64_t B, Sq, Sk, H, Hk, hd;
+  int64_t count;
+  float softmax_scale;
+  int dtype;
+} aa_sparse_fwd_args;
+
+/* Bytes of workspace aa_sparse_fwd needs on the current device, 16-byte aligned:
+ * fp32 partial results where there are fewer blocks of queries than SIMDs and
+ * the lists are split, else 0. */
+size_t aa_sparse_fwd_workspace(int64_t B, int64_t Sq, int64_t H, int64_t count);
+
+/*
+ * out = softmax(q k^T * softmax_scale) v over the keys of the listed blocks below
+ * seqused_k, lse its natural-log row log-sum-exp. One launch, plus a combine pass
+ * when aa_sparse_fwd_workspace() > 0. Rows of k and v at or past seqused_k are
+ * not read. With lse, rest may be asked for: out + rest is the output to 16
+ * bits or more. Stands beside src/attention.py:43-81, which attends every key.
+ */
+int aa_sparse_fwd(const aa_sparse_fwd_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+typedef struct aa_sparse_bwd_args {
+  const void* dout;         /* [B, Sq, H, hd] */
+  const void* q;            /* as in the forward */
+  const void* k;
+  const void* v;
+  const void* out;          /* from aa_sparse_fwd */
+  const void* rest;         /* from aa_sparse_fwd, or NULL: D of the rounded out */
+  const float* lse;         /* [B, H, Sq] contiguous, from aa_sparse_fwd */
+  const int32_t* seqused_k;
+  const int32_t* blocks;
+  void* dq;                 /* [B, Sq, H, hd] */
+  void* dk;                 /* [B, Sk, Hk, hd]: 0 where no list names a key's block */
+  void* dv;
+  int64_t dout_stride[3];
+  int64_t q_stride[3];
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t out_stride[3];
+  int64_t dq_stride[3];
+  int64_t dk_stride[3];
+  int64_t dv_stride[3];
+  int64_t B, Sq, Sk, H, Hk, hd;
+  int64_t count;
+  float softmax_scale;
+  int dtype;
+} aa_sparse_bwd_args;
+
+/* Bytes of workspace aa_sparse_bwd needs, 16-byte aligned: 1 KB of softmax
+ * statistics per block of queries, and the lists turned round. */
+size_t aa_sparse_bwd_workspace(int64_t B, int64_t Sq, int64_t Sk, int64_t H);
+
+/*
+ * dq, dk, dv of aa_sparse_fwd, softmax recomputed from lse; dk and dv are sums
+ * over the heads of q that share a head of k. Deterministic: no atomics on
+ * floats, every sum in a fixed order. With Sq == 0 or Sk == 0 nothing is written.
+ */
+int aa_sparse_bwd(const aa_sparse_bwd_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
