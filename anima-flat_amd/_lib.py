@@ -290,7 +290,6 @@ class SparseFwdArgs(Structure):
         ("k", c_void_p),
         ("v", c_void_p),
         ("out", c_void_p),
-        ("rest", c_void_p),
         ("lse", c_void_p),
         ("seqused_k", c_void_p),
         ("blocks", c_void_p),
@@ -319,7 +318,6 @@ class SparseBwdArgs(Structure):
         ("k", c_void_p),
         ("v", c_void_p),
         ("out", c_void_p),
-        ("rest", c_void_p),
         ("lse", c_void_p),
         ("seqused_k", c_void_p),
         ("blocks", c_void_p),

@@ -22,7 +22,6 @@ constexpr int64_t kMaxCount = kMaxBlocks;
 struct SparseParams {
   const bf16 *q, *k, *v;
   bf16* o;
-  bf16* rest;               // o's rounding error, laid out as o, or null (only with lse)
   float* lse;               // [B, H, Sq] or null
   const int32_t* seqused;   // [B] or null
   const int32_t* blocks;

@@ -24,7 +24,6 @@ namespace sparse {
 
 struct BwdParams {
   bwd::Params a;           // tensors, strides, statistics [B][H][nq][kStat]; ntq = nq, ntk = nk
-  const bf16* rest;        // O's rounding error, laid out as O, or null
   const int32_t* seqused;
   const int32_t* blocks;
   uint64_t* turned;        // [B][H][nk][nqw]: bit i of word w: query block 64 w + i lists the key block
@@ -148,26 +147,20 @@ void sparse_dq_kernel(BwdParams sp) {
     dma.all_k();
   }
   // Each query's statistics: lse2 = lse log2(e) and -D, D = rowsum(dO o O)
-  // (this lane's 64 values, then the partner lane's half; O, and what its
-  // rounding left out, straight from memory). Queries past Sq, and those that attended nothing: lse2 = +inf, so
+  // (this lane's 64 values, then the partner lane's half; O straight from
+  // memory). Queries past Sq, and those that attended nothing: lse2 = +inf, so
   // that P = 0.
-  const int64_t oat = b * p.s_o[0] + h * p.s_o[2];
+  const bf16* op = p.o + b * p.s_o[0] + h * p.s_o[2];
 #pragma unroll
   for (int qb = 0; qb < 2; ++qb) {
     const int q = qrow0 + 32 * qb + li;
-    const int64_t row = oat + (int64_t)min(q, p.Sq - 1) * p.s_o[1] + 8 * hh;
+    const bf16* orow = op + (int64_t)min(q, p.Sq - 1) * p.s_o[1] + 8 * hh;
     float nd = 0.f;
 #pragma unroll
     for (int kk = 0; kk < 8; ++kk) {
       float x[8], y[8];
-      unpack8(ld16(p.o + row + 16 * kk), x);
+      unpack8(ld16(orow + 16 * kk), x);
       unpack8(__builtin_bit_cast(u32x4, w.dop[qb][kk]), y);
-      if (sp.rest) {
-        float more[8];
-        unpack8(ld16(sp.rest + row + 16 * kk), more);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] += more[i];
-      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) nd = fmaf(y[i], x[i], nd);
     }
@@ -715,7 +708,7 @@ extern "C" int aa_sparse_bwd(const aa_sparse_bwd_args* a, void* workspace, size_
   const void* all[] = {a->dout, a->q, a->k, a->v, a->out, a->lse, a->blocks, a->dq, a->dk, a->dv};
   for (const void* ptr : all)
     if (!ptr) return fail(AA_EINVAL, "sparse_bwd: null pointer");
-  const void* rows[] = {a->dout, a->q, a->k, a->v, a->out, a->rest, a->dq, a->dk, a->dv};
+  const void* rows[] = {a->dout, a->q, a->k, a->v, a->out, a->dq, a->dk, a->dv};
   for (const void* ptr : rows)
     if (!aligned16(ptr)) return fail(AA_EINVAL, "sparse_bwd: tensors must be 16-byte aligned");
   const int64_t* strides[] = {a->dout_stride, a->q_stride, a->k_stride, a->v_stride, a->out_stride, a->dq_stride, a->dk_stride, a->dv_stride};
@@ -757,7 +750,6 @@ extern "C" int aa_sparse_bwd(const aa_sparse_bwd_args* a, void* workspace, size_
   p.c = a->softmax_scale * kLog2e;
   p.scale = a->softmax_scale;
   p.stats = (float*)workspace;
-  sp.rest = (const bf16*)a->rest;
   sp.seqused = a->seqused_k;
   sp.blocks = a->blocks;
   sp.group = (int)(a->H / a->Hk);

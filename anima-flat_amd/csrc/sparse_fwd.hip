@@ -248,26 +248,11 @@ void sparse_fwd_kernel(SparseParams p) {
   for (int q = 0; q < 2; ++q) {
     const bool any = lsum[q] != 0.f;
     const float scale = any ? 1.0f / lsum[q] : 0.f;
-    f32x16 o[4] = {w.o[0][q], w.o[1][q], w.o[2][q], w.o[3][q]};
+    const f32x16 o[4] = {w.o[0][q], w.o[1][q], w.o[2][q], w.o[3][q]};
     bf16* area = ktile + q * 32 * kD;
     stage_acc_rows(o, scale, lane, area);
     stage_rows_out(p.o + at, p.os[1], qrow0 + 32 * q, p.Sq, lane, area);
     if constexpr (LSE) {
-      if (p.rest) {
-        // The backward's D = rowsum(dO o O) stands beside a dP of its own size:
-        // with O rounded to bf16, dQ is off by that rounding times the mean
-        // key, 3.4e-3 of itself where its other roundings make 2.4e-3.
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float y = o[dt][r] * scale;
-            o[dt][r] = y - round_bf16(y);
-          }
-        bf16* more = vtile + q * 32 * kD;
-        stage_acc_rows(o, 1.0f, lane, more);
-        stage_rows_out(p.rest + at, p.os[1], qrow0 + 32 * q, p.Sq, lane, more);
-      }
       const float lf = pair_sum(w.lf[q][0] + w.lf[q][1]);
       const int row = qrow0 + 32 * q + li;
       if (hh == 0 && row < p.Sq)
@@ -301,11 +286,8 @@ __global__ __launch_bounds__(64 * kCombineWaves) void sparse_combine_kernel(Spar
   }
   const bool any = sum != 0.f;
   const float scale = any ? 1.0f / sum : 0.f;
-  o0 *= scale;
-  o1 *= scale;
   const int64_t at = b * p.os[0] + q * p.os[1] + h * p.os[2] + 2 * lane;
-  *reinterpret_cast<uint32_t*>(p.o + at) = pack_bf16(o0, o1);
-  if (p.rest) *reinterpret_cast<uint32_t*>(p.rest + at) = pack_bf16(o0 - round_bf16(o0), o1 - round_bf16(o1));
+  *reinterpret_cast<uint32_t*>(p.o + at) = pack_bf16(o0 * scale, o1 * scale);
   if (p.lse && lane == 0) p.lse[r] = any ? (mx * p.c + __log2f(fsum)) * kLn2 : -INFINITY;
 }
 
@@ -346,8 +328,7 @@ extern "C" int aa_sparse_fwd(const aa_sparse_fwd_args* a, void* workspace, size_
     return fail(AA_EUNSUPPORTED, "sparse_fwd: too many query blocks");
   if (a->B == 0 || a->Sq == 0) return AA_OK;
   if (!a->q || !a->out || !a->blocks || (a->Sk && (!a->k || !a->v))) return fail(AA_EINVAL, "sparse_fwd: null pointer");
-  if (a->rest && !a->lse) return fail(AA_EINVAL, "sparse_fwd: rest comes with lse");
-  for (const void* ptr : {a->q, a->k, a->v, (const void*)a->out, (const void*)a->rest})
+  for (const void* ptr : {a->q, a->k, a->v, (const void*)a->out})
     if (!aligned16(ptr)) return fail(AA_EINVAL, "sparse_fwd: tensors must be 16-byte aligned");
   for (const int64_t* st : {a->q_stride, a->k_stride, a->v_stride, a->out_stride})
     for (int i = 0; i < 3; ++i)
@@ -359,7 +340,6 @@ extern "C" int aa_sparse_fwd(const aa_sparse_fwd_args* a, void* workspace, size_
   p.k = (const bf16*)a->k;
   p.v = (const bf16*)a->v;
   p.o = (bf16*)a->out;
-  p.rest = (bf16*)a->rest;
   p.lse = a->lse;
   p.seqused = a->seqused_k;
   p.blocks = a->blocks;

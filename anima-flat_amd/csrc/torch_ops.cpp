@@ -846,23 +846,17 @@ Tensor select_blocks(const Tensor& q, const Tensor& k, int64_t count, const OptT
   return python_impl<Tensor>("select_blocks", q, k, count, seqused);
 }
 
-T3 sparse_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& blocks, const OptT& seqused, bool keep) {
+T2 sparse_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& blocks, const OptT& seqused, bool keep) {
   if (grouped_ready(q, k, &v, seqused) && blocks_ready(blocks, q)) {
     const c10::DeviceGuard guard(q.device());
-    Tensor out = at::empty(q.sizes(), q.options()), lse, rest;
-    if (keep) {
-      lse = at::empty({q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
-      rest = at::empty(q.sizes(), q.options());
-    } else {
-      lse = at::empty({0}, q.options().dtype(at::kFloat));
-      rest = no_elements(q);
-    }
+    const auto fopt = q.options().dtype(at::kFloat);
+    Tensor out = at::empty(q.sizes(), q.options());
+    Tensor lse = keep ? at::empty({q.size(0), q.size(2), q.size(1)}, fopt) : at::empty({0}, fopt);
     aa_sparse_fwd_args a = {};
     a.q = q.data_ptr();
     a.k = k.data_ptr();
     a.v = v.data_ptr();
     a.out = out.data_ptr();
-    a.rest = keep ? rest.data_ptr() : nullptr;
     a.lse = keep ? lse.data_ptr<float>() : nullptr;
     a.seqused_k = lengths_ptr(seqused);
     a.blocks = blocks.data_ptr<int32_t>();
@@ -874,18 +868,18 @@ T3 sparse_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& b
     a.softmax_scale = (float)(1.0 / std::sqrt(128.0));
     const size_t bytes = aa_sparse_fwd_workspace(a.B, a.Sq, a.H, a.count);
     const Tensor ws = workspace(bytes, q);
-    if (launched(aa_sparse_fwd(&a, workspace_ptr(ws), bytes, stream_of(q)), "sparse_attention")) return {out, lse, rest};
+    if (launched(aa_sparse_fwd(&a, workspace_ptr(ws), bytes, stream_of(q)), "sparse_attention")) return {out, lse};
   }
-  return python_impl<T3>("sparse_fwd", q, k, v, blocks, seqused, keep);
+  return python_impl<T2>("sparse_fwd", q, k, v, blocks, seqused, keep);
 }
 
 T3 sparse_bwd(const Tensor& dout_, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out,
-              const Tensor& rest, const Tensor& lse, const Tensor& blocks, const OptT& seqused) {
-  const auto slow = [&] { return python_impl<T3>("sparse_bwd", dout_, q, k, v, out, rest, lse, blocks, seqused); };
+              const Tensor& lse, const Tensor& blocks, const OptT& seqused) {
+  const auto slow = [&] { return python_impl<T3>("sparse_bwd", dout_, q, k, v, out, lse, blocks, seqused); };
   if (!grouped_ready(q, k, &v, seqused) || !blocks_ready(blocks, q)) return slow();
-  for (const Tensor* t : {&dout_, &out, &rest})
+  for (const Tensor* t : {&dout_, &out})
     if (!t->sizes().equals(q.sizes()) || !bf16_on(*t, q)) return slow();
-  if (!out.is_contiguous() || !rest.is_contiguous() || !aligned16(out) || !aligned16(rest)) return slow();
+  if (!kernel_ready(out)) return slow();
   if (lse.dim() != 3 || lse.size(0) != q.size(0) || lse.size(1) != q.size(2) || lse.size(2) != q.size(1) ||
       lse.scalar_type() != at::kFloat || !on_gpu(lse, q) || !lse.is_contiguous())
     return slow();
@@ -899,7 +893,6 @@ T3 sparse_bwd(const Tensor& dout_, const Tensor& q, const Tensor& k, const Tenso
   a.k = k.data_ptr();
   a.v = v.data_ptr();
   a.out = out.data_ptr();
-  a.rest = rest.data_ptr();
   a.lse = lse.data_ptr<float>();
   a.seqused_k = lengths_ptr(seqused);
   a.blocks = blocks.data_ptr<int32_t>();
@@ -973,8 +966,8 @@ ANIMA_OP(op_lora_down8_bwd, "anima_flat_amd::lora_down8_bwd", T2, CT, CT, CT, CT
 ANIMA_OP(op_rotary_tables, "anima_flat_amd::rotary_tables", T2, CT, Ints, Doubles, Doubles, int64_t, double)
 ANIMA_OP(op_rotary, "anima_flat_amd::rotary", T2, CT, CO, CT, CT, bool, bool)
 ANIMA_OP(op_select_blocks, "anima_flat_amd::select_blocks", Tensor, CT, CT, int64_t, CO)
-ANIMA_OP(op_sparse_fwd, "anima_flat_amd::sparse_fwd", T3, CT, CT, CT, CT, CO, bool)
-ANIMA_OP(op_sparse_bwd, "anima_flat_amd::sparse_bwd", T3, CT, CT, CT, CT, CT, CT, CT, CT, CO)
+ANIMA_OP(op_sparse_fwd, "anima_flat_amd::sparse_fwd", T2, CT, CT, CT, CT, CO, bool)
+ANIMA_OP(op_sparse_bwd, "anima_flat_amd::sparse_bwd", T3, CT, CT, CT, CT, CT, CT, CT, CO)
 #undef ANIMA_OP
 
 // Whether a call is recorded for the backward; no op here has a forward-mode
@@ -1338,29 +1331,29 @@ T2 rotary_autograd(CT q, CO k, CT cos, CT sin, bool interleaved, bool inverse) {
 
 struct SparseFwd : torch::autograd::Function<SparseFwd> {
   static constexpr bool is_traceable = true;
-  static Tensor forward(AutogradContext* ctx, CT q, CT k, CT v, CT blocks, CO seqused, Tensor* lse, Tensor* rest) {
+  static Tensor forward(AutogradContext* ctx, CT q, CT k, CT v, CT blocks, CO seqused, Tensor* lse) {
     Tensor out;
-    std::tie(out, *lse, *rest) = op_sparse_fwd().below(q, k, v, blocks, seqused, true);
+    std::tie(out, *lse) = op_sparse_fwd().below(q, k, v, blocks, seqused, true);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({q, k, v, out, *rest, *lse, blocks, seqused.value_or(Tensor())});
+    ctx->save_for_backward({q, k, v, out, *lse, blocks, seqused.value_or(Tensor())});
     return out;
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
-    variable_list grads(7);
+    variable_list grads(6);
     if (!g[0].defined()) return grads;
     const variable_list s = ctx->get_saved_variables();
-    const T3 r = op_sparse_bwd()(g[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7].defined() ? OptT(s[7]) : OptT());
+    const T3 r = op_sparse_bwd()(g[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6].defined() ? OptT(s[6]) : OptT());
     std::tie(grads[0], grads[1], grads[2]) = r;
     return grads;
   }
 };
 
-T3 sparse_fwd_autograd(CT q, CT k, CT v, CT blocks, CO seqused, bool keep) {
+T2 sparse_fwd_autograd(CT q, CT k, CT v, CT blocks, CO seqused, bool keep) {
   if (!needs_grad(q, k, v)) return op_sparse_fwd().below(q, k, v, blocks, seqused, keep);
   check_capture(q, k, v);
-  Tensor lse, rest;
-  Tensor out = SparseFwd::apply(q, k, v, blocks, seqused, &lse, &rest);
-  return {out, lse, rest};
+  Tensor lse;
+  Tensor out = SparseFwd::apply(q, k, v, blocks, seqused, &lse);
+  return {out, lse};
 }
 
 // ------------------------------------------------------------- registration --
@@ -1414,7 +1407,7 @@ void add_kernels(const std::string& ns, const std::string& name) {
   ANIMA_PLAIN(rotary_tables, T2, CT, Ints, Doubles, Doubles, int64_t, double);
   ANIMA_ADD(sparse_fwd, &sparse_fwd_autograd);
   ANIMA_PLAIN(select_blocks, Tensor, CT, CT, int64_t, CO);
-  ANIMA_PLAIN(sparse_bwd, T3, CT, CT, CT, CT, CT, CT, CT, CT, CO);
+  ANIMA_PLAIN(sparse_bwd, T3, CT, CT, CT, CT, CT, CT, CT, CO);
   TORCH_CHECK(false, "no native kernels for ", ns, "::", name);
 }
 

@@ -122,18 +122,17 @@ def _(q, k, count, seqused_k):
 def _sparse_fwd(
     q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, blocks: torch.Tensor, seqused_k: Optional[torch.Tensor],
     keep: bool,
-) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+) -> tuple[torch.Tensor, torch.Tensor]:
     _check_heads(q, k, v, seqused_k, (blocks,))
     _check_blocks(q, blocks)
     B, Sq, H, _ = q.shape
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty((B, H, Sq) if keep else 0, dtype=torch.float32, device=q.device)
-    rest = torch.empty(q.shape if keep else 0, dtype=q.dtype, device=q.device)
     if out.numel() == 0:
-        return out, lse, rest
+        return out, lse
     q, k, v, lengths, blocks = _prep(q), _prep(k), _prep(v), _lengths(seqused_k), blocks.contiguous()
     a = _lib.SparseFwdArgs(
-        q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(), rest=rest.data_ptr() if keep else None,
+        q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(),
         lse=lse.data_ptr() if keep else None, seqused_k=_lib.ptr(lengths), blocks=blocks.data_ptr(), softmax_scale=1.0 / math.sqrt(q.shape[3]),
         **_sizes(q, k, blocks.shape[3]),
     )
@@ -142,7 +141,7 @@ def _sparse_fwd(
         n = _lib.lib().aa_sparse_fwd_workspace(B, Sq, H, blocks.shape[3])
         ws = _workspace(n, q)
         _lib.check(_lib.lib().aa_sparse_fwd(ctypes.byref(a), _lib.ptr(ws), n, _lib.stream(q)), "sparse_attention")
-    return out, lse, rest
+    return out, lse
 
 
 @_sparse_fwd.register_fake
@@ -150,29 +149,28 @@ def _(q, k, v, blocks, seqused_k, keep):
     _check_heads(q, k, v, seqused_k, (blocks,))
     _check_blocks(q, blocks)
     B, Sq, H, _ = q.shape
-    lse = q.new_empty((B, H, Sq) if keep else (0,), dtype=torch.float32)
-    return q.new_empty(q.shape), lse, q.new_empty(q.shape if keep else (0,))
+    return q.new_empty(q.shape), q.new_empty((B, H, Sq) if keep else (0,), dtype=torch.float32)
 
 
 @custom_op("anima_flat_amd::sparse_bwd", mutates_args=())
 def _sparse_bwd(
-    dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, rest: torch.Tensor,
-    lse: torch.Tensor, blocks: torch.Tensor, seqused_k: Optional[torch.Tensor],
+    dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, lse: torch.Tensor,
+    blocks: torch.Tensor, seqused_k: Optional[torch.Tensor],
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    _check_heads(q, k, v, seqused_k, (blocks, dout, out, rest, lse))
+    _check_heads(q, k, v, seqused_k, (blocks, dout, out, lse))
     _check_blocks(q, blocks)
     B, Sq, H, _ = q.shape
-    if any(t.shape != q.shape or t.dtype != q.dtype for t in (dout, out, rest)):
-        raise ValueError("dout, out and rest must have q's shape and dtype")
+    if any(t.shape != q.shape or t.dtype != q.dtype for t in (dout, out)):
+        raise ValueError("dout and out must have q's shape and dtype")
     if lse.shape != (B, H, Sq) or lse.dtype != torch.float32:
         raise ValueError(f"lse must be float32 [B, H, Sq]={(B, H, Sq)}")
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
     if q.numel() == 0 or k.numel() == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
-    dout, q, k, v, out, rest = (_prep(t) for t in (dout, q, k, v, out.contiguous(), rest.contiguous()))
+    dout, q, k, v, out = (_prep(t) for t in (dout, q, k, v, out))
     lse, lengths, blocks = lse.contiguous(), _lengths(seqused_k), blocks.contiguous()
     a = _lib.SparseBwdArgs(
-        dout=dout.data_ptr(), q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(), rest=rest.data_ptr(),
+        dout=dout.data_ptr(), q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(),
         lse=lse.data_ptr(), seqused_k=_lib.ptr(lengths), blocks=blocks.data_ptr(), dq=dq.data_ptr(), dk=dk.data_ptr(), dv=dv.data_ptr(),
         softmax_scale=1.0 / math.sqrt(q.shape[3]), **_sizes(q, k, blocks.shape[3]),
     )
@@ -185,7 +183,7 @@ def _sparse_bwd(
 
 
 @_sparse_bwd.register_fake
-def _(dout, q, k, v, out, rest, lse, blocks, seqused_k):
+def _(dout, q, k, v, out, lse, blocks, seqused_k):
     return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
 
 
@@ -194,13 +192,13 @@ def _sparse_setup(ctx, inputs, output):
     q, k, v, blocks, seqused_k, keep = inputs
     if not keep:
         raise RuntimeError("sparse_attention: a call that needs gradients keeps its statistics (keep)")
-    out, lse, rest = output
-    ctx.mark_non_differentiable(lse, rest)
+    out, lse = output
+    ctx.mark_non_differentiable(lse)
     ctx.set_materialize_grads(False)
-    ctx.save_for_backward(q, k, v, out, rest, lse, blocks, seqused_k)
+    ctx.save_for_backward(q, k, v, out, lse, blocks, seqused_k)
 
 
-def _sparse_backward(ctx, dout, _, __):
+def _sparse_backward(ctx, dout, _):
     if dout is None:
         return (None,) * 6
     return *_sparse_bwd(dout, *ctx.saved_tensors), None, None, None

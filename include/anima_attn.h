@@ -589,7 +589,6 @@ typedef struct aa_sparse_fwd_args {
   const void* k;            /* [B, Sk, Hk, hd]; k, v may be NULL when Sk == 0 */
   const void* v;
   void* out;                /* [B, Sq, H, hd] */
-  void* rest;               /* what out's rounding left out, laid out as out, or NULL */
   float* lse;               /* [B, H, Sq] contiguous, or NULL */
   const int32_t* seqused_k; /* [B], or NULL */
   const int32_t* blocks;    /* [B, H, nq, count] */
@@ -612,8 +611,7 @@ size_t aa_sparse_fwd_workspace(int64_t B, int64_t Sq, int64_t H, int64_t count);
  * out = softmax(q k^T * softmax_scale) v over the keys of the listed blocks below
  * seqused_k, lse its natural-log row log-sum-exp. One launch, plus a combine pass
  * when aa_sparse_fwd_workspace() > 0. Rows of k and v at or past seqused_k are
- * not read. With lse, rest may be asked for: out + rest is the output to 16
- * bits or more. Stands beside src/attention.py:43-81, which attends every key.
+ * not read. Stands beside src/attention.py:43-81, which attends every key.
  */
 int aa_sparse_fwd(const aa_sparse_fwd_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
@@ -623,7 +621,6 @@ typedef struct aa_sparse_bwd_args {
   const void* k;
   const void* v;
   const void* out;          /* from aa_sparse_fwd */
-  const void* rest;         /* from aa_sparse_fwd, or NULL: D of the rounded out */
   const float* lse;         /* [B, H, Sq] contiguous, from aa_sparse_fwd */
   const int32_t* seqused_k;
   const int32_t* blocks;
