@@ -2,9 +2,9 @@
 // and keys by them, for gfx950. Both are bound by HBM.
 //
 // Tables: angle = position * frequency. A position of 10^6 leaves no digit of
-//   its angle in fp32, so the frequency is kept in turns (radians / 2 pi) in
-//   fp64, the product's whole turns are dropped in fp64 and only the rest, in
-//   [-1/2, 1/2], goes to fp32: one sincospif, rounded once.
+//   its angle in fp32, so the frequency is kept in quarter turns (radians /
+//   (pi / 2)) in fp64, the product's whole quarters are dropped in fp64 and only
+//   the rest r in [-1/2, 1/2] goes to fp32, for sin and cos of (pi / 2) r.
 //
 // Turn: a pair (a, b) becomes (a cos - b sin, b cos + a sin), in fp32, rounded
 //   once to the type of q and k. A pair is (i, i + part / 2) of a head or
@@ -32,10 +32,11 @@ struct TableParams {
   const void* positions;  // [rows, axes]
   float* cos;             // [rows, pairs]
   float* sin;
-  uint32_t total;         // rows * pairs / VEC
+  uint32_t total;         // threads: step * pairs / VEC
+  uint32_t rows, step;    // a thread's rows: row, row + step, ...
   int axes, pairs;
   float amplitude;
-  double turns[kMaxPairs];    // a position's turns of pair i
+  double quarters[kMaxPairs]; // a position's quarter turns of pair i
   uint8_t axis[kMaxPairs];
 };
 
@@ -48,30 +49,67 @@ __device__ __forceinline__ double position(const void* p, uint64_t i, int type) 
   }
 }
 
-// VEC pairs of one row a thread.
-template <int VEC>
+// sin and cos of q quarter turns. Polynomials of r^2 for |r| <= 1/2, fitted to
+// the least largest error (3e-9 relative for sin, 6e-11 for cos) and rounded to
+// fp32, in place of a library sine for any argument (11 fp32 instructions; with
+// one the kernel was bound by its instructions, 131072 positions x 64 pairs 23 us).
+__device__ __forceinline__ void sincos_quarters(double q, float& s, float& c) {
+  const double whole = rint(q);
+  const float r = (float)(q - whole);
+  const float y = r * r;
+  const float sn = r * fmaf(y, fmaf(y, fmaf(y, -0.004601658f, 0.07968003f), -0.6459635f), 1.5707964f);
+  const float cs = fmaf(y, fmaf(y, fmaf(y, fmaf(y, 0.000903363f, -0.020859936f), 0.25366917f), -1.2337005f), 1.0f);
+  // The quarter modulo 4: its two low bits, of a double of up to 2^53.
+  const int n = (int)(whole - 4.0 * floor(0.25 * whole));
+  s = n & 1 ? cs : sn;
+  c = n & 1 ? sn : cs;
+  s = n & 2 ? -s : s;
+  c = (n + 1) & 2 ? -c : c;
+}
+
+// VEC pairs of ROWS rows a thread, whose frequencies stay in registers; the rows
+// of a workgroup's threads on one unit are `step` apart.
+template <int VEC, int ROWS>
 __global__ __launch_bounds__(kThreads) void tables_kernel(const TableParams p, int type) {
   const uint32_t idx = blockIdx.x * kThreads + threadIdx.x;
   if (idx >= p.total) return;
   const uint32_t units = (uint32_t)p.pairs / VEC;
-  const uint32_t row = idx / units;
-  const int i0 = (int)(idx - row * units) * VEC;
-  float c[VEC], s[VEC];
+  const uint32_t row0 = idx / units;
+  const int i0 = (int)(idx - row0 * units) * VEC;
+  double quarters[VEC];
+  int axis[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; ++j) {
-    const double pos = position(p.positions, (uint64_t)row * p.axes + p.axis[i0 + j], type);
-    const double t = pos * p.turns[i0 + j];
-    sincospif(2.0f * (float)(t - rint(t)), &s[j], &c[j]);
-    c[j] *= p.amplitude;
-    s[j] *= p.amplitude;
+    quarters[j] = p.quarters[i0 + j];
+    axis[j] = p.axis[i0 + j];
   }
-  const uint64_t at = (uint64_t)row * p.pairs + i0;
-  if constexpr (VEC == 4) {
-    *reinterpret_cast<f32x4*>(p.cos + at) = f32x4{c[0], c[1], c[2], c[3]};
-    *reinterpret_cast<f32x4*>(p.sin + at) = f32x4{s[0], s[1], s[2], s[3]};
-  } else {
-    p.cos[at] = c[0];
-    p.sin[at] = s[0];
+  double pos[ROWS][VEC];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const uint64_t row = row0 + (uint64_t)r * p.step;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j)
+      pos[r][j] = row < p.rows ? position(p.positions, row * p.axes + axis[j], type) : 0;
+  }
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const uint64_t row = row0 + (uint64_t)r * p.step;
+    if (row >= p.rows) return;
+    float c[VEC], s[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      sincos_quarters(pos[r][j] * quarters[j], s[j], c[j]);
+      c[j] *= p.amplitude;
+      s[j] *= p.amplitude;
+    }
+    const uint64_t at = row * p.pairs + i0;
+    if constexpr (VEC == 4) {
+      __builtin_nontemporal_store(f32x4{c[0], c[1], c[2], c[3]}, reinterpret_cast<f32x4*>(p.cos + at));
+      __builtin_nontemporal_store(f32x4{s[0], s[1], s[2], s[3]}, reinterpret_cast<f32x4*>(p.sin + at));
+    } else {
+      p.cos[at] = c[0];
+      p.sin[at] = s[0];
+    }
   }
 }
 
@@ -177,10 +215,16 @@ __global__ __launch_bounds__(kThreads) void turn_kernel(const TurnParams p) {
 
 template <typename T, int W, bool INTERLEAVED>
 void launch_turn(TurnParams p, int64_t tokens, hipStream_t stream) {
-  constexpr int PER = 4;
-  p.slices = (p.heads + PER - 1) / PER;
-  p.total = (uint32_t)(tokens * p.slices * p.units);
-  turn_kernel<T, W, INTERLEAVED, PER><<<(p.total + kThreads - 1) / kThreads, kThreads, 0, stream>>>(p);
+  const auto run = [&](auto per) {
+    constexpr int PER = decltype(per)::value;
+    p.slices = (p.heads + PER - 1) / PER;
+    p.total = (uint32_t)(tokens * p.slices * p.units);
+    turn_kernel<T, W, INTERLEAVED, PER><<<(p.total + kThreads - 1) / kThreads, kThreads, 0, stream>>>(p);
+  };
+  // One head a thread while that fills no more than half of the chip (256
+  // tokens, 32 heads of 128: 5.2 -> 3.7 us; 3003 tokens of 16 x 80: 6.0 -> 7.9).
+  if (tokens * p.heads * p.units <= 1024 * (int64_t)device_cu_count()) run(std::integral_constant<int, 1>{});
+  else run(std::integral_constant<int, 4>{});
 }
 
 template <typename T>
@@ -241,7 +285,7 @@ extern "C" int aa_rotary_tables(const aa_rotary_tables_args* a, void* stream) {
         const double keep = std::min(1.0, std::max(0.0, (turns - 1) / 31));
         f *= keep + (1 - keep) / scale;
       }
-      p.turns[p.pairs] = f / (2 * M_PI);
+      p.quarters[p.pairs] = f / M_PI_2;
       p.axis[p.pairs++] = (uint8_t)x;
     }
   }
@@ -258,11 +302,21 @@ extern "C" int aa_rotary_tables(const aa_rotary_tables_args* a, void* stream) {
   p.cos = a->cos;
   p.sin = a->sin;
   p.axes = (int)a->axes;
-  p.total = (uint32_t)(a->rows * p.pairs / vec);
+  p.rows = (uint32_t)a->rows;
+  // Four rows a thread where that still fills the chip (131072 positions of 64
+  // pairs 21.8 -> 18.5 us, 16384 with one row 5.8, with four 7.1).
+  const int rows = a->rows * p.pairs / vec >= 4096 * (int64_t)device_cu_count() ? 4 : 1;
+  p.step = (p.rows + rows - 1) / rows;
+  p.total = (uint32_t)(p.step * (uint64_t)p.pairs / vec);
   const uint32_t blocks = (uint32_t)(((uint64_t)p.total + kThreads - 1) / kThreads);
   if (!grid_fits(blocks, kThreads)) return fail(AA_EUNSUPPORTED, "rotary_tables: too many positions");
-  if (vec == 4) tables_kernel<4><<<blocks, kThreads, 0, (hipStream_t)stream>>>(p, a->position_type);
-  else tables_kernel<1><<<blocks, kThreads, 0, (hipStream_t)stream>>>(p, a->position_type);
+  const auto run = [&](auto v, auto r) {
+    tables_kernel<decltype(v)::value, decltype(r)::value><<<blocks, kThreads, 0, (hipStream_t)stream>>>(p, a->position_type);
+  };
+  using I1 = std::integral_constant<int, 1>;
+  using I4 = std::integral_constant<int, 4>;
+  if (vec == 4) rows == 4 ? run(I4{}, I4{}) : run(I4{}, I1{});
+  else rows == 4 ? run(I1{}, I4{}) : run(I1{}, I1{});
   return check_launch("rotary_tables");
 }
 

@@ -515,9 +515,12 @@ struct TileWalk {
     const int i = 64 * pg + lane;
     return i < total ? words[(int64_t)(i / nqw) * head + i % nqw] : 0;
   }
-  __device__ __forceinline__ int count(int lane) {
-    int sum = 0;
-    for (int pg = 0; 64 * pg < total; ++pg) sum += __popcll(load(pg, lane));
+  // The first page opened, and the number of tiles.
+  __device__ __forceinline__ int start(int lane) {
+    open(0, lane);
+    word = 0;
+    int sum = __popcll(mine);
+    for (int pg = 1; 64 * pg < total; ++pg) sum += __popcll(load(pg, lane));
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
     return __builtin_amdgcn_readfirstlane(sum);
@@ -569,8 +572,16 @@ void sparse_dkdv_kernel(BwdParams sp) {
   walk.head = (int64_t)p.ntk * sp.nqw;
   walk.nqw = sp.nqw;
   walk.total = sp.group * sp.nqw;
-  walk.word = 0;
-  const int n = walk.count(lane);
+
+  // The wave's K and V rows staged in ring stages 2 and 3 (16 KB per wave), free
+  // until tile 2's DMA, on their way while the list is read. Keys past klen
+  // re-read its last key (their gradients are not stored).
+  bf16* kst = ring + 2 * (2 * kTileElems) + wave * 8192;
+  if (klen > 0) {
+    stage_rows_in(p.k + b * p.s_k[0] + hk * p.s_k[2], p.s_k[1], key0, klen, lane, kst);
+    stage_rows_in(p.v + b * p.s_v[0] + hk * p.s_v[2], p.s_v[1], key0, klen, lane, kst + 4096);
+  }
+  const int n = walk.start(lane);
 
   const uint32_t ring0 = lds_addr(ring);
   const uint32_t stat0 = lds_addr(stat);
@@ -601,13 +612,6 @@ void sparse_dkdv_kernel(BwdParams sp) {
     if (stats_dma) dma.issue_stats(lane);
   };
   if (n > 0) {
-    walk.open(0, lane);
-    // The wave's K and V rows staged in ring stages 2 and 3 (16 KB per wave),
-    // free until tile 2's DMA. Keys past klen re-read its last key (their
-    // gradients are not stored).
-    bf16* kst = ring + 2 * (2 * kTileElems) + wave * 8192;
-    stage_rows_in(p.k + b * p.s_k[0] + hk * p.s_k[2], p.s_k[1], key0, klen, lane, kst);
-    stage_rows_in(p.v + b * p.s_v[0] + hk * p.s_v[2], p.s_v[1], key0, klen, lane, kst + 4096);
     issue_job(0);
     issue_job(1);
     if (stats_dma) asm volatile("s_waitcnt vmcnt(9)" ::: "memory");

@@ -37,54 +37,22 @@ using ks::WaveDma;
 
 constexpr uint32_t kTileBytes = kTileElems * sizeof(bf16);
 
-// The row sum of query 32 qb + lane % 32 again, in plain arithmetic, where the
-// sum on the matrix pipe took in another row's NaN or infinity (FwdWave::setup;
-// O did not). From the staged Q rows and K in memory, half of a block's keys
-// per lane of a pair; only runs where a row holds no finite numbers.
-__device__ __forceinline__ float row_sum_again(const SparseParams& p, const bf16* kp, const bf16* stage, BlockWalk walk,
-                                               int lane, int klen, float m) {
-  const float mc = m * p.c;
-  float sum = 0.f;
-#pragma unroll 1
-  for (int i = 0; i < walk.n; ++i) {
-    const int lo = walk.next() * kB, hi = min(lo + kB, klen);
-#pragma unroll 1
-    for (int key = lo + (lane >> 5); key < hi; key += 2) {
-      const bf16* kr = kp + (int64_t)key * p.ks[1];
-      float s = 0.f;
-#pragma unroll 1
-      for (int ch = 0; ch < kD / 8; ++ch) {
-        float x[8], y[8];
-        unpack8(ld16(stage + stage_at(lane & 31, ch)), x);
-        unpack8(ld16(kr + 8 * ch), y);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s = fmaf(x[e], y[e], s);
-      }
-      sum += round_bf16(fast_exp2(fmaf(s, p.c, -mc)));
-    }
-  }
-  return pair_sum(sum);
-}
-
-// LSE: something reads the log-sum-exp, so the fp32 probabilities are summed
-// too (attn_fwd_ks_kernel's comment).
-template <bool LSE, bool SPLIT>
-__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1)))
-void sparse_fwd_kernel(SparseParams p) {
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kTileBytes];
-  __shared__ __attribute__((aligned(16))) uint32_t bits[2 * 64];
-
-  int item = item_of(blockIdx.x, gridDim.x, p.items * (SPLIT ? p.nsplit : 1));
-  if (item < 0) return;
-  int split = 0;
-  if constexpr (SPLIT) {
-    split = item % p.nsplit;
-    item = item / p.nsplit;
-  }
+// One work item: query block and part of its list. TRACK: with a running
+// maximum; without, each row keeps the maximum of its first tile, and `again` is
+// set, with nothing written, if a sum left the exponent range by that.
+template <bool LSE, bool SPLIT, bool TRACK>
+__device__ __forceinline__ void run_item(int item, int split, uint8_t* lds, uint32_t* bits, uint32_t& again) {
+  // The kernel's arguments and the lane, as if unknown before: what two bodies
+  // of a kernel have in common would be kept in registers through the first.
+  constexpr bool FSUM = LSE || TRACK;
+  typedef const __attribute__((address_space(4))) SparseParams* Args;
+  Args args = (Args)__builtin_amdgcn_kernarg_segment_ptr();
+  int lane = threadIdx.x;
+  asm volatile("" : "+s"(args), "+s"(item), "+v"(lane));
+  const __attribute__((address_space(4))) SparseParams& p = *args;
   const int qblk = item % p.nq;
   const int bh = item / p.nq;
   const int b = bh / p.H, h = bh - b * p.H, hk = h / p.group;
-  const int lane = threadIdx.x;
   const int li = lane & 31, hh = lane >> 5;
   const int qrow0 = qblk * kB;
   const int klen = key_length(p.seqused, b, p.Sk);
@@ -183,9 +151,9 @@ void sparse_fwd_kernel(SparseParams p) {
       k_tile(x2);
       v3_tile(x0);
       v_tile(x1);
-      w.tile<SB, NEXT, true, LSE>(0, x1 == part, x1 * kB, klen, dma);
+      w.tile<SB, NEXT, TRACK, FSUM>(0, x1 == part, x1 * kB, klen, dma);
       if constexpr (NEXT) {
-        w.update_max<LSE>();
+        if constexpr (TRACK) w.update_max<FSUM>();
         x0 = x1;
         x1 = x2;
         x2 = next_block();
@@ -206,15 +174,20 @@ void sparse_fwd_kernel(SparseParams p) {
   }
   wait_dma();
   w.fence_o();
-  float lsum[2] = {w.lsum[0][0], w.lsum[1][0]};
-  if (__builtin_amdgcn_ballot_w64(!(lsum[0] <= FLT_MAX && lsum[1] <= FLT_MAX))) {
-    stage_q(ktile);
-    read_list();
-    wait_dma();
+  if constexpr (!TRACK) {
+    const uint64_t out = __builtin_amdgcn_ballot_w64(!w.sums_in_range());
+    again = (uint32_t)(out | (out >> 32));
+    if (again) return;
+  }
+  // The fp32 probabilities' sum stands in for the rounded ones' where that took
+  // in another row's NaN or infinity on the matrix pipe (FwdWave::setup; O did
+  // not).
+  float lsum[2] = {w.lsum[0][0], w.lsum[1][0]}, lf[2] = {0.f, 0.f};
+  if constexpr (FSUM) {
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const float sum = row_sum_again(p, kp, ktile + q * 32 * kD, walk, lane, klen, w.m_raw[q]);
-      if (!(lsum[q] <= FLT_MAX)) lsum[q] = sum;
+      lf[q] = pair_sum(w.lf[q][0] + w.lf[q][1]);
+      if (TRACK && !(lsum[q] <= FLT_MAX)) lsum[q] = lf[q];
     }
   }
 
@@ -223,9 +196,8 @@ void sparse_fwd_kernel(SparseParams p) {
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       const int row = 32 * q + li;
-      const float lf = LSE ? pair_sum(w.lf[q][0] + w.lf[q][1]) : 0.f;
       if (qrow0 + row >= p.Sq) continue;
-      if (hh == 0) p.part_stat[rec + row] = f32x4{w.m_raw[q], lsum[q], lf, 0.f};
+      if (hh == 0) p.part_stat[rec + row] = f32x4{w.m_raw[q], lsum[q], lf[q], 0.f};
       if (n == 0) continue;  // the combine kernel reads no O of a part without keys
       float* to = p.part_o + (rec + row) * kD;
 #pragma unroll
@@ -247,42 +219,81 @@ void sparse_fwd_kernel(SparseParams p) {
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
     const bool any = lsum[q] != 0.f;
-    const float scale = any ? 1.0f / lsum[q] : 0.f;
     const f32x16 o[4] = {w.o[0][q], w.o[1][q], w.o[2][q], w.o[3][q]};
     bf16* area = ktile + q * 32 * kD;
-    stage_acc_rows(o, scale, lane, area);
+    stage_acc_rows(o, any ? 1.0f / lsum[q] : 0.f, lane, area);
     stage_rows_out(p.o + at, p.os[1], qrow0 + 32 * q, p.Sq, lane, area);
     if constexpr (LSE) {
-      const float lf = pair_sum(w.lf[q][0] + w.lf[q][1]);
       const int row = qrow0 + 32 * q + li;
       if (hh == 0 && row < p.Sq)
-        p.lse[(int64_t)bh * p.Sq + row] = any ? (w.m_raw[q] * p.c + __log2f(lf)) * kLn2 : -INFINITY;
+        p.lse[(int64_t)bh * p.Sq + row] = any ? (w.m_raw[q] * p.c + __log2f(lf[q])) * kLn2 : -INFINITY;
     }
   }
 }
 
-// One wave per query: the parts' O, two head dims a lane, by their weights.
+// LSE: something reads the log-sum-exp, so the fp32 probabilities are summed
+// too (attn_fwd_ks_kernel's comment).
+template <bool LSE, bool SPLIT>
+__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1)))
+void sparse_fwd_kernel(SparseParams p) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kTileBytes];
+  __shared__ __attribute__((aligned(16))) uint32_t bits[2 * 64];
+  int item = item_of(blockIdx.x, gridDim.x, p.items * (SPLIT ? p.nsplit : 1));
+  if (item < 0) return;
+  int split = 0;
+  if constexpr (SPLIT) {
+    split = item % p.nsplit;
+    item = item / p.nsplit;
+  }
+  // (Opaque: joined to the first body, the second one's code spilled registers.)
+  uint32_t again = 0;
+  run_item<LSE, SPLIT, false>(item, split, lds, bits, again);
+  again = __builtin_amdgcn_readfirstlane(again);
+  asm volatile("" : "+s"(again)::"memory");
+  if (again) run_item<LSE, SPLIT, true>(item, split, lds, bits, again);
+}
+
+// One workgroup per query: wave w takes the parts w, w + 4, ..., two head dims a
+// lane, and the waves' sums meet in LDS in order. (The parts come from other
+// XCDs' workgroups, a long way; 8 loads a lane are on it at once.)
 constexpr int kCombineWaves = 4;
-__global__ __launch_bounds__(64 * kCombineWaves) void sparse_combine_kernel(SparseParams p, int64_t rows) {
-  const int64_t r = (int64_t)blockIdx.x * kCombineWaves + (threadIdx.x >> 6);
-  if (r >= rows) return;
-  const int lane = threadIdx.x & 63;
+__global__ __launch_bounds__(64 * kCombineWaves) void sparse_combine_kernel(SparseParams p) {
+  __shared__ float sums[kCombineWaves][4][64];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t r = blockIdx.x;
   const int64_t bh = r / p.Sq;
   const int q = (int)(r - bh * p.Sq);
   const int64_t b = bh / p.H, h = bh - b * p.H;
   const int64_t rec = (bh * p.nq + q / kB) * p.nsplit * kB + q % kB;
   float mx = -INFINITY;
-  for (int s = 0; s < p.nsplit; ++s) mx = fmaxf(mx, p.part_stat[rec + (int64_t)s * kB][0]);
+  for (int s = lane; s < p.nsplit; s += 64) mx = fmaxf(mx, p.part_stat[rec + (int64_t)s * kB][0]);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off));
   float sum = 0.f, fsum = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int s = 0; s < p.nsplit; ++s) {
+#pragma unroll 8
+  for (int s = wave; s < p.nsplit; s += kCombineWaves) {
     const f32x4 st = p.part_stat[rec + (int64_t)s * kB];
-    if (st[0] == -INFINITY) continue;  // no keys
-    const float a = fast_exp2((st[0] - mx) * p.c);
     const float2 o = *reinterpret_cast<const float2*>(p.part_o + (rec + (int64_t)s * kB) * kD + 2 * lane);
+    // The O of a part without keys was never written and does not count.
+    const bool keys = st[0] != -INFINITY;
+    const float a = keys ? fast_exp2((st[0] - mx) * p.c) : 0.f;
     sum += st[1] * a;
     fsum += st[2] * a;
-    o0 += o.x * a;
-    o1 += o.y * a;
+    o0 += keys ? o.x * a : 0.f;
+    o1 += keys ? o.y * a : 0.f;
+  }
+  sums[wave][0][lane] = sum;
+  sums[wave][1][lane] = fsum;
+  sums[wave][2][lane] = o0;
+  sums[wave][3][lane] = o1;
+  __syncthreads();
+  if (wave != 0) return;
+#pragma unroll
+  for (int w = 1; w < kCombineWaves; ++w) {
+    sum += sums[w][0][lane];
+    fsum += sums[w][1][lane];
+    o0 += sums[w][2][lane];
+    o1 += sums[w][3][lane];
   }
   const bool any = sum != 0.f;
   const float scale = any ? 1.0f / sum : 0.f;
@@ -291,10 +302,14 @@ __global__ __launch_bounds__(64 * kCombineWaves) void sparse_combine_kernel(Spar
   if (p.lse && lane == 0) p.lse[r] = any ? (mx * p.c + __log2f(fsum)) * kLn2 : -INFINITY;
 }
 
-// Parts of a list: as many as give every SIMD a wave, and no more than blocks.
+// Parts of a list: as many as give every SIMD a wave, of equal numbers of blocks;
+// none where that takes fewer than 4 blocks (about 2 us each) off the longest
+// part: the second launch costs as much.
 static int plan_split(int64_t items, int64_t count) {
   const int64_t slots = 4 * (int64_t)device_cu_count();
-  return (int)std::max<int64_t>(1, std::min<int64_t>(items ? slots / items : 1, count));
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(items ? slots / items : 1, count));
+  const int64_t longest = (count + parts - 1) / parts;
+  return count - longest < 4 ? 1 : (int)((count + longest - 1) / longest);
 }
 
 }  // namespace sparse
@@ -373,7 +388,6 @@ extern "C" int aa_sparse_fwd(const aa_sparse_fwd_args* a, void* workspace, size_
   const unsigned grid = grid_of((int64_t)p.items * p.nsplit);
   if (p.lse) sparse_fwd_kernel<true, true><<<grid, 64, 0, st>>>(p);
   else sparse_fwd_kernel<false, true><<<grid, 64, 0, st>>>(p);
-  const int64_t rows = a->B * a->H * a->Sq;
-  sparse_combine_kernel<<<(unsigned)((rows + kCombineWaves - 1) / kCombineWaves), 64 * kCombineWaves, 0, st>>>(p, rows);
+  sparse_combine_kernel<<<(unsigned)(a->B * a->H * a->Sq), 64 * kCombineWaves, 0, st>>>(p);
   return check_launch("sparse_fwd");
 }

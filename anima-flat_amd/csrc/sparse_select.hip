@@ -11,10 +11,10 @@
 // 16384 tokens, 134 M fp64 FMAs beside the attention's 137 G.
 //
 //   means_kernel   one wave per block of rows: HBM-bound, q and k once
-//   select_kernel  one workgroup per R query blocks of one head: scores into
-//                  LDS, a key block per lane (k's means are transposed for
-//                  that), then a wave per row finds the count-th largest score
-//                  bit by bit
+//   select_kernel  one workgroup per 4 query blocks of one head: scores into LDS,
+//                  a key block per lane (k's means are transposed for that, q's
+//                  are scalars), then a wave per row finds the count-th largest
+//                  score bit by bit
 #include <string>
 
 #include "sparse.h"
@@ -93,7 +93,8 @@ __device__ __forceinline__ uint64_t order_of(double x) {
   return u >> 63 ? ~u : u | (uint64_t{1} << 63);
 }
 
-constexpr int kSelectThreads = 256;
+constexpr int kSelectThreads = 512;
+constexpr int kRows = 4;  // query blocks of a workgroup
 
 // A row's scores for one wave: score 64 j + lane of lane `lane`, j < nj. Up to 1024
 // stay in registers; more are read from LDS again for every bit (at 4096 they
@@ -156,38 +157,70 @@ __device__ __forceinline__ void pick(const Scores& scores, int have, int count, 
   for (int i = at + lane; i < count; i += 64) out[i] = -1;
 }
 
-template <int R>
-__global__ __launch_bounds__(kSelectThreads) void select_kernel(SelectParams p, int rgroups, int items) {
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  double* qrow = reinterpret_cast<double*>(lds);              // [128][R]
-  uint64_t* score = reinterpret_cast<uint64_t*>(qrow + R * kD);  // [R][nk]
-  const int item = item_of(blockIdx.x, gridDim.x, items);
-  if (item < 0) return;
-  const int bh = item / rgroups, r0 = (item - bh * rgroups) * R;
-  const int b = bh / p.H, h = bh - b * p.H;
-  const int rows = min(R, p.nq - r0);
-  const int have = (key_length(p.seqused, b, p.Sk) + kB - 1) / kB;
-
-  for (int i = threadIdx.x; i < R * kD; i += kSelectThreads) {
-    const int r = i / kD, d = i - r * kD;
-    qrow[d * R + r] = r < rows ? p.qm[((int64_t)bh * p.nq + r0 + r) * kD + d] : 0.0;
-  }
-  __syncthreads();
-  const double* km = p.km + (int64_t)(b * p.Hk + h / (p.H / p.Hk)) * kD * p.nk;
-  for (int j = threadIdx.x; j < have; j += kSelectThreads) {
-    double acc[R] = {};
-#pragma unroll 8
-    for (int d = 0; d < kD; ++d) {
-      const double x = km[(int64_t)d * p.nk + j];
+// Scores of the workgroup's query blocks against the blocks of keys: the former's
+// means are scalar operands, the latter's are read once for all of them. The
+// waves share the blocks of keys and, with few of them, the head dims (PARTS
+// parts, which meet in LDS in a fixed order): what bounds it is how many reads
+// are on their way at once.
+template <int PARTS>
+__device__ __forceinline__ void dot_rows(const double* qm, const double* km, int nk, int have, int rows, double* partial,
+                                         uint64_t* score) {
+  constexpr int kWidth = kSelectThreads / PARTS, kSpan = kD / PARTS;
+  // Written by the launch before: constant here, so that the uniform reads of
+  // qm are scalar loads.
+  typedef const __attribute__((address_space(4))) double* Const;
+  const int part = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWidth);
+  for (int j = threadIdx.x - part * kWidth; j < have; j += kWidth) {
+    double acc[kRows] = {};
+#pragma unroll 2
+    for (int d0 = 0; d0 < kSpan; d0 += 16) {
+      double x[16];
 #pragma unroll
-      for (int r = 0; r < R; ++r) acc[r] = fma(qrow[d * R + r], x, acc[r]);
+      for (int i = 0; i < 16; ++i) x[i] = km[(int64_t)(part * kSpan + d0 + i) * nk + j];
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        Const q = (Const)(uintptr_t)(qm + min(r, rows - 1) * kD + part * kSpan + d0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[r] = fma(q[i], x[i], acc[r]);
+      }
     }
 #pragma unroll
-    for (int r = 0; r < R; ++r) score[r * p.nk + j] = order_of(acc[r]);
+    for (int r = 0; r < kRows; ++r) {
+      if constexpr (PARTS == 1) score[r * nk + j] = order_of(acc[r]);
+      else partial[(part * kRows + r) * kWidth + j] = acc[r];
+    }
   }
   __syncthreads();
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (int r = wave; r < rows; r += kSelectThreads / 64) {
+  if constexpr (PARTS > 1) {
+    for (int i = threadIdx.x; i < kRows * kWidth; i += kSelectThreads) {
+      const int r = i / kWidth, j = i % kWidth;
+      if (j >= have) continue;
+      double sum = 0;
+#pragma unroll
+      for (int s = 0; s < PARTS; ++s) sum += partial[(s * kRows + r) * kWidth + j];
+      score[r * nk + j] = order_of(sum);
+    }
+    __syncthreads();
+  }
+}
+
+__global__ __launch_bounds__(kSelectThreads) void select_kernel(SelectParams p, int rgroups, int items) {
+  extern __shared__ __attribute__((aligned(16))) uint64_t score[];  // [kRows][nk]
+  __shared__ double partial[kRows * kSelectThreads];
+  const int item = item_of(blockIdx.x, gridDim.x, items);
+  if (item < 0) return;
+  const int bh = item / rgroups, r0 = (item - bh * rgroups) * kRows;
+  const int b = bh / p.H, h = bh - b * p.H;
+  const int rows = min(kRows, p.nq - r0);
+  const int have = (key_length(p.seqused, b, p.Sk) + kB - 1) / kB;
+  const double* qm = p.qm + ((int64_t)bh * p.nq + r0) * kD;
+  const double* km = p.km + (int64_t)(b * p.Hk + h / (p.H / p.Hk)) * kD * p.nk;
+  if (have <= 64) dot_rows<8>(qm, km, p.nk, have, rows, partial, score);
+  else if (have <= 128) dot_rows<4>(qm, km, p.nk, have, rows, partial, score);
+  else if (have <= 256) dot_rows<2>(qm, km, p.nk, have, rows, partial, score);
+  else dot_rows<1>(qm, km, p.nk, have, rows, partial, score);
+  const int lane = threadIdx.x & 63;
+  for (int r = threadIdx.x >> 6; r < rows; r += kSelectThreads / 64) {
     int32_t* out = p.blocks + ((int64_t)bh * p.nq + r0 + r) * p.count;
     const uint64_t* row = score + r * p.nk;
     if (have <= 64) pick(Held<1>(row, have, lane), have, p.count, out, lane);
@@ -260,12 +293,8 @@ extern "C" int aa_block_select(const aa_block_select_args* a, void* workspace, s
   const int64_t qtotal = a->B * a->H * qg, total = qtotal + a->B * a->Hk * kg;
   if (!grid_fits(total, 64 * kMeanWaves)) return fail(AA_EUNSUPPORTED, "block_select: too many blocks");
   means_kernel<<<(unsigned)total, 64 * kMeanWaves, 0, st>>>(p, (int)qg, (int)kg, (int)qtotal);
-  // R rows share each read of k's means; few rows leave CUs idle, and 4096
-  // blocks of 4 rows fill the LDS.
-  constexpr int R = 4;
-  const int64_t rg = (nq + R - 1) / R, items = a->B * a->H * rg;
-  const size_t lds = (size_t)R * (kD + nk) * sizeof(double);
-  if (!grid_fits(grid_of(items), kSelectThreads)) return fail(AA_EUNSUPPORTED, "block_select: too many query blocks");
-  select_kernel<R><<<grid_of(items), kSelectThreads, lds, st>>>(p, (int)rg, (int)items);
+  if (!grid_fits(grid_of(a->B * a->H * nq), kSelectThreads)) return fail(AA_EUNSUPPORTED, "block_select: too many query blocks");
+  const int64_t rg = (nq + kRows - 1) / kRows, items = a->B * a->H * rg;
+  select_kernel<<<grid_of(items), kSelectThreads, (size_t)(kRows * nk) * sizeof(uint64_t), st>>>(p, (int)rg, (int)items);
   return check_launch("block_select");
 }
