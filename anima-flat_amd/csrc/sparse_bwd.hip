@@ -49,18 +49,31 @@ void sparse_dq_kernel(BwdParams sp) {
   const int qrow0 = qblk * kB;
   const int klen = key_length(sp.seqused, b, p.Sk);
 
-  // Q into the second and third K place, dO into the V places (areas of 32
-  // rows, tile_io.h); the list through the first K place, whose block comes
-  // when it is known.
+  // Three waits stand before the first MFMA, and all waves of a round wait
+  // together: for the list with Q, dO, O and the log-sum-exp; for the first two
+  // halves of K and V; and for nothing else. dO and O come straight into the
+  // registers' layout (32 rows an instruction, 1 us for a CU's four waves), Q
+  // through LDS (areas of 32 rows, tile_io.h) into places that the list's
+  // bits, in the first K place, leave free.
   auto area = [&](uint32_t off) { return reinterpret_cast<bf16*>(lds + off); };
   const bf16* qp = p.q + b * p.s_q[0] + h * p.s_q[2];
-  const bf16* dop = p.dout + b * p.s_do[0] + h * p.s_do[2];
   bf16* aq[2] = {area(kBlock), area(2 * kBlock)};
-  bf16* ado[2] = {area(kVRing), area(kVRing + kBlock)};
+#pragma unroll
+  for (int qb = 0; qb < 2; ++qb) stage_rows_in(qp, p.s_q[1], qrow0 + 32 * qb, p.Sq, lane, aq[qb]);
+  DqWave w;
+  u32x4 orow[2][8];
+  float lse[2];
 #pragma unroll
   for (int qb = 0; qb < 2; ++qb) {
-    stage_rows_in(qp, p.s_q[1], qrow0 + 32 * qb, p.Sq, lane, aq[qb]);
-    stage_rows_in(dop, p.s_do[1], qrow0 + 32 * qb, p.Sq, lane, ado[qb]);
+    const int q = min(qrow0 + 32 * qb + li, p.Sq - 1);
+    const bf16* dop = p.dout + b * p.s_do[0] + h * p.s_do[2] + (int64_t)q * p.s_do[1] + 8 * hh;
+    const bf16* op = p.o + b * p.s_o[0] + h * p.s_o[2] + (int64_t)q * p.s_o[1] + 8 * hh;
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) {
+      w.dop[qb][kk] = __builtin_bit_cast(bf16x8, ld16(dop + 16 * kk));
+      orow[qb][kk] = ld16(op + 16 * kk);
+    }
+    lse[qb] = p.lse[(int64_t)bh * p.Sq + q];
   }
   BlockWalk walk;
   walk.read(sp.blocks + (int64_t)item * sp.count, sp.count, (klen + kB - 1) / kB, reinterpret_cast<uint32_t*>(lds), lane);
@@ -107,17 +120,51 @@ void sparse_dq_kernel(BwdParams sp) {
   };
   const int l0 = next_half();
   int l1 = next_half(), l2 = next_half(), l3 = 0;
-  if (n > 0) {
-    k_job(0, l0);
-    dma.all_k();
-  }
   wait_dma();
-  __syncthreads();
-
-  DqWave w;
   w.li = li;
   w.hh = hh;
   w.c = p.c;
+#pragma unroll
+  for (int qb = 0; qb < 2; ++qb)
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) {
+      w.qop[qb][kk] = staged_operand(aq[qb], lane, kk);
+      asm volatile("" : "+a"(w.qop[qb][kk]));
+    }
+  // Statistics of each query: lse2 = lse log2(e) and -D, D = rowsum(dO o O) (this
+  // lane's 64 values, then the partner lane's half). O is the rounded output:
+  // D is off by its rounding, beside the rounding of dZ to bf16 for the MFMAs
+  // (dQ 3.4e-3 of its norm from 64 bits, one rounding is 1.7e-3). Queries past
+  // Sq, and those that attended nothing: lse2 = +inf, so that P = 0.
+#pragma unroll
+  for (int qb = 0; qb < 2; ++qb) {
+    const int q = qrow0 + 32 * qb + li;
+    float nd = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) {
+      float x[8], y[8];
+      unpack8(orow[qb][kk], x);
+      unpack8(__builtin_bit_cast(u32x4, w.dop[qb][kk]), y);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) nd = fmaf(y[i], x[i], nd);
+    }
+    nd = pair_sum(nd);
+    nd = q < p.Sq ? -nd : 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) w.nd[qb][r] = nd;
+    w.lse2[qb] = q >= p.Sq || lse[qb] == -INFINITY ? INFINITY : lse[qb] * kLog2e;
+  }
+  __syncthreads();  // the staged rows are read: their places are free
+  if (n > 0) {
+    k_job(0, l0);
+    dma.all_k();
+    v_job(0, l0);
+    dma.all_v();
+    k_job(1, l1);
+    dma.all_k();
+    v_job(1, l1);
+    dma.all_v();
+  }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     w.krd[j] = mine + 2u * (uint32_t)dual_row_rd(lane, j);
@@ -131,60 +178,8 @@ void sparse_dq_kernel(BwdParams sp) {
       w.dq[dt][qb] = f32x16{};
       asm volatile("" : "+a"(w.dq[dt][qb]));
     }
-#pragma unroll
-  for (int qb = 0; qb < 2; ++qb)
-#pragma unroll
-    for (int kk = 0; kk < 8; ++kk) {
-      w.qop[qb][kk] = staged_operand(aq[qb], lane, kk);
-      w.dop[qb][kk] = staged_operand(ado[qb], lane, kk);
-      asm volatile("" : "+a"(w.qop[qb][kk]));
-    }
-  __syncthreads();  // the staged rows are read: their places are free
+  wait_vm<16>();  // K and V of the first half
   if (n > 0) {
-    v_job(0, l0);
-    dma.all_v();
-    k_job(1, l1);
-    dma.all_k();
-  }
-  // Each query's statistics: lse2 = lse log2(e) and -D, D = rowsum(dO o O)
-  // (this lane's 64 values, then the partner lane's half; O straight from
-  // memory). Queries past Sq, and those that attended nothing: lse2 = +inf, so
-  // that P = 0.
-  const bf16* op = p.o + b * p.s_o[0] + h * p.s_o[2];
-#pragma unroll
-  for (int qb = 0; qb < 2; ++qb) {
-    const int q = qrow0 + 32 * qb + li;
-    const bf16* orow = op + (int64_t)min(q, p.Sq - 1) * p.s_o[1] + 8 * hh;
-    float nd = 0.f;
-#pragma unroll
-    for (int kk = 0; kk < 8; ++kk) {
-      float x[8], y[8];
-      unpack8(ld16(orow + 16 * kk), x);
-      unpack8(__builtin_bit_cast(u32x4, w.dop[qb][kk]), y);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) nd = fmaf(y[i], x[i], nd);
-    }
-    nd = pair_sum(nd);
-    nd = q < p.Sq ? -nd : 0.f;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) w.nd[qb][r] = nd;
-    const float lse = q < p.Sq ? p.lse[(int64_t)bh * p.Sq + q] : -INFINITY;
-    w.lse2[qb] = lse == -INFINITY ? INFINITY : lse * kLog2e;
-  }
-  if (hh == 0) {
-    float* st = p.stats + (int64_t)item * bwd::kStat;
-#pragma unroll
-    for (int qb = 0; qb < 2; ++qb) {
-      st[32 * qb + li] = w.lse2[qb];
-      st[kB + 32 * qb + li] = w.nd[qb][0];
-    }
-  }
-  // The loads and stores above leave the vmcnt counts to the DMA.
-  wait_dma();
-
-  if (n > 0) {
-    v_job(1, l1);
-    dma.all_v();
     const int b0 = (n - 1) & 1;  // the last half's S^T is in buffer 0
     const bool m0 = l0 + kKeys > klen;
     if (b0) {
@@ -235,6 +230,16 @@ void sparse_dq_kernel(BwdParams sp) {
     run(I0{}, std::false_type{}, i);
   }
   wait_dma();
+  // The record that the dK/dV kernel reads (at the end: stores ahead of the
+  // loop would be waited for with its first loads).
+  if (hh == 0) {
+    float* st = p.stats + (int64_t)item * bwd::kStat;
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+      st[32 * qb + li] = w.lse2[qb];
+      st[kB + 32 * qb + li] = w.nd[qb][0];
+    }
+  }
   // Keeps dQ in AGPRs up to here and orders the reads after its MFMAs.
   asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3"
                : "+a"(w.dq[0][0]), "+a"(w.dq[1][0]), "+a"(w.dq[2][0]), "+a"(w.dq[3][0]),
@@ -309,8 +314,8 @@ constexpr int kWaves = 4;
 constexpr int kStages = 4;
 constexpr int kLead = kStages - 1;  // tile t + kLead is fetched during tile t
 // Operand reads ahead of their MFMA, and queues of them (attn_bwd_dkdv.hip).
-constexpr int kRPf = 3, kRQ = kRPf + 1;
-constexpr int kTPf = 3, kTQ = kTPf + 2;
+constexpr int kRPf = 4, kRQ = kRPf + 1;
+constexpr int kTPf = 4, kTQ = kTPf + 2;
 constexpr int rread_slot(int j) { return j < kRPf ? 0 : j - kRPf; }
 constexpr int tread_slot(int j) { return 16 + j - kTPf; }
 // Unit u: scores 2 jp, 2 jp + 1 of the P / dZ operand of query chunk c (u =

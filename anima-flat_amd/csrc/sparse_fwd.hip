@@ -119,8 +119,9 @@ __device__ __forceinline__ void run_item(int item, int split, uint8_t* lds, uint
       constexpr int i = decltype(I)::value;
       dma.template issue_k<(i >> 2), (i & 3)>();
     });
-    wait_dma();
+    ks::wait_vm<16>();  // the Q rows
     w.read_q(vtile, lane);
+    wait_dma();
     // As if a tile -1 came before: the K quarters of tile 1, then V chunks
     // 0-2 of tile 0.
     k_tile(x1);

@@ -148,3 +148,31 @@ def test_tile_order(sp, h, w):
         y, c = x[order].view(-1, 64) // w, x[order].view(-1, 64) % w
         assert ((y // 8) == (y[:, :1] // 8)).all() and ((c // 8) == (c[:, :1] // 8)).all()
         assert torch.equal(x[order][:3], torch.tensor([0, 1, 2])) and x[order][8] == w
+
+
+def test_captured_training_without_the_extension(pkg, sp, monkeypatch):
+    """The Python autograd setups cannot look for a live eager graph: they refuse a captured
+    forward with gradients, and an op call that kept no statistics."""
+    from types import SimpleNamespace
+
+    rotary = importlib.import_module("anima_flat_amd.kernels.rotary")
+    x, t, blocks = torch.zeros(1, 4, 1, 128, dtype=BF), torch.zeros(4, 64), torch.zeros(1, 1, 1, 1, dtype=torch.int32)
+    cases = [
+        ("rotary", rotary._rotary_setup, (x, None, t, t, False, False), (x, x[:0])),
+        ("sparse_attention", sp._sparse_setup, (x, x, x, blocks, None, True), (x, t)),
+    ]
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: True)
+    for name, setup, inputs, output in cases:
+        saved = []
+        needs = tuple(isinstance(i, torch.Tensor) and i.dtype == BF for i in inputs)
+        ctx = SimpleNamespace(needs_input_grad=needs, set_materialize_grads=lambda on: None, mark_non_differentiable=lambda *a: None,
+                              save_for_backward=lambda *a: saved.append(a))
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        with pytest.raises(RuntimeError, match=f"{name}: .* only with the torch extension"):
+            setup(ctx, inputs, output)
+        assert not saved
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+        setup(ctx, inputs, output)
+        assert saved
+    with pytest.raises(RuntimeError, match="keeps its statistics"):
+        sp._sparse_setup(ctx, (x, x, x, blocks, None, False), (x, t))
