@@ -91,7 +91,7 @@ _PROTOTYPES: dict[str, tuple[object, list[object]]] = {
     "aa_block_select": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
     "aa_sparse_fwd_workspace": (c_size_t, [_I64] * 4),
     "aa_sparse_fwd": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
-    "aa_sparse_bwd_workspace": (c_size_t, [_I64] * 4),
+    "aa_sparse_bwd_workspace": (c_size_t, [_I64] * 6),
     "aa_sparse_bwd": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
 }
 

@@ -8,6 +8,8 @@
 // with a key are no blocks, a block that is named twice is attended once.
 #pragma once
 
+#include <algorithm>
+
 #include "tile_io.h"
 
 namespace aa {
@@ -116,6 +118,16 @@ struct BlockWalk {
     return x;
   }
 };
+
+// Parts of a list: as many as give every SIMD a wave, of equal numbers of blocks;
+// none where that takes fewer than 4 blocks (about 2 us each) off the longest
+// part: the second launch costs as much.
+inline int plan_split(int64_t items, int64_t count) {
+  const int64_t slots = 4 * (int64_t)device_cu_count();
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(items ? slots / items : 1, count));
+  const int64_t longest = (count + parts - 1) / parts;
+  return count - longest < 4 ? 1 : (int)((count + longest - 1) / longest);
+}
 
 }  // namespace sparse
 }  // namespace aa

@@ -13,6 +13,8 @@
 //                       block of queries that names it
 //   sparse_dkdv_kernel  one workgroup of 4 waves per block of 64 keys of one key
 //                       head, over the query blocks of all heads that share it
+//   sparse_sum_kernel   where few blocks would leave SIMDs or CUs idle, their
+//                       lists are split and the parts' fp32 sums added up here
 #include <type_traits>
 
 #include "attn_bwd_dq_wave.h"
@@ -28,7 +30,19 @@ struct BwdParams {
   const int32_t* blocks;
   uint64_t* turned;        // [B][H][nk][nqw]: bit i of word w: query block 64 w + i lists the key block
   int group, count, nqw, items, kitems;
+  // Parts of a query block's list (dQ) and of a key block's (dK, dV); with more
+  // than one, sparse_sum_kernel adds up the parts' 32 x 32 accumulators in fp32.
+  int qparts, kparts;
+  f32x4* sums;             // [item][part][tile][4][64]
 };
+constexpr int kQTiles = 8, kKTiles = 16;  // accumulators of a dQ item; of a dK / dV item
+
+// Accumulator tile of 32 rows x 32 head dims, as the MFMA holds it.
+__device__ __forceinline__ void store_tile(f32x4* to, const f32x16& acc, int lane) {
+#pragma unroll
+  for (int rq = 0; rq < 4; ++rq)
+    __builtin_nontemporal_store(f32x4{acc[4 * rq], acc[4 * rq + 1], acc[4 * rq + 2], acc[4 * rq + 3]}, to + rq * 64 + lane);
+}
 
 // ---------------------------------------------------------------------- dQ --
 
@@ -39,8 +53,11 @@ void sparse_dq_kernel(BwdParams sp) {
   const bwd::Params& p = sp.a;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kWaveBytes];
 
-  const int item = item_of(blockIdx.x, gridDim.x, sp.items);
+  int item = item_of(blockIdx.x, gridDim.x, sp.items * sp.qparts);
   if (item < 0) return;
+  const int whole = item;
+  const int part = item % sp.qparts;
+  item /= sp.qparts;
   const int qblk = item % p.ntq;
   const int bh = item / p.ntq;
   const int b = bh / p.H, h = bh - b * p.H, hk = h / sp.group;
@@ -77,6 +94,7 @@ void sparse_dq_kernel(BwdParams sp) {
   }
   BlockWalk walk;
   walk.read(sp.blocks + (int64_t)item * sp.count, sp.count, (klen + kB - 1) / kB, reinterpret_cast<uint32_t*>(lds), lane);
+  if (sp.qparts > 1) walk.part(part, sp.qparts, lane);
   walk.start();
   // Halves of 32 keys; the last one may hold none.
   const int nblk = walk.n;
@@ -232,7 +250,7 @@ void sparse_dq_kernel(BwdParams sp) {
   wait_dma();
   // The record that the dK/dV kernel reads (at the end: stores ahead of the
   // loop would be waited for with its first loads).
-  if (hh == 0) {
+  if (hh == 0 && part == 0) {
     float* st = p.stats + (int64_t)item * bwd::kStat;
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) {
@@ -244,6 +262,14 @@ void sparse_dq_kernel(BwdParams sp) {
   asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3"
                : "+a"(w.dq[0][0]), "+a"(w.dq[1][0]), "+a"(w.dq[2][0]), "+a"(w.dq[3][0]),
                  "+a"(w.dq[0][1]), "+a"(w.dq[1][1]), "+a"(w.dq[2][1]), "+a"(w.dq[3][1]));
+  if (sp.qparts > 1) {
+    f32x4* to = sp.sums + (int64_t)whole * kQTiles * 256;
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb)
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) store_tile(to + (4 * qb + dt) * 256, w.dq[dt][qb], lane);
+    return;
+  }
   __syncthreads();
   bf16* ob = p.dq + b * p.s_dq[0] + h * p.s_dq[2];
 #pragma unroll
@@ -535,17 +561,32 @@ struct TileWalk {
     mine = load(pg, lane);
     lanes = __builtin_amdgcn_ballot_w64(mine != 0);
   }
+  // The next word with tiles; only while there is one.
+  __device__ __forceinline__ void next_word(int lane) {
+    while (lanes == 0) open(page + 1, lane);
+    const int l = __builtin_ctzll(lanes);
+    lanes &= lanes - 1;
+    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)mine, l);
+    const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(mine >> 32), l);
+    word = (uint64_t)lo | ((uint64_t)hi << 32);
+    at = 64 * page + l;
+  }
+  // Past the next k tiles; there are more than k.
+  __device__ __forceinline__ void skip(int k, int lane) {
+    while (k > 0) {
+      if (word == 0) next_word(lane);
+      const int c = __builtin_popcountll(word);
+      if (c <= k) {
+        word = 0;
+        k -= c;
+      } else {
+        for (; k > 0; --k) word &= word - 1;
+      }
+    }
+  }
   // Only while there is one: (head of the group, query tile).
   __device__ __forceinline__ void next(int lane, int& g, int& tile) {
-    if (word == 0) {
-      while (lanes == 0) open(page + 1, lane);
-      const int l = __builtin_ctzll(lanes);
-      lanes &= lanes - 1;
-      const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)mine, l);
-      const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(mine >> 32), l);
-      word = (uint64_t)lo | ((uint64_t)hi << 32);
-      at = 64 * page + l;
-    }
+    if (word == 0) next_word(lane);
     g = at / nqw;
     tile = 64 * (at - g * nqw) + __builtin_ctzll(word);
     word &= word - 1;
@@ -558,8 +599,11 @@ void sparse_dkdv_kernel(BwdParams sp) {
   __shared__ __attribute__((aligned(1024))) bf16 ring[kStages * 2 * kTileElems];
   __shared__ __attribute__((aligned(1024))) float stat[kStages * kStat];
 
-  const int item = item_of(blockIdx.x, gridDim.x, sp.kitems);
+  int item = item_of(blockIdx.x, gridDim.x, sp.kitems * sp.kparts);
   if (item < 0) return;
+  const int whole = item;
+  const int part = item % sp.kparts;
+  item /= sp.kparts;
   const int kblk = item % p.ntk;
   const int bhk = item / p.ntk;
   const int heads_k = p.H / sp.group;
@@ -578,15 +622,22 @@ void sparse_dkdv_kernel(BwdParams sp) {
   walk.nqw = sp.nqw;
   walk.total = sp.group * sp.nqw;
 
-  // The wave's K and V rows staged in ring stages 2 and 3 (16 KB per wave), free
-  // until tile 2's DMA, on their way while the list is read. Keys past klen
-  // re-read its last key (their gradients are not stored).
-  bf16* kst = ring + 2 * (2 * kTileElems) + wave * 8192;
-  if (klen > 0) {
-    stage_rows_in(p.k + b * p.s_k[0] + hk * p.s_k[2], p.s_k[1], key0, klen, lane, kst);
-    stage_rows_in(p.v + b * p.s_v[0] + hk * p.s_v[2], p.s_v[1], key0, klen, lane, kst + 4096);
+  const int all = walk.start(lane);
+  const int from = (int)((int64_t)all * part / sp.kparts);
+  const int n = (int)((int64_t)all * (part + 1) / sp.kparts) - from;
+  if (n > 0) {
+    walk.skip(from, lane);
+  } else if (sp.kparts == 1) {
+    // No list names the block: zeros (each wave 32 rows of dV or dK).
+    bf16* to = hq ? p.dk + b * p.s_dk[0] + hk * p.s_dk[2] : p.dv + b * p.s_dv[0] + hk * p.s_dv[2];
+    const int64_t rs = hq ? p.s_dk[1] : p.s_dv[1];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = key0 + 4 * i + (lane >> 4);
+      if (row < p.Sk) st16_nt(to + row * rs + 8 * (lane & 15), u32x4{0, 0, 0, 0});
+    }
+    return;
   }
-  const int n = walk.start(lane);
 
   const uint32_t ring0 = lds_addr(ring);
   const uint32_t stat0 = lds_addr(stat);
@@ -617,6 +668,12 @@ void sparse_dkdv_kernel(BwdParams sp) {
     if (stats_dma) dma.issue_stats(lane);
   };
   if (n > 0) {
+    // The wave's K and V rows staged in ring stages 2 and 3 (16 KB per wave),
+    // free until tile 2's DMA. Keys past klen re-read its last key (their
+    // gradients are not stored).
+    bf16* kst = ring + 2 * (2 * kTileElems) + wave * 8192;
+    stage_rows_in(p.k + b * p.s_k[0] + hk * p.s_k[2], p.s_k[1], key0, klen, lane, kst);
+    stage_rows_in(p.v + b * p.s_v[0] + hk * p.s_v[2], p.s_v[1], key0, klen, lane, kst + 4096);
     issue_job(0);
     issue_job(1);
     if (stats_dma) asm volatile("s_waitcnt vmcnt(9)" ::: "memory");
@@ -681,6 +738,12 @@ void sparse_dkdv_kernel(BwdParams sp) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) own[dt][4 * rq + e] = there ? own[dt][4 * rq + e] + v[e] : 0.f;
     }
+  if (sp.kparts > 1) {
+    f32x4* dst = sp.sums + ((int64_t)whole * kKTiles + 4 * wave) * 256;
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) store_tile(dst + dt * 256, own[dt], lane);
+    return;
+  }
   bf16* ostage = ring + 2 * (2 * kTileElems) + wave * 4096;
   stage_acc_rows(own, hq ? p.scale : 1.0f, lane, ostage);
   bf16* to = hq ? p.dk + b * p.s_dk[0] + hk * p.s_dk[2] : p.dv + b * p.s_dv[0] + hk * p.s_dv[2];
@@ -688,15 +751,83 @@ void sparse_dkdv_kernel(BwdParams sp) {
 }
 
 }  // namespace kv
+
+// ------------------------------------------------------------ sums of parts --
+
+// One wave per accumulator tile of an item: its parts' sum, in order, to the
+// gradient's rows. Q: dQ's items (tile 4 qb + dt); else dK's and dV's (tile 4
+// wave + dt of sparse_dkdv_kernel).
+template <bool Q>
+__global__ __launch_bounds__(256) void sparse_sum_kernel(BwdParams sp) {
+  constexpr int kTiles = Q ? kQTiles : kKTiles;
+  const bwd::Params& p = sp.a;
+  const int parts = Q ? sp.qparts : sp.kparts, items = Q ? sp.items : sp.kitems;
+  const int id = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int item = id / kTiles, tile = id % kTiles;
+  if (item >= items) return;
+  const f32x4* from = sp.sums + ((int64_t)item * parts * kTiles + tile) * 256 + lane;
+  f32x4 acc[4] = {};
+#pragma unroll 4
+  for (int s = 0; s < parts; ++s)
+#pragma unroll
+    for (int rq = 0; rq < 4; ++rq) acc[rq] += from[(int64_t)s * kTiles * 256 + rq * 64];
+
+  const int blocks = Q ? p.ntq : p.ntk, heads = Q ? p.H : p.H / sp.group;
+  const int blk = item % blocks, bh = item / blocks;
+  const int64_t b = bh / heads, h = bh - b * heads;
+  const int group = tile >> 2;  // Q: the row half; else the wave: key half, then dV / dK
+  const int row = blk * kB + 32 * (group & 1) + (lane & 31);
+  const bool dk = !Q && group >= 2;
+  const int64_t* st = Q ? p.s_dq : dk ? p.s_dk : p.s_dv;
+  bf16* to = (Q ? p.dq : dk ? p.dk : p.dv) + b * st[0] + row * st[1] + h * st[2] + 32 * (tile & 3) + 4 * (lane >> 5);
+  const float scale = Q || dk ? p.scale : 1.0f;
+  if (row >= (Q ? p.Sq : p.Sk)) return;
+#pragma unroll
+  for (int rq = 0; rq < 4; ++rq)
+    *reinterpret_cast<u32x2*>(to + 8 * rq) = u32x2{pack_bf16(acc[rq][0] * scale, acc[rq][1] * scale),
+                                                   pack_bf16(acc[rq][2] * scale, acc[rq][3] * scale)};
+}
+
+// Parts of the lists of key blocks: as many as give every CU a workgroup, of 4
+// query tiles or more where the lists are as long as on average.
+static int plan_kparts(int64_t kitems, int64_t group, int64_t nq, int64_t nk, int64_t count) {
+  const int64_t tiles = std::min(group * nq, (group * nq * count + nk - 1) / nk);
+  const int64_t parts = std::min<int64_t>(device_cu_count() / std::max<int64_t>(kitems, 1), tiles / 4);
+  return (int)std::max<int64_t>(1, parts);
+}
+
+struct BwdPlan {
+  int64_t nq, nk, nqw, items, kitems;
+  int qparts, kparts;
+  size_t stats, turned, sums;  // bytes
+};
+
+static BwdPlan plan_bwd(int64_t B, int64_t Sq, int64_t Sk, int64_t H, int64_t Hk, int64_t count) {
+  BwdPlan r = {};
+  r.nq = (Sq + kB - 1) / kB;
+  r.nk = (Sk + kB - 1) / kB;
+  r.nqw = (r.nq + 63) / 64;
+  r.items = B * H * r.nq;
+  r.kitems = B * Hk * r.nk;
+  r.qparts = plan_split(r.items, count);
+  r.kparts = plan_kparts(r.kitems, H / Hk, r.nq, r.nk, count);
+  r.stats = (size_t)r.items * bwd::kStat * sizeof(float);
+  r.turned = ((size_t)(B * H * r.nk * r.nqw) * sizeof(uint64_t) + 15) / 16 * 16;
+  const size_t q = r.qparts > 1 ? (size_t)r.items * r.qparts * kQTiles : 0;
+  const size_t k = r.kparts > 1 ? (size_t)r.kitems * r.kparts * kKTiles : 0;
+  r.sums = std::max(q, k) * 256 * sizeof(f32x4);  // one after the other
+  return r;
+}
+
 }  // namespace sparse
 }  // namespace aa
 
 using namespace aa;
 
-extern "C" size_t aa_sparse_bwd_workspace(int64_t B, int64_t Sq, int64_t Sk, int64_t H) {
-  if (B <= 0 || Sq <= 0 || Sk <= 0 || H <= 0) return 0;
-  const int64_t nq = (Sq + sparse::kB - 1) / sparse::kB, nk = (Sk + sparse::kB - 1) / sparse::kB;
-  return (size_t)(B * H * (nq * bwd::kStat * (int64_t)sizeof(float) + nk * ((nq + 63) / 64) * (int64_t)sizeof(uint64_t)));
+extern "C" size_t aa_sparse_bwd_workspace(int64_t B, int64_t Sq, int64_t Sk, int64_t H, int64_t Hk, int64_t count) {
+  if (B <= 0 || Sq <= 0 || Sk <= 0 || H <= 0 || Hk <= 0 || H % Hk || count < 1) return 0;
+  const sparse::BwdPlan plan = sparse::plan_bwd(B, Sq, Sk, H, Hk, count);
+  return plan.stats + plan.turned + plan.sums;
 }
 
 extern "C" int aa_sparse_bwd(const aa_sparse_bwd_args* a, void* workspace, size_t workspace_bytes, void* stream) {
@@ -710,7 +841,7 @@ extern "C" int aa_sparse_bwd(const aa_sparse_bwd_args* a, void* workspace, size_
   if (a->count < 1 || a->count > kMaxCount) return fail(AA_EUNSUPPORTED, "sparse_bwd: count must be 1 to 4096");
   if (a->Sk > kMaxBlocks * kB) return fail(AA_EUNSUPPORTED, "sparse_bwd: at most 262144 keys");
   const int64_t nq = (a->Sq + kB - 1) / kB, nk = (a->Sk + kB - 1) / kB;
-  if (a->Sq > 0x7fffffc0 || a->B > 0x7fffffff || a->H > 65535 || (nq && a->B * a->H > 0x1fffff0 / nq) ||
+  if (a->Sq > 0x7fffffc0 || a->B > 0x7fffffff || a->H > 65535 || (nq && a->B * a->H > 0xfffff0 / nq) ||
       (nk && a->B * a->Hk > 0x7fffff / nk))
     return fail(AA_EUNSUPPORTED, "sparse_bwd: too many blocks");
   if (a->B == 0 || a->Sq == 0 || a->Sk == 0) return AA_OK;
@@ -727,7 +858,8 @@ extern "C" int aa_sparse_bwd(const aa_sparse_bwd_args* a, void* workspace, size_
   for (int i = 0; i < 4; ++i)
     if (strides[i][1] < 0 || strides[i][1] >= kMaxRowStride)
       return fail(AA_EUNSUPPORTED, "sparse_bwd: sequence stride of dout, q, k or v out of range");
-  if (!workspace || !aligned16(workspace) || workspace_bytes < aa_sparse_bwd_workspace(a->B, a->Sq, a->Sk, a->H))
+  const BwdPlan plan = plan_bwd(a->B, a->Sq, a->Sk, a->H, a->Hk, a->count);
+  if (!workspace || !aligned16(workspace) || workspace_bytes < plan.stats + plan.turned + plan.sums)
     return fail(AA_EINVAL, "sparse_bwd: workspace too small or misaligned");
 
   BwdParams sp = {};
@@ -763,13 +895,18 @@ extern "C" int aa_sparse_bwd(const aa_sparse_bwd_args* a, void* workspace, size_
   sp.blocks = a->blocks;
   sp.group = (int)(a->H / a->Hk);
   sp.count = (int)a->count;
-  sp.nqw = (int)((nq + 63) / 64);
-  sp.items = (int)(a->B * a->H * nq);
-  sp.kitems = (int)(a->B * a->Hk * nk);
-  sp.turned = (uint64_t*)(p.stats + (int64_t)sp.items * bwd::kStat);
+  sp.nqw = (int)plan.nqw;
+  sp.items = (int)plan.items;
+  sp.kitems = (int)plan.kitems;
+  sp.qparts = plan.qparts;
+  sp.kparts = plan.kparts;
+  sp.turned = (uint64_t*)((char*)workspace + plan.stats);
+  sp.sums = (f32x4*)((char*)workspace + plan.stats + plan.turned);
   hipStream_t st = (hipStream_t)stream;
   sparse_turn_kernel<<<(unsigned)(a->B * a->H * sp.nqw), kTurnThreads, (size_t)nk * 8, st>>>(sp);
-  sparse_dq_kernel<<<grid_of(sp.items), 64, 0, st>>>(sp);
-  kv::sparse_dkdv_kernel<<<grid_of(sp.kitems), kv::kWaves * 64, 0, st>>>(sp);
+  sparse_dq_kernel<<<grid_of(plan.items * sp.qparts), 64, 0, st>>>(sp);
+  if (sp.qparts > 1) sparse_sum_kernel<true><<<(unsigned)(plan.items * kQTiles / 4), 256, 0, st>>>(sp);
+  kv::sparse_dkdv_kernel<<<grid_of(plan.kitems * sp.kparts), kv::kWaves * 64, 0, st>>>(sp);
+  if (sp.kparts > 1) sparse_sum_kernel<false><<<(unsigned)(plan.kitems * kKTiles / 4), 256, 0, st>>>(sp);
   return check_launch("sparse_bwd");
 }

@@ -303,16 +303,6 @@ __global__ __launch_bounds__(64 * kCombineWaves) void sparse_combine_kernel(Spar
   if (p.lse && lane == 0) p.lse[r] = any ? (mx * p.c + __log2f(fsum)) * kLn2 : -INFINITY;
 }
 
-// Parts of a list: as many as give every SIMD a wave, of equal numbers of blocks;
-// none where that takes fewer than 4 blocks (about 2 us each) off the longest
-// part: the second launch costs as much.
-static int plan_split(int64_t items, int64_t count) {
-  const int64_t slots = 4 * (int64_t)device_cu_count();
-  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(items ? slots / items : 1, count));
-  const int64_t longest = (count + parts - 1) / parts;
-  return count - longest < 4 ? 1 : (int)((count + longest - 1) / longest);
-}
-
 }  // namespace sparse
 }  // namespace aa
 

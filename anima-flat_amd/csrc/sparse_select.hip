@@ -160,8 +160,10 @@ __device__ __forceinline__ void pick(const Scores& scores, int have, int count, 
 // Scores of the workgroup's query blocks against the blocks of keys: the former's
 // means are scalar operands, the latter's are read once for all of them. The
 // waves share the blocks of keys and, with few of them, the head dims (PARTS
-// parts, which meet in LDS in a fixed order): what bounds it is how many reads
-// are on their way at once.
+// parts, which meet in LDS in a fixed order): latency bounds it, so many loads
+// are on their way at once and 512 threads take 4 rows (2048 query blocks x 64 of
+// keys: 256 threads 10.1 us, 512 6.8; 4096 x 256 25 us, 7 of them the search.
+// 16 rows a workgroup by fp64 matrix instructions: 8.9 and 22).
 template <int PARTS>
 __device__ __forceinline__ void dot_rows(const double* qm, const double* km, int nk, int have, int rows, double* partial,
                                          uint64_t* score) {
@@ -172,14 +174,17 @@ __device__ __forceinline__ void dot_rows(const double* qm, const double* km, int
   const int part = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWidth);
   for (int j = threadIdx.x - part * kWidth; j < have; j += kWidth) {
     double acc[kRows] = {};
-#pragma unroll 2
+#pragma unroll 1
     for (int d0 = 0; d0 < kSpan; d0 += 16) {
       double x[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] = km[(int64_t)(part * kSpan + d0 + i) * nk + j];
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
-        Const q = (Const)(uintptr_t)(qm + min(r, rows - 1) * kD + part * kSpan + d0);
+        // Opaque: the scalar loads of all rows at once would spill.
+        uint64_t at = (uint64_t)(uintptr_t)(qm + min(r, rows - 1) * kD + part * kSpan + d0);
+        asm volatile("" : "+s"(at));
+        const Const q = (Const)at;
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[r] = fma(q[i], x[i], acc[r]);
       }

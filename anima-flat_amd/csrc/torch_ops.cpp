@@ -909,7 +909,7 @@ T3 sparse_bwd(const Tensor& dout_, const Tensor& q, const Tensor& k, const Tenso
   set_strides(a.dv_stride, dv);
   set_sizes(a, q, k, blocks.size(3));
   a.softmax_scale = (float)(1.0 / std::sqrt(128.0));
-  const size_t bytes = aa_sparse_bwd_workspace(a.B, a.Sq, a.Sk, a.H);
+  const size_t bytes = aa_sparse_bwd_workspace(a.B, a.Sq, a.Sk, a.H, a.Hk, a.count);
   const Tensor ws = workspace(bytes, q);
   if (!launched(aa_sparse_bwd(&a, workspace_ptr(ws), bytes, stream_of(q)), "sparse_attention backward")) return slow();
   return {dq, dk, dv};

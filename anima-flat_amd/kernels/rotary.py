@@ -110,7 +110,8 @@ def _ready(t: torch.Tensor) -> torch.Tensor:
     bytes), or a copy."""
     unit = 16 // t.element_size()
     if t.stride(3) != 1 or any(s % unit for s in t.stride()[:3]):
-        t = t.contiguous()
+        # (contiguous() keeps the strides of dimensions of size 1.)
+        return t.clone(memory_format=torch.contiguous_format)
     return aligned(t)
 
 

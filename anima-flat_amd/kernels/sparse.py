@@ -53,7 +53,7 @@ def _check_heads(q, k, v, seqused_k, more=()) -> None:
     if seqused_k is not None and (
         seqused_k.shape != q.shape[:1] or seqused_k.dtype not in (torch.int32, torch.int64)
     ):
-        raise ValueError(f"seqused_k must be int32 [B]={q.shape[0]}")
+        raise ValueError(f"seqused_k must be [B]={q.shape[0]}, int32 or int64")
 
 
 def _check_blocks(q, blocks) -> None:
@@ -69,7 +69,11 @@ def _blocks_of(rows: int) -> int:
 
 
 def _lengths(seqused_k):
-    return None if seqused_k is None else seqused_k.to(torch.int32).contiguous()
+    if seqused_k is None:
+        return None
+    if seqused_k.dtype != torch.int32:
+        seqused_k = seqused_k.clamp(0, MAX_KEYS).to(torch.int32)
+    return seqused_k.contiguous()
 
 
 def _workspace(nbytes: int, like: torch.Tensor):
@@ -176,7 +180,7 @@ def _sparse_bwd(
     )
     _set_strides(a, dout=dout, q=q, k=k, v=v, out=out, dq=dq, dk=dk, dv=dv)
     with torch.cuda.device(q.device):
-        n = _lib.lib().aa_sparse_bwd_workspace(B, Sq, k.shape[1], H)
+        n = _lib.lib().aa_sparse_bwd_workspace(B, Sq, k.shape[1], H, k.shape[2], blocks.shape[3])
         ws = _workspace(n, q)
         _lib.check(_lib.lib().aa_sparse_bwd(ctypes.byref(a), _lib.ptr(ws), n, _lib.stream(q)), "sparse_attention backward")
     return dq, dk, dv
@@ -221,7 +225,8 @@ def select_blocks(q, k, count, seqused_k=None):
         q: Queries, bfloat16 `[B, Sq, H, 128]`.
         k: Keys, bfloat16 `[B, Sk, Hk, 128]` (H a multiple of Hk; at most 262144 keys).
         count: Blocks of keys per block of queries, 1 to 4096.
-        seqused_k: Number of keys of each batch item, int32 `[B]`, or None for all.
+        seqused_k: Number of keys of each batch item, int32 or int64 `[B]` (below 0 is 0, beyond Sk
+            all of them), or None for all.
 
     Returns:
         int32 `[B, H, ceil(Sq / 64), count]`, each list in ascending order, -1 behind its
@@ -243,7 +248,8 @@ def sparse_attention(q, k, v, blocks, seqused_k=None):
         blocks: int32 `[B, H, ceil(Sq / 64), count]`, as `select_blocks` gives them, or any
             other: in any order, a block named twice counts once, numbers that are no block
             with a key are passed over.
-        seqused_k: Number of keys of each batch item, int32 `[B]`, or None for all.
+        seqused_k: Number of keys of each batch item, int32 or int64 `[B]` (below 0 is 0, beyond Sk
+            all of them), or None for all.
 
     Returns:
         Attention output with heads merged, `[B, Sq, H * 128]`; 0 for queries whose list is

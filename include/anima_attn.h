@@ -641,9 +641,10 @@ typedef struct aa_sparse_bwd_args {
   int dtype;
 } aa_sparse_bwd_args;
 
-/* Bytes of workspace aa_sparse_bwd needs, 16-byte aligned: 1 KB of softmax
- * statistics per block of queries, and the lists turned round. */
-size_t aa_sparse_bwd_workspace(int64_t B, int64_t Sq, int64_t Sk, int64_t H);
+/* Bytes of workspace aa_sparse_bwd needs on the current device, 16-byte aligned:
+ * 1 KB of softmax statistics per block of queries, the lists turned round and,
+ * where few blocks are split over more of the device, fp32 partial sums. */
+size_t aa_sparse_bwd_workspace(int64_t B, int64_t Sq, int64_t Sk, int64_t H, int64_t Hk, int64_t count);
 
 /*
  * dq, dk, dv of aa_sparse_fwd, softmax recomputed from lse; dk and dv are sums

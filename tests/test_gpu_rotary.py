@@ -180,6 +180,16 @@ def test_special_values_stay_in_their_pair(rot):
     assert torch.isfinite(y[0, 1, 0, :15]).all() and y[0, 1, 0, 15] == math.inf
 
 
+def test_strides_of_single_elements(rot):
+    """Dimensions of size 1 have strides that address nothing, and that contiguous() keeps."""
+    g = gen(8)
+    base = torch.randn(1, 5, 3, 67, generator=g).cuda().to(torch.bfloat16)
+    x = base[:, :1, :1, :64]
+    x = x.as_strided(x.shape, (7, 3, 5, 1))
+    cos, sin = _angles(g, 1, 32)
+    assert torch.equal(rot.rotary(x, cos, sin), rot.rotary(x.clone(memory_format=torch.contiguous_format), cos, sin))
+
+
 def test_empty(rot):
     cos = torch.ones(0, 4, device="cuda")
     q, k = rot.rotary_qk(torch.empty(2, 0, 3, 8, device="cuda"), torch.empty(2, 0, 1, 8, device="cuda"), cos, cos)

@@ -57,7 +57,12 @@ def test_forward(sp, size):
     _check_forward(sp, q, k, v, random_blocks(g, B, H, Sq, Sk, count, lens), lens)
 
 
-@pytest.mark.parametrize("size", SIZES)
+# Lists of few blocks of keys, split over workgroups: tiles of three heads, and more words of
+# tiles than a wave has lanes.
+LONG = [(1, 4500, 150, 6, 2, 2, None), (1, 33000, 70, 8, 1, 1, [65]), (2, 40, 4000, 3, 3, 30, [4000, 900])]
+
+
+@pytest.mark.parametrize("size", SIZES + LONG)
 def test_gradients(sp, size):
     B, Sq, Sk, H, Hk, count, lens = size
     g = gen(12)
@@ -274,6 +279,15 @@ def test_views(sp, form):
         dout = torch.cos(torch.arange(out.numel(), device="cuda")).view(out.shape).to(BF)
         seen.append([sp.select_blocks(tensors[0], tensors[1], 2), out, *torch.autograd.grad(out, leaves, dout)])
     assert all(torch.equal(a, b) for a, b in zip(*seen))
+
+
+def test_strides_of_single_elements(sp):
+    """Dimensions of size 1 have strides that address nothing, and that contiguous() keeps."""
+    q, k = heads(gen(24), 1, 1, 1), heads(gen(25), 1, 90, 1)
+    odd = q.as_strided(q.shape, (3, 5, 7, 1))
+    blocks = torch.tensor([0, 1], dtype=torch.int32, device="cuda").view(1, 1, 1, 2)
+    assert torch.equal(sp.sparse_attention(odd, k, k, blocks), sp.sparse_attention(q, k, k, blocks))
+    assert torch.equal(sp.select_blocks(odd, k, 1), sp.select_blocks(q, k, 1))
 
 
 def test_every_block_is_the_dense_attention(pkg, sp):

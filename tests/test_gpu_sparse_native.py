@@ -168,8 +168,9 @@ def test_refusals_on_the_gpu(mods):
         with pytest.raises(ValueError, match=says):
             call(*args)
     # Lengths of another integer type are read as they are.
-    lens = torch.tensor([5, 90], device="cuda")
-    assert torch.equal(sparse.select_blocks(q, k, 2, lens), sparse.select_blocks(q, k, 2, lens.int()))
+    for values in ([5, 90], [-(2**40), 2**40]):
+        lens = torch.tensor(values, device="cuda")
+        assert torch.equal(sparse.select_blocks(q, k, 2, lens), sparse.select_blocks(q, k, 2, lens.clamp(0, 90).int()))
 
 
 def _refused(call, *tensors):
