@@ -39,6 +39,9 @@ __device__ __forceinline__ void wait_vm() {
 __device__ __forceinline__ void mfma_acc(f32x16& acc, bf16x8 a, bf16x8 b) {
   asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
 }
+__device__ __forceinline__ void mfma_sum(f32x4& acc, bf16x8 a, bf16x8 b) {
+  asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+}
 __device__ __forceinline__ void keep_alive(bf16x8 v) { asm volatile("" ::"v"(v)); }
 
 // Unit u of a block: scores 2 jp, 2 jp + 1 of the dZ operand (c, qb), c =
@@ -107,6 +110,28 @@ struct DqWave {
   int li, hh;
   uint32_t krd[4], vrd[4];      // LDS byte addresses of the next block's K / V row operands
   uint32_t ktr[4];              // ... of this block's K transposed operands
+  // With SUMS: sums of the rounded dZ of each query, in AGPRs, one small MFMA per
+  // operand: element 2 qb + i of lane l < 16 for query 32 qb + 16 i + l. And the
+  // squares of an eighth of the blocks' dZ; lane l: those of the blocks of group l.
+  f32x4 zsum;
+  float zsq, weight;
+
+  // zb as the B operand [32 keys][16 queries] of a 16 x 16 x 32 MFMA: lanes 0-15
+  // and 32-47 hold queries 0-15, the others 16-31. Ones in row 2 qb of A sum the
+  // former, in row 2 qb + 1 the latter.
+  template <int qb>
+  __device__ __forceinline__ u32x4 sum_rows() const {
+    uint32_t ones = (li & 15) == 2 * qb + (li >> 4) ? 0x3f803f80u : 0;
+    asm volatile("" : "+v"(ones));
+    u32x4 rows = {ones, ones, ones, ones};
+    asm volatile("" : "+v"(rows));
+    return rows;
+  }
+  // The sum of this lane's query (32 qb + li).
+  __device__ __forceinline__ float query_sum(int qb) const {
+    const float lo = __shfl(zsum[2 * qb], li & 15), hi = __shfl(zsum[2 * qb + 1], li & 15);
+    return li & 16 ? hi : lo;
+  }
 
   template <int j>
   __device__ __forceinline__ bf16x8 k_row() const {
@@ -179,13 +204,15 @@ struct DqWave {
   }
 
   // Block j: dZ^T and dQ^T of block j (its S^T, dP^T - D in buffer SB) and,
-  // with NEXT, those of block j+1 into the other buffer.
-  template <int SB, bool NEXT>
+  // with NEXT, those of block j+1 into the other buffer. SUMS: sums of dZ too,
+  // the block one of `group`.
+  template <int SB, bool NEXT, bool SUMS = false>
   __device__ __forceinline__ void block(bool mask_next, int kb_next, int lo_next, int Sk,
-                                        const BlockDma& dma) {
+                                        const BlockDma& dma, int group = 0) {
     constexpr int NB = 1 - SB;
     bf16x8 rq[kRowQ], tq[kTrQ];
     float fa[2][2], fe[2][2];
+    u32x4 rows;
     static_for<0, 48>([&](auto G) {
       constexpr int g = decltype(G)::value;
       if constexpr (NEXT && g == krow_slot(0)) wait_vm<16>();  // K of block j+1
@@ -223,11 +250,37 @@ struct DqWave {
           asm volatile("" : "+v"(fe[u & 1][0]), "+v"(fe[u & 1][1]));
         }
         if constexpr (unit_slot(u) + 2 == g) {
-          zb[cz][qb][2 * jp] = (bf16)(fe[u & 1][0] * dp[SB][qb][r]);
-          zb[cz][qb][2 * jp + 1] = (bf16)(fe[u & 1][1] * dp[SB][qb][r + 1]);
+          const float z0 = fe[u & 1][0] * dp[SB][qb][r], z1 = fe[u & 1][1] * dp[SB][qb][r + 1];
+          zb[cz][qb][2 * jp] = (bf16)z0;
+          zb[cz][qb][2 * jp + 1] = (bf16)z1;
+          if constexpr (SUMS && qb == 0 && (jp & 1)) zsq = fmaf(z1, z1, zsq);
           asm volatile("" : "+v"(zb[cz][qb]));
         }
       });
+      // (From slot 40 on there are registers: the scores are used up.)
+      if constexpr (SUMS && g == 40) rows = sum_rows<0>();
+      if constexpr (SUMS && g == 43) rows = sum_rows<1>();
+      if constexpr (SUMS && (g == 41 || g == 42)) mfma_sum(zsum, __builtin_bit_cast(bf16x8, rows), zb[g - 41][0]);
+      if constexpr (SUMS && (g == 44 || g == 45)) mfma_sum(zsum, __builtin_bit_cast(bf16x8, rows), zb[g - 44][1]);
+      // The wave's sum of squares, of two blocks, one step a slot, to the group's
+      // lane. A lane's that is not finite does not count.
+      if constexpr (SUMS && SB == 0 && g == 39) zsq = zsq < INFINITY ? zsq : 0.f;
+      if constexpr (SUMS && SB == 0 && g >= 40 && g < 46) {
+        constexpr int step[6] = {0x111, 0x112, 0x114, 0x118, 0x142, 0x143};  // row_shr 1, 2, 4, 8; row_bcast 15, 31
+        zsq += __builtin_bit_cast(
+            float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, zsq), step[(g - 40) % 6], 0xf, 0xf, false));
+        asm volatile("" : "+v"(zsq));
+      }
+      if constexpr (SUMS && g == 46) {
+        asm volatile("" ::"v"(rows));
+        keep_alive(zb[1][1]);
+      }
+      if constexpr (SUMS && SB == 0 && g == 46) {
+        const float all = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, zsq), 63));
+        weight += li + 32 * hh == group ? all : 0.f;
+        zsq = 0.f;
+        asm volatile("" : "+v"(weight), "+v"(zsq));
+      }
       if constexpr (NEXT && g == 40) {
         if (mask_next) mask<NB>(kb_next, lo_next, Sk);
       }
@@ -242,6 +295,7 @@ struct DqWave {
         constexpr int op = g - 33;
         keep_alive(tq[(op >> 1) % kTrQ]);
         keep_alive(zb[op >> 3][op & 1]);
+        if constexpr (SUMS && (g == 42 || g == 45)) keep_alive(zb[0][g == 45]);
       }
       __builtin_amdgcn_sched_barrier(0);
     });

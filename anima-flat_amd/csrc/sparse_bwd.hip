@@ -10,7 +10,7 @@
 //                       (attn_bwd_dq_wave.h); it also writes the statistics
 //                       record (lse, D) of its queries
 //   sparse_turn_kernel  the lists turned round: for each block of keys a bit per
-//                       block of queries that names it
+//                       block of queries that names it; and its mean key
 //   sparse_dkdv_kernel  one workgroup of 4 waves per block of 64 keys of one key
 //                       head, over the query blocks of all heads that share it
 //   sparse_sum_kernel   where few blocks would leave SIMDs or CUs idle, their
@@ -34,7 +34,12 @@ struct BwdParams {
   // than one, sparse_sum_kernel adds up the parts' 32 x 32 accumulators in fp32.
   int qparts, kparts;
   f32x4* sums;             // [item][part][tile][4][64]
+  float* means;            // [B][Hk][nk][128]: mean key of each block
+  float* recs;             // [item][part][kRec]: what a dQ part's correction needs
 };
+// A part's record: the sum of dZ of each query, then the weighted sum of the
+// mean keys and that of the weights.
+constexpr int kRecMean = kB, kRecWeight = kB + kD, kRec = 256;
 constexpr int kQTiles = 8, kKTiles = 16;  // accumulators of a dQ item; of a dK / dV item
 
 // Accumulator tile of 32 rows x 32 head dims, as the MFMA holds it.
@@ -44,7 +49,28 @@ __device__ __forceinline__ void store_tile(f32x4* to, const f32x16& acc, int lan
     __builtin_nontemporal_store(f32x4{acc[4 * rq], acc[4 * rq + 1], acc[4 * rq + 2], acc[4 * rq + 3]}, to + rq * 64 + lane);
 }
 
+// Mean key of weighted mean keys: 0 where nothing or nothing finite is known.
+__device__ __forceinline__ float mean_of(float sum, float weight) {
+  const float m = sum / weight;
+  return fabsf(m) < INFINITY ? m : 0.f;
+}
+
 // ---------------------------------------------------------------------- dQ --
+//
+// A query's dZ sum to 0 over its keys, but those that the MFMAs take do not
+// quite: each is rounded to bf16, and D is that of the rounded O. What stands out
+// of those errors in dQ is their sum times what the keys have in common: for
+// normed keys whose neighbours are alike dQ was 3.3e-3 to 4.6e-3 of its norm off,
+// where one rounding is 1.7e-3. So the kernel sums the rounded dZ (four MFMAs of 16
+// x 16 x 32 in a half's 48 slots; v_dot2 of pairs took twice their time) and
+// takes sum x mean key off at the end: 2.4e-3, two roundings. The mean is that of the
+// listed blocks, weighted by a sample of their squares of dZ, as it is there that the
+// errors come from (unweighted 2.6e-3, the first block's 3.2e-3); any would be
+// right, as the exact sum is 0. It costs 3 to 5% of the backward, half of it in the
+// loop (4096 tokens 158 -> 164 us, 9216 471 -> 492).
+//
+// What bounds the loop is one wave's issue: 410 instructions in a half's 48 slots
+// (MFMA busy in half of the cycles). 1.35 us a half in a full CU.
 
 __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1)))
 void sparse_dq_kernel(BwdParams sp) {
@@ -142,6 +168,9 @@ void sparse_dq_kernel(BwdParams sp) {
   w.li = li;
   w.hh = hh;
   w.c = p.c;
+  w.zsum = f32x4{};
+  asm volatile("" : "+a"(w.zsum));
+  w.zsq = w.weight = 0.f;
 #pragma unroll
   for (int qb = 0; qb < 2; ++qb)
 #pragma unroll
@@ -150,10 +179,8 @@ void sparse_dq_kernel(BwdParams sp) {
       asm volatile("" : "+a"(w.qop[qb][kk]));
     }
   // Statistics of each query: lse2 = lse log2(e) and -D, D = rowsum(dO o O) (this
-  // lane's 64 values, then the partner lane's half). O is the rounded output:
-  // D is off by its rounding, beside the rounding of dZ to bf16 for the MFMAs
-  // (dQ 3.4e-3 of its norm from 64 bits, one rounding is 1.7e-3). Queries past
-  // Sq, and those that attended nothing: lse2 = +inf, so that P = 0.
+  // lane's 64 values, then the partner lane's half). Queries past Sq, and those
+  // that attended nothing: lse2 = +inf, so that P = 0.
 #pragma unroll
   for (int qb = 0; qb < 2; ++qb) {
     const int q = qrow0 + 32 * qb + li;
@@ -226,7 +253,7 @@ void sparse_dq_kernel(BwdParams sp) {
         ka_job(i + 3, l3);
         v_job(i + 3, l3);
       }
-      w.block<SB, NEXT>(l1 + kKeys > klen, row_of(l1), l1, klen, dma);
+      w.block<SB, NEXT, true>(l1 + kKeys > klen, row_of(l1), l1, klen, dma, (i >> 1) & 63);
       w.advance_tr((i + 1) % 3 == 0 ? 0u - 2u * kBlock : kBlock);
       if constexpr (NEXT) {
         l1 = l2;
@@ -261,9 +288,44 @@ void sparse_dq_kernel(BwdParams sp) {
   // Keeps dQ in AGPRs up to here and orders the reads after its MFMAs.
   asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3"
                : "+a"(w.dq[0][0]), "+a"(w.dq[1][0]), "+a"(w.dq[2][0]), "+a"(w.dq[3][0]),
-                 "+a"(w.dq[0][1]), "+a"(w.dq[1][1]), "+a"(w.dq[2][1]), "+a"(w.dq[3][1]));
+                 "+a"(w.dq[0][1]), "+a"(w.dq[1][1]), "+a"(w.dq[2][1]), "+a"(w.dq[3][1]),
+                 "+a"(w.zsum));
+  // The sums of dZ, of both lanes of a query (0 where they are not finite: so is
+  // the query's dQ then), and the weighted sum of the mean keys, two head dims a
+  // lane.
+  float zsum[2], m[2] = {0.f, 0.f}, weight = 0.f;
+#pragma unroll
+  for (int qb = 0; qb < 2; ++qb) {
+    zsum[qb] = w.query_sum(qb);
+    if (!(fabsf(zsum[qb]) < INFINITY)) zsum[qb] = 0.f;
+  }
+  // (No square at all, of gradients below 1e-22 for example: the plain mean.)
+  if (sp.qparts == 1 && __builtin_amdgcn_ballot_w64(w.weight > 0.f) == 0) w.weight = 1.f;
+  walk.lanes = __builtin_amdgcn_ballot_w64(walk.mine != 0);
+  walk.word = 0;
+  const float* means = sp.means + ((int64_t)b * (p.H / sp.group) + hk) * p.ntk * kD + 2 * lane;
+  for (int i0 = 0; i0 < nblk; i0 += 8) {
+    float2 x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      x[e] = i0 + e < nblk ? *reinterpret_cast<const float2*>(means + (int64_t)walk.next() * kD) : float2{0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+            const float g = i0 + e < nblk ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w.weight), (i0 + e) & 63)) : 0.f;
+      m[0] = fmaf(g, x[e].x, m[0]);
+      m[1] = fmaf(g, x[e].y, m[1]);
+      weight += g;
+    }
+  }
   if (sp.qparts > 1) {
     f32x4* to = sp.sums + (int64_t)whole * kQTiles * 256;
+    float* rec = sp.recs + (int64_t)whole * kRec;
+    if (hh == 0) {
+      rec[li] = zsum[0];
+      rec[32 + li] = zsum[1];
+    }
+    *reinterpret_cast<float2*>(rec + kRecMean + 2 * lane) = float2{m[0], m[1]};
+    if (lane == 0) rec[kRecWeight] = weight;
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb)
 #pragma unroll
@@ -271,10 +333,22 @@ void sparse_dq_kernel(BwdParams sp) {
     return;
   }
   __syncthreads();
+  float* mean = reinterpret_cast<float*>(lds + 2 * kBlock);
+  mean[2 * lane] = mean_of(m[0], weight);
+  mean[2 * lane + 1] = mean_of(m[1], weight);
+  __syncthreads();
   bf16* ob = p.dq + b * p.s_dq[0] + h * p.s_dq[2];
 #pragma unroll
   for (int qb = 0; qb < 2; ++qb) {
-    const f32x16 acc[4] = {w.dq[0][qb], w.dq[1][qb], w.dq[2][qb], w.dq[3][qb]};
+    f32x16 acc[4] = {w.dq[0][qb], w.dq[1][qb], w.dq[2][qb], w.dq[3][qb]};
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+      for (int rq = 0; rq < 4; ++rq) {
+        const f32x4 km = *reinterpret_cast<const f32x4*>(mean + 32 * dt + 8 * rq + 4 * hh);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[dt][4 * rq + e] = fmaf(-zsum[qb], km[e], acc[dt][4 * rq + e]);
+      }
     bf16* stage = area((uint32_t)qb * kBlock);
     stage_acc_rows(acc, p.scale, lane, stage);
     stage_rows_out(ob, p.s_dq[1], qrow0 + 32 * qb, p.Sq, lane, stage);
@@ -285,12 +359,56 @@ void sparse_dq_kernel(BwdParams sp) {
 
 constexpr int kTurnThreads = 256;
 
+// The mean key of each block, one wave a block: 16 lanes a row, 4 rows an
+// instruction. Blocks without a key are left out: nothing reads them.
+__device__ __forceinline__ void mean_keys(const BwdParams& sp, int64_t blk, int lane) {
+  const bwd::Params& p = sp.a;
+  if (blk >= sp.kitems) return;
+  const int x = (int)(blk % p.ntk), bhk = (int)(blk / p.ntk);
+  const int heads = p.H / sp.group, b = bhk / heads, hk = bhk - b * heads;
+  const int n = min(key_length(sp.seqused, b, p.Sk) - x * kB, kB);
+  if (n <= 0) return;
+  const int c = lane & 15, r0 = lane >> 4;
+  const bf16* base = p.k + b * p.s_k[0] + hk * p.s_k[2] + (int64_t)x * kB * p.s_k[1] + 8 * c;
+  u32x4 raw[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int r = 4 * i + r0;
+    raw[i] = r < n ? ld16(base + r * p.s_k[1]) : u32x4{0, 0, 0, 0};
+  }
+  float sum[8] = {};
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    float v[8];
+    unpack8(raw[i], v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[e] += v[e];
+  }
+  const float inv = 1.0f / (float)n;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    sum[e] += __shfl_xor(sum[e], 16);
+    sum[e] += __shfl_xor(sum[e], 32);
+    sum[e] *= inv;
+  }
+  if (r0 == 0) {
+    f32x4* to = reinterpret_cast<f32x4*>(sp.means + blk * kD + 8 * c);
+    to[0] = f32x4{sum[0], sum[1], sum[2], sum[3]};
+    to[1] = f32x4{sum[4], sum[5], sum[6], sum[7]};
+  }
+}
+
 // One workgroup per 64 query blocks of one (batch, head): a bit each in LDS for
 // every block of keys, then out. (An OR of bits: the order of the atomics does
-// not matter.)
-__global__ __launch_bounds__(kTurnThreads) void sparse_turn_kernel(BwdParams sp) {
+// not matter.) The workgroups from `lists` on: mean keys.
+__global__ __launch_bounds__(kTurnThreads) void sparse_turn_kernel(BwdParams sp, int lists) {
   extern __shared__ uint32_t word[];  // [nk][2]
   const bwd::Params& p = sp.a;
+  if ((int)blockIdx.x >= lists) {
+    const int64_t wg = (int)blockIdx.x - lists;
+    mean_keys(sp, wg * (kTurnThreads / 64) + (threadIdx.x >> 6), threadIdx.x & 63);
+    return;
+  }
   const int w = blockIdx.x % sp.nqw, bh = blockIdx.x / sp.nqw;
   const int b = bh / p.H;
   const int have = (key_length(sp.seqused, b, p.Sk) + kB - 1) / kB;
@@ -782,6 +900,23 @@ __global__ __launch_bounds__(256) void sparse_sum_kernel(BwdParams sp) {
   bf16* to = (Q ? p.dq : dk ? p.dk : p.dv) + b * st[0] + row * st[1] + h * st[2] + 32 * (tile & 3) + 4 * (lane >> 5);
   const float scale = Q || dk ? p.scale : 1.0f;
   if (row >= (Q ? p.Sq : p.Sk)) return;
+  if constexpr (Q) {
+    // The correction of sparse_dq_kernel, over all parts.
+    f32x4 m[4] = {};
+    float zsum = 0.f, weight = 0.f;
+    for (int s = 0; s < parts; ++s) {
+      const float* rec = sp.recs + ((int64_t)item * parts + s) * kRec;
+      zsum += rec[row - blk * kB];
+      weight += rec[kRecWeight];
+#pragma unroll
+      for (int rq = 0; rq < 4; ++rq)
+        m[rq] += *reinterpret_cast<const f32x4*>(rec + kRecMean + 32 * (tile & 3) + 8 * rq + 4 * (lane >> 5));
+    }
+#pragma unroll
+    for (int rq = 0; rq < 4; ++rq)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[rq][e] = fmaf(-zsum, mean_of(m[rq][e], weight), acc[rq][e]);
+  }
 #pragma unroll
   for (int rq = 0; rq < 4; ++rq)
     *reinterpret_cast<u32x2*>(to + 8 * rq) = u32x2{pack_bf16(acc[rq][0] * scale, acc[rq][1] * scale),
@@ -799,7 +934,8 @@ static int plan_kparts(int64_t kitems, int64_t group, int64_t nq, int64_t nk, in
 struct BwdPlan {
   int64_t nq, nk, nqw, items, kitems;
   int qparts, kparts;
-  size_t stats, turned, sums;  // bytes
+  size_t stats, turned, sums, means, recs;  // bytes
+  size_t total() const { return stats + turned + sums + means + recs; }
 };
 
 static BwdPlan plan_bwd(int64_t B, int64_t Sq, int64_t Sk, int64_t H, int64_t Hk, int64_t count) {
@@ -816,6 +952,8 @@ static BwdPlan plan_bwd(int64_t B, int64_t Sq, int64_t Sk, int64_t H, int64_t Hk
   const size_t q = r.qparts > 1 ? (size_t)r.items * r.qparts * kQTiles : 0;
   const size_t k = r.kparts > 1 ? (size_t)r.kitems * r.kparts * kKTiles : 0;
   r.sums = std::max(q, k) * 256 * sizeof(f32x4);  // one after the other
+  r.means = (size_t)r.kitems * kD * sizeof(float);
+  r.recs = r.qparts > 1 ? (size_t)r.items * r.qparts * kRec * sizeof(float) : 0;
   return r;
 }
 
@@ -827,7 +965,7 @@ using namespace aa;
 extern "C" size_t aa_sparse_bwd_workspace(int64_t B, int64_t Sq, int64_t Sk, int64_t H, int64_t Hk, int64_t count) {
   if (B <= 0 || Sq <= 0 || Sk <= 0 || H <= 0 || Hk <= 0 || H % Hk || count < 1) return 0;
   const sparse::BwdPlan plan = sparse::plan_bwd(B, Sq, Sk, H, Hk, count);
-  return plan.stats + plan.turned + plan.sums;
+  return plan.total();
 }
 
 extern "C" int aa_sparse_bwd(const aa_sparse_bwd_args* a, void* workspace, size_t workspace_bytes, void* stream) {
@@ -859,7 +997,7 @@ extern "C" int aa_sparse_bwd(const aa_sparse_bwd_args* a, void* workspace, size_
     if (strides[i][1] < 0 || strides[i][1] >= kMaxRowStride)
       return fail(AA_EUNSUPPORTED, "sparse_bwd: sequence stride of dout, q, k or v out of range");
   const BwdPlan plan = plan_bwd(a->B, a->Sq, a->Sk, a->H, a->Hk, a->count);
-  if (!workspace || !aligned16(workspace) || workspace_bytes < plan.stats + plan.turned + plan.sums)
+  if (!workspace || !aligned16(workspace) || workspace_bytes < plan.total())
     return fail(AA_EINVAL, "sparse_bwd: workspace too small or misaligned");
 
   BwdParams sp = {};
@@ -900,10 +1038,14 @@ extern "C" int aa_sparse_bwd(const aa_sparse_bwd_args* a, void* workspace, size_
   sp.kitems = (int)plan.kitems;
   sp.qparts = plan.qparts;
   sp.kparts = plan.kparts;
-  sp.turned = (uint64_t*)((char*)workspace + plan.stats);
-  sp.sums = (f32x4*)((char*)workspace + plan.stats + plan.turned);
+  char* at = (char*)workspace + plan.stats;
+  sp.turned = (uint64_t*)at;
+  sp.sums = (f32x4*)(at += plan.turned);
+  sp.means = (float*)(at += plan.sums);
+  sp.recs = (float*)(at += plan.means);
   hipStream_t st = (hipStream_t)stream;
-  sparse_turn_kernel<<<(unsigned)(a->B * a->H * sp.nqw), kTurnThreads, (size_t)nk * 8, st>>>(sp);
+  const int lists = (int)(a->B * a->H * sp.nqw), means = (int)((plan.kitems + kTurnThreads / 64 - 1) / (kTurnThreads / 64));
+  sparse_turn_kernel<<<lists + means, kTurnThreads, (size_t)nk * 8, st>>>(sp, lists);
   sparse_dq_kernel<<<grid_of(plan.items * sp.qparts), 64, 0, st>>>(sp);
   if (sp.qparts > 1) sparse_sum_kernel<true><<<(unsigned)(plan.items * kQTiles / 4), 256, 0, st>>>(sp);
   kv::sparse_dkdv_kernel<<<grid_of(plan.kitems * sp.kparts), kv::kWaves * 64, 0, st>>>(sp);

@@ -8,7 +8,8 @@ the instruction; together eps. The probability that weights V is rounded to bf16
     |out - o| <= sum_j p_j (w + eps) |v_j - o| / (1 - w - eps) + n u sum_j p_j |v_j| + w |o|
 (the sum of the same rounded probabilities divides). The backward forms p from the
 log-sum-exp, off by eps + n u + 2^-20 (1 + |lse|), rounds p and dz once each, and takes D from
-the rounded out.
+the rounded out. dq takes (sum of dz) x (a mean of keys) off: as the exact dz sum to 0, that
+adds the sum of their errors times what a mean can be, the largest block's.
 """
 
 from __future__ import annotations
@@ -115,7 +116,11 @@ def attend(q, k, v, blocks, lens=None, dout=None):
             ):
                 by_scale = 1.0 if name == "dv" else scale
                 ref[name][b, :, at] += by_scale * (val @ by)
-                err[name][b, :, at] += by_scale * ((bad + max(Sq, Sk) * U32 * val.abs()) @ by.abs())
+                bad = bad + max(Sq, Sk) * U32 * val.abs()
+                err[name][b, :, at] += by_scale * (bad @ by.abs())
+                if name == "dq" and Sk:
+                    means = torch.stack([r.mean(0) for r in K[: ends_of(lens, B, Sk)[b] or 1].split(B64)])
+                    err[name][b, :, at] += by_scale * 1.01 * bad.sum(1, keepdim=True) * means.abs().amax(0)
     for name in ("dq", "dk", "dv"):
         if name in ref:
             err[name] = 1.01 * err[name] + U16 * ref[name].abs()

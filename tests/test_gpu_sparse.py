@@ -79,6 +79,37 @@ def test_gradients(sp, size):
     assert all(torch.equal(a, b) for a, b in zip(got, again))
 
 
+@pytest.mark.parametrize("size", [(1, 100, 500, 4, 2, 3, None), (2, 70, 700, 2, 2, 9, [700, 130]), (1, 40, 9000, 2, 1, 70, None),
+                                  (3, 7, 30, 2, 2, 1, None), (1, 33000, 150, 8, 4, 2, None)])
+def test_gradients_of_keys_in_common(sp, size):
+    """Keys of 8 times what differs between them: dq is what differs times dz, the rest cancels.
+    Two roundings of it are left, of dz and of dq, half a step of 2^-8 at most each."""
+    B, Sq, Sk, H, Hk, count, lens = size
+    g = gen(31)
+    q, v, dout = heads(g, B, Sq, H), heads(g, B, Sk, Hk), heads(g, B, Sq, H)
+    k = (8 * heads(g, 1, 1, Hk).float() + heads(g, B, Sk, Hk).float()).to(BF)
+    lens = _lens(lens)
+    blocks = random_blocks(g, B, H, Sq, Sk, count, lens)
+    q.requires_grad_(True)
+    (dq,) = torch.autograd.grad(sp.sparse_attention(q, k, v, blocks, lens), [q], dout.flatten(2))
+    ref, _ = attend(q, k, v, blocks, lens, dout)
+    assert (dq.double() - ref["dq"]).norm() <= 2 * 2.0**-8 * ref["dq"].norm()
+
+
+@pytest.mark.parametrize("scale", [2.0**-80, 2.0**75])
+@pytest.mark.parametrize("sk", [150, 1500])
+def test_gradients_of_any_scale(sp, scale, sk):
+    """dz whose squares leave the range of float32: the mean key falls back to the plain one, in
+    split lists to none."""
+    g = gen(32)
+    q, k, v, dout = heads(g, 1, 70, 2), heads(g, 1, sk, 1), heads(g, 1, sk, 1), heads(g, 1, 70, 2) * scale
+    blocks = random_blocks(g, 1, 2, 70, sk, 20)
+    q.requires_grad_(True)
+    (dq,) = torch.autograd.grad(sp.sparse_attention(q, k, v, blocks), [q], dout.flatten(2))
+    ref, err = attend(q, k, v, blocks, None, dout)
+    _close("dq", dq, ref["dq"], err["dq"])
+
+
 def test_gradients_by_differences(sp):
     """Along a direction: the loss, in 64 bits from the kernel's inputs, moves as the gradients
     say. A step of 2^-6 leaves a relative error of its square, (2^-6)^2 / 6 times third

@@ -129,7 +129,7 @@ def test_workspaces(lib):
     assert lib.aa_block_select_workspace(2, 65, 64, 6, 3) == 2 * (6 * 2 + 3 * 1) * 128 * 8
     # No device here, so no split: 1 KB a query block, 8 bytes a key block and 64 query blocks.
     if not torch.cuda.is_available():
-        assert lib.aa_sparse_bwd_workspace(2, 65, 130, 6, 3, 2) == 2 * 6 * (2 * 1024 + 3 * 8)
+        assert lib.aa_sparse_bwd_workspace(2, 65, 130, 6, 3, 2) == 2 * 6 * (2 * 1024 + 3 * 8) + 2 * 3 * 3 * 512
         assert lib.aa_sparse_fwd_workspace(2, 65, 6, 100) == 0
     assert lib.aa_block_select_workspace(1, 64, 64, 3, 2) == lib.aa_sparse_bwd_workspace(1, 0, 64, 1, 1, 1) == 0
     assert lib.aa_sparse_bwd_workspace(1, 64, 64, 3, 2, 1) == lib.aa_sparse_fwd_workspace(0, 1, 1, 1) == 0
