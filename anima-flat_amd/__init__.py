@@ -26,6 +26,11 @@ Opt-in modules, not imported here (import them explicitly):
                  quantize_weight, int8_linear), inference; the reference's are FP8.
   kernels.ckpt8  training with activations kept in 8 bits (gelu8, lora_down8); no counterpart
                  in the reference.
+  kernels.rotary rotary positions of any form, apart from the norm (rotary_tables, rotary,
+                 rotary_qk); the reference turns whole heads inside qkv_norm_rope only.
+  kernels.sparse attention of blocks of queries over selected blocks of keys (select_blocks,
+                 sparse_attention, tile_order), for images beyond the trained size; no counterpart
+                 in the reference.
 
 Every op is registered through kernels.common.custom_op, which raises if the name is already
 registered in the process (torch.library would otherwise re-bind it silently). Ops this package

@@ -398,6 +398,9 @@ __device__ __forceinline__ void mean_keys(const BwdParams& sp, int64_t blk, int 
   }
 }
 
+// (With the mean keys 5.2 us at 4096 tokens of 16 heads, 8.1 at 9216, where K is
+// 38 MB; the lists alone are a chain of latencies of 4.8 us.)
+//
 // One workgroup per 64 query blocks of one (batch, head): a bit each in LDS for
 // every block of keys, then out. (An OR of bits: the order of the atomics does
 // not matter.) The workgroups from `lists` on: mean keys.
@@ -442,6 +445,11 @@ __global__ __launch_bounds__(kTurnThreads) void sparse_turn_kernel(BwdParams sp,
 //   slots  8-15: dP - D of tile t+1   |   scores every 2-3 slots from slot 2
 //   slots 16-31: dV^T and dK^T of tile t, alternating
 // The DMA of tile t+3 goes out one instruction in 4 slots; one barrier a tile.
+//
+// What bounds it: the waves' issue (matrix pipe busy in 40% of the cycles, 21%
+// waits), 1.05 us a tile, and per key block the start (its bits, K and V, the
+// first tiles) and the end: 4096 tokens x 16 heads over 1, 16, 64 blocks 36.5, 102
+// and 304 us; 9216 over 24 blocks 303 us, 765 TFLOP/s over its four products.
 namespace kv {
 
 using bwd::kStat;

@@ -10,7 +10,8 @@
 // means something. That costs 1/16 of the inputs' bytes for the means and, at
 // 16384 tokens, 134 M fp64 FMAs beside the attention's 137 G.
 //
-//   means_kernel   one wave per block of rows: HBM-bound, q and k once
+//   means_kernel   one wave per block of rows: HBM-bound, q and k once (2 x 4096
+//                  tokens of 16 + 16 heads 14.8 us, 4.5 TB/s)
 //   select_kernel  one workgroup per 4 query blocks of one head: scores into LDS,
 //                  a key block per lane (k's means are transposed for that, q's
 //                  are scalars), then a wave per row finds the count-th largest

@@ -5,7 +5,9 @@
  * the QK-RMSNorm + 3D-RoPE prologue, per-head RMSNorm of cross-attention
  * queries, the non-causal flash-attention forward (self, and key-length
  * masked cross-attention with an optional fused padding correction), the
- * flash-attention backward, and the padding-correction kernels on their own.
+ * flash-attention backward, and the padding-correction kernels on their own;
+ * around them the block's norms, int8 products and 8-bit copies, rotary
+ * positions on their own and the attention over selected blocks.
  *
  * Conventions shared by every entry point:
  *   - Tensors are device pointers. Attention tensors are [B, S, H, hd]
@@ -20,10 +22,12 @@
  *     AA_EUNSUPPORTED (-2) for a shape or dtype the kernels do not
  *     implement; AA_EHIP (-3) when a HIP launch reports an error.
  *     aa_last_error() returns the calling thread's last message.
- *   - Only dtype AA_DTYPE_BF16 is implemented for activations; weights,
- *     rotary tables, LSE and padding logs are float32; key lengths int32.
+ *   - Only dtype AA_DTYPE_BF16 is implemented for activations (aa_rotary also
+ *     takes FP16 and FP32); weights, rotary tables, LSE and padding logs are
+ *     float32; key lengths and block lists int32.
  *   - hd (head_dim) must be 128; aa_attn_fwd (and its workspace and no-alloc
- *     forms) also takes 384, the VAE decoder's single-head attention.
+ *     forms) also takes 384, the VAE decoder's single-head attention, and
+ *     aa_rotary multiples of 8 up to 512.
  *
  * The reference (anima-flat) has no C FFI of its own: its path is Python
  * calling FlashAttention-4 (CuTe DSL) and Triton kernels. Each entry point
@@ -642,8 +646,9 @@ typedef struct aa_sparse_bwd_args {
 } aa_sparse_bwd_args;
 
 /* Bytes of workspace aa_sparse_bwd needs on the current device, 16-byte aligned:
- * 1 KB of softmax statistics per block of queries, the lists turned round and,
- * where few blocks are split over more of the device, fp32 partial sums. */
+ * 1 KB of softmax statistics per block of queries, the lists turned round, the
+ * mean key of each block and, where few blocks are split over more of the device,
+ * fp32 partial sums. */
 size_t aa_sparse_bwd_workspace(int64_t B, int64_t Sq, int64_t Sk, int64_t H, int64_t Hk, int64_t count);
 
 /*
