@@ -1005,6 +1005,8 @@ extern "C" int aa_sparse_bwd(const aa_sparse_bwd_args* a, void* workspace, size_
     if (strides[i][1] < 0 || strides[i][1] >= kMaxRowStride)
       return fail(AA_EUNSUPPORTED, "sparse_bwd: sequence stride of dout, q, k or v out of range");
   const BwdPlan plan = plan_bwd(a->B, a->Sq, a->Sk, a->H, a->Hk, a->count);
+  const int64_t lists = a->B * a->H * plan.nqw, means = (plan.kitems + kTurnThreads / 64 - 1) / (kTurnThreads / 64);
+  if (!grid_fits(lists + means, kTurnThreads)) return fail(AA_EUNSUPPORTED, "sparse_bwd: too many blocks");
   if (!workspace || !aligned16(workspace) || workspace_bytes < plan.total())
     return fail(AA_EINVAL, "sparse_bwd: workspace too small or misaligned");
 
@@ -1052,8 +1054,7 @@ extern "C" int aa_sparse_bwd(const aa_sparse_bwd_args* a, void* workspace, size_
   sp.means = (float*)(at += plan.sums);
   sp.recs = (float*)(at += plan.means);
   hipStream_t st = (hipStream_t)stream;
-  const int lists = (int)(a->B * a->H * sp.nqw), means = (int)((plan.kitems + kTurnThreads / 64 - 1) / (kTurnThreads / 64));
-  sparse_turn_kernel<<<lists + means, kTurnThreads, (size_t)nk * 8, st>>>(sp, lists);
+  sparse_turn_kernel<<<(unsigned)(lists + means), kTurnThreads, (size_t)nk * 8, st>>>(sp, (int)lists);
   sparse_dq_kernel<<<grid_of(plan.items * sp.qparts), 64, 0, st>>>(sp);
   if (sp.qparts > 1) sparse_sum_kernel<true><<<(unsigned)(plan.items * kQTiles / 4), 256, 0, st>>>(sp);
   kv::sparse_dkdv_kernel<<<grid_of(plan.kitems * sp.kparts), kv::kWaves * 64, 0, st>>>(sp);

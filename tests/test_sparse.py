@@ -117,6 +117,7 @@ def test_library_refusals(pkg, lib):
         for name in tensors:
             assert call(kind, **{name: None}) == call(kind, **{name: fake + 8}) == L.AA_EINVAL, (kind, name)
             assert call(kind, **{name + "_stride": L.c_strides((1 << 15, 2044, 128))}) == L.AA_EINVAL, (kind, name)
+    assert call("bwd", B=1048575, Hk=8, Sq=1, Sk=1) == L.AA_EUNSUPPORTED
     assert call("select", ws=None) == call("select", ws_bytes=64) == call("select", ws=fake + 8) == L.AA_EINVAL
     assert call("bwd", ws=None) == call("bwd", ws_bytes=64) == call("bwd", ws=fake + 8) == call("bwd", lse=None) == L.AA_EINVAL
     for kind, names in (("fwd", ("k", "v")), ("bwd", ("dout", "q", "k", "v"))):
