@@ -63,7 +63,8 @@ struct BlockDma {
   uint32_t kdst, vdst, kadst;  // LDS byte addresses of their places
 
   // Rows at or past Sk are never fetched: fewer than 32 keys re-read the last
-  // one, more have no block that reaches past them (row_of in the kernel).
+  // one, more have no block that reaches past them (row_of in the dense kernel),
+  // or one that re-reads its own last row (end_k, end_v in the sparse one).
   __device__ __forceinline__ void setup(int64_t ks1, int64_t vs1, int Sk, int lane) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -71,6 +72,21 @@ struct BlockDma {
       ko[i] = (uint32_t)(r * ks1 + col) * 2u;
       vo[i] = (uint32_t)(r * vs1 + col) * 2u;
     }
+  }
+  // From now on the rows past `last` re-read it: min(r, last) rows are the smaller
+  // of the two offsets, as no stride is negative. Of K the 8-row blocks I .. I + 1
+  // (0: issue_ka's, 2: issue_kb's). (Opaque: the loop around has no registers for
+  // what does not change in it.)
+  template <int I>
+  __device__ __forceinline__ void end_k(int64_t ks1, int last, int lane) {
+    asm volatile("" : "+v"(lane));
+#pragma unroll
+    for (int i = I; i < I + 2; ++i) ko[i] = min(ko[i], (uint32_t)(last * ks1 + 8 * dual_chunk(lane, i & 1)) * 2u);
+  }
+  __device__ __forceinline__ void end_v(int64_t vs1, int last, int lane) {
+    asm volatile("" : "+v"(lane));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) vo[i] = min(vo[i], (uint32_t)(last * vs1 + 8 * dual_chunk(lane, i & 1)) * 2u);
   }
   template <int i>
   __device__ __forceinline__ void issue_k() const {

@@ -132,8 +132,11 @@ void sparse_dq_kernel(BwdParams sp) {
   }
 
   // First keys of the halves i + 1, i + 2, i + 3; past the list its last half
-  // again, into places that nothing reads. A half that reaches past klen is
-  // moved back to end there, its keys below its own first masked.
+  // again, into places that nothing reads. In the half that klen ends in, which is
+  // the last one of any list that has it, the rows from klen on re-read the one
+  // before it, masked. (Moved back to end at klen, as in the dense kernel, the half
+  // would read keys of the block before, which the list need not name: a NaN there
+  // spoilt dQ.)
   int blk = 0, half = 0, left = n, lo = 0;
   auto next_half = [&]() {
     if (left > 0) {
@@ -144,23 +147,25 @@ void sparse_dq_kernel(BwdParams sp) {
     }
     return lo;
   };
-  auto row_of = [&](int first) { return min(first, max(klen - kKeys, 0)); };
   const bf16* kp = p.k + b * p.s_k[0] + hk * p.s_k[2];
   const bf16* vp = p.v + b * p.s_v[0] + hk * p.s_v[2];
   const uint32_t mine = lds_addr(lds);
   BlockDma dma;
-  dma.setup(p.s_k[1], p.s_v[1], klen, lane);
-  auto k_job = [&](int i, int first) {
-    dma.kt = kp + (int64_t)row_of(first) * p.s_k[1];
+  dma.setup(p.s_k[1], p.s_v[1], kKeys, lane);
+  auto k_job = [&](int i, int first) {  // its last 16 keys; the others' rows are ka_job's
+    dma.kt = kp + (int64_t)first * p.s_k[1];
     dma.kdst = mine + (uint32_t)(i % 3) * kBlock;
+    if (first + kKeys > klen) dma.end_k<2>(p.s_k[1], klen - 1 - first, lane);
   };
   auto ka_job = [&](int i, int first) {
-    dma.ka = kp + (int64_t)row_of(first) * p.s_k[1];
+    dma.ka = kp + (int64_t)first * p.s_k[1];
     dma.kadst = mine + (uint32_t)(i % 3) * kBlock;
+    if (first + kKeys > klen) dma.end_k<0>(p.s_k[1], klen - 1 - first, lane);
   };
   auto v_job = [&](int i, int first) {
-    dma.vt = vp + (int64_t)row_of(first) * p.s_v[1];
+    dma.vt = vp + (int64_t)first * p.s_v[1];
     dma.vdst = mine + kVRing + (uint32_t)(i & 1) * kBlock;
+    if (first + kKeys > klen) dma.end_v(p.s_v[1], klen - 1 - first, lane);
   };
   const int l0 = next_half();
   int l1 = next_half(), l2 = next_half(), l3 = 0;
@@ -201,10 +206,12 @@ void sparse_dq_kernel(BwdParams sp) {
   }
   __syncthreads();  // the staged rows are read: their places are free
   if (n > 0) {
+    ka_job(0, l0);
     k_job(0, l0);
     dma.all_k();
     v_job(0, l0);
     dma.all_v();
+    ka_job(1, l1);
     k_job(1, l1);
     dma.all_k();
     v_job(1, l1);
@@ -229,10 +236,10 @@ void sparse_dq_kernel(BwdParams sp) {
     const bool m0 = l0 + kKeys > klen;
     if (b0) {
       w.first<1>();
-      if (m0) w.mask<1>(row_of(l0), l0, klen);
+      if (m0) w.mask<1>(l0, l0, klen);
     } else {
       w.first<0>();
-      if (m0) w.mask<0>(row_of(l0), l0, klen);
+      if (m0) w.mask<0>(l0, l0, klen);
     }
     v_job(2, l2);
     dma.all_v();
@@ -253,7 +260,7 @@ void sparse_dq_kernel(BwdParams sp) {
         ka_job(i + 3, l3);
         v_job(i + 3, l3);
       }
-      w.block<SB, NEXT, true>(l1 + kKeys > klen, row_of(l1), l1, klen, dma, (i >> 1) & 63);
+      w.block<SB, NEXT, true>(l1 + kKeys > klen, l1, l1, klen, dma, (i >> 1) & 63);
       w.advance_tr((i + 1) % 3 == 0 ? 0u - 2u * kBlock : kBlock);
       if constexpr (NEXT) {
         l1 = l2;
