@@ -39,8 +39,11 @@ __device__ __forceinline__ void wait_vm() {
 __device__ __forceinline__ void mfma_acc(f32x16& acc, bf16x8 a, bf16x8 b) {
   asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
 }
-__device__ __forceinline__ void mfma_sum(f32x4& acc, bf16x8 a, bf16x8 b) {
-  asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+// 16 products of 4 x 4 x 4: with ones for A, every element of a lane's result is
+// the sum of the lane's own four values of B. (Two on one accumulator stand two
+// instructions apart or more.)
+__device__ __forceinline__ void mfma_sum(f32x4& acc, u32x2 ones, bf16x4 b) {
+  asm volatile("v_mfma_f32_4x4x4_16b_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(ones), "v"(b));
 }
 __device__ __forceinline__ void keep_alive(bf16x8 v) { asm volatile("" ::"v"(v)); }
 
@@ -126,28 +129,12 @@ struct DqWave {
   int li, hh;
   uint32_t krd[4], vrd[4];      // LDS byte addresses of the next block's K / V row operands
   uint32_t ktr[4];              // ... of this block's K transposed operands
-  // With SUMS: sums of the rounded dZ of each query, in AGPRs, one small MFMA per
-  // operand: element 2 qb + i of lane l < 16 for query 32 qb + 16 i + l. And the
-  // squares of an eighth of the blocks' dZ; lane l: those of the blocks of group l.
-  f32x4 zsum;
+  // With SUMS: sums of this lane's rounded dZ of query 32 qb + li, in AGPRs (every
+  // element). Nothing of another lane is in them: what a product over more lanes
+  // multiplies by 0 is NaN where a query's dZ are. And the squares of an eighth of
+  // the blocks' dZ; lane l: those of the blocks of group l.
+  f32x4 zsum[2];
   float zsq, weight;
-
-  // zb as the B operand [32 keys][16 queries] of a 16 x 16 x 32 MFMA: lanes 0-15
-  // and 32-47 hold queries 0-15, the others 16-31. Ones in row 2 qb of A sum the
-  // former, in row 2 qb + 1 the latter.
-  template <int qb>
-  __device__ __forceinline__ u32x4 sum_rows() const {
-    uint32_t ones = (li & 15) == 2 * qb + (li >> 4) ? 0x3f803f80u : 0;
-    asm volatile("" : "+v"(ones));
-    u32x4 rows = {ones, ones, ones, ones};
-    asm volatile("" : "+v"(rows));
-    return rows;
-  }
-  // The sum of this lane's query (32 qb + li).
-  __device__ __forceinline__ float query_sum(int qb) const {
-    const float lo = __shfl(zsum[2 * qb], li & 15), hi = __shfl(zsum[2 * qb + 1], li & 15);
-    return li & 16 ? hi : lo;
-  }
 
   template <int j>
   __device__ __forceinline__ bf16x8 k_row() const {
@@ -228,7 +215,7 @@ struct DqWave {
     constexpr int NB = 1 - SB;
     bf16x8 rq[kRowQ], tq[kTrQ];
     float fa[2][2], fe[2][2];
-    u32x4 rows;
+    u32x2 ones;
     static_for<0, 48>([&](auto G) {
       constexpr int g = decltype(G)::value;
       if constexpr (NEXT && g == krow_slot(0)) wait_vm<16>();  // K of block j+1
@@ -273,11 +260,20 @@ struct DqWave {
           asm volatile("" : "+v"(zb[cz][qb]));
         }
       });
-      // (From slot 40 on there are registers: the scores are used up.)
-      if constexpr (SUMS && g == 40) rows = sum_rows<0>();
-      if constexpr (SUMS && g == 43) rows = sum_rows<1>();
-      if constexpr (SUMS && (g == 41 || g == 42)) mfma_sum(zsum, __builtin_bit_cast(bf16x8, rows), zb[g - 41][0]);
-      if constexpr (SUMS && (g == 44 || g == 45)) mfma_sum(zsum, __builtin_bit_cast(bf16x8, rows), zb[g - 44][1]);
+      // (From slot 39 on there are registers: the scores are used up.)
+      if constexpr (SUMS && g == 39) {
+        ones = u32x2{0x3f803f80u, 0x3f803f80u};
+        asm volatile("" : "+v"(ones));
+      }
+      // (Even slots: the odd ones have a DMA.)
+      if constexpr (SUMS && g >= 40 && (g & 1) == 0) {
+        constexpr int s = (g - 40) >> 1;
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb) {
+          const bf16x8& z = zb[s >> 1][qb];
+          mfma_sum(zsum[qb], ones, (s & 1) ? __builtin_shufflevector(z, z, 4, 5, 6, 7) : __builtin_shufflevector(z, z, 0, 1, 2, 3));
+        }
+      }
       // The wave's sum of squares, of two blocks, one step a slot, to the group's
       // lane. A lane's that is not finite does not count.
       if constexpr (SUMS && SB == 0 && g == 39) zsq = zsq < INFINITY ? zsq : 0.f;
@@ -286,10 +282,6 @@ struct DqWave {
         zsq += __builtin_bit_cast(
             float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, zsq), step[(g - 40) % 6], 0xf, 0xf, false));
         asm volatile("" : "+v"(zsq));
-      }
-      if constexpr (SUMS && g == 46) {
-        asm volatile("" ::"v"(rows));
-        keep_alive(zb[1][1]);
       }
       if constexpr (SUMS && SB == 0 && g == 46) {
         const float all = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, zsq), 63));
@@ -311,12 +303,16 @@ struct DqWave {
         constexpr int op = g - 33;
         keep_alive(tq[(op >> 1) % kTrQ]);
         keep_alive(zb[op >> 3][op & 1]);
-        if constexpr (SUMS && (g == 42 || g == 45)) keep_alive(zb[0][g == 45]);
+        if constexpr (SUMS && g > 40 && (g & 1)) {
+          keep_alive(zb[(g - 41) >> 2][0]);
+          keep_alive(zb[(g - 41) >> 2][1]);
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
     });
     keep_alive(tq[7 % kTrQ]);
     keep_alive(zb[1][1]);
+    if constexpr (SUMS) asm volatile("" ::"v"(ones));
   }
 };
 

@@ -61,9 +61,9 @@ __device__ __forceinline__ float mean_of(float sum, float weight) {
 // quite: each is rounded to bf16, and D is that of the rounded O. What stands out
 // of those errors in dQ is their sum times what the keys have in common: for
 // normed keys whose neighbours are alike dQ was 3.3e-3 to 4.6e-3 of its norm off,
-// where one rounding is 1.7e-3. So the kernel sums the rounded dZ (four MFMAs of 16
-// x 16 x 32 in a half's 48 slots; v_dot2 of pairs took twice their time) and
-// takes sum x mean key off at the end: 2.4e-3, two roundings. The mean is that of the
+// where one rounding is 1.7e-3. So the kernel sums the rounded dZ (eight MFMAs of 4
+// x 4 x 4, whose sums are a lane's own, in a half's last slots; v_dot2 of pairs
+// took twice their time) and takes sum x mean key off at the end: 2.4e-3, two roundings. The mean is that of the
 // listed blocks, weighted by a sample of their squares of dZ, as it is there that the
 // errors come from (unweighted 2.6e-3, the first block's 3.2e-3); any would be
 // right, as the exact sum is 0. It costs 3 to 5% of the backward, half of it in the
@@ -173,8 +173,8 @@ void sparse_dq_kernel(BwdParams sp) {
   w.li = li;
   w.hh = hh;
   w.c = p.c;
-  w.zsum = f32x4{};
-  asm volatile("" : "+a"(w.zsum));
+  w.zsum[0] = w.zsum[1] = f32x4{};
+  asm volatile("" : "+a"(w.zsum[0]), "+a"(w.zsum[1]));
   w.zsq = w.weight = 0.f;
 #pragma unroll
   for (int qb = 0; qb < 2; ++qb)
@@ -296,14 +296,14 @@ void sparse_dq_kernel(BwdParams sp) {
   asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3"
                : "+a"(w.dq[0][0]), "+a"(w.dq[1][0]), "+a"(w.dq[2][0]), "+a"(w.dq[3][0]),
                  "+a"(w.dq[0][1]), "+a"(w.dq[1][1]), "+a"(w.dq[2][1]), "+a"(w.dq[3][1]),
-                 "+a"(w.zsum));
+                 "+a"(w.zsum[0]), "+a"(w.zsum[1]));
   // The sums of dZ, of both lanes of a query (0 where they are not finite: so is
   // the query's dQ then), and the weighted sum of the mean keys, two head dims a
   // lane.
   float zsum[2], m[2] = {0.f, 0.f}, weight = 0.f;
 #pragma unroll
   for (int qb = 0; qb < 2; ++qb) {
-    zsum[qb] = w.query_sum(qb);
+    zsum[qb] = pair_sum(w.zsum[qb][0]);
     if (!(fabsf(zsum[qb]) < INFINITY)) zsum[qb] = 0.f;
   }
   // (No square at all, of gradients below 1e-22 for example: the plain mean.)
