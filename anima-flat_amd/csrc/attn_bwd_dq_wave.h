@@ -274,7 +274,7 @@ struct DqWave {
           mfma_sum(zsum[qb], ones, (s & 1) ? __builtin_shufflevector(z, z, 4, 5, 6, 7) : __builtin_shufflevector(z, z, 0, 1, 2, 3));
         }
       }
-      // The wave's sum of squares, of two blocks, one step a slot, to the group's
+      // The wave's sum of squares, of two blocks (or of the first one), one step a slot, to the group's
       // lane. A lane's that is not finite does not count.
       if constexpr (SUMS && SB == 0 && g == 39) zsq = zsq < INFINITY ? zsq : 0.f;
       if constexpr (SUMS && SB == 0 && g >= 40 && g < 46) {

@@ -64,7 +64,7 @@ __device__ __forceinline__ float mean_of(float sum, float weight) {
 // where one rounding is 1.7e-3. So the kernel sums the rounded dZ (eight MFMAs of 4
 // x 4 x 4, whose sums are a lane's own, in a half's last slots; v_dot2 of pairs
 // took twice their time) and takes sum x mean key off at the end: 2.4e-3, two roundings. The mean is that of the
-// listed blocks, weighted by a sample of their squares of dZ, as it is there that the
+// listed blocks, weighted by a sample of their own squares of dZ, as it is there that the
 // errors come from (unweighted 2.6e-3, the first block's 3.2e-3); any would be
 // right, as the exact sum is 0. It costs 3 to 5% of the backward, half of it in the
 // loop (4096 tokens 158 -> 164 us, 9216 471 -> 492).
@@ -122,7 +122,8 @@ void sparse_dq_kernel(BwdParams sp) {
   walk.read(sp.blocks + (int64_t)item * sp.count, sp.count, (klen + kB - 1) / kB, reinterpret_cast<uint32_t*>(lds), lane);
   if (sp.qparts > 1) walk.part(part, sp.qparts, lane);
   walk.start();
-  // Halves of 32 keys; the last one may hold none.
+  // Halves of 32 keys; the last one may hold none, and the one before it then
+  // comes first: a block's two halves stay a pair that ends in buffer 0.
   const int nblk = walk.n;
   int n = 2 * nblk;
   if (nblk > 0 && klen % kB != 0 && klen % kB <= kKeys) {
@@ -132,8 +133,8 @@ void sparse_dq_kernel(BwdParams sp) {
   }
 
   // First keys of the halves i + 1, i + 2, i + 3; past the list its last half
-  // again, into places that nothing reads. In the half that klen ends in, which is
-  // the last one of any list that has it, the rows from klen on re-read the one
+  // again, into places that nothing reads. In the half that klen ends in, which
+  // comes last or, alone of its block, first, the rows from klen on re-read the one
   // before it, masked. (Moved back to end at klen, as in the dense kernel, the half
   // would read keys of the block before, which the list need not name: a NaN there
   // spoilt dQ.)
@@ -167,7 +168,12 @@ void sparse_dq_kernel(BwdParams sp) {
     dma.vdst = mine + kVRing + (uint32_t)(i & 1) * kBlock;
     if (first + kKeys > klen) dma.end_v(p.s_v[1], klen - 1 - first, lane);
   };
-  const int l0 = next_half();
+  const bool single = n & 1;
+  if (single) {
+    lo = klen / kB * kB;
+    --left;
+  }
+  const int l0 = single ? lo : next_half();
   int l1 = next_half(), l2 = next_half(), l3 = 0;
   wait_dma();
   w.li = li;
@@ -211,6 +217,7 @@ void sparse_dq_kernel(BwdParams sp) {
     dma.all_k();
     v_job(0, l0);
     dma.all_v();
+    if (single) dma.setup(p.s_k[1], p.s_v[1], kKeys, lane);
     ka_job(1, l1);
     k_job(1, l1);
     dma.all_k();
@@ -318,7 +325,9 @@ void sparse_dq_kernel(BwdParams sp) {
       x[e] = i0 + e < nblk ? *reinterpret_cast<const float2*>(means + (int64_t)walk.next() * kD) : float2{0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-            const float g = i0 + e < nblk ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w.weight), (i0 + e) & 63)) : 0.f;
+      // The group of the list's block i0 + e: a single half's block, its last, was first.
+      const int group = !single ? i0 + e : i0 + e + 1 < nblk ? i0 + e + 1 : 0;
+      const float g = i0 + e < nblk ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w.weight), group & 63)) : 0.f;
       m[0] = fmaf(g, x[e].x, m[0]);
       m[1] = fmaf(g, x[e].y, m[1]);
       weight += g;
