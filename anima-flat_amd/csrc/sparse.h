@@ -129,5 +129,18 @@ inline int plan_split(int64_t items, int64_t count) {
   return count - longest < 4 ? 1 : (int)((count + longest - 1) / longest);
 }
 
+// What the backward launches: a wave per block of queries (dQ), a workgroup of 256
+// threads per 64 of them and per 4 blocks of keys (turned lists, mean keys), and
+// one per block of keys (dK, dV). A forward that keeps statistics is held to it.
+constexpr int64_t kTurnThreads = 256, kKvThreads = 256;
+inline int64_t turn_lists(int64_t B, int64_t H, int64_t nq) { return B * H * ((nq + 63) / 64); }
+inline int64_t turn_means(int64_t kitems) { return (kitems + kTurnThreads / 64 - 1) / (kTurnThreads / 64); }
+inline bool backward_fits(int64_t B, int64_t Sq, int64_t Sk, int64_t H, int64_t Hk) {
+  const int64_t nq = (Sq + kB - 1) / kB, nk = (Sk + kB - 1) / kB;
+  if ((nq && B * H > 0x1fffff0 / nq) || (nk && B * Hk > 0x1fffff0 / nk)) return false;
+  return grid_fits(turn_lists(B, H, nq) + turn_means(B * Hk * nk), kTurnThreads) &&
+         grid_fits(grid_of(B * Hk * nk), kKvThreads);
+}
+
 }  // namespace sparse
 }  // namespace aa

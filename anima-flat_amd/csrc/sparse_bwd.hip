@@ -373,8 +373,6 @@ void sparse_dq_kernel(BwdParams sp) {
 
 // ------------------------------------------------------- lists turned round --
 
-constexpr int kTurnThreads = 256;
-
 // The mean key of each block, one wave a block: 16 lanes a row, 4 rows an
 // instruction. Blocks without a key are left out: nothing reads them.
 __device__ __forceinline__ void mean_keys(const BwdParams& sp, int64_t blk, int lane) {
@@ -479,6 +477,7 @@ using bwd::w1::mfma_acc;
 using bwd::w1::QdoDma;
 
 constexpr int kWaves = 4;
+static_assert(kWaves * 64 == kKvThreads, "backward_fits");
 constexpr int kStages = 4;
 constexpr int kLead = kStages - 1;  // tile t + kLead is fetched during tile t
 // Operand reads ahead of their MFMA, and queues of them (attn_bwd_dkdv.hip).
@@ -1003,8 +1002,7 @@ extern "C" int aa_sparse_bwd(const aa_sparse_bwd_args* a, void* workspace, size_
   if (a->count < 1 || a->count > kMaxCount) return fail(AA_EUNSUPPORTED, "sparse_bwd: count must be 1 to 4096");
   if (a->Sk > kMaxBlocks * kB) return fail(AA_EUNSUPPORTED, "sparse_bwd: at most 262144 keys");
   const int64_t nq = (a->Sq + kB - 1) / kB, nk = (a->Sk + kB - 1) / kB;
-  if (a->Sq > 0x7fffffc0 || a->B > 0x7fffffff || a->H > 65535 || (nq && a->B * a->H > 0xfffff0 / nq) ||
-      (nk && a->B * a->Hk > 0x7fffff / nk))
+  if (a->Sq > 0x7fffffc0 || a->B > 0x7fffffff || a->H > 65535 || !backward_fits(a->B, a->Sq, a->Sk, a->H, a->Hk))
     return fail(AA_EUNSUPPORTED, "sparse_bwd: too many blocks");
   if (a->B == 0 || a->Sq == 0 || a->Sk == 0) return AA_OK;
   const void* all[] = {a->dout, a->q, a->k, a->v, a->out, a->lse, a->blocks, a->dq, a->dk, a->dv};
@@ -1021,8 +1019,7 @@ extern "C" int aa_sparse_bwd(const aa_sparse_bwd_args* a, void* workspace, size_
     if (strides[i][1] < 0 || strides[i][1] >= kMaxRowStride)
       return fail(AA_EUNSUPPORTED, "sparse_bwd: sequence stride of dout, q, k or v out of range");
   const BwdPlan plan = plan_bwd(a->B, a->Sq, a->Sk, a->H, a->Hk, a->count);
-  const int64_t lists = a->B * a->H * plan.nqw, means = (plan.kitems + kTurnThreads / 64 - 1) / (kTurnThreads / 64);
-  if (!grid_fits(lists + means, kTurnThreads)) return fail(AA_EUNSUPPORTED, "sparse_bwd: too many blocks");
+  const int64_t lists = turn_lists(a->B, a->H, nq), means = turn_means(plan.kitems);
   if (!workspace || !aligned16(workspace) || workspace_bytes < plan.total())
     return fail(AA_EINVAL, "sparse_bwd: workspace too small or misaligned");
 

@@ -339,6 +339,8 @@ extern "C" int aa_sparse_fwd(const aa_sparse_fwd_args* a, void* workspace, size_
   const int64_t nq = (a->Sq + kB - 1) / kB;
   if (a->Sq > 0x7fffffc0 || a->B > 0x7fffffff || a->H > 65535 || (nq && a->B * a->H > 0x1fffff0 / nq))
     return fail(AA_EUNSUPPORTED, "sparse_fwd: too many query blocks");
+  if (a->lse && a->Sk && !backward_fits(a->B, a->Sq, a->Sk, a->H, a->Hk))
+    return fail(AA_EUNSUPPORTED, "sparse_fwd: too many blocks for a backward pass (without lse there is none)");
   if (a->B == 0 || a->Sq == 0) return AA_OK;
   if (!a->q || !a->out || !a->blocks || (a->Sk && (!a->k || !a->v))) return fail(AA_EINVAL, "sparse_fwd: null pointer");
   for (const void* ptr : {a->q, a->k, a->v, (const void*)a->out})

@@ -256,7 +256,9 @@ def sparse_attention(q, k, v, blocks, seqused_k=None):
         empty. Differentiable in q, k and v, once.
 
     Raises:
-        ValueError: If a tensor is not on CUDA, or a shape, dtype or size is not supported.
+        ValueError: If a tensor is not on CUDA, or a shape, dtype or size is not supported (blocks
+            of queries beyond 33 million; with gradients B H ceil(Sq / 4096) + B Hk ceil(Sk / 64) / 4
+            or B Hk ceil(Sk / 64) beyond 16 million).
     """
     keep = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     return _sparse_fwd(q, k, v, blocks, seqused_k, keep)[0].flatten(2)

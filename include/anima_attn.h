@@ -615,7 +615,7 @@ size_t aa_sparse_fwd_workspace(int64_t B, int64_t Sq, int64_t H, int64_t count);
  * out = softmax(q k^T * softmax_scale) v over the keys of the listed blocks below
  * seqused_k, lse its natural-log row log-sum-exp. One launch, plus a combine pass
  * when aa_sparse_fwd_workspace() > 0. Rows of k and v at or past seqused_k are
- * not read. Stands beside src/attention.py:43-81, which attends every key.
+ * not read. B H nq at most 0x1fffff0; with lse also what aa_sparse_bwd takes. Stands beside src/attention.py:43-81, which attends every key.
  */
 int aa_sparse_fwd(const aa_sparse_fwd_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
@@ -655,6 +655,8 @@ size_t aa_sparse_bwd_workspace(int64_t B, int64_t Sq, int64_t Sk, int64_t H, int
  * dq, dk, dv of aa_sparse_fwd, softmax recomputed from lse; dk and dv are sums
  * over the heads of q that share a head of k. Deterministic: no atomics on
  * floats, every sum in a fixed order. With Sq == 0 or Sk == 0 nothing is written.
+ * With nk = ceil(Sk / 64): B H nq and B Hk nk at most 0x1fffff0, B H ceil(nq / 64) +
+ * B Hk nk / 4 and B Hk nk below 2^24.
  */
 int aa_sparse_bwd(const aa_sparse_bwd_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
