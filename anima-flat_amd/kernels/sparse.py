@@ -30,6 +30,7 @@ from .common import _check, custom_op, refuse_captured_training
 BLOCK = 64
 MAX_KEYS = 262144
 MAX_COUNT = 4096
+MAX_ROW_STRIDE = 1 << 24
 
 
 def _check_heads(q, k, v, seqused_k, more=()) -> None:
@@ -74,6 +75,13 @@ def _lengths(seqused_k):
     if seqused_k.dtype != torch.int32:
         seqused_k = seqused_k.clamp(0, MAX_KEYS).to(torch.int32)
     return seqused_k.contiguous()
+
+
+def _near(t: torch.Tensor) -> torch.Tensor:
+    """`_prep`, and a copy where tokens are further apart than the backward's 32-bit row offsets
+    reach."""
+    t = _prep(t)
+    return t if t.stride(1) < MAX_ROW_STRIDE else t.clone(memory_format=torch.contiguous_format)
 
 
 def _workspace(nbytes: int, like: torch.Tensor):
@@ -171,7 +179,7 @@ def _sparse_bwd(
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
     if q.numel() == 0 or k.numel() == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
-    dout, q, k, v, out = (_prep(t) for t in (dout, q, k, v, out))
+    dout, q, k, v, out = _near(dout), _near(q), _prep(k), _prep(v), _prep(out)
     lse, lengths, blocks = lse.contiguous(), _lengths(seqused_k), blocks.contiguous()
     a = _lib.SparseBwdArgs(
         dout=dout.data_ptr(), q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(),
@@ -244,7 +252,8 @@ def sparse_attention(q, k, v, blocks, seqused_k=None):
     Args:
         q: Queries, bfloat16 `[B, Sq, H, 128]`.
         k, v: Keys and values, bfloat16 `[B, Sk, Hk, 128]` (H a multiple of Hk; at most 262144
-            keys). Rows at or past `seqused_k` are not read.
+            keys, less than 2^24 values from one to the next). Rows at or past `seqused_k` are
+            not read.
         blocks: int32 `[B, H, ceil(Sq / 64), count]`, as `select_blocks` gives them, or any
             other: in any order, a block named twice counts once, numbers that are no block
             with a key are passed over.

@@ -655,7 +655,8 @@ size_t aa_sparse_bwd_workspace(int64_t B, int64_t Sq, int64_t Sk, int64_t H, int
  * dq, dk, dv of aa_sparse_fwd, softmax recomputed from lse; dk and dv are sums
  * over the heads of q that share a head of k. Deterministic: no atomics on
  * floats, every sum in a fixed order. With Sq == 0 or Sk == 0 nothing is written.
- * With nk = ceil(Sk / 64): B H nq and B Hk nk at most 0x1fffff0, B H ceil(nq / 64) +
+ * Sequence strides of dout, q, k and v are 0 to 2^24 - 1 (in the forward those of
+ * k and v). With nk = ceil(Sk / 64): B H nq and B Hk nk at most 0x1fffff0, B H ceil(nq / 64) +
  * B Hk nk / 4 and B Hk nk below 2^24.
  */
 int aa_sparse_bwd(const aa_sparse_bwd_args* args, void* workspace, size_t workspace_bytes, void* stream);
