@@ -1350,6 +1350,7 @@ struct SparseFwd : torch::autograd::Function<SparseFwd> {
 
 T2 sparse_fwd_autograd(CT q, CT k, CT v, CT blocks, CO seqused, bool keep) {
   if (!needs_grad(q, k, v)) return op_sparse_fwd().below(q, k, v, blocks, seqused, keep);
+  TORCH_CHECK(keep, "sparse_attention: a call that needs gradients keeps its statistics (keep)");
   check_capture(q, k, v);
   Tensor lse;
   Tensor out = SparseFwd::apply(q, k, v, blocks, seqused, &lse);
