@@ -306,7 +306,7 @@ extern "C" int aa_rotary_tables(const aa_rotary_tables_args* a, void* stream) {
   // Four rows a thread where that still fills the chip (131072 positions of 64
   // pairs 21.8 -> 18.5 us, 16384 with one row 5.8, with four 7.1).
   const int rows = a->rows * p.pairs / vec >= 4096 * (int64_t)device_cu_count() ? 4 : 1;
-  p.step = (p.rows + rows - 1) / rows;
+  p.step = (uint32_t)((a->rows + rows - 1) / rows);
   p.total = (uint32_t)(p.step * (uint64_t)p.pairs / vec);
   const uint32_t blocks = (uint32_t)(((uint64_t)p.total + kThreads - 1) / kThreads);
   if (!grid_fits(blocks, kThreads)) return fail(AA_EUNSUPPORTED, "rotary_tables: too many positions");
