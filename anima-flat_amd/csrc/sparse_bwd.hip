@@ -66,11 +66,15 @@ __device__ __forceinline__ float mean_of(float sum, float weight) {
 // took twice their time) and takes sum x mean key off at the end: 2.4e-3, two roundings. The mean is that of the
 // listed blocks, weighted by a sample of their own squares of dZ, as it is there that the
 // errors come from (unweighted 2.6e-3, the first block's 3.2e-3); any would be
-// right, as the exact sum is 0. It costs 3 to 5% of the backward, half of it in the
-// loop (4096 tokens 158 -> 164 us, 9216 471 -> 492).
+// right, as the exact sum is 0. (Of lists of more than 64 blocks, blocks 64 apart
+// have one weight, of both.) It costs 3 to 4% of the backward, most of it in the
+// loop (forward and backward at 4096 tokens x 16 blocks 193 -> 197 us, 9216 x 24
+// 632 -> 650).
 //
-// What bounds the loop is one wave's issue: 410 instructions in a half's 48 slots
-// (MFMA busy in half of the cycles). 1.35 us a half in a full CU.
+// What bounds the loop is one wave's issue: 420 instructions in a half's 48 slots
+// (MFMA busy in half of the cycles), 1.43 us a half in a full CU. Beside it stands
+// what a round of lists does together, start and end (4096 tokens x 16 heads x 16 blocks:
+// 19 of 63 us), and a last round that is not full (9216 x 24: 2.25 rounds, 235 us).
 
 __global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(1, 1)))
 void sparse_dq_kernel(BwdParams sp) {
@@ -412,7 +416,7 @@ __device__ __forceinline__ void mean_keys(const BwdParams& sp, int64_t blk, int 
   }
 }
 
-// (With the mean keys 5.2 us at 4096 tokens of 16 heads, 8.1 at 9216, where K is
+// (With the mean keys 5.1 us at 4096 tokens of 16 heads, 8.3 at 9216, where K is
 // 38 MB; the lists alone are a chain of latencies of 4.8 us.)
 //
 // One workgroup per 64 query blocks of one (batch, head): a bit each in LDS for
@@ -461,9 +465,10 @@ __global__ __launch_bounds__(kTurnThreads) void sparse_turn_kernel(BwdParams sp,
 // The DMA of tile t+3 goes out one instruction in 4 slots; one barrier a tile.
 //
 // What bounds it: the waves' issue (matrix pipe busy in 40% of the cycles, 21%
-// waits), 1.05 us a tile, and per key block the start (its bits, K and V, the
-// first tiles) and the end: 4096 tokens x 16 heads over 1, 16, 64 blocks 36.5, 102
-// and 304 us; 9216 over 24 blocks 303 us, 765 TFLOP/s over its four products.
+// waits), 0.95 us a tile, and per key block 7 us with nothing beside them for the
+// start (its bits, K and V, the first tiles) and the end: 4096 tokens x 16 heads over
+// 1, 16, 64 blocks 37, 88-91 and 276 us; 9216 over 24 blocks 272 us, 850 TFLOP/s
+// over its four products.
 namespace kv {
 
 using bwd::kStat;

@@ -18,16 +18,18 @@
 // Work list order: query blocks of one head are neighbours on one XCD, so the
 // keys that they have in common come from its L2.
 //
-// What bounds it: one wave's issue beside its MFMAs, as in the dense forward; the
-// matrix pipe is busy in 50% of the cycles, 21% are waits. A tile takes a wave
-// 1.9 us. 2 x 4096 tokens of 16 heads over 16 blocks each 81 us (850 TFLOP/s),
-// 16384 tokens over 32 blocks 285-318 us (870-960); over one block each it is
-// bound by HBM (4096 tokens 13.3 us, 5 TB/s).
+// What bounds it: one wave's issue beside its MFMAs, as in the dense forward (1.9 us
+// a tile), and what a round of lists does together, start and end: 13 of 43 us for
+// 4096 tokens of 16 heads over 16 blocks each, one round. The matrix pipe is busy in 50% of
+// the cycles, 21% are waits. 2 x 4096 tokens 82 us (840 TFLOP/s), 16384 tokens over 32
+// blocks 280 us (980); 9216 over 24 blocks 158 us (730), 2.25 rounds of which the last
+// leaves three of four SIMDs idle. Over one block each it is bound by HBM (4096 tokens
+// 15.6 us, 4.3 TB/s).
 //
 // Few query blocks (fewer than the chip's SIMDs): each list is cut into
 // `nsplit` parts of whole blocks, the parts write O and their row statistics
 // in fp32 and a second launch merges them (one query, 16 heads, 32 blocks:
-// 8.9 + 4.0 us; unsplit the list alone would take 60).
+// 9.7 + 4.0 us; unsplit the list alone would take 60).
 #include <algorithm>
 #include <cfloat>
 #include <cmath>

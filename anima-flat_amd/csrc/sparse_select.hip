@@ -163,7 +163,7 @@ __device__ __forceinline__ void pick(const Scores& scores, int have, int count, 
 // waves share the blocks of keys and, with few of them, the head dims (PARTS
 // parts, which meet in LDS in a fixed order): latency bounds it, so many loads
 // are on their way at once and 512 threads take 4 rows (2048 query blocks x 64 of
-// keys: 256 threads 10.1 us, 512 6.8; 4096 x 256 25 us, 7 of them the search.
+// keys: 256 threads 10.1 us, 512 6.8; 4096 x 256 24 us, 7 of them the search.
 // 16 rows a workgroup by fp64 matrix instructions: 8.9 and 22).
 template <int PARTS>
 __device__ __forceinline__ void dot_rows(const double* qm, const double* km, int nk, int have, int rows, double* partial,

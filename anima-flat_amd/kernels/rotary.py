@@ -198,7 +198,9 @@ def rotary_tables(positions, dims, theta=10000.0, scale=1.0, scaling="ntk", orig
       "yarn"    pairs that turn at most once in the trained length `original` are stretched,
                 those that turn 32 times or more are not, a ramp between, and both tables are
                 multiplied by `0.1 ln(scale) + 1` (arXiv 2309.00071; the largest scale, with
-                several axes)
+                several axes). The ramp is linear in the number of turns, as in the paper's
+                section 3.2; a ramp in the pair's index between two rounded bounds, which
+                other programs have under this name, has other angles on it
 
     Args:
         positions: `[..., axes]` int32, int64, float32 or float64, or, where `dims` is one

@@ -518,7 +518,8 @@ typedef struct aa_rotary_tables_args {
  *   AA_SCALING_NTK     theta s^(d / (d - 2)) in theta's place (d > 2);
  *   AA_SCALING_LINEAR  f_i / s;
  *   AA_SCALING_YARN    f_i (g + (1 - g) / s), g = (original f_i / (2 pi) - 1) / 31
- *                      clamped to 0 .. 1, and both tables times 0.1 ln(max s) + 1.
+ *                      clamped to 0 .. 1 (linear in the number of turns, not in i),
+ *                      and both tables times 0.1 ln(max s) + 1.
  * The angle is exact to 2^-52 of itself: positions up to 10^8 are told apart.
  * Generalises src/model.py:51-84 (rope_tables), whose tables at 1 x 1 to h x w
  * are AA_SCALING_NTK's of axes (t, y, x).
